@@ -354,17 +354,18 @@ def _plain_append(s):
         x = x.view(B, n, BT, H, D).permute(0, 1, 3, 2, 4)[keep]         # [blocks, H, 16, 64]
         isnew = new.view(B, n, 1, BT, 1)[keep]
         isold = old.view(B, n, 1, BT, 1)[keep]
+        begun = isold.any(3, keepdim=True)  # (slots behind the last token: left as they were)
         was = cells[ids].reshape(x.shape)
         if c["fmt"] == BF16:
-            y = torch.where(isnew, x.to(torch.bfloat16), torch.where(isold, was, torch.zeros_like(was)))
+            y = torch.where(isnew, x.to(torch.bfloat16), torch.where(begun, was, torch.zeros_like(was)))
             cells[ids] = y.view(cells[ids].shape)
             continue
-        so = torch.where(isold.any(3)[..., 0], s["sc"][ids, :, i], torch.zeros_like(s["sc"][ids, :, i]))
+        so = torch.where(begun[..., 0, 0], s["sc"][ids, :, i], torch.zeros_like(s["sc"][ids, :, i]))
         sn = torch.maximum(so, _scale_of((x.abs() * isnew).amax((2, 3))))
         ratio = torch.where(sn > 0, so / sn, torch.zeros_like(sn))[..., None, None]
         moved = (_codes(was) * ratio).to(torch.float8_e4m3fn).view(torch.uint8)
         y = torch.where(isnew, _to_codes(x, sn[..., None, None]).view(torch.uint8),
-                        torch.where(isold, moved, torch.zeros_like(moved)))
+                        torch.where(isold, moved, torch.where(begun, was, torch.zeros_like(was))))
         cells[ids] = y.view(cells[ids].shape)
         s["sc"][ids, :, i] = sn
     if c["pack"]:
@@ -615,11 +616,10 @@ def exact(case, seed):
             for i, (pool, xs, place) in enumerate(zip(pools, (kn, vn), _places(c["fmt"]))):
                 cell = torch.from_numpy(place).cuda()
                 was = pool[phys][:, cell]                                 # [H, 16, 64]
-                now = torch.zeros_like(was)
                 x = xs[lo - int(start[b]):hi - int(start[b])].transpose(0, 1)
                 n_old = lo - j * BT
+                now = was.clone() if n_old else torch.zeros_like(was)
                 if not f8:
-                    now[:, :n_old] = was[:, :n_old]
                     now[:, n_old:n_old + x.shape[1]] = x
                 else:
                     a = x.abs().amax((1, 2))
