@@ -354,7 +354,7 @@ def _plain_append(s):
         x = x.view(B, n, BT, H, D).permute(0, 1, 3, 2, 4)[keep]         # [blocks, H, 16, 64]
         isnew = new.view(B, n, 1, BT, 1)[keep]
         isold = old.view(B, n, 1, BT, 1)[keep]
-        begun = isold.any(3, keepdim=True)  # (slots behind the last token: left as they were)
+        begun = isold.any(2, keepdim=True)  # (slots behind the last token: left as they were)
         was = cells[ids].reshape(x.shape)
         if c["fmt"] == BF16:
             y = torch.where(isnew, x.to(torch.bfloat16), torch.where(begun, was, torch.zeros_like(was)))
