@@ -84,28 +84,42 @@ typedef enum { GKV_F32 = 0, GKV_BF16 = 1 } gkv_dtype;
  * and 64 of V, each with one fp32 scale = max|x| / 448, code = the nearest
  * e4m3 value (ties to even) of min(max(x * (448 / max|x|), -448), 448); an
  * all-zero head has scale 0 and codes 0. No counterpart in the reference,
- * which names FP8 K/V as its next step after int8 V. */
-typedef enum { GKV_V_BF16 = 0, GKV_V_INT8 = 1, GKV_KV_FP8 = 2 } gkv_v_format;
+ * which names FP8 K/V as its next step after int8 V.
+ * GKV_KV_FP8_BLOCK stores the same codes in the same places with one fp32
+ * scale of K and one of V per BLOCK of 16 tokens and head (129 bytes a token and
+ * head for K and V together, against 136): for the gkv_kept_* entry points,
+ * gkv_copy_blocks and the pool; the other kernels refuse it. Readers take any
+ * finite scale >= 0; gkv_kept_append writes powers of two (see there). */
+typedef enum {
+  GKV_V_BF16 = 0,
+  GKV_V_INT8 = 1,
+  GKV_KV_FP8 = 2,
+  GKV_KV_FP8_BLOCK = 3
+} gkv_v_format;
 
 /* A paged cache of one layer as the kernels see it. */
 typedef struct {
   void *k;                     /* bf16 [num_blocks][n_kv_heads][1024] (K block layout);
-                                  GKV_KV_FP8: e4m3 [num_blocks][n_kv_heads][1024], code of
+                                  GKV_KV_FP8, GKV_KV_FP8_BLOCK: e4m3
+                                  [num_blocks][n_kv_heads][1024], code of
                                   token t, dim d at ((d % 32) / 8 * 16 + t) * 16 + (d / 32) * 8
                                   + d % 8 */
   void *v;                     /* GKV_V_BF16: bf16 [num_blocks][n_kv_heads][1024] (V block
                                   layout);
-                                  GKV_V_INT8 / GKV_KV_FP8: int8 / e4m3
+                                  GKV_V_INT8 / GKV_KV_FP8 / GKV_KV_FP8_BLOCK: int8 / e4m3
                                   [num_blocks][n_kv_heads][1024], code of dim d, token t at
                                   ((d % 16) * 4 + t / 4) * 16 + (d / 16) * 4 + t % 4 */
   const int32_t *block_table;  /* int32 [B][table_stride] (device) */
   int32_t table_stride;        /* entries per table row */
   int32_t num_blocks;          /* physical blocks in k / v (ids are checked against it) */
   int32_t n_kv_heads;
-  int32_t ring;                /* 0: slot = position; W > 0: slot = position % W */
+  int32_t ring;                /* 0: slot = position; W > 0: slot = position % W (the
+                                  gkv_kept_* entry points: window + 16, see there) */
   void *v_scale;               /* GKV_V_INT8: fp32 [num_blocks][n_kv_heads][16] (V scale of
                                   token t at t); GKV_KV_FP8: fp32 [num_blocks][n_kv_heads][32]
-                                  (K scale of token t at t, V scale at 16 + t); else NULL */
+                                  (K scale of token t at t, V scale at 16 + t);
+                                  GKV_KV_FP8_BLOCK: fp32 [num_blocks][n_kv_heads][2] (the
+                                  block's K scale, its V scale); else NULL */
   int32_t v_format;            /* gkv_v_format (0: bf16) */
 } gkv_cache_view;
 
@@ -407,6 +421,97 @@ int gkv_prefill_paged(void *stream, int32_t B, const int32_t *cu_seqlens,
                       const float *sinks, int32_t window, void *out, int64_t out_stride,
                       int32_t out_dtype, uint32_t *dev_err);
 
+/* ---- First tokens kept, whole blocks --------------------------------------- */
+
+/* Attention in which position p sees position t iff t <= p and (t < kept or
+ * t > p - window): a sliding window and the first tokens, which stay visible
+ * however far the sequence runs; window = 0: every t <= p (kept is then
+ * ignored). kept and window are multiples of 16 (GKV_ERR_UNSUPPORTED otherwise).
+ * No counterpart in the reference. The cache holds whole blocks, in the formats
+ * GKV_V_BF16 and GKV_KV_FP8_BLOCK (the others: GKV_ERR_UNSUPPORTED):
+ *   cache.ring = 0            logical block j (positions 16 j .. 16 j + 15) is entry
+ *                             j of the sequence's table row; entries of blocks that
+ *                             nothing sees any more may hold any id
+ *   cache.ring = window + 16  entry j for the kept blocks (j < kept / 16), behind
+ *                             them a ring: entry kept / 16 + (j - kept / 16) %
+ *                             (window / 16 + 1). One block more than the window,
+ *                             so a block is begun anew only when none of its
+ *                             tokens is seen any more. table_stride >= kept / 16 +
+ *                             window / 16 + 1 (GKV_ERR_ARG otherwise).
+ * gkv_pool_create_kept makes such caches; full layers of any pool in these formats
+ * are the ring = 0 form. sinks: fp32 [Hq] logits, or NULL (no sink). Masked
+ * positions count for nothing, whatever their slots hold; in a prefill a V that
+ * is not finite reaches every row of its workgroup's 32 that is not masked off
+ * it by a whole block. */
+
+/* Append by whole blocks: the rows of sequence b, cu_seqlens[b] ..
+ * cu_seqlens[b+1] - 1 (device int32 [B+1]; NULL: row b alone, as in a decode
+ * step), are its positions seq_lens[b] - n .. seq_lens[b] - 1 (seq_lens: device
+ * int32 [B], tokens after the append; rows at positions below 0 are skipped, so
+ * a length of 0 is an idle place in a batch). K is rotated as gkv_kv_append
+ * rotates it.
+ *   GKV_V_BF16        K and V as bf16, round to nearest even
+ *   GKV_KV_FP8_BLOCK  the scale of a block that the call begins is the smallest
+ *                     power of two s with max|x| <= 448 s over its tokens (finite
+ *                     values; 0 if all are 0); of one that it continues the larger of
+ *                     that and the scale the block has, to which the older codes move
+ *                     (code' = e4m3(code * s / s'), an exponent shift, exact unless
+ *                     the result is subnormal). code = e4m3 of min(max(x / s,
+ *                     -448), 448), ties to even; NaN stays NaN.
+ * Unwritten slots of a block that the call begins become 0, those of one that
+ * it continues stay as they are. On a ring, blocks that later ones of the same call
+ * replace are not stored. max_rows: host bound of the rows of a sequence (a
+ * sequence with more sets GKV_DEVERR_LENGTH and its further blocks are not
+ * stored). A block beyond the table row: GKV_DEVERR_LENGTH, not stored. k_pack,
+ * v_pack: NULL, or bf16 [rows][Hkv][64] as gkv_kv_append's (cache.k = cache.v =
+ * NULL: packed rows only). Two sequences of one call must not share a block
+ * that either appends to. B <= 65535. qkv, tables and packed rows are 16-byte
+ * aligned, row_stride is a multiple of 4. */
+int gkv_kept_append(void *stream, int32_t B, const int32_t *cu_seqlens, const int32_t *seq_lens,
+                    int32_t max_rows, const float *qkv, int64_t row_stride, int32_t n_q_heads,
+                    const float *cos_tab, const float *sin_tab, gkv_cache_view cache,
+                    int32_t kept, int32_t window, void *k_pack, void *v_pack,
+                    uint32_t *dev_err);
+
+/* Bytes of workspace gkv_kept_decode needs (0: none, workspace may be NULL). */
+size_t gkv_kept_workspace_bytes(int32_t B, int32_t n_kv_heads, int32_t max_seq_len, int32_t kept,
+                                int32_t window);
+
+/* Decode attention: one query token per sequence, at position seq_lens[b] - 1,
+ * its own token already appended. q, cos_tab / sin_tab, out as in
+ * gkv_decode_attention; max_seq_len: host bound of seq_lens, which the angle
+ * tables cover (a longer sequence, or one past the table row, sets
+ * GKV_DEVERR_LENGTH and is taken at the bound). A sequence of length 0 gets
+ * zeros; so does a head that sees nothing (every block id bad, no sink). At most 8
+ * kv heads and 8 query heads per kv head. Calls that may overlap need
+ * workspaces of their own. Rows are 16-byte aligned (out in bf16: 8-byte), their
+ * strides multiples of 4. */
+int gkv_kept_decode(void *stream, int32_t B, int32_t n_q_heads, const float *q, int64_t q_stride,
+                    const float *cos_tab, const float *sin_tab, const int32_t *seq_lens,
+                    int32_t max_seq_len, gkv_cache_view cache, int32_t kept, int32_t window,
+                    const float *sinks, void *workspace, size_t workspace_bytes, void *out,
+                    int64_t out_stride, int32_t out_dtype, uint32_t *dev_err);
+
+/* Causal attention of prompts (cache.k NULL, start_pos NULL: every key from the
+ * packed rows; cache.n_kv_heads counts) or of chunks that continue a cached
+ * history (start_pos: multiples of 16), with gkv_prefill_paged's arguments and
+ * rules: keys before start_pos[b] from the cache, those from there on from the
+ * packed rows (k = v = NULL: from the cache too, ring = 0 only). On a ring,
+ * append the chunk after this call. */
+int gkv_kept_prefill(void *stream, int32_t B, const int32_t *cu_seqlens, const int32_t *start_pos,
+                     int32_t max_len, int32_t n_q_heads, const float *q, int64_t q_stride,
+                     const float *cos_tab, const float *sin_tab, const void *k, const void *v,
+                     gkv_cache_view cache, int32_t kept, int32_t window, const float *sinks,
+                     void *out, int64_t out_stride, int32_t out_dtype, uint32_t *dev_err);
+
+/* Copies block src[i] to block dst[i] (device int32 [n_pairs]) in every one of
+ * n_views caches (host array; any format, K, V and scales; the block tables are
+ * not used), all in one launch per 32 views. The targets are distinct and no
+ * target is a source. An id outside a cache sets GKV_DEVERR_BLOCK_ID and is not
+ * copied there. No counterpart in the reference. */
+int gkv_copy_blocks(void *stream, const gkv_cache_view *views, int32_t n_views, int32_t n_pairs,
+                    const int32_t *src, const int32_t *dst, uint32_t *dev_err);
+
 /* ---- Exact path (fp32 caches, bit for bit with the CPU forward) ---------- */
 
 /* The reference's GPTOSS_EXACT engine build (getp-csrc/engine/gpu_engine.hpp:
@@ -477,13 +582,45 @@ typedef struct {
 } gkv_pool_config;
 
 int gkv_pool_create(const gkv_pool_config *cfg, gkv_pool **out);
+/* A pool whose window layers keep the first `kept` tokens (a multiple of 16, 0
+ * allowed) and a ring of window + 16 slots behind them, for the gkv_kept_*
+ * entry points; cfg->window > 0, formats GKV_V_BF16 and GKV_KV_FP8_BLOCK.
+ * (gkv_pool_create refuses GKV_KV_FP8_BLOCK with a window: its rings hold
+ * exactly W slots.) */
+int gkv_pool_create_kept(const gkv_pool_config *cfg, int32_t kept, gkv_pool **out);
 int gkv_pool_destroy(gkv_pool *pool);
 /* Takes a free sequence id (its length starts at 0). */
 int gkv_pool_seq_alloc(gkv_pool *pool, int32_t *seq_id);
 /* Makes room for seq_len tokens of seq_id (allocating blocks; never shrinks). */
 int gkv_pool_seq_reserve(gkv_pool *pool, int32_t seq_id, int32_t seq_len);
-/* Returns the sequence's blocks to the free list. */
+/* Returns the sequence's blocks to the free list (those that no other
+ * sequence holds). */
 int gkv_pool_seq_free(gkv_pool *pool, int32_t seq_id);
+/* A new sequence that holds the first n_tokens of parent's: the full layers'
+ * blocks are shared (freed with their last holder), the partly filled last one
+ * and the window layers' rings are copied, on stream, at once. The tokens are
+ * already appended (their kernels queued before this call on the same stream), and
+ * both sequences append behind their own lengths only. Window layers: a ring
+ * holds what it holds, so there n_tokens is the parent's length.
+ * GKV_ERR_CAPACITY (no sequence id, no block left) and GKV_ERR_ARG (more tokens
+ * than the parent has room for) take nothing. The child's table entries
+ * reach the device with the next gkv_pool_sync. */
+int gkv_pool_seq_fork(gkv_pool *pool, int32_t parent, int32_t n_tokens, void *stream,
+                      int32_t *child);
+/* Cuts the sequence back to n_tokens: returns the full layers' blocks behind
+ * them. A partly filled last block that other sequences hold is replaced by a
+ * copy (on stream), as appends go on in it; GKV_ERR_CAPACITY if that needs
+ * a block and none is left (nothing is taken then). The rings stay: what the
+ * dropped tokens overwrote is gone (on a ring of window + 16 slots nothing
+ * that is seen, if n_tokens does not go back behind the start of the block
+ * that was begun last). */
+int gkv_pool_seq_trim(gkv_pool *pool, int32_t seq_id, int32_t n_tokens, void *stream);
+/* Moves the full layers' blocks in use to the ids 0 .. n - 1 (n in *n_used, which
+ * may be NULL): one launch per 32 layers copies what lies behind, on stream, and
+ * the next gkv_pool_sync brings the tables; a kernel queued between the two
+ * on that stream still reads the old places, whose data stays until they are
+ * handed out again. */
+int gkv_pool_compact(gkv_pool *pool, void *stream, int64_t *n_used);
 /* Brings the device block tables up to date after alloc/reserve/free, on
  * stream, without waiting: only the entries changed since the last sync go,
  * from a pinned staging buffer the pool owns (one of two, each reused only

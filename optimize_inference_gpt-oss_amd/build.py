@@ -29,6 +29,9 @@ SOURCES = [
     "qkv_append.hip",
     "yardstick.hip",
     "exact_attention.hip",
+    "block_copy.hip",
+    "kept_append.hip",
+    "kept_decode.hip",
     "rope_table.cpp",
     "kv_pool.cpp",
     "capi.cpp",

@@ -1,0 +1,873 @@
+// Decode attention over a cache of whole blocks: bf16, or e4m3 codes with one
+// scale per block and kv head; every position, or a sliding window and the first
+// tokens that stay visible.
+//
+// One query token per sequence and head: score = q.k / 8, softmax over the
+// positions seen and (if given) the head's sink logit, out = sum p v. Each K and V
+// byte is read once for the whole group of query heads; 2 * 64 * 2 operations a
+// head and token against 128 (bf16: 256) bytes a kv head and token: bound by HBM.
+//
+// Matrix cores, 16x16 output, K = 32, the operand arrangement of the block
+// layouts (kv_append.hpp): S^T = K Q^T and O^T += V^T P^T, columns 0..7 the high
+// pieces of query head col's q and p, columns 8..15 the rest, added afterwards.
+// Block codes enter without their scale, which is one number per block and
+// wave: K's goes into the factor of the exponent, V's into the weights, so the
+// stream costs no scale loads per token. Against codes q is split into fp16 pieces
+// (e4m3 values are fp16 values; 22 bits of q, scaled by a power of two per head so
+// that no range is lost), against bf16 K into bf16 pieces (16 bits); p always into
+// bf16 pieces (its range is that of exp2).
+//
+// A step is two blocks (32 tokens). A wave takes the steps of one (sequence, kv
+// head), loads the next step's blocks while it computes this one's, and leaves it
+// to the other waves of its SIMD to cover the chain of matrix op, exponential,
+// matrix op: 4 waves per SIMD for codes (a step is 16 registers of data),
+// 2 for bf16 with a ring of 3 steps. Two ways to deal the steps out:
+//   whole   few steps a sequence (a window, short contexts): a (sequence, kv
+//           head) belongs to 1 .. 8 waves of one workgroup, which cut its steps and
+//           merge in LDS. One launch, no workspace.
+//   ranges  the sequences laid end to end are cut into equal ranges, one per
+//           resident wave; every workgroup finds its own range from the lengths
+//           in its prologue. A sequence inside one range is finished there,
+//           the pieces of the others go to the workspace and a second launch
+//           merges them, a workgroup per (sequence, kv head).
+#include "kept.hpp"
+
+#include <algorithm>
+
+namespace gkv {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+constexpr int kKeptAux = 2;            // nontemporal: each K/V byte is read once
+constexpr int kKeptStep = 32;          // tokens per step
+constexpr int kHeads = 8;              // query heads per kv head, at most
+constexpr int kSplitWgs = 512;         // range workgroups: two per CU (bf16: 256, one per CU)
+constexpr int kMinRangeSteps = 4;      // steps per range, at least
+constexpr int kPieceFloats = kHeads * kHeadDim;
+constexpr int kPieceMl = 2 * kHeads;   // (m, l) of a piece's heads
+constexpr float kLowest = -1e30f;      // the running maximum before any score (log2 units)
+constexpr int kMergeThreads = 512;
+constexpr int kMergeChunk = 256;       // pieces whose weights are held in LDS at a time
+
+struct KeptDecodeArgs {
+  const float *q;
+  int64_t q_stride;
+  const float *cos_tab, *sin_tab;
+  const int32_t *seq_lens;
+  const char *kc, *vc;
+  const float *scales;
+  const int32_t *table;
+  int table_stride, num_blocks;
+  KeptRow row;
+  int window, max_len;
+  const float *sinks; // NULL: none
+  int B, G, n_kv_heads;
+  int parts, heads_per_wg; // whole: waves per (sequence, head), heads per workgroup
+  int max_ranges;          // ranges: waves launched per kv head
+  int32_t *plan;           // ranges: {T, n}, then the B + 1 prefix sums of the steps
+  float *ws_ml, *ws_o;     // [range][2][n_kv_heads]: a range's first and last piece
+  void *out;
+  int64_t out_stride;
+  int out_bf16;
+  uint32_t *dev_err;
+};
+
+// What a sequence's query sees: blocks 0 .. first_blocks - 1, then from
+// logical block win0 on, n_blocks in all.
+struct Span {
+  int L, first_blocks, win0, n_blocks;
+  int ring0; // win0's place in the ring
+};
+
+__device__ __forceinline__ int span_len(const KeptDecodeArgs &a, int b) {
+  return max(min(a.seq_lens[b], a.max_len), 0);
+}
+
+__device__ __forceinline__ Span span_of(const KeptDecodeArgs &a, int L) {
+  Span s;
+  s.L = L;
+  const int nb = (L + kBlockTokens - 1) / kBlockTokens;
+  if (a.window == 0) {
+    s.first_blocks = s.n_blocks = nb;
+    s.win0 = s.ring0 = 0;
+    return s;
+  }
+  s.first_blocks = min(a.row.kept_blocks, nb);
+  s.win0 = max(max(L - a.window, 0) / kBlockTokens, a.row.kept_blocks);
+  s.n_blocks = s.first_blocks + max(nb - s.win0, 0);
+  s.ring0 = a.row.ring_blocks
+                ? (int)((uint32_t)(s.win0 - a.row.kept_blocks) % (uint32_t)a.row.ring_blocks)
+                : 0;
+  return s;
+}
+
+__device__ __forceinline__ int span_steps(const Span &s) { return (s.n_blocks + 1) / 2; }
+
+// Table entry of the span's i-th block (a window spans at most the ring).
+__device__ __forceinline__ int span_entry(const KeptDecodeArgs &a, const Span &s, int i) {
+  if (i < s.first_blocks)
+    return i;
+  const int w = i - s.first_blocks;
+  if (a.row.ring_blocks == 0)
+    return s.win0 + w;
+  const int e = s.ring0 + w;
+  return a.row.kept_blocks + (e >= a.row.ring_blocks ? e - a.row.ring_blocks : e);
+}
+
+__device__ __forceinline__ void put(void *out, int64_t i, f32x4 v, int bf16) {
+  if (bf16)
+    *(u32x2 *)((uint16_t *)out + i) =
+        u32x2{f32x2_to_bf16_rne(v[0], v[1]), f32x2_to_bf16_rne(v[2], v[3])};
+  else
+    *(f32x4 *)((float *)out + i) = v;
+}
+
+// The running state of one wave: maximum (log2 units) and weight sum of this
+// lane's column, its part of O^T.
+struct State {
+  float m, l;
+  f32x4 o[4];
+};
+
+template <bool BLK>
+struct StepData {
+  u32x4 k[BLK ? 2 : 4], v[BLK ? 2 : 4];
+  f32x2 sc[2]; // per block: K scale, V scale (wave-uniform)
+};
+
+typedef const __attribute__((address_space(4))) int32_t *ScalarI32;
+typedef const __attribute__((address_space(4))) f32x2 *ScalarF2;
+
+// Four e4m3 codes -> four fp16 (exact).
+__device__ __forceinline__ u32x2 codes_to_f16(uint32_t w) {
+  const f16x2 a = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
+  const f16x2 b = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true));
+  return u32x2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
+}
+
+// Steps s0 .. s1 - 1 of sequence b for kv head g, by one wave. R: steps of data in
+// registers.
+template <bool BLK, int R>
+__device__ __forceinline__ State attend(const KeptDecodeArgs &a, int b, int g, const Span &sp,
+                                        int s0, int s1) {
+  constexpr int D = kHeadDim;
+  constexpr int kHeadBytes = kBlockTokens * D * (BLK ? 1 : 2);
+  const int lane = threadIdx.x & 63, col = lane & 15, kg = lane >> 4;
+  const bool low = col >= 8;
+  const int head = col & 7;
+  const bool head_ok = head < a.G;
+  const uint32_t k_off = lane * 16;
+  const uint32_t v_off = BLK ? (col * 4 + kg) * 16 : lane * 16;
+
+  // The block ids of a step (-1: none, or outside the pool), read through the
+  // scalar cache a step before they are used.
+  const int64_t trow = (int64_t)b * a.table_stride;
+  bool bad = false;
+  auto ids_of = [&](int s) -> int2 {
+    int2 r{-1, -1};
+    if (s < s1) {
+      r.x = ((ScalarI32)a.table)[trow + span_entry(a, sp, 2 * s)];
+      if (2 * s + 1 < sp.n_blocks)
+        r.y = ((ScalarI32)a.table)[trow + span_entry(a, sp, 2 * s + 1)];
+    }
+    return r;
+  };
+  auto load = [&](StepData<BLK> &x, int2 ids, int s) {
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      int id = uniform(j ? ids.y : ids.x);
+      const bool ok = id >= 0 && id < a.num_blocks;
+      bad |= !ok && s < s1 && 2 * s + j < sp.n_blocks;
+      id = ok ? id : 0;
+      const int64_t hb = (int64_t)id * a.n_kv_heads + g;
+      // a missing block reads nothing: its resource covers 0 bytes
+      const __amdgpu_buffer_rsrc_t kr = head_rsrc(a.kc + hb * kHeadBytes, ok ? kHeadBytes : 0);
+      const __amdgpu_buffer_rsrc_t vr = head_rsrc(a.vc + hb * kHeadBytes, ok ? kHeadBytes : 0);
+      if (BLK) {
+        x.sc[j] = ((ScalarF2)a.scales)[hb];
+        x.k[j] = __builtin_amdgcn_raw_buffer_load_b128(kr, k_off, 0, kKeptAux);
+        x.v[j] = __builtin_amdgcn_raw_buffer_load_b128(vr, v_off, 0, kKeptAux);
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          x.k[2 * j + h] = __builtin_amdgcn_raw_buffer_load_b128(kr, k_off + h * 1024, 0, kKeptAux);
+          x.v[2 * j + h] = __builtin_amdgcn_raw_buffer_load_b128(vr, v_off + h * 1024, 0, kKeptAux);
+        }
+      }
+      if (!ok)
+        x.sc[j] = f32x2{-1.0f, 0.0f}; // (the mark of a missing block)
+      else if (!BLK)
+        x.sc[j] = f32x2{0.0f, 0.0f};
+    }
+  };
+
+  StepData<BLK> buf[R];
+  int2 ids = ids_of(s0);
+#pragma unroll
+  for (int i = 0; i < R - 1; i++) {
+    const int2 next = ids_of(s0 + i + 1);
+    load(buf[i], ids, s0 + i);
+    ids = next;
+  }
+
+  // The query: dims 8kg .. +7 and 32+8kg .. +7 of the column's head, rotated at
+  // the sequence's last position, scaled, in two pieces.
+  float qa[8], qb[8];
+  {
+    const f32x4 *qp =
+        (const f32x4 *)(a.q + (int64_t)b * a.q_stride + (g * a.G + (head_ok ? head : 0)) * D + 8 * kg);
+    const f32x4 x0 = qp[0], x1 = qp[1], x2 = qp[8], x3 = qp[9];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      qa[i] = x0[i];
+      qa[4 + i] = x1[i];
+      qb[i] = x2[i];
+      qb[4 + i] = x3[i];
+    }
+    if (a.cos_tab) {
+      const f32x4 *cp = (const f32x4 *)(a.cos_tab + (int64_t)(sp.L - 1) * (D / 2) + 8 * kg);
+      const f32x4 *np = (const f32x4 *)(a.sin_tab + (int64_t)(sp.L - 1) * (D / 2) + 8 * kg);
+#pragma unroll
+      for (int i4 = 0; i4 < 2; i4++) {
+        const f32x4 c = cp[i4], n = np[i4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          const float y1 = qa[4 * i4 + i], y2 = qb[4 * i4 + i];
+          qa[4 * i4 + i] = rope_first(y1, y2, c[i], n[i]);
+          qb[4 * i4 + i] = rope_second(y1, y2, c[i], n[i]);
+        }
+      }
+    }
+  }
+  float qf = 0.125f * kLog2e; // 1 / sqrt(64); exp -> exp2
+  if (BLK) {
+    // q * 2^-e has its largest element in [1, 2)
+    float mx = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+      mx = fmaxf(mx, fmaxf(fabsf(qa[i]), fabsf(qb[i])));
+    mx = fmaxf(mx, __shfl_xor(mx, 16));
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
+    const int e = min(max((int)(__float_as_uint(mx) >> 23), 27), 227);
+    const float down = __uint_as_float((uint32_t)(254 - e) << 23);
+    qf *= __uint_as_float((uint32_t)e << 23);
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      qa[i] *= down;
+      qb[i] *= down;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      qa[i] *= qf;
+      qb[i] *= qf;
+    }
+  }
+  u32x4 q0, q1;
+  {
+    typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+    if (BLK) {
+      f16x8 x, y;
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const _Float16 hx = (_Float16)qa[i], hy = (_Float16)qb[i];
+        x[i] = low ? (_Float16)(qa[i] - (float)hx) : hx;
+        y[i] = low ? (_Float16)(qb[i] - (float)hy) : hy;
+      }
+      q0 = __builtin_bit_cast(u32x4, x);
+      q1 = __builtin_bit_cast(u32x4, y);
+    } else {
+      bf16x8_t x, y;
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const __bf16 hx = (__bf16)qa[i], hy = (__bf16)qb[i];
+        x[i] = low ? (__bf16)(qa[i] - (float)hx) : hx;
+        y[i] = low ? (__bf16)(qb[i] - (float)hy) : hy;
+      }
+      q0 = __builtin_bit_cast(u32x4, x);
+      q1 = __builtin_bit_cast(u32x4, y);
+    }
+    if (!head_ok)
+      q0 = q1 = u32x4{0, 0, 0, 0};
+  }
+
+  State st;
+  st.m = kLowest;
+  st.l = 0.0f;
+#pragma unroll
+  for (int nn = 0; nn < 4; nn++)
+    st.o[nn] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+  auto compute = [&](StepData<BLK> &x, int s) {
+    float t[8];
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (BLK) {
+        const u32x2 c0 = codes_to_f16(x.k[j][0]), c1 = codes_to_f16(x.k[j][1]);
+        const u32x2 c2 = codes_to_f16(x.k[j][2]), c3 = codes_to_f16(x.k[j][3]);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+            __builtin_bit_cast(f16x8, u32x4{c0[0], c0[1], c1[0], c1[1]}),
+            __builtin_bit_cast(f16x8, q0), acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+            __builtin_bit_cast(f16x8, u32x4{c2[0], c2[1], c3[0], c3[1]}),
+            __builtin_bit_cast(f16x8, q1), acc, 0, 0, 0);
+      } else {
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x.k[2 * j]),
+                                                      __builtin_bit_cast(bf16x8, q0), acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x.k[2 * j + 1]),
+                                                      __builtin_bit_cast(bf16x8, q1), acc, 0, 0, 0);
+      }
+      const float c = BLK ? qf * x.sc[j][0] : 1.0f;
+#pragma unroll
+      for (int r = 0; r < 4; r++) {
+        t[4 * j + r] = acc[r] + swap8(acc[r]);
+        if (BLK)
+          t[4 * j + r] *= c;
+      }
+    }
+    // The tokens of the block that are seen: all but in a sequence's last block
+    // and in a window's first. The others get weight 0, and their values (never
+    // written, or no longer seen) become 0.
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+      const int i = 2 * s + j;
+      const int blk = i < sp.first_blocks ? i : sp.win0 + i - sp.first_blocks;
+      int hi = min(sp.L - blk * kBlockTokens, kBlockTokens);
+      int lo = 0;
+      if (a.window > 0 && i >= sp.first_blocks)
+        lo = max(sp.L - a.window - blk * kBlockTokens, 0);
+      if (i >= sp.n_blocks || x.sc[j][0] < 0.0f)
+        hi = 0;
+      if (lo > 0 || hi < kBlockTokens) {
+        uint32_t keep = 0;
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+          const int tk = 4 * kg + r;
+          const bool in = tk >= lo && tk < hi;
+          keep |= in ? 0xffu << (8 * r) : 0u;
+          if (!in)
+            t[4 * j + r] = -INFINITY;
+        }
+        if (BLK) {
+#pragma unroll
+          for (int nn = 0; nn < 4; nn++)
+            x.v[j][nn] &= keep;
+        } else {
+          const uint32_t m0 = (keep & 0xffu ? 0xffffu : 0u) | (keep & 0xff00u ? 0xffff0000u : 0u);
+          const uint32_t m1 =
+              (keep & 0xff0000u ? 0xffffu : 0u) | (keep & 0xff000000u ? 0xffff0000u : 0u);
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            u32x4 &v = x.v[2 * j + h];
+            v = u32x4{v[0] & m0, v[1] & m1, v[2] & m0, v[3] & m1};
+          }
+        }
+      }
+    }
+    float mx = t[0];
+#pragma unroll
+    for (int i = 1; i < 8; i++)
+      mx = fmaxf(mx, t[i]);
+    // The running maximum moves only when a score passes it by more than 8
+    // (weights stay below 2^8); the test needs no cross-lane maximum, only the
+    // move does (m is the same in the 4 lanes of a column).
+    if (__any(mx > st.m + 8.0f)) {
+      mx = fmaxf(mx, __shfl_xor(mx, 16));
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      const float m = fmaxf(st.m, mx);
+      const float f = __builtin_amdgcn_exp2f(st.m - m);
+      st.m = m;
+      st.l *= f;
+#pragma unroll
+      for (int nn = 0; nn < 4; nn++)
+        st.o[nn] *= f;
+    }
+    float p[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      p[i] = __builtin_amdgcn_exp2f(t[i] - st.m);
+      st.l += p[i];
+      if (BLK)
+        p[i] *= x.sc[i >> 2][1];
+    }
+    bf16x8 pw;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const __bf16 h = (__bf16)p[i];
+      pw[i] = low ? (__bf16)(p[i] - (float)h) : h;
+    }
+#pragma unroll
+    for (int nn = 0; nn < 4; nn++) {
+      u32x4 w;
+      if (BLK) {
+        const u32x2 y0 = fp8x4_to_bf16x4(x.v[0][nn]), y1 = fp8x4_to_bf16x4(x.v[1][nn]);
+        w = u32x4{y0[0], y0[1], y1[0], y1[1]};
+      } else {
+        // half h = nn / 2 of each block, dims col + 32 h + 16 (nn % 2)
+        const u32x4 y0 = x.v[nn / 2], y1 = x.v[2 + nn / 2];
+        const int k = 2 * (nn & 1);
+        w = u32x4{y0[k], y0[k + 1], y1[k], y1[k + 1]};
+      }
+      st.o[nn] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), pw,
+                                                         st.o[nn], 0, 0, 0);
+    }
+  };
+
+  for (int s = s0; s < s1; s += R) {
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      if (s + r >= s1)
+        break;
+      const int2 next = ids_of(s + r + R);
+      load(buf[(r + R - 1) % R], ids, s + r + R - 1);
+      ids = next;
+      compute(buf[r], s + r);
+    }
+  }
+  if (bad && lane == 0 && a.dev_err)
+    atomicOr(a.dev_err, GKV_DEVERR_BLOCK_ID);
+  // the four lanes of a column hold its weights, the two columns of a head the
+  // pieces of its output
+  st.l += __shfl_xor(st.l, 16);
+  st.l += __shfl_xor(st.l, 32);
+#pragma unroll
+  for (int nn = 0; nn < 4; nn++)
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+      st.o[nn][r] += swap8(st.o[nn][r]);
+  return st;
+}
+
+// The factor that turns sum p v (weights against the maximum m, sum l) into the
+// output: 1 / (l + sink weight), 0 where nothing was seen.
+__device__ __forceinline__ float out_factor(float m, float l, float sink2) {
+  const float M = fmaxf(m, sink2);
+  const float f = __builtin_amdgcn_exp2f(m - M);
+  const float den = fmaf(l, f, __builtin_amdgcn_exp2f(sink2 - M));
+  return den == 0.0f ? 0.0f : f / den; // (a NaN stays one)
+}
+
+__device__ __forceinline__ float sink_of(const KeptDecodeArgs &a, int g, int head) {
+  return a.sinks ? a.sinks[g * a.G + head] * kLog2e : -INFINITY;
+}
+
+// The finished output of one (sequence, kv head), from the wave that holds it all.
+__device__ __forceinline__ void put_whole(const KeptDecodeArgs &a, int b, int g, const State &st) {
+  const int lane = threadIdx.x & 63, col = lane & 15, kg = lane >> 4;
+  if (col >= a.G) // (at most 8: the high pieces' columns)
+    return;
+  const float f = out_factor(st.m, st.l, sink_of(a, g, col));
+  const int64_t ob = (int64_t)b * a.out_stride + (int64_t)(g * a.G + col) * kHeadDim + 4 * kg;
+#pragma unroll
+  for (int nn = 0; nn < 4; nn++)
+    put(a.out, ob + 16 * nn, st.o[nn] * f, a.out_bf16);
+}
+
+__device__ __forceinline__ void put_zeros(const KeptDecodeArgs &a, int64_t at, int n, int t, int nt) {
+  for (int i = 4 * t; i < n; i += 4 * nt)
+    put(a.out, at + i, f32x4{0.0f, 0.0f, 0.0f, 0.0f}, a.out_bf16);
+}
+
+// ---- whole: one workgroup holds every step of its (sequence, kv head)s --------------
+
+template <bool BLK, int R, int WPE>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(WPE)))
+void kept_decode_whole_kernel(KeptDecodeArgs a) {
+  __shared__ float s_o[8][kPieceFloats];
+  __shared__ float2 s_ml[8][kHeads];
+  const int n_groups = (a.n_kv_heads + a.heads_per_wg - 1) / a.heads_per_wg;
+  const int b = blockIdx.x / n_groups;
+  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int slot = wave / a.parts, part = wave % a.parts;
+  const int g = (int)(blockIdx.x % n_groups) * a.heads_per_wg + slot;
+  const int len = uniform(a.seq_lens[b]);
+  if (len > a.max_len && threadIdx.x == 0 && a.dev_err)
+    atomicOr(a.dev_err, GKV_DEVERR_LENGTH);
+  const Span sp = span_of(a, max(min(len, a.max_len), 0));
+  const int n = span_steps(sp);
+  const bool ok = g < a.n_kv_heads;
+  if (n == 0) { // an empty sequence: zeros
+    if (ok)
+      put_zeros(a, (int64_t)b * a.out_stride + (int64_t)g * a.G * kHeadDim, a.G * kHeadDim,
+                part * 64 + lane, a.parts * 64);
+    return;
+  }
+  State st;
+  if (ok) {
+    const int s0 = part * n / a.parts, s1 = (part + 1) * n / a.parts;
+    if (s0 < s1) {
+      st = attend<BLK, R>(a, b, g, sp, s0, s1);
+    } else {
+      st.m = kLowest;
+      st.l = 0.0f;
+#pragma unroll
+      for (int nn = 0; nn < 4; nn++)
+        st.o[nn] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    if (a.parts == 1) {
+      put_whole(a, b, g, st);
+      return;
+    }
+    const int col = lane & 15, kg = lane >> 4;
+    if (col < kHeads) {
+#pragma unroll
+      for (int nn = 0; nn < 4; nn++)
+        *(f32x4 *)&s_o[wave][col * kHeadDim + 16 * nn + 4 * kg] = st.o[nn];
+      if (kg == 0)
+        s_ml[wave][col] = float2{st.m, st.l};
+    }
+  }
+  if (a.parts == 1)
+    return;
+  __syncthreads();
+  if (!ok)
+    return;
+  // the parts' sums against their common maximum, 4 dims a thread
+  const int w0 = slot * a.parts;
+  for (int e = part * 64 + lane; e < a.G * (kHeadDim / 4); e += a.parts * 64) {
+    const int h = e / (kHeadDim / 4);
+    float m = kLowest, l = 0.0f;
+    for (int p = 0; p < a.parts; p++)
+      m = fmaxf(m, s_ml[w0 + p][h].x);
+    f32x4 o{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int p = 0; p < a.parts; p++) {
+      const float f = __builtin_amdgcn_exp2f(s_ml[w0 + p][h].x - m);
+      l = fmaf(s_ml[w0 + p][h].y, f, l);
+      o += *(const f32x4 *)&s_o[w0 + p][4 * e] * f;
+    }
+    put(a.out, (int64_t)b * a.out_stride + (int64_t)g * a.G * kHeadDim + 4 * e,
+        o * out_factor(m, l, sink_of(a, g, h)), a.out_bf16);
+  }
+}
+
+// ---- ranges ----------------------------------------------------------------------
+
+// Range r of the T steps cut into n.
+__device__ __forceinline__ int range_begin(int r, int T, int n) {
+  return (int)((int64_t)r * T / n);
+}
+
+template <bool BLK, int R, int WPE>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(WPE)))
+void kept_decode_split_kernel(KeptDecodeArgs a) {
+  __shared__ int s_wave[8];
+  __shared__ int s_b[8], s_c[8];
+  const int t = threadIdx.x, lane = t & 63, wave = uniform(t >> 6), nt = blockDim.x;
+  const int n_waves = nt >> 6, subs = n_waves / a.n_kv_heads; // ranges in this workgroup
+
+  // Prefix sums of the sequences' steps: thread t holds sequences t * per ..
+  const int per = (a.B + nt - 1) / nt;
+  const int b0 = min(t * per, a.B), b1 = min(b0 + per, a.B);
+  int mine = 0;
+  bool over = false;
+  for (int b = b0; b < b1; b++) {
+    over |= a.seq_lens[b] > a.max_len;
+    mine += span_steps(span_of(a, span_len(a, b)));
+  }
+  int incl = mine;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int v = __shfl_up(incl, off, 64);
+    if (lane >= off)
+      incl += v;
+  }
+  if (lane == 63)
+    s_wave[wave] = incl;
+  __syncthreads();
+  int before = 0, T = 0;
+  for (int w = 0; w < n_waves; w++) {
+    const int v = s_wave[w];
+    before += w < wave ? v : 0;
+    T += v;
+  }
+  T = uniform(T);
+  const int n = min(a.max_ranges, max(T / kMinRangeSteps, 1));
+  const int r0 = blockIdx.x * subs;
+  int c = before + incl - mine;
+  // each of the workgroup's ranges: the sequence that holds its first step
+  for (int b = b0; b < b1; b++) {
+    const int m = span_steps(span_of(a, span_len(a, b)));
+    for (int k = 0; k < subs; k++) {
+      const int at = r0 + k < n ? range_begin(r0 + k, T, n) : -1;
+      if (c <= at && at < c + m) {
+        s_b[k] = b;
+        s_c[k] = c;
+      }
+    }
+    if (blockIdx.x == 0)
+      a.plan[2 + b] = c;
+    c += m;
+  }
+  if (blockIdx.x == 0 && t == 0) {
+    a.plan[0] = T;
+    a.plan[1] = n;
+    a.plan[2 + a.B] = T;
+  }
+  if (blockIdx.x == 0 && over && a.dev_err)
+    atomicOr(a.dev_err, GKV_DEVERR_LENGTH);
+  // sequences without tokens: zeros
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x)
+    if (a.seq_lens[b] <= 0 || a.max_len <= 0)
+      put_zeros(a, (int64_t)b * a.out_stride, a.n_kv_heads * a.G * kHeadDim, t, nt);
+  __syncthreads();
+
+  const int sub = wave / a.n_kv_heads, g = wave % a.n_kv_heads;
+  const int r = r0 + sub;
+  if (r >= n || T == 0)
+    return;
+  const int rs = range_begin(r, T, n), re = range_begin(r + 1, T, n);
+  int b = uniform(s_b[sub]), cb = uniform(s_c[sub]);
+  while (cb < re) {
+    const Span sp = span_of(a, uniform(span_len(a, b)));
+    const int m = span_steps(sp);
+    const int s0 = max(rs - cb, 0), s1 = min(re - cb, m);
+    if (s0 < s1) {
+      const State st = attend<BLK, R>(a, b, g, sp, s0, s1);
+      if (s0 == 0 && s1 == m) {
+        put_whole(a, b, g, st);
+      } else {
+        const int col = lane & 15, kg = lane >> 4;
+        const int64_t piece = ((int64_t)r * 2 + (cb + s0 == rs ? 0 : 1)) * a.n_kv_heads + g;
+        if (col < kHeads) {
+          float *o = a.ws_o + piece * kPieceFloats + col * kHeadDim + 4 * kg;
+#pragma unroll
+          for (int nn = 0; nn < 4; nn++)
+            *(f32x4 *)(o + 16 * nn) = st.o[nn];
+          if (kg == 0)
+            *(float2 *)(a.ws_ml + piece * kPieceMl + 2 * col) = float2{st.m, st.l};
+        }
+      }
+    }
+    cb += m;
+    b++;
+  }
+}
+
+// The pieces of one (sequence, kv head) that was cut: M = max m_i, out =
+// sum o_i 2^(m_i - M) / (sum l_i 2^(m_i - M) + 2^(sink - M)). The weights of up to
+// kMergeChunk pieces stand in LDS; then each group of 128 threads (4 dims of a
+// query head a thread) sums every fourth piece. Bound by latency: the plan, the
+// (m, l), the pieces.
+__global__ __launch_bounds__(kMergeThreads) void kept_decode_merge_kernel(KeptDecodeArgs a) {
+  constexpr int kGroups = kMergeThreads / 128, kWaves = kMergeThreads / 64;
+  __shared__ float s_w[kMergeChunk][kHeads];
+  __shared__ float s_red[kWaves][kHeads], s_m[kHeads], s_l[kHeads];
+  __shared__ f32x4 s_o[kGroups][128];
+  const int b = blockIdx.x / a.n_kv_heads, g = blockIdx.x % a.n_kv_heads;
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  const int T = a.plan[0], n = a.plan[1], c0 = a.plan[2 + b], c1 = a.plan[3 + b];
+  if (c0 == c1)
+    return;
+  const int w0 = (int)(((int64_t)(c0 + 1) * n - 1) / T), w1 = (int)(((int64_t)c1 * n - 1) / T);
+  if (w0 == w1)
+    return; // finished by its range
+  const int first_slot = range_begin(w0, T, n) < c0 ? 1 : 0;
+  auto piece = [&](int i) {
+    return ((int64_t)(w0 + i) * 2 + (i == 0 ? first_slot : 0)) * a.n_kv_heads + g;
+  };
+  const int np = w1 - w0 + 1, h = t & 7;
+  float m = kLowest;
+  for (int i = t >> 3; i < np; i += kMergeThreads / 8)
+    m = fmaxf(m, a.ws_ml[piece(i) * kPieceMl + 2 * h]);
+#pragma unroll
+  for (int off = 8; off < 64; off <<= 1)
+    m = fmaxf(m, __shfl_xor(m, off));
+  if (lane < 8)
+    s_red[wave][lane] = m;
+  __syncthreads();
+  if (t < 8) {
+    for (int w = 0; w < kWaves; w++)
+      m = fmaxf(m, s_red[w][t]);
+    s_m[t] = m;
+  }
+  __syncthreads();
+  m = s_m[h];
+  float l = 0.0f;
+  f32x4 o{0.0f, 0.0f, 0.0f, 0.0f};
+  const int grp = t / 128, e = t % 128, eh = e / 16;
+  for (int i0 = 0; i0 < np; i0 += kMergeChunk) {
+    const int cnt = min(np - i0, kMergeChunk);
+    for (int i = t >> 3; i < cnt; i += kMergeThreads / 8) {
+      const float2 ml = *(const float2 *)(a.ws_ml + piece(i0 + i) * kPieceMl + 2 * h);
+      const float w = __builtin_amdgcn_exp2f(ml.x - m);
+      s_w[i][h] = w;
+      l = fmaf(ml.y, w, l);
+    }
+    __syncthreads();
+    for (int i = grp; i < cnt; i += 4 * kGroups) {
+      f32x4 x[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        x[j] = *(const f32x4 *)(a.ws_o + piece(i0 + min(i + j * kGroups, cnt - 1)) * kPieceFloats + 4 * e);
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        if (i + j * kGroups < cnt)
+          o += x[j] * s_w[i + j * kGroups][eh];
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int off = 8; off < 64; off <<= 1)
+    l += __shfl_xor(l, off);
+  if (lane < 8)
+    s_red[wave][lane] = l;
+  s_o[grp][e] = o;
+  __syncthreads();
+  if (t < 8) {
+    l = 0.0f;
+    for (int w = 0; w < kWaves; w++)
+      l += s_red[w][t];
+    s_l[t] = l;
+  }
+  __syncthreads();
+  if (t >= 128 || eh >= a.G)
+    return;
+#pragma unroll
+  for (int k = 1; k < kGroups; k++)
+    o += s_o[k][e];
+  put(a.out, (int64_t)b * a.out_stride + (int64_t)g * a.G * kHeadDim + 4 * e,
+      o * out_factor(s_m[eh], s_l[eh], sink_of(a, g, eh)), a.out_bf16);
+}
+
+// ---- host side --------------------------------------------------------------------
+
+// Steps of the longest sequence that a call with these bounds can meet.
+static int64_t steps_bound(int32_t max_seq_len, int32_t kept, int32_t window) {
+  int64_t blocks = ((int64_t)max_seq_len + kBlockTokens - 1) / kBlockTokens;
+  if (window > 0)
+    blocks = std::min<int64_t>(blocks, ((int64_t)kept + window) / kBlockTokens + 1);
+  return (blocks + 1) / 2;
+}
+
+static bool use_whole(int32_t B, int32_t n_kv_heads, int32_t max_seq_len, int32_t kept,
+                      int32_t window) {
+  (void)B;
+  (void)n_kv_heads;
+  return steps_bound(max_seq_len, kept, window) <= (window > 0 ? 160 : 16);
+}
+
+static int range_subs(int n_kv_heads) { return 8 / n_kv_heads; }
+
+struct KeptWorkspace {
+  size_t ml, o, total;
+};
+static KeptWorkspace kept_workspace(int32_t B, int32_t n_kv_heads) {
+  auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
+  const size_t pieces = (size_t)kSplitWgs * range_subs(n_kv_heads) * 2 * n_kv_heads;
+  KeptWorkspace w;
+  w.ml = up(((size_t)B + 3) * 4);
+  w.o = w.ml + up(pieces * kPieceMl * 4);
+  w.total = w.o + pieces * kPieceFloats * 4;
+  return w;
+}
+
+} // namespace gkv
+
+extern "C" size_t gkv_kept_workspace_bytes(int32_t B, int32_t n_kv_heads, int32_t max_seq_len,
+                                           int32_t kept, int32_t window) {
+  using namespace gkv;
+  if (B <= 0 || n_kv_heads <= 0 || n_kv_heads > 8 || max_seq_len < 0 || kept < 0 || window < 0 ||
+      use_whole(B, n_kv_heads, max_seq_len, kept, window))
+    return 0;
+  return kept_workspace(B, n_kv_heads).total;
+}
+
+extern "C" int gkv_kept_decode(void *stream, int32_t B, int32_t n_q_heads, const float *q,
+                               int64_t q_stride, const float *cos_tab, const float *sin_tab,
+                               const int32_t *seq_lens, int32_t max_seq_len, gkv_cache_view cache,
+                               int32_t kept, int32_t window, const float *sinks, void *workspace,
+                               size_t workspace_bytes, void *out, int64_t out_stride,
+                               int32_t out_dtype, uint32_t *dev_err) {
+  using namespace gkv;
+  if (B < 0 || n_q_heads <= 0 || max_seq_len < 0 || !q || !seq_lens || !out ||
+      (out_dtype != GKV_F32 && out_dtype != GKV_BF16) || (cos_tab == nullptr) != (sin_tab == nullptr))
+    return GKV_ERR_ARG;
+  int st = kept_check(cache, kept, window, true);
+  if (st != GKV_OK)
+    return st;
+  if (n_q_heads % cache.n_kv_heads != 0)
+    return GKV_ERR_ARG;
+  const int G = n_q_heads / cache.n_kv_heads;
+  if (cache.n_kv_heads > 8 || G > kHeads)
+    return GKV_ERR_UNSUPPORTED;
+  if (q_stride < (int64_t)n_q_heads * kHeadDim || out_stride < (int64_t)n_q_heads * kHeadDim)
+    return GKV_ERR_ARG;
+  // 16-byte loads of the query rows and the angles, 16- (bf16: 8-) byte stores
+  if (q_stride % 4 != 0 || out_stride % 4 != 0 ||
+      ((uintptr_t)q | (uintptr_t)cos_tab | (uintptr_t)sin_tab) % 16 != 0 ||
+      (uintptr_t)out % (out_dtype == GKV_BF16 ? 8 : 16) != 0)
+    return GKV_ERR_ARG;
+  const int64_t steps = steps_bound(max_seq_len, kept, window);
+  if ((int64_t)B * steps >= INT32_MAX || (int64_t)B * cache.n_kv_heads >= INT32_MAX)
+    return GKV_ERR_UNSUPPORTED; // 32-bit step counts
+  const bool blk = cache.v_format == GKV_KV_FP8_BLOCK;
+  KeptDecodeArgs a{};
+  a.q = q;
+  a.q_stride = q_stride;
+  a.cos_tab = cos_tab;
+  a.sin_tab = sin_tab;
+  a.seq_lens = seq_lens;
+  a.kc = (const char *)cache.k;
+  a.vc = (const char *)cache.v;
+  a.scales = (const float *)cache.v_scale;
+  a.table = cache.block_table;
+  a.table_stride = cache.table_stride;
+  a.num_blocks = cache.num_blocks;
+  a.row = KeptRow{kept / kBlockTokens, cache.ring / kBlockTokens};
+  a.window = window;
+  a.max_len = (int)std::min<int64_t>(max_seq_len, kept_capacity(cache.table_stride, cache.ring) - 1);
+  if (cache.ring == 0)
+    a.max_len = (int)std::min<int64_t>(max_seq_len, kept_capacity(cache.table_stride, 0));
+  a.sinks = sinks;
+  a.B = B;
+  a.G = G;
+  a.n_kv_heads = cache.n_kv_heads;
+  a.out = out;
+  a.out_stride = out_stride;
+  a.out_bf16 = out_dtype == GKV_BF16;
+  a.dev_err = dev_err;
+  hipStream_t s = (hipStream_t)stream;
+  if (use_whole(B, a.n_kv_heads, max_seq_len, kept, window)) {
+    if (B == 0)
+      return GKV_OK;
+    // waves per (sequence, head): as many as leave every wave slot of the GPU
+    // taken, at most 8 and no more than there are steps
+    const int64_t slots = 256 * (blk ? 16 : 8);
+    int parts = 1;
+    while (parts < 8 && 2 * parts * (int64_t)B * a.n_kv_heads <= slots && 2 * parts <= steps)
+      parts *= 2;
+    a.parts = parts;
+    a.heads_per_wg = std::min(8 / parts, a.n_kv_heads);
+    const dim3 grid((unsigned)((int64_t)B * ((a.n_kv_heads + a.heads_per_wg - 1) / a.heads_per_wg)));
+    const dim3 block(64 * parts * a.heads_per_wg);
+    if (blk)
+      hipLaunchKernelGGL((kept_decode_whole_kernel<true, 2, 4>), grid, block, 0, s, a);
+    else
+      hipLaunchKernelGGL((kept_decode_whole_kernel<false, 3, 2>), grid, block, 0, s, a);
+    return launch_status("kept_decode_whole_kernel");
+  }
+  const KeptWorkspace w = kept_workspace(B, a.n_kv_heads);
+  if (B > 0 && (!workspace || workspace_bytes < w.total))
+    return GKV_ERR_WORKSPACE;
+  if ((uintptr_t)workspace % 16 != 0)
+    return GKV_ERR_ARG;
+  if (B == 0)
+    return GKV_OK;
+  const int n_wg = blk ? kSplitWgs : kSplitWgs / 2, subs = range_subs(a.n_kv_heads);
+  a.max_ranges = n_wg * subs;
+  a.plan = (int32_t *)workspace;
+  a.ws_ml = (float *)((char *)workspace + w.ml);
+  a.ws_o = (float *)((char *)workspace + w.o);
+  const dim3 block(64 * subs * a.n_kv_heads);
+  if (blk)
+    hipLaunchKernelGGL((kept_decode_split_kernel<true, 2, 4>), dim3(n_wg), block, 0, s, a);
+  else
+    hipLaunchKernelGGL((kept_decode_split_kernel<false, 3, 2>), dim3(n_wg), block, 0, s, a);
+  if ((st = launch_status("kept_decode_split_kernel")))
+    return st;
+  hipLaunchKernelGGL(kept_decode_merge_kernel, dim3((unsigned)(B * a.n_kv_heads)),
+                     dim3(kMergeThreads), 0, s, a);
+  return launch_status("kept_decode_merge_kernel");
+}

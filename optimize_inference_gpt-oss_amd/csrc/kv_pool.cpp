@@ -9,7 +9,12 @@
 //                  layer; per layer K and V [num_blocks][Hkv][1024] bf16 in
 //                  the block layouts of kv_append.hpp (32 KB per block at Hkv=8)
 //   window layers  a ring of W/16 blocks per sequence id, fixed at create time
-//                  (the reference's slots = window, gpu_engine.hpp:318-319)
+//                  (the reference's slots = window, gpu_engine.hpp:318-319); a
+//                  pool that keeps first tokens: kept/16 + W/16 + 1 blocks
+//   sharing        a fork holds its parent's full blocks too: every block counts
+//                  its holders and returns to the free list with the last one;
+//                  the partly filled last block is copied, so that nobody
+//                  appends to a block that another sequence reads
 //   tables         int32 [max_seqs][ceil(max_seq_len/16)] and [max_seqs][W/16],
 //                  mirrored on the host; gkv_pool_sync uploads the entries that
 //                  changed since the last sync, without waiting
@@ -23,11 +28,13 @@
 #include <algorithm>
 #include <cstdint>
 #include <cstring>
+#include <exception>
 #include <new>
 #include <numeric>
 #include <random>
 #include <vector>
 
+#include "block_copy.hpp"
 #include "gkv.h"
 
 namespace {
@@ -41,13 +48,15 @@ struct gkv_pool {
   std::vector<char> layer_is_window;
   int n_full = 0, n_window = 0;
   int table_stride = 0; // full-table entries per sequence
-  int ring_blocks = 0;  // W / 16
+  int ring_blocks = 0;  // window layers' table entries per sequence: W / 16, or kept / 16 + W / 16 + 1
+  int ring = 0;         // slots of the window layers' ring: W, or W + 16
   int64_t num_blocks = 0, num_ring_blocks = 0;
   std::vector<void *> k_full, v_full, k_ring, v_ring;
   std::vector<void *> s_full, s_ring; // fp32 V scales (int8 V only)
   int32_t *d_table = nullptr, *d_ring_table = nullptr;
   std::vector<int32_t> h_table, h_ring_table;
   std::vector<int32_t> free_blocks; // stack; back() is handed out next
+  std::vector<int32_t> refs;        // per block: the sequences that hold it
   std::vector<int32_t> seq_blocks;  // blocks held per sequence
   std::vector<char> seq_live;
   std::vector<int32_t> free_seqs;
@@ -81,6 +90,81 @@ struct gkv_pool {
     stage_cap = 0;
   }
 
+  // The staging buffer for the next n pairs (grown if need be), free to be
+  // filled: its previous copy (two uses ago) has long completed in practice,
+  // the wait only guards the case where it has not.
+  int stage_for(size_t n, int *k) {
+    if (n > stage_cap) {
+      free_stage();
+      const size_t cap = std::max<size_t>(n, 4096);
+      for (int i = 0; i < 2; i++)
+        if (hipHostMalloc((void **)&h_stage[i], cap * sizeof(int2), hipHostMallocDefault) !=
+                hipSuccess ||
+            hipMalloc((void **)&d_stage[i], cap * sizeof(int2)) != hipSuccess ||
+            hipEventCreateWithFlags(&stage_done[i], hipEventDisableTiming) != hipSuccess) {
+          free_stage();
+          return GKV_ERR_HIP;
+        }
+      stage_cap = cap;
+    }
+    *k = stage_i;
+    return hipEventSynchronize(stage_done[stage_i]) == hipSuccess ? GKV_OK : GKV_ERR_HIP;
+  }
+
+  gkv_cache_view layer_view(int layer) const {
+    const int i = layer_index[layer];
+    gkv_cache_view v{};
+    v.n_kv_heads = cfg.n_kv_heads;
+    v.v_format = cfg.v_format;
+    if (layer_is_window[layer]) {
+      v.k = k_ring[i];
+      v.v = v_ring[i];
+      v.v_scale = s_ring[i];
+      v.block_table = d_ring_table;
+      v.table_stride = ring_blocks;
+      v.num_blocks = (int32_t)num_ring_blocks;
+      v.ring = ring;
+    } else {
+      v.k = k_full[i];
+      v.v = v_full[i];
+      v.v_scale = s_full[i];
+      v.block_table = d_table;
+      v.table_stride = table_stride;
+      v.num_blocks = (int32_t)num_blocks;
+    }
+    return v;
+  }
+
+  // Copies blocks {src, dst} in every full (or window) layer, on stream: one
+  // launch per 32 layers. The ids travel as kernel arguments, or, many of
+  // them, through a staging buffer.
+  int copy(const std::vector<int2> &pairs, bool window, hipStream_t s) {
+    std::vector<gkv_cache_view> views;
+    for (int l = 0; l < cfg.n_layers; l++)
+      if ((layer_is_window[l] != 0) == window)
+        views.push_back(layer_view(l));
+    const int n = (int)pairs.size(), n_views = (int)views.size();
+    if (n == 0 || n_views == 0)
+      return GKV_OK;
+    if (n <= gkv::kInlinePairs)
+      return gkv::copy_blocks(s, views.data(), n_views, n, nullptr, nullptr, 0, pairs.data(),
+                              nullptr);
+    int k = 0;
+    int st = stage_for(pairs.size(), &k);
+    if (st != GKV_OK)
+      return st;
+    std::memcpy(h_stage[k], pairs.data(), pairs.size() * sizeof(int2));
+    if (hipMemcpyAsync(d_stage[k], h_stage[k], pairs.size() * sizeof(int2), hipMemcpyHostToDevice,
+                       s) != hipSuccess)
+      return GKV_ERR_HIP;
+    st = gkv::copy_blocks(s, views.data(), n_views, n, (const int32_t *)d_stage[k],
+                          (const int32_t *)d_stage[k] + 1, 2, nullptr, nullptr);
+    if (hipEventRecord(stage_done[k], s) != hipSuccess)
+      st = GKV_ERR_HIP;
+    stage_i ^= 1;
+    return st;
+  }
+
   ~gkv_pool() {
     free_stage();
     for (auto *vec : {&k_full, &v_full, &k_ring, &v_ring, &s_full, &s_ring})
@@ -94,24 +178,7 @@ struct gkv_pool {
   }
 };
 
-// Bytes of one 16-token block of one layer: K bf16 (or e4m3), V bf16 (or int8
-// or e4m3 codes) + fp32 scales (V's, or K's and V's).
-static int64_t k_bytes(int n_kv_heads, int v_format) {
-  return (int64_t)n_kv_heads * kBT * kD * (v_format == GKV_KV_FP8 ? 1 : 2);
-}
-static int64_t v_bytes(int n_kv_heads, int v_format) {
-  return (int64_t)n_kv_heads * kBT * kD * (v_format == GKV_V_BF16 ? 2 : 1);
-}
-static int64_t s_bytes(int n_kv_heads, int v_format) {
-  return (int64_t)n_kv_heads * kBT * 4 *
-         (v_format == GKV_V_INT8 ? 1 : v_format == GKV_KV_FP8 ? 2 : 0);
-}
-static int64_t block_bytes_per_layer(int n_kv_heads, int v_format) {
-  return k_bytes(n_kv_heads, v_format) + v_bytes(n_kv_heads, v_format) +
-         s_bytes(n_kv_heads, v_format);
-}
-
-extern "C" int gkv_pool_create(const gkv_pool_config *cfg, gkv_pool **out) {
+static int pool_create(const gkv_pool_config *cfg, int32_t kept, int32_t slack, gkv_pool **out) {
   if (!cfg || !out)
     return GKV_ERR_ARG;
   *out = nullptr;
@@ -121,7 +188,8 @@ extern "C" int gkv_pool_create(const gkv_pool_config *cfg, gkv_pool **out) {
     return GKV_ERR_ARG;
   if (c.head_dim != kD || c.window % kBT != 0)
     return GKV_ERR_UNSUPPORTED;
-  if (c.v_format != GKV_V_BF16 && c.v_format != GKV_V_INT8 && c.v_format != GKV_KV_FP8)
+  gkv::BlockBytes bb;
+  if (c.n_kv_heads > 65536 || gkv::block_bytes(c.n_kv_heads, c.v_format, &bb) != GKV_OK)
     return GKV_ERR_ARG;
   gkv_pool *p = new (std::nothrow) gkv_pool();
   if (!p)
@@ -135,9 +203,10 @@ extern "C" int gkv_pool_create(const gkv_pool_config *cfg, gkv_pool **out) {
     p->layer_index[l] = win ? p->n_window++ : p->n_full++;
   }
   p->table_stride = (c.max_seq_len + kBT - 1) / kBT;
-  p->ring_blocks = c.window / kBT;
+  p->ring = c.window > 0 ? c.window + slack : 0;
+  p->ring_blocks = c.window > 0 ? (kept + c.window + slack) / kBT : 0;
   p->num_ring_blocks = (int64_t)c.max_seqs * p->ring_blocks;
-  const int64_t bpl = block_bytes_per_layer(c.n_kv_heads, c.v_format);
+  const int64_t bpl = bb.k + bb.v + bb.s;
   const int64_t ring_bytes = p->num_ring_blocks * bpl * p->n_window;
   const int64_t table_bytes =
       ((int64_t)c.max_seqs * p->table_stride + (int64_t)c.max_seqs * p->ring_blocks) * 4;
@@ -178,8 +247,7 @@ extern "C" int gkv_pool_create(const gkv_pool_config *cfg, gkv_pool **out) {
     p->device_bytes += bytes;
     return true;
   };
-  const int64_t kb = k_bytes(c.n_kv_heads, c.v_format), vb = v_bytes(c.n_kv_heads, c.v_format);
-  const int64_t sb = s_bytes(c.n_kv_heads, c.v_format);
+  const int64_t kb = bb.k, vb = bb.v, sb = bb.s;
   bool ok = true;
   p->k_full.assign(p->n_full, nullptr);
   p->v_full.assign(p->n_full, nullptr);
@@ -218,6 +286,7 @@ extern "C" int gkv_pool_create(const gkv_pool_config *cfg, gkv_pool **out) {
     std::shuffle(ring_ids.begin(), ring_ids.end(), rng);
   }
   std::copy(ring_ids.begin(), ring_ids.end(), p->h_ring_table.begin());
+  p->refs.assign(p->num_blocks, 0);
   p->seq_blocks.assign(c.max_seqs, 0);
   p->seq_live.assign(c.max_seqs, 0);
   p->free_seqs.resize(c.max_seqs);
@@ -229,6 +298,29 @@ extern "C" int gkv_pool_create(const gkv_pool_config *cfg, gkv_pool **out) {
   }
   *out = p;
   return GKV_OK;
+}
+
+extern "C" int gkv_pool_create(const gkv_pool_config *cfg, gkv_pool **out) {
+  // the block format's scale needs whole blocks to leave a window at once
+  if (cfg && cfg->v_format == GKV_KV_FP8_BLOCK && cfg->window > 0) {
+    if (out)
+      *out = nullptr;
+    return GKV_ERR_UNSUPPORTED;
+  }
+  return pool_create(cfg, 0, 0, out);
+}
+
+extern "C" int gkv_pool_create_kept(const gkv_pool_config *cfg, int32_t kept, gkv_pool **out) {
+  if (!cfg || !out)
+    return GKV_ERR_ARG;
+  *out = nullptr;
+  if (kept < 0 || kept > INT32_MAX / 4 || cfg->window <= 0 || cfg->window > INT32_MAX / 4)
+    return GKV_ERR_ARG;
+  if (kept % kBT != 0)
+    return GKV_ERR_UNSUPPORTED;
+  if (cfg->v_format != GKV_V_BF16 && cfg->v_format != GKV_KV_FP8_BLOCK)
+    return GKV_ERR_UNSUPPORTED; // what the gkv_kept_* entry points read
+  return pool_create(cfg, kept, kBT, out);
 }
 
 extern "C" int gkv_pool_destroy(gkv_pool *pool) {
@@ -272,6 +364,7 @@ extern "C" int gkv_pool_seq_reserve(gkv_pool *pool, int32_t seq_id, int32_t seq_
   for (int32_t j = have; j < need; j++) {
     row[j] = pool->free_blocks.back();
     pool->free_blocks.pop_back();
+    pool->refs[row[j]] = 1;
     pool->pending.push_back(int2{(int)(base + j), row[j]});
   }
   pool->seq_blocks[seq_id] = need;
@@ -286,7 +379,8 @@ extern "C" int gkv_pool_seq_free(gkv_pool *pool, int32_t seq_id) {
   const size_t base = (size_t)seq_id * pool->table_stride;
   int32_t *row = &pool->h_table[base];
   for (int32_t j = pool->seq_blocks[seq_id] - 1; j >= 0; j--) {
-    pool->free_blocks.push_back(row[j]);
+    if (--pool->refs[row[j]] == 0) // (the capacity for every block is there)
+      pool->free_blocks.push_back(row[j]);
     row[j] = -1;
     pool->pending.push_back(int2{(int)(base + j), -1});
   }
@@ -294,6 +388,163 @@ extern "C" int gkv_pool_seq_free(gkv_pool *pool, int32_t seq_id) {
   pool->seq_live[seq_id] = 0;
   pool->free_seqs.push_back(seq_id);
   return GKV_OK;
+}
+
+// ---- sharing, trimming, compacting ---------------------------------------------
+//
+// The copies go out on the caller's stream at once, the table entries with the
+// next gkv_pool_sync on it. Nothing is taken before the copies are queued, so
+// a failed call leaves the bookkeeping as it was.
+
+extern "C" int gkv_pool_seq_fork(gkv_pool *pool, int32_t parent, int32_t n_tokens, void *stream,
+                                 int32_t *child) try {
+  if (!pool || !child || n_tokens < 0)
+    return GKV_ERR_ARG;
+  if (parent < 0 || parent >= pool->cfg.max_seqs || !pool->seq_live[parent])
+    return GKV_ERR_BLOCK;
+  const int32_t shared = n_tokens / kBT, part = n_tokens % kBT != 0;
+  if (n_tokens > pool->cfg.max_seq_len ||
+      (pool->n_full > 0 && shared + part > pool->seq_blocks[parent]))
+    return GKV_ERR_ARG; // more tokens than the parent holds
+  const bool full = pool->n_full > 0;
+  if (pool->free_seqs.empty() || (full && part && pool->free_blocks.empty()))
+    return GKV_ERR_CAPACITY;
+  const int32_t id = pool->free_seqs.back();
+  const size_t from = (size_t)parent * pool->table_stride, to = (size_t)id * pool->table_stride;
+  if (full)
+    pool->pending.reserve(pool->pending.size() + shared + part);
+  hipStream_t s = (hipStream_t)stream;
+  if (full && part) {
+    const int st = pool->copy({int2{pool->h_table[from + shared], pool->free_blocks.back()}}, false, s);
+    if (st != GKV_OK)
+      return st;
+  }
+  if (pool->n_window > 0) {
+    // the ring's blocks in use (the kept tokens' first), slot by slot
+    std::vector<int2> ring;
+    const size_t rb = pool->ring_blocks;
+    for (size_t j = 0; j < std::min<size_t>(rb, shared + part); j++)
+      ring.push_back(int2{pool->h_ring_table[parent * rb + j], pool->h_ring_table[id * rb + j]});
+    const int st = pool->copy(ring, true, s);
+    if (st != GKV_OK)
+      return st;
+  }
+  if (full) {
+    for (int32_t j = 0; j < shared; j++) {
+      pool->h_table[to + j] = pool->h_table[from + j];
+      pool->refs[pool->h_table[from + j]]++;
+    }
+    if (part) {
+      const int32_t blk = pool->free_blocks.back();
+      pool->free_blocks.pop_back();
+      pool->refs[blk] = 1;
+      pool->h_table[to + shared] = blk;
+    }
+    for (int32_t j = 0; j < shared + part; j++)
+      pool->pending.push_back(int2{(int)(to + j), pool->h_table[to + j]});
+    pool->seq_blocks[id] = shared + part;
+  } else {
+    pool->seq_blocks[id] = 0;
+  }
+  pool->free_seqs.pop_back();
+  pool->seq_live[id] = 1;
+  *child = id;
+  return GKV_OK;
+} catch (const std::exception &) {
+  return GKV_ERR_CAPACITY; // out of host memory
+}
+
+extern "C" int gkv_pool_seq_trim(gkv_pool *pool, int32_t seq_id, int32_t n_tokens,
+                                 void *stream) try {
+  if (!pool || n_tokens < 0)
+    return GKV_ERR_ARG;
+  if (seq_id < 0 || seq_id >= pool->cfg.max_seqs || !pool->seq_live[seq_id])
+    return GKV_ERR_BLOCK;
+  if (pool->n_full == 0)
+    return GKV_OK;
+  const int32_t have = pool->seq_blocks[seq_id], keep = n_tokens / kBT + (n_tokens % kBT != 0);
+  if (keep > have)
+    return GKV_ERR_ARG;
+  const size_t base = (size_t)seq_id * pool->table_stride;
+  int32_t *row = &pool->h_table[base];
+  pool->pending.reserve(pool->pending.size() + (have - keep) + 1);
+  // appends go on inside the last block: it has to be this sequence's own
+  int32_t own = -1;
+  if (n_tokens % kBT != 0 && pool->refs[row[keep - 1]] > 1) {
+    if (!pool->free_blocks.empty())
+      own = pool->free_blocks.back();
+    for (int32_t j = keep; own < 0 && j < have; j++)
+      if (pool->refs[row[j]] == 1)
+        own = row[j]; // one of those that this call frees
+    if (own < 0)
+      return GKV_ERR_CAPACITY;
+    const int st = pool->copy({int2{row[keep - 1], own}}, false, (hipStream_t)stream);
+    if (st != GKV_OK)
+      return st;
+  }
+  for (int32_t j = have - 1; j >= keep; j--) {
+    if (--pool->refs[row[j]] == 0)
+      pool->free_blocks.push_back(row[j]);
+    row[j] = -1;
+    pool->pending.push_back(int2{(int)(base + j), -1});
+  }
+  if (own >= 0) {
+    pool->free_blocks.erase(std::find(pool->free_blocks.begin(), pool->free_blocks.end(), own));
+    pool->refs[row[keep - 1]]--;
+    pool->refs[own] = 1;
+    row[keep - 1] = own;
+    pool->pending.push_back(int2{(int)(base + keep - 1), own});
+  }
+  pool->seq_blocks[seq_id] = keep;
+  return GKV_OK;
+} catch (const std::exception &) {
+  return GKV_ERR_CAPACITY; // out of host memory
+}
+
+extern "C" int gkv_pool_compact(gkv_pool *pool, void *stream, int64_t *n_used) try {
+  if (!pool)
+    return GKV_ERR_ARG;
+  const int64_t nb = pool->num_blocks, live = nb - (int64_t)pool->free_blocks.size();
+  // block `live` and those behind move into the holes before it: the sources
+  // and the targets are disjoint, so the copies need no order
+  std::vector<int2> moves;
+  std::vector<int32_t> now(nb);
+  std::iota(now.begin(), now.end(), 0);
+  int32_t hole = 0;
+  for (int64_t i = live; i < nb; i++) {
+    if (pool->refs[i] == 0)
+      continue;
+    while (pool->refs[hole] != 0)
+      hole++;
+    moves.push_back(int2{(int)i, hole});
+    now[i] = hole++;
+  }
+  size_t entries = 0;
+  for (int32_t q = 0; q < pool->cfg.max_seqs; q++)
+    entries += pool->seq_blocks[q];
+  pool->pending.reserve(pool->pending.size() + (moves.empty() ? 0 : entries));
+  const int st = pool->copy(moves, false, (hipStream_t)stream);
+  if (st != GKV_OK)
+    return st;
+  for (const int2 &m : moves)
+    std::swap(pool->refs[m.x], pool->refs[m.y]);
+  for (int32_t q = 0; q < pool->cfg.max_seqs; q++) {
+    const size_t base = (size_t)q * pool->table_stride;
+    for (int32_t j = 0; j < pool->seq_blocks[q]; j++) {
+      int32_t &id = pool->h_table[base + j];
+      if (now[id] != id) {
+        id = now[id];
+        pool->pending.push_back(int2{(int)(base + j), id});
+      }
+    }
+  }
+  for (int64_t i = 0; i < nb - live; i++) // the lowest free block is handed out next
+    pool->free_blocks[i] = (int32_t)(nb - 1 - i);
+  if (n_used)
+    *n_used = live;
+  return GKV_OK;
+} catch (const std::exception &) {
+  return GKV_ERR_CAPACITY; // out of host memory
 }
 
 // Applies n staged (index, value) pairs to the device table, in order (a
@@ -337,24 +588,10 @@ extern "C" int gkv_pool_sync(gkv_pool *pool, void *stream) {
   for (int2 &e : pend)
     e.y = pool->h_table[e.x];
   const size_t n = pend.size();
-  if (n > pool->stage_cap) {
-    pool->free_stage();
-    const size_t cap = std::max<size_t>(n, 4096);
-    for (int i = 0; i < 2; i++)
-      if (hipHostMalloc((void **)&pool->h_stage[i], cap * sizeof(int2), hipHostMallocDefault) !=
-              hipSuccess ||
-          hipMalloc((void **)&pool->d_stage[i], cap * sizeof(int2)) != hipSuccess ||
-          hipEventCreateWithFlags(&pool->stage_done[i], hipEventDisableTiming) != hipSuccess) {
-        pool->free_stage();
-        return GKV_ERR_HIP;
-      }
-    pool->stage_cap = cap;
-  }
-  const int k = pool->stage_i;
-  // the staging buffer's previous copy (two syncs ago) has long completed
-  // in practice; the wait only guards the case where it has not
-  if (hipEventSynchronize(pool->stage_done[k]) != hipSuccess)
-    return GKV_ERR_HIP;
+  int k = 0;
+  const int st = pool->stage_for(n, &k);
+  if (st != GKV_OK)
+    return st;
   std::memcpy(pool->h_stage[k], pend.data(), n * sizeof(int2));
   if (hipMemcpyAsync(pool->d_stage[k], pool->h_stage[k], n * sizeof(int2), hipMemcpyHostToDevice,
                      s) != hipSuccess)
@@ -373,27 +610,8 @@ extern "C" int gkv_pool_layer_view_from(const gkv_pool *pool, int32_t layer, int
   if (!pool || !view || layer < 0 || layer >= pool->cfg.n_layers || first_seq < 0 ||
       first_seq >= pool->cfg.max_seqs)
     return GKV_ERR_ARG;
-  const int i = pool->layer_index[layer];
-  gkv_cache_view v{};
-  v.n_kv_heads = pool->cfg.n_kv_heads;
-  v.v_format = pool->cfg.v_format;
-  if (pool->layer_is_window[layer]) {
-    v.k = pool->k_ring[i];
-    v.v = pool->v_ring[i];
-    v.v_scale = pool->s_ring[i];
-    v.block_table = pool->d_ring_table + (size_t)first_seq * pool->ring_blocks;
-    v.table_stride = pool->ring_blocks;
-    v.num_blocks = (int32_t)pool->num_ring_blocks;
-    v.ring = pool->cfg.window;
-  } else {
-    v.k = pool->k_full[i];
-    v.v = pool->v_full[i];
-    v.v_scale = pool->s_full[i];
-    v.block_table = pool->d_table + (size_t)first_seq * pool->table_stride;
-    v.table_stride = pool->table_stride;
-    v.num_blocks = (int32_t)pool->num_blocks;
-    v.ring = 0;
-  }
+  gkv_cache_view v = pool->layer_view(layer);
+  v.block_table += (size_t)first_seq * v.table_stride;
   *view = v;
   return GKV_OK;
 }

@@ -41,7 +41,7 @@ class CacheView(ctypes.Structure):
                 ("v_scale", _vp), ("v_format", _i32)]
 
 
-V_BF16, V_INT8, KV_FP8 = 0, 1, 2
+V_BF16, V_INT8, KV_FP8, KV_FP8_BLOCK = 0, 1, 2, 3
 
 
 def block_offsets(kind: str):
@@ -50,7 +50,8 @@ def block_offsets(kind: str):
     - "k": [16 tokens][64 dims] of the bf16 K block (2 KB),
     - "v": [64 dims][16 tokens] of the bf16 V block (2 KB),
     - "v_int8": [64 dims][16 tokens] of the int8 V block (1 KB), also the e4m3 V block,
-    - "k_fp8": [16 tokens][64 dims] of the e4m3 K block (1 KB)."""
+    - "k_fp8": [16 tokens][64 dims] of the e4m3 K block (1 KB).
+    (KV_FP8_BLOCK has the code blocks of KV_FP8.)"""
     if kind == "k_fp8":
         return [[((d % 32) // 8 * 16 + t) * 16 + (d // 32) * 8 + d % 8 for d in range(64)]
                 for t in range(16)]
@@ -129,12 +130,27 @@ SIGNATURES = {
                                              _vp, _vp, _vp, _vp, _i32, _vp, _i64, _i32]),
     "gkv_prefill_paged": (ctypes.c_int, [_vp, _i32, _vp, _vp, _i32, _i32, _vp, _i64, _vp, _vp,
                                          _vp, _vp, CacheView, _vp, _i32, _vp, _i64, _i32, _vp]),
+    "gkv_kept_append": (ctypes.c_int, [_vp, _i32, _vp, _vp, _i32, _vp, _i64, _i32, _vp, _vp,
+                                       CacheView, _i32, _i32, _vp, _vp, _vp]),
+    "gkv_kept_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32]),
+    "gkv_kept_decode": (ctypes.c_int, [_vp, _i32, _i32, _vp, _i64, _vp, _vp, _vp, _i32, CacheView,
+                                       _i32, _i32, _vp, _vp, _sz, _vp, _i64, _i32, _vp]),
+    "gkv_kept_prefill": (ctypes.c_int, [_vp, _i32, _vp, _vp, _i32, _i32, _vp, _i64, _vp, _vp,
+                                        _vp, _vp, CacheView, _i32, _i32, _vp, _vp, _i64, _i32,
+                                        _vp]),
+    "gkv_copy_blocks": (ctypes.c_int, [_vp, ctypes.POINTER(CacheView), _i32, _i32, _vp, _vp,
+                                       _vp]),
     "gkv_rope_exact": (ctypes.c_int, [_vp, _i32, _vp, _i64, _vp, _vp, _vp, _i32]),
     "gkv_kv_write_exact": (ctypes.c_int, [_vp, _i32, _vp, _i64, _i32, _i32, _vp, _vp, _i32, _i32,
                                           _i32, _vp, _i32, _vp]),
     "gkv_attention_exact": (ctypes.c_int, [_vp, _i32, _i32, _i32, _vp, _i64, _vp, _vp, _i32, _vp,
                                            _i32, _vp, _i32, _i32, _vp, _i64, _vp]),
     "gkv_pool_create": (ctypes.c_int, [ctypes.POINTER(PoolConfig), ctypes.POINTER(_vp)]),
+    "gkv_pool_create_kept": (ctypes.c_int, [ctypes.POINTER(PoolConfig), _i32,
+                                            ctypes.POINTER(_vp)]),
+    "gkv_pool_seq_fork": (ctypes.c_int, [_vp, _i32, _i32, _vp, ctypes.POINTER(_i32)]),
+    "gkv_pool_seq_trim": (ctypes.c_int, [_vp, _i32, _i32, _vp]),
+    "gkv_pool_compact": (ctypes.c_int, [_vp, _vp, ctypes.POINTER(_i64)]),
     "gkv_pool_destroy": (ctypes.c_int, [_vp]),
     "gkv_pool_seq_alloc": (ctypes.c_int, [_vp, ctypes.POINTER(_i32)]),
     "gkv_pool_seq_reserve": (ctypes.c_int, [_vp, _i32, _i32]),
@@ -242,7 +258,9 @@ def cache_view(k, v, block_table, n_kv_heads: int, ring: int = 0, v_scale=None,
     """View over torch tensors k [NB, Hkv, 16, 64], v [NB, Hkv, 64, 16] (bf16 or int16),
     block_table int32 [B, stride]. With v_scale (fp32 [NB, Hkv, 16]) the V cache is
     int8 codes [NB, Hkv, 1024] (GKV_V_INT8); v_format=KV_FP8: k and v are e4m3 codes
-    [NB, Hkv, 1024] and v_scale fp32 [NB, Hkv, 32] (K scales, then V scales)."""
+    [NB, Hkv, 1024] and v_scale fp32 [NB, Hkv, 32] (K scales, then V scales);
+    v_format=KV_FP8_BLOCK: the same codes and v_scale fp32 [NB, Hkv, 2] (the block's
+    K scale, its V scale)."""
     if v_format is None:
         v_format = V_INT8 if v_scale is not None else V_BF16
     return CacheView(ptr(k), ptr(v), ptr(block_table), int(block_table.shape[1]),
@@ -426,14 +444,81 @@ def prefill_paged(cu_seqlens, max_len, q, cache: CacheView, sinks, out, start_po
     check("gkv_prefill_paged", st)
 
 
+def kept_append(qkv, n_q_heads, cos_tab, sin_tab, seq_lens, view: CacheView, kept=0, window=0,
+                cu_seqlens=None, max_rows=1, k_pack=None, v_pack=None, dev_err=None, stream=None):
+    """gkv_kept_append: the rows cu_seqlens[b] .. cu_seqlens[b+1]-1 (None: row b) as the last
+    positions of sequence b, seq_lens[b] tokens long with them, into whole blocks of bf16, or
+    of e4m3 codes with one scale per block and head."""
+    st = lib().gkv_kept_append(stream_handle(stream), seq_lens.shape[0], ptr(cu_seqlens),
+                               ptr(seq_lens), max_rows, ptr(qkv), qkv.stride(0), n_q_heads,
+                               ptr(cos_tab), ptr(sin_tab), view, kept, window, ptr(k_pack),
+                               ptr(v_pack), ptr(dev_err))
+    check("gkv_kept_append", st)
+
+
+def kept_workspace_bytes(B, n_kv_heads, max_seq_len, kept=0, window=0) -> int:
+    return lib().gkv_kept_workspace_bytes(B, n_kv_heads, max_seq_len, kept, window)
+
+
+def kept_decode(q, n_q_heads, seq_lens, max_seq_len, view: CacheView, out, sinks=None, kept=0,
+                window=0, cos_tab=None, sin_tab=None, workspace=None, dev_err=None, stream=None):
+    """gkv_kept_decode: one query per sequence, which sees the first `kept` positions and
+    the last `window` (window 0: all)."""
+    import torch
+    out_dtype = BF16 if out.dtype == torch.bfloat16 else F32
+    ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
+    st = lib().gkv_kept_decode(stream_handle(stream), q.shape[0], n_q_heads, ptr(q), q.stride(0),
+                               ptr(cos_tab), ptr(sin_tab), ptr(seq_lens), max_seq_len, view, kept,
+                               window, ptr(sinks), ptr(workspace), ws_bytes, ptr(out),
+                               out.stride(0), out_dtype, ptr(dev_err))
+    check("gkv_kept_decode", st)
+
+
+def kept_prefill(cu_seqlens, max_len, q, n_q_heads, view: CacheView, out, start_pos=None, k=None,
+                 v=None, sinks=None, kept=0, window=0, cos_tab=None, sin_tab=None, dev_err=None,
+                 stream=None):
+    """gkv_kept_prefill: prompts (a view without a cache: CacheView(n_kv_heads=...)), or chunks
+    continuing the sequences in `view`, with the mask of kept_decode."""
+    import torch
+    out_dtype = BF16 if out.dtype == torch.bfloat16 else F32
+    st = lib().gkv_kept_prefill(stream_handle(stream), cu_seqlens.shape[0] - 1, ptr(cu_seqlens),
+                                ptr(start_pos), max_len, n_q_heads, ptr(q), q.stride(0),
+                                ptr(cos_tab), ptr(sin_tab), ptr(k), ptr(v), view, kept, window,
+                                ptr(sinks), ptr(out), out.stride(0), out_dtype, ptr(dev_err))
+    check("gkv_kept_prefill", st)
+
+
+def cache_views(views):
+    """The array of cache views that copy_blocks takes (made once, kept by the caller)."""
+    return (CacheView * len(views))(*views)
+
+
+def copy_blocks(views, src, dst, dev_err=None, stream=None):
+    """gkv_copy_blocks: block src[i] to dst[i] (int32 device tensors) in every view (a
+    cache_views array, or a list of CacheView)."""
+    if not isinstance(views, ctypes.Array):
+        views = cache_views(views)
+    if src.shape != dst.shape:
+        raise ValueError("src and dst differ in length")
+    st = lib().gkv_copy_blocks(stream_handle(stream), views, len(views), src.numel(), ptr(src),
+                               ptr(dst), ptr(dev_err))
+    check("gkv_copy_blocks", st)
+
+
 class Pool:
     """Paged KV pool (gkv_pool_*)."""
 
     def __init__(self, n_layers, n_kv_heads, max_seqs, max_seq_len, window=128, num_blocks=0,
-                 bytes_budget=0, shuffle_seed=0, head_dim=64, v_format=0):
+                 bytes_budget=0, shuffle_seed=0, head_dim=64, v_format=0, kept=None):
         self.cfg = PoolConfig(n_layers, n_kv_heads, head_dim, window, max_seqs, max_seq_len,
                               num_blocks, bytes_budget, shuffle_seed, v_format)
         h = _vp()
+        self.h = None
+        if kept is not None:  # the window layers keep the first tokens (gkv_pool_create_kept)
+            check("gkv_pool_create_kept", lib().gkv_pool_create_kept(ctypes.byref(self.cfg), kept,
+                                                                     ctypes.byref(h)))
+            self.h = h
+            return
         check("gkv_pool_create", lib().gkv_pool_create(ctypes.byref(self.cfg), ctypes.byref(h)))
         self.h = h
 
@@ -458,6 +543,22 @@ class Pool:
 
     def free(self, seq: int) -> int:
         return lib().gkv_pool_seq_free(self.h, seq)
+
+    def fork(self, parent: int, n_tokens: int, stream=None) -> int:
+        s = _i32()
+        check("gkv_pool_seq_fork", lib().gkv_pool_seq_fork(self.h, parent, n_tokens,
+                                                           stream_handle(stream), ctypes.byref(s)))
+        return s.value
+
+    def trim(self, seq: int, n_tokens: int, stream=None):
+        check("gkv_pool_seq_trim", lib().gkv_pool_seq_trim(self.h, seq, n_tokens,
+                                                           stream_handle(stream)))
+
+    def compact(self, stream=None) -> int:
+        n = _i64()
+        check("gkv_pool_compact", lib().gkv_pool_compact(self.h, stream_handle(stream),
+                                                         ctypes.byref(n)))
+        return n.value
 
     def sync(self, stream=None):
         check("gkv_pool_sync", lib().gkv_pool_sync(self.h, stream_handle(stream)))
