@@ -29,7 +29,7 @@
 //           resident wave; every workgroup finds its own range from the lengths
 //           in its prologue. A sequence inside one range is finished there,
 //           the pieces of the others go to the workspace and a second launch
-//           merges them, a workgroup per (sequence, kv head).
+//           merges them, a workgroup per range.
 #include "kept.hpp"
 
 #include <algorithm>
@@ -48,7 +48,7 @@ constexpr int kPieceFloats = kHeads * kHeadDim;
 constexpr int kPieceMl = 2 * kHeads;   // (m, l) of a piece's heads
 constexpr float kLowest = -1e30f;      // the running maximum before any score (log2 units)
 constexpr int kMergeThreads = 512;
-constexpr int kMergeChunk = 256;       // pieces whose weights are held in LDS at a time
+constexpr int kMaxRanges = 8 * kSplitWgs; // one kv head: 8 ranges a workgroup
 
 struct KeptDecodeArgs {
   const float *q;
@@ -65,7 +65,8 @@ struct KeptDecodeArgs {
   int B, G, n_kv_heads;
   int parts, heads_per_wg; // whole: waves per (sequence, head), heads per workgroup
   int max_ranges;          // ranges: waves launched per kv head
-  int32_t *plan;           // ranges: {T, n}, then the B + 1 prefix sums of the steps
+  int4 *cuts;              // ranges: {sequence, its first step, its end, T} of the sequence that range
+                           // r starts inside of (sequence -1: at a sequence's start, or no range)
   float *ws_ml, *ws_o;     // [range][2][n_kv_heads]: a range's first and last piece
   void *out;
   int64_t out_stride;
@@ -133,8 +134,10 @@ struct State {
 template <bool BLK>
 struct StepData {
   u32x4 k[BLK ? 2 : 4], v[BLK ? 2 : 4];
-  f32x2 sc[2]; // per block: K scale, V scale (wave-uniform)
+  f32x2 sc[2];   // per block: K scale, V scale (wave-uniform)
+  uint32_t miss; // bit j: block j is not there (padding, or an id outside the pool)
 };
+constexpr int kNoBlock = INT32_MIN; // the id of a step's missing second block
 
 typedef const __attribute__((address_space(4))) int32_t *ScalarI32;
 typedef const __attribute__((address_space(4))) f32x2 *ScalarF2;
@@ -160,32 +163,56 @@ __device__ __forceinline__ State attend(const KeptDecodeArgs &a, int b, int g, c
   const uint32_t k_off = lane * 16;
   const uint32_t v_off = BLK ? (col * 4 + kg) * 16 : lane * 16;
 
-  // The block ids of a step (-1: none, or outside the pool), read through the
-  // scalar cache a step before they are used.
-  const int64_t trow = (int64_t)b * a.table_stride;
+  // The query's rows and angles: dims 8kg .. +7 and 32+8kg .. +7 of the column's
+  // head. Their loads go out first, as their address depends on nothing else.
+  f32x4 qr[4], an[4];
+  {
+    const f32x4 *qp =
+        (const f32x4 *)(a.q + (int64_t)b * a.q_stride + (g * a.G + (head_ok ? head : 0)) * D + 8 * kg);
+    qr[0] = qp[0];
+    qr[1] = qp[1];
+    qr[2] = qp[8];
+    qr[3] = qp[9];
+    if (a.cos_tab) {
+      const f32x4 *cp = (const f32x4 *)(a.cos_tab + (int64_t)(sp.L - 1) * (D / 2) + 8 * kg);
+      const f32x4 *np = (const f32x4 *)(a.sin_tab + (int64_t)(sp.L - 1) * (D / 2) + 8 * kg);
+      an[0] = cp[0];
+      an[1] = cp[1];
+      an[2] = np[0];
+      an[3] = np[1];
+    }
+  }
+
+  // The block ids of a step, read through the scalar cache a step before they are
+  // used.
+  const ScalarI32 trow = (ScalarI32)a.table + (int64_t)b * a.table_stride;
   bool bad = false;
   auto ids_of = [&](int s) -> int2 {
-    int2 r{-1, -1};
+    int2 r{kNoBlock, kNoBlock};
     if (s < s1) {
-      r.x = ((ScalarI32)a.table)[trow + span_entry(a, sp, 2 * s)];
+      r.x = trow[span_entry(a, sp, 2 * s)];
       if (2 * s + 1 < sp.n_blocks)
-        r.y = ((ScalarI32)a.table)[trow + span_entry(a, sp, 2 * s + 1)];
+        r.y = trow[span_entry(a, sp, 2 * s + 1)];
     }
     return r;
   };
-  auto load = [&](StepData<BLK> &x, int2 ids, int s) {
+  const char *k_head = a.kc + g * kHeadBytes, *v_head = a.vc + g * kHeadBytes;
+  const char *s_head = (const char *)a.scales + g * 8;
+  const uint32_t stride = (uint32_t)a.n_kv_heads * kHeadBytes; // bytes of a block
+  auto load = [&](StepData<BLK> &x, int2 ids) {
+    x.miss = 0;
 #pragma unroll
     for (int j = 0; j < 2; j++) {
-      int id = uniform(j ? ids.y : ids.x);
-      const bool ok = id >= 0 && id < a.num_blocks;
-      bad |= !ok && s < s1 && 2 * s + j < sp.n_blocks;
-      id = ok ? id : 0;
-      const int64_t hb = (int64_t)id * a.n_kv_heads + g;
+      const int id = uniform(j ? ids.y : ids.x);
+      const bool ok = (uint32_t)id < (uint32_t)a.num_blocks;
+      bad |= !ok && id != kNoBlock;
+      x.miss |= ok ? 0u : 1u << j;
+      const uint64_t off = (uint64_t)(ok ? (uint32_t)id : 0u) * stride;
       // a missing block reads nothing: its resource covers 0 bytes
-      const __amdgpu_buffer_rsrc_t kr = head_rsrc(a.kc + hb * kHeadBytes, ok ? kHeadBytes : 0);
-      const __amdgpu_buffer_rsrc_t vr = head_rsrc(a.vc + hb * kHeadBytes, ok ? kHeadBytes : 0);
+      const __amdgpu_buffer_rsrc_t kr = head_rsrc(k_head + off, ok ? kHeadBytes : 0);
+      const __amdgpu_buffer_rsrc_t vr = head_rsrc(v_head + off, ok ? kHeadBytes : 0);
       if (BLK) {
-        x.sc[j] = ((ScalarF2)a.scales)[hb];
+        x.sc[j] = *(ScalarF2)(s_head + off / 128);
         x.k[j] = __builtin_amdgcn_raw_buffer_load_b128(kr, k_off, 0, kKeptAux);
         x.v[j] = __builtin_amdgcn_raw_buffer_load_b128(vr, v_off, 0, kKeptAux);
       } else {
@@ -195,49 +222,29 @@ __device__ __forceinline__ State attend(const KeptDecodeArgs &a, int b, int g, c
           x.v[2 * j + h] = __builtin_amdgcn_raw_buffer_load_b128(vr, v_off + h * 1024, 0, kKeptAux);
         }
       }
-      if (!ok)
-        x.sc[j] = f32x2{-1.0f, 0.0f}; // (the mark of a missing block)
-      else if (!BLK)
-        x.sc[j] = f32x2{0.0f, 0.0f};
     }
   };
 
+  const int last_step = (sp.n_blocks - 1) / 2, win_step = a.window > 0 ? sp.first_blocks / 2 : -1;
   StepData<BLK> buf[R];
   int2 ids = ids_of(s0);
 #pragma unroll
   for (int i = 0; i < R - 1; i++) {
     const int2 next = ids_of(s0 + i + 1);
-    load(buf[i], ids, s0 + i);
+    load(buf[i], ids);
     ids = next;
   }
 
-  // The query: dims 8kg .. +7 and 32+8kg .. +7 of the column's head, rotated at
-  // the sequence's last position, scaled, in two pieces.
+  // The query, rotated at the sequence's last position, scaled, in two pieces.
   float qa[8], qb[8];
-  {
-    const f32x4 *qp =
-        (const f32x4 *)(a.q + (int64_t)b * a.q_stride + (g * a.G + (head_ok ? head : 0)) * D + 8 * kg);
-    const f32x4 x0 = qp[0], x1 = qp[1], x2 = qp[8], x3 = qp[9];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      qa[i] = x0[i];
-      qa[4 + i] = x1[i];
-      qb[i] = x2[i];
-      qb[4 + i] = x3[i];
-    }
+  for (int i = 0; i < 8; i++) {
+    const float y1 = qr[i / 4][i % 4], y2 = qr[2 + i / 4][i % 4];
+    qa[i] = y1;
+    qb[i] = y2;
     if (a.cos_tab) {
-      const f32x4 *cp = (const f32x4 *)(a.cos_tab + (int64_t)(sp.L - 1) * (D / 2) + 8 * kg);
-      const f32x4 *np = (const f32x4 *)(a.sin_tab + (int64_t)(sp.L - 1) * (D / 2) + 8 * kg);
-#pragma unroll
-      for (int i4 = 0; i4 < 2; i4++) {
-        const f32x4 c = cp[i4], n = np[i4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const float y1 = qa[4 * i4 + i], y2 = qb[4 * i4 + i];
-          qa[4 * i4 + i] = rope_first(y1, y2, c[i], n[i]);
-          qb[4 * i4 + i] = rope_second(y1, y2, c[i], n[i]);
-        }
-      }
+      qa[i] = rope_first(y1, y2, an[i / 4][i % 4], an[2 + i / 4][i % 4]);
+      qb[i] = rope_second(y1, y2, an[i / 4][i % 4], an[2 + i / 4][i % 4]);
     }
   }
   float qf = 0.125f * kLog2e; // 1 / sqrt(64); exp -> exp2
@@ -299,61 +306,67 @@ __device__ __forceinline__ State attend(const KeptDecodeArgs &a, int b, int g, c
   for (int nn = 0; nn < 4; nn++)
     st.o[nn] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
+  // One step. After the scores' matrix ops a column's two halves hold what q's
+  // pieces make of the same tokens; each lane takes the sum of both for four
+  // tokens only: block 0's in the columns below 8, block 1's above. Maximum,
+  // exponential and sum run on those, and the halves swap p's pieces for the
+  // second matrix op: half the vector instructions of keeping both blocks in
+  // both.
   auto compute = [&](StepData<BLK> &x, int s) {
-    float t[8];
+    f32x4 acc[2];
 #pragma unroll
     for (int j = 0; j < 2; j++) {
-      f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+      acc[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       if (BLK) {
         const u32x2 c0 = codes_to_f16(x.k[j][0]), c1 = codes_to_f16(x.k[j][1]);
         const u32x2 c2 = codes_to_f16(x.k[j][2]), c3 = codes_to_f16(x.k[j][3]);
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
             __builtin_bit_cast(f16x8, u32x4{c0[0], c0[1], c1[0], c1[1]}),
-            __builtin_bit_cast(f16x8, q0), acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+            __builtin_bit_cast(f16x8, q0), acc[j], 0, 0, 0);
+        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
             __builtin_bit_cast(f16x8, u32x4{c2[0], c2[1], c3[0], c3[1]}),
-            __builtin_bit_cast(f16x8, q1), acc, 0, 0, 0);
+            __builtin_bit_cast(f16x8, q1), acc[j], 0, 0, 0);
       } else {
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x.k[2 * j]),
-                                                      __builtin_bit_cast(bf16x8, q0), acc, 0, 0, 0);
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x.k[2 * j + 1]),
-                                                      __builtin_bit_cast(bf16x8, q1), acc, 0, 0, 0);
-      }
-      const float c = BLK ? qf * x.sc[j][0] : 1.0f;
-#pragma unroll
-      for (int r = 0; r < 4; r++) {
-        t[4 * j + r] = acc[r] + swap8(acc[r]);
-        if (BLK)
-          t[4 * j + r] *= c;
+        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x.k[2 * j]),
+                                                         __builtin_bit_cast(bf16x8, q0), acc[j], 0, 0, 0);
+        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x.k[2 * j + 1]),
+                                                         __builtin_bit_cast(bf16x8, q1), acc[j], 0, 0, 0);
       }
     }
+    float t[4];
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+      t[r] = (low ? acc[1][r] : acc[0][r]) + swap8(low ? acc[0][r] : acc[1][r]);
+    // the scale of this lane's block (never 0: a masked score of -inf stays one)
+    const float c = BLK ? fmaxf(qf * (low ? x.sc[1][0] : x.sc[0][0]), 1e-37f) : 1.0f;
     // The tokens of the block that are seen: all but in a sequence's last block
     // and in a window's first. The others get weight 0, and their values (never
     // written, or no longer seen) become 0.
+    if (s == last_step || s == win_step || x.miss != 0) {
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
-      const int i = 2 * s + j;
-      const int blk = i < sp.first_blocks ? i : sp.win0 + i - sp.first_blocks;
-      int hi = min(sp.L - blk * kBlockTokens, kBlockTokens);
-      int lo = 0;
-      if (a.window > 0 && i >= sp.first_blocks)
-        lo = max(sp.L - a.window - blk * kBlockTokens, 0);
-      if (i >= sp.n_blocks || x.sc[j][0] < 0.0f)
-        hi = 0;
-      if (lo > 0 || hi < kBlockTokens) {
+      for (int j = 0; j < 2; j++) {
+        const int i = 2 * s + j;
+        const int blk = i < sp.first_blocks ? i : sp.win0 + i - sp.first_blocks;
+        int hi = min(sp.L - blk * kBlockTokens, kBlockTokens);
+        int lo = 0;
+        if (a.window > 0 && i >= sp.first_blocks)
+          lo = max(sp.L - a.window - blk * kBlockTokens, 0);
+        if ((x.miss >> j) & 1)
+          hi = 0;
         uint32_t keep = 0;
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-          const int tk = 4 * kg + r;
-          const bool in = tk >= lo && tk < hi;
+          const bool in = 4 * kg + r >= lo && 4 * kg + r < hi;
           keep |= in ? 0xffu << (8 * r) : 0u;
-          if (!in)
-            t[4 * j + r] = -INFINITY;
+          if (!in && low == (j == 1))
+            t[r] = -INFINITY;
         }
         if (BLK) {
 #pragma unroll
           for (int nn = 0; nn < 4; nn++)
             x.v[j][nn] &= keep;
+          if (hi == 0)
+            x.sc[j][1] = 0.0f; // (a missing block's scale is another block's)
         } else {
           const uint32_t m0 = (keep & 0xffu ? 0xffffu : 0u) | (keep & 0xff00u ? 0xffff0000u : 0u);
           const uint32_t m1 =
@@ -366,16 +379,14 @@ __device__ __forceinline__ State attend(const KeptDecodeArgs &a, int b, int g, c
         }
       }
     }
-    float mx = t[0];
-#pragma unroll
-    for (int i = 1; i < 8; i++)
-      mx = fmaxf(mx, t[i]);
+    float mx = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * c;
     // The running maximum moves only when a score passes it by more than 8
     // (weights stay below 2^8); the test needs no cross-lane maximum, only the
-    // move does (m is the same in the 4 lanes of a column).
+    // move does (m is the same in the 8 lanes of a query head).
     if (__any(mx > st.m + 8.0f)) {
       mx = fmaxf(mx, __shfl_xor(mx, 16));
       mx = fmaxf(mx, __shfl_xor(mx, 32));
+      mx = fmaxf(mx, swap8(mx));
       const float m = fmaxf(st.m, mx);
       const float f = __builtin_amdgcn_exp2f(st.m - m);
       st.m = m;
@@ -384,20 +395,29 @@ __device__ __forceinline__ State attend(const KeptDecodeArgs &a, int b, int g, c
       for (int nn = 0; nn < 4; nn++)
         st.o[nn] *= f;
     }
-    float p[8];
+    float p[4];
+    const float vs = low ? x.sc[1][1] : x.sc[0][1];
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      p[i] = __builtin_amdgcn_exp2f(t[i] - st.m);
-      st.l += p[i];
+    for (int r = 0; r < 4; r++) {
+      p[r] = __builtin_amdgcn_exp2f(fmaf(t[r], c, -st.m));
+      st.l += p[r];
       if (BLK)
-        p[i] *= x.sc[i >> 2][1];
+        p[r] *= vs;
     }
-    bf16x8 pw;
+    // p in bf16 and what that leaves, for the 4 tokens; the columns below 8 need
+    // the first of both blocks, those above the second
+    uint32_t hi[2], lo[2], w0[2], w1[2];
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const __bf16 h = (__bf16)p[i];
-      pw[i] = low ? (__bf16)(p[i] - (float)h) : h;
+    for (int k = 0; k < 2; k++) {
+      const float x0 = p[2 * k], x1 = p[2 * k + 1];
+      hi[k] = f32x2_to_bf16_rne(x0, x1);
+      lo[k] = f32x2_to_bf16_rne(x0 - __uint_as_float(hi[k] << 16),
+                                x1 - __uint_as_float(hi[k] & 0xffff0000u));
+      const uint32_t got = __float_as_uint(swap8(__uint_as_float(low ? hi[k] : lo[k])));
+      w0[k] = low ? got : hi[k];
+      w1[k] = low ? lo[k] : got;
     }
+    const bf16x8 pw = __builtin_bit_cast(bf16x8, u32x4{w0[0], w0[1], w1[0], w1[1]});
 #pragma unroll
     for (int nn = 0; nn < 4; nn++) {
       u32x4 w;
@@ -421,17 +441,18 @@ __device__ __forceinline__ State attend(const KeptDecodeArgs &a, int b, int g, c
       if (s + r >= s1)
         break;
       const int2 next = ids_of(s + r + R);
-      load(buf[(r + R - 1) % R], ids, s + r + R - 1);
+      load(buf[(r + R - 1) % R], ids);
       ids = next;
       compute(buf[r], s + r);
     }
   }
   if (bad && lane == 0 && a.dev_err)
     atomicOr(a.dev_err, GKV_DEVERR_BLOCK_ID);
-  // the four lanes of a column hold its weights, the two columns of a head the
-  // pieces of its output
+  // the eight lanes of a query head hold its weights, its two columns the pieces
+  // of its output
   st.l += __shfl_xor(st.l, 16);
   st.l += __shfl_xor(st.l, 32);
+  st.l += swap8(st.l);
 #pragma unroll
   for (int nn = 0; nn < 4; nn++)
 #pragma unroll
@@ -544,9 +565,15 @@ void kept_decode_whole_kernel(KeptDecodeArgs a) {
 
 // ---- ranges ----------------------------------------------------------------------
 
-// Range r of the T steps cut into n.
+// Range r of the T steps cut into n (n <= 4096): floor(r T / n), in 32 bits.
 __device__ __forceinline__ int range_begin(int r, int T, int n) {
-  return (int)((int64_t)r * T / n);
+  const uint32_t q = (uint32_t)T / (uint32_t)n, m = (uint32_t)T % (uint32_t)n;
+  return (int)(r * q + r * m / (uint32_t)n);
+}
+
+// The range that holds step p.
+__device__ __forceinline__ int range_of(int p, int T, int n) {
+  return (int)(((int64_t)(p + 1) * n - 1) / T);
 }
 
 template <bool BLK, int R, int WPE>
@@ -587,24 +614,23 @@ void kept_decode_split_kernel(KeptDecodeArgs a) {
   const int r0 = blockIdx.x * subs;
   int c = before + incl - mine;
   // each of the workgroup's ranges: the sequence that holds its first step
+  int at[8];
+#pragma unroll
+  for (int k = 0; k < 8; k++)
+    at[k] = k < subs && r0 + k < n ? range_begin(r0 + k, T, n) : -1;
   for (int b = b0; b < b1; b++) {
     const int m = span_steps(span_of(a, span_len(a, b)));
-    for (int k = 0; k < subs; k++) {
-      const int at = r0 + k < n ? range_begin(r0 + k, T, n) : -1;
-      if (c <= at && at < c + m) {
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+      if (c <= at[k] && at[k] < c + m) {
         s_b[k] = b;
         s_c[k] = c;
+        a.cuts[r0 + k] = int4{c < at[k] ? b : -1, c, c + m, T};
       }
-    }
-    if (blockIdx.x == 0)
-      a.plan[2 + b] = c;
     c += m;
   }
-  if (blockIdx.x == 0 && t == 0) {
-    a.plan[0] = T;
-    a.plan[1] = n;
-    a.plan[2 + a.B] = T;
-  }
+  if (t < subs && (r0 + t >= n || T == 0))
+    a.cuts[r0 + t] = int4{-1, 0, 0, 0};
   if (blockIdx.x == 0 && over && a.dev_err)
     atomicOr(a.dev_err, GKV_DEVERR_LENGTH);
   // sequences without tokens: zeros
@@ -645,90 +671,200 @@ void kept_decode_split_kernel(KeptDecodeArgs a) {
   }
 }
 
-// The pieces of one (sequence, kv head) that was cut: M = max m_i, out =
-// sum o_i 2^(m_i - M) / (sum l_i 2^(m_i - M) + 2^(sink - M)). The weights of up to
-// kMergeChunk pieces stand in LDS; then each group of 128 threads (4 dims of a
-// query head a thread) sums every fourth piece. Bound by latency: the plan, the
-// (m, l), the pieces.
+// The pieces of a sequence that was cut: M = max m_i, out = sum o_i 2^(m_i - M) /
+// (sum l_i 2^(m_i - M) + 2^(sink - M)). One workgroup per range, whose record
+// (left by the split) names the sequence that the range starts inside of. A
+// sequence of at most kMergeFew pieces is merged by the first such range's, a
+// wave per kv head, every piece's loads at once. The kv heads of a longer one are
+// dealt over all of them, a wave taking every eighth piece, four at a time, the waves
+// joined in LDS. In one of more pieces than there are query heads each of those
+// has a workgroup: 16 threads a piece (4 dims each), 32 pieces at a time, the first
+// four of each thread loaded before the weights are known. Bound by latency: the
+// record, then the pieces.
+constexpr int kMergeFew = 4;
 __global__ __launch_bounds__(kMergeThreads) void kept_decode_merge_kernel(KeptDecodeArgs a) {
-  constexpr int kGroups = kMergeThreads / 128, kWaves = kMergeThreads / 64;
-  __shared__ float s_w[kMergeChunk][kHeads];
-  __shared__ float s_red[kWaves][kHeads], s_m[kHeads], s_l[kHeads];
-  __shared__ f32x4 s_o[kGroups][128];
-  const int b = blockIdx.x / a.n_kv_heads, g = blockIdx.x % a.n_kv_heads;
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int T = a.plan[0], n = a.plan[1], c0 = a.plan[2 + b], c1 = a.plan[3 + b];
-  if (c0 == c1)
+  constexpr int D = kHeadDim, kWaves = kMergeThreads / 64, kGroups = kMergeThreads / 16;
+  __shared__ float s_w[kMaxRanges];
+  __shared__ float s_red[kWaves];
+  __shared__ f32x4 s_o[kWaves][64][2];
+  __shared__ float2 s_ml[kWaves][kHeads];
+  const int4 cut = a.cuts[blockIdx.x];
+  if (cut.x < 0)
     return;
-  const int w0 = (int)(((int64_t)(c0 + 1) * n - 1) / T), w1 = (int)(((int64_t)c1 * n - 1) / T);
-  if (w0 == w1)
-    return; // finished by its range
-  const int first_slot = range_begin(w0, T, n) < c0 ? 1 : 0;
-  auto piece = [&](int i) {
+  const int T = cut.w, n = min(a.max_ranges, max(T / kMinRangeSteps, 1)), b = cut.x;
+  const int w0 = range_of(cut.y, T, n), np = range_of(cut.z - 1, T, n) - w0 + 1;
+  const int inside = (int)blockIdx.x - w0 - 1;
+  if (np <= kMergeFew && inside > 0)
+    return;
+  // the first piece is its range's last one, unless the sequence starts there
+  const int first_slot = range_begin(w0, T, n) < cut.y ? 1 : 0;
+  auto piece = [&](int i, int g) {
     return ((int64_t)(w0 + i) * 2 + (i == 0 ? first_slot : 0)) * a.n_kv_heads + g;
   };
-  const int np = w1 - w0 + 1, h = t & 7;
-  float m = kLowest;
-  for (int i = t >> 3; i < np; i += kMergeThreads / 8)
-    m = fmaxf(m, a.ws_ml[piece(i) * kPieceMl + 2 * h]);
+  const int t = threadIdx.x, lane = t & 63, wave = uniform(t >> 6);
+  if (np <= kMergeFew) {
+    const int g = wave, h = lane >> 3, d0 = 8 * (lane & 7);
+    if (g >= a.n_kv_heads || h >= a.G)
+      return;
+    float2 ml[kMergeFew];
+    f32x4 x[kMergeFew][2];
 #pragma unroll
-  for (int off = 8; off < 64; off <<= 1)
-    m = fmaxf(m, __shfl_xor(m, off));
-  if (lane < 8)
-    s_red[wave][lane] = m;
-  __syncthreads();
-  if (t < 8) {
-    for (int w = 0; w < kWaves; w++)
-      m = fmaxf(m, s_red[w][t]);
-    s_m[t] = m;
-  }
-  __syncthreads();
-  m = s_m[h];
-  float l = 0.0f;
-  f32x4 o{0.0f, 0.0f, 0.0f, 0.0f};
-  const int grp = t / 128, e = t % 128, eh = e / 16;
-  for (int i0 = 0; i0 < np; i0 += kMergeChunk) {
-    const int cnt = min(np - i0, kMergeChunk);
-    for (int i = t >> 3; i < cnt; i += kMergeThreads / 8) {
-      const float2 ml = *(const float2 *)(a.ws_ml + piece(i0 + i) * kPieceMl + 2 * h);
-      const float w = __builtin_amdgcn_exp2f(ml.x - m);
-      s_w[i][h] = w;
-      l = fmaf(ml.y, w, l);
+    for (int i = 0; i < kMergeFew; i++) {
+      const int64_t p = piece(min(i, np - 1), g);
+      ml[i] = *(const float2 *)(a.ws_ml + p * kPieceMl + 2 * h);
+      const f32x4 *o = (const f32x4 *)(a.ws_o + p * kPieceFloats + h * D + d0);
+      x[i][0] = o[0];
+      x[i][1] = o[1];
     }
-    __syncthreads();
-    for (int i = grp; i < cnt; i += 4 * kGroups) {
-      f32x4 x[4];
+    float m = kLowest, l = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 4; j++)
-        x[j] = *(const f32x4 *)(a.ws_o + piece(i0 + min(i + j * kGroups, cnt - 1)) * kPieceFloats + 4 * e);
+    for (int i = 0; i < kMergeFew; i++)
+      m = fmaxf(m, ml[i].x);
+    f32x4 o0{0.0f, 0.0f, 0.0f, 0.0f}, o1{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int j = 0; j < 4; j++)
-        if (i + j * kGroups < cnt)
-          o += x[j] * s_w[i + j * kGroups][eh];
-    }
-    __syncthreads();
-  }
-#pragma unroll
-  for (int off = 8; off < 64; off <<= 1)
-    l += __shfl_xor(l, off);
-  if (lane < 8)
-    s_red[wave][lane] = l;
-  s_o[grp][e] = o;
-  __syncthreads();
-  if (t < 8) {
-    l = 0.0f;
-    for (int w = 0; w < kWaves; w++)
-      l += s_red[w][t];
-    s_l[t] = l;
-  }
-  __syncthreads();
-  if (t >= 128 || eh >= a.G)
+    for (int i = 0; i < kMergeFew; i++)
+      if (i < np) {
+        const float f = __builtin_amdgcn_exp2f(ml[i].x - m);
+        l = fmaf(ml[i].y, f, l);
+        o0 += x[i][0] * f;
+        o1 += x[i][1] * f;
+      }
+    const float f = out_factor(m, l, sink_of(a, g, h));
+    const int64_t ob = (int64_t)b * a.out_stride + (int64_t)(g * a.G + h) * D + d0;
+    put(a.out, ob, o0 * f, a.out_bf16);
+    put(a.out, ob + 4, o1 * f, a.out_bf16);
     return;
+  }
+  if (np - 1 < a.n_kv_heads * a.G) {
+    const int h = lane >> 3, d0 = 8 * (lane & 7), hc = min(h, a.G - 1);
+    for (int g = inside; g < a.n_kv_heads; g += np - 1) {
+      float m = kLowest, l = 0.0f;
+      f32x4 o0{0.0f, 0.0f, 0.0f, 0.0f}, o1{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int i0 = wave; i0 < np; i0 += 4 * kWaves) {
+        float2 ml[4];
+        f32x4 x[4][2];
 #pragma unroll
-  for (int k = 1; k < kGroups; k++)
-    o += s_o[k][e];
-  put(a.out, (int64_t)b * a.out_stride + (int64_t)g * a.G * kHeadDim + 4 * e,
-      o * out_factor(s_m[eh], s_l[eh], sink_of(a, g, eh)), a.out_bf16);
+        for (int j = 0; j < 4; j++) {
+          const int64_t p = piece(min(i0 + j * kWaves, np - 1), g);
+          ml[j] = *(const float2 *)(a.ws_ml + p * kPieceMl + 2 * hc);
+          const f32x4 *o = (const f32x4 *)(a.ws_o + p * kPieceFloats + hc * D + d0);
+          x[j][0] = o[0];
+          x[j][1] = o[1];
+        }
+        float mn = m;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          mn = fmaxf(mn, ml[j].x); // (a repeated last piece moves no maximum)
+        const float f0 = __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= f0;
+        o0 *= f0;
+        o1 *= f0;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          if (i0 + j * kWaves < np) {
+            const float f = __builtin_amdgcn_exp2f(ml[j].x - m);
+            l = fmaf(ml[j].y, f, l);
+            o0 += x[j][0] * f;
+            o1 += x[j][1] * f;
+          }
+      }
+      __syncthreads(); // (the arrays may still be read for another head)
+      s_o[wave][lane][0] = o0;
+      s_o[wave][lane][1] = o1;
+      if ((lane & 7) == 0)
+        s_ml[wave][h] = float2{m, l};
+      __syncthreads();
+      // thread t < 128: 4 dims of query head t / 16
+      const int th = t / 16;
+      if (t < 128 && th < a.G) {
+        float mt = kLowest, lt = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; w++)
+          mt = fmaxf(mt, s_ml[w][th].x);
+        f32x4 ot{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) {
+          const float f = __builtin_amdgcn_exp2f(s_ml[w][th].x - mt);
+          lt = fmaf(s_ml[w][th].y, f, lt);
+          ot += s_o[w][t / 2][t & 1] * f;
+        }
+        put(a.out, (int64_t)b * a.out_stride + (int64_t)g * a.G * D + 4 * t,
+            ot * out_factor(mt, lt, sink_of(a, g, th)), a.out_bf16);
+      }
+    }
+    return;
+  }
+  const int grp = t >> 4, e = t & 15;
+  for (int item = inside; item < a.n_kv_heads * a.G; item += np - 1) {
+    const int g = item / a.G, h = item % a.G;
+    auto load = [&](int i) {
+      return *(const f32x4 *)(a.ws_o + piece(min(i, np - 1), g) * kPieceFloats + h * D + 4 * e);
+    };
+    f32x4 x[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      x[j] = load(grp + j * kGroups);
+    // the common maximum, the pieces' weights, the sum
+    float m = kLowest;
+    for (int i = t; i < np; i += kMergeThreads)
+      m = fmaxf(m, a.ws_ml[piece(i, g) * kPieceMl + 2 * h]);
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1)
+      m = fmaxf(m, __shfl_xor(m, off));
+    __syncthreads(); // (the arrays may still be read for another head)
+    if (lane == 0)
+      s_red[wave] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWaves; w++)
+      m = fmaxf(m, s_red[w]);
+    float l = 0.0f;
+    for (int i = t; i < np; i += kMergeThreads) {
+      const float2 ml = *(const float2 *)(a.ws_ml + piece(i, g) * kPieceMl + 2 * h);
+      const float f = __builtin_amdgcn_exp2f(ml.x - m);
+      s_w[i] = f;
+      l = fmaf(ml.y, f, l);
+    }
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1)
+      l += __shfl_xor(l, off);
+    __syncthreads();
+    if (lane == 0)
+      s_red[wave] = l;
+    f32x4 o{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = grp; i < np; i += 4 * kGroups) {
+      f32x4 y[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        y[j] = i + 4 * kGroups < np ? load(i + (4 + j) * kGroups) : x[j];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        if (i + j * kGroups < np)
+          o += x[j] * s_w[i + j * kGroups];
+        x[j] = y[j];
+      }
+    }
+#pragma unroll
+    for (int off = 16; off <= 32; off <<= 1)
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+        o[r] += __shfl_xor(o[r], off);
+    if (lane < 16)
+      s_o[wave][lane][0] = o;
+    __syncthreads();
+    if (t < 16) {
+      o = s_o[0][t][0];
+      l = s_red[0];
+#pragma unroll
+      for (int w = 1; w < kWaves; w++) {
+        o += s_o[w][t][0];
+        l += s_red[w];
+      }
+      put(a.out, (int64_t)b * a.out_stride + (int64_t)(g * a.G + h) * D + 4 * t,
+          o * out_factor(m, l, sink_of(a, g, h)), a.out_bf16);
+    }
+  }
 }
 
 // ---- host side --------------------------------------------------------------------
@@ -751,13 +887,13 @@ static bool use_whole(int32_t B, int32_t n_kv_heads, int32_t max_seq_len, int32_
 static int range_subs(int n_kv_heads) { return 8 / n_kv_heads; }
 
 struct KeptWorkspace {
-  size_t ml, o, total;
+  size_t ml, o, total; // (the ranges' records come first)
 };
-static KeptWorkspace kept_workspace(int32_t B, int32_t n_kv_heads) {
+static KeptWorkspace kept_workspace(int32_t n_kv_heads) {
   auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
   const size_t pieces = (size_t)kSplitWgs * range_subs(n_kv_heads) * 2 * n_kv_heads;
   KeptWorkspace w;
-  w.ml = up(((size_t)B + 3) * 4);
+  w.ml = up((size_t)kSplitWgs * range_subs(n_kv_heads) * sizeof(int4));
   w.o = w.ml + up(pieces * kPieceMl * 4);
   w.total = w.o + pieces * kPieceFloats * 4;
   return w;
@@ -771,7 +907,7 @@ extern "C" size_t gkv_kept_workspace_bytes(int32_t B, int32_t n_kv_heads, int32_
   if (B <= 0 || n_kv_heads <= 0 || n_kv_heads > 8 || max_seq_len < 0 || kept < 0 || window < 0 ||
       use_whole(B, n_kv_heads, max_seq_len, kept, window))
     return 0;
-  return kept_workspace(B, n_kv_heads).total;
+  return kept_workspace(n_kv_heads).total;
 }
 
 extern "C" int gkv_kept_decode(void *stream, int32_t B, int32_t n_q_heads, const float *q,
@@ -845,10 +981,10 @@ extern "C" int gkv_kept_decode(void *stream, int32_t B, int32_t n_q_heads, const
     if (blk)
       hipLaunchKernelGGL((kept_decode_whole_kernel<true, 2, 4>), grid, block, 0, s, a);
     else
-      hipLaunchKernelGGL((kept_decode_whole_kernel<false, 3, 2>), grid, block, 0, s, a);
+      hipLaunchKernelGGL((kept_decode_whole_kernel<false, 2, 4>), grid, block, 0, s, a);
     return launch_status("kept_decode_whole_kernel");
   }
-  const KeptWorkspace w = kept_workspace(B, a.n_kv_heads);
+  const KeptWorkspace w = kept_workspace(a.n_kv_heads);
   if (B > 0 && (!workspace || workspace_bytes < w.total))
     return GKV_ERR_WORKSPACE;
   if ((uintptr_t)workspace % 16 != 0)
@@ -857,17 +993,17 @@ extern "C" int gkv_kept_decode(void *stream, int32_t B, int32_t n_q_heads, const
     return GKV_OK;
   const int n_wg = blk ? kSplitWgs : kSplitWgs / 2, subs = range_subs(a.n_kv_heads);
   a.max_ranges = n_wg * subs;
-  a.plan = (int32_t *)workspace;
+  a.cuts = (int4 *)workspace;
   a.ws_ml = (float *)((char *)workspace + w.ml);
   a.ws_o = (float *)((char *)workspace + w.o);
   const dim3 block(64 * subs * a.n_kv_heads);
   if (blk)
     hipLaunchKernelGGL((kept_decode_split_kernel<true, 2, 4>), dim3(n_wg), block, 0, s, a);
   else
-    hipLaunchKernelGGL((kept_decode_split_kernel<false, 3, 2>), dim3(n_wg), block, 0, s, a);
+    hipLaunchKernelGGL((kept_decode_split_kernel<false, 2, 4>), dim3(n_wg), block, 0, s, a);
   if ((st = launch_status("kept_decode_split_kernel")))
     return st;
-  hipLaunchKernelGGL(kept_decode_merge_kernel, dim3((unsigned)(B * a.n_kv_heads)),
-                     dim3(kMergeThreads), 0, s, a);
+  hipLaunchKernelGGL(kept_decode_merge_kernel, dim3((unsigned)a.max_ranges), dim3(kMergeThreads), 0, s,
+                     a);
   return launch_status("kept_decode_merge_kernel");
 }
