@@ -32,6 +32,7 @@ SOURCES = [
     "block_copy.hip",
     "kept_append.hip",
     "kept_decode.hip",
+    "kept_prefill.hip",
     "rope_table.cpp",
     "kv_pool.cpp",
     "capi.cpp",

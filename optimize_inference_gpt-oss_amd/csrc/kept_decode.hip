@@ -36,9 +36,6 @@
 
 namespace gkv {
 
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-
 constexpr int kKeptAux = 2;            // nontemporal: each K/V byte is read once
 constexpr int kKeptStep = 32;          // tokens per step
 constexpr int kHeads = 8;              // query heads per kv head, at most
@@ -141,13 +138,6 @@ constexpr int kNoBlock = INT32_MIN; // the id of a step's missing second block
 
 typedef const __attribute__((address_space(4))) int32_t *ScalarI32;
 typedef const __attribute__((address_space(4))) f32x2 *ScalarF2;
-
-// Four e4m3 codes -> four fp16 (exact).
-__device__ __forceinline__ u32x2 codes_to_f16(uint32_t w) {
-  const f16x2 a = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
-  const f16x2 b = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true));
-  return u32x2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
-}
 
 // Steps s0 .. s1 - 1 of sequence b for kv head g, by one wave. R: steps of data in
 // registers.

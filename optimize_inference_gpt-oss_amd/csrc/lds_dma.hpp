@@ -36,11 +36,8 @@ __device__ __forceinline__ void lds_barrier() {
 // for all of them before unrelated LDS reads, leaves their waits to the
 // pipeline's explicit wait_vmcnt; the compiler's own waits for its loads can
 // then only be stricter than needed, never weaker.
-__device__ __forceinline__ uint32_t lds_addr(const void *p) {
-  return (uint32_t)(uintptr_t)(lds_ptr)p;
-}
-__device__ __forceinline__ void dma16(const void *src, uint32_t lds) {
-  const uint32_t m = __builtin_amdgcn_readfirstlane(lds);
+__device__ __forceinline__ void dma16(const void *src, void *l_base) {
+  const uint32_t m = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_ptr)l_base);
   uint32_t saved;
   asm volatile("s_mov_b32 %0, m0\n\t"
                "s_mov_b32 m0, %2\n\t"
@@ -52,16 +49,14 @@ __device__ __forceinline__ void dma16(const void *src, uint32_t lds) {
                : "memory");
 }
 
-__device__ __forceinline__ void dma16(const void *src, void *l_base) { dma16(src, lds_addr(l_base)); }
-
 // dma16 with a wave-uniform base address (held in SGPRs) and a 32-bit byte
 // offset per lane: no 64-bit address per lane is formed or kept. The base's
 // halves may come from v_readfirstlane right before the asm, and a memory
 // instruction may read an SGPR five wait states after a vector instruction
 // wrote it at the earliest. The compiler waits in front of its own
 // instructions only, so the asm brings all five (the moves count one each).
-__device__ __forceinline__ void dma16_s(const void *base, uint32_t byte_off, uint32_t lds) {
-  const uint32_t m = __builtin_amdgcn_readfirstlane(lds);
+__device__ __forceinline__ void dma16_s(const void *base, uint32_t byte_off, void *l_base) {
+  const uint32_t m = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_ptr)l_base);
   const uint64_t b = (uint64_t)(uintptr_t)base;
   // (readfirstlane returns a signed int: each half is taken as unsigned
   // before it is widened, or a low half >= 2^31 would fill the high one)
@@ -88,6 +83,9 @@ __device__ __forceinline__ void dma16_s(const void *base, uint32_t byte_off, uin
 // from v_readfirstlane, and the asm brings all five. (9507 projection rows, in turn
 // with loads of two wait states that leave M0 changed: 2% slower with the five and
 // M0 saved in every form, 243.0 / 248.0 us; level so, 252.6 / 252.4 on another GPU.)
+__device__ __forceinline__ uint32_t lds_addr(const void *p) {
+  return (uint32_t)(uintptr_t)(lds_ptr)p;
+}
 template <bool kSalu>
 __device__ __forceinline__ void dma16_at(const void *base, uint32_t byte_off, uint32_t lds) {
   const uint64_t b = (uint64_t)(uintptr_t)base;
@@ -113,25 +111,6 @@ __device__ __forceinline__ void dma4(const void *src, void *l_base) {
                "s_mov_b32 m0, %0"
                : "=&s"(saved)
                : "v"(src), "s"(m)
-               : "memory");
-}
-
-// dma4 with a wave-uniform base and a 32-bit byte offset per lane, with dma16_s's
-// wait states.
-__device__ __forceinline__ void dma4_s(const void *base, uint32_t byte_off, uint32_t lds) {
-  const uint32_t m = __builtin_amdgcn_readfirstlane(lds);
-  const uint64_t b = (uint64_t)(uintptr_t)base;
-  const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(b >> 32));
-  const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)b);
-  const uint64_t sb = ((uint64_t)hi << 32) | lo;
-  uint32_t saved;
-  asm volatile("s_mov_b32 %0, m0\n\t"
-               "s_mov_b32 m0, %3\n\t"
-               "s_nop 2\n\t"
-               "global_load_lds_dword %1, %2\n\t"
-               "s_mov_b32 m0, %0"
-               : "=&s"(saved)
-               : "v"(byte_off), "s"(sb), "s"(m)
                : "memory");
 }
 

@@ -59,7 +59,7 @@
 // (events, two runs): 8 chunks of 100 .. 700 tokens after 1536 cached ones 231 -> 216
 // us with int8 V, 254 -> 249 with the e4m3 cache, level (216) with bf16; 64 prompts of
 // 64 .. 512 tokens 192 - 194 -> 187 - 190 us (full layer), 160 - 162 -> 158 - 160 (window).
-#include "kept.hpp"
+#include "gkv_device.hpp"
 #include "lds_dma.hpp"
 
 #include <algorithm>
@@ -73,7 +73,6 @@ constexpr int kKTile = 64;          // keys per LDS tile
 constexpr int kVRow = kKTile + 8;   // fp16 per V^T row in LDS
 constexpr float kVScale = 0x1p-10f; // V is staged as fp16 of v * kVScale
 constexpr float kQScale = 0.125f * kLog2e; // 1/sqrt(64); exp -> exp2 (on the scores)
-constexpr int kUnseen = -2;         // KEPT: a cached block that no query of the workgroup sees
 constexpr int kStages = 3;          // K/V tile pipeline depth (tiles held in LDS)
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -98,8 +97,6 @@ struct PrefillArgs {
   int64_t out_stride;
   int out_bf16;
   uint32_t *dev_err;
-  int kept;    // KEPT: first positions that stay visible
-  KeptRow row; // KEPT: where the cached blocks stand
 };
 
 // HIST: prompts may continue a cached history (start positions, keys from
@@ -108,17 +105,10 @@ struct PrefillArgs {
 // bf16 K and V; 1 int8 V codes with a scale per token and head; 2 e4m3 K and
 // V codes, each with a scale per token and head. A cached group's stage of a
 // quantized K or V holds the block's 1 KB of codes, then its scales (int8 V:
-// 16 floats; e4m3: the block's 32, K scales then V scales). 3 (with KEPT): e4m3
-// codes with one K and one V scale per block and kv head, which a 4-byte load
-// per lane repeats behind the codes.
-// KEPT: positions before a.kept stay visible behind the window: their tiles come
-// first, then the window's. V of positions that no query of the block sees is
-// staged as 0.
-template <int NW, bool HIST, int VF = 0, bool KEPT = false>
+// 16 floats; e4m3: the block's 32, K scales then V scales).
+template <int NW, bool HIST, int VF = 0>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW >= 8 ? 4 : 1))) void prefill_kernel(PrefillArgs a) {
   static_assert(HIST || VF == 0, "codes come from the cache");
-  static_assert(KEPT || VF != 3, "block scales: the kept form");
-  constexpr bool F8 = VF >= 2; // K and V as e4m3 codes
   constexpr int D = kHeadDim;
   constexpr int NT = NW * 64;
   constexpr int kPieces = kKTile * D / 8 / NT; // V^T conversion: key pairs x 4 dims per thread
@@ -172,21 +162,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW >= 8
   const int W = a.window;
   int k_lo = W > 0 ? max(0, p0 - W + 1) : 0;
   k_lo &= ~(kKTile - 1);
-  // KEPT: tiles before the window's (those of the kept positions), and how far
-  // the window's tiles stand behind them
-  const int n_first = KEPT && W > 0 ? min((a.kept + kKTile - 1) / kKTile, k_lo / kKTile) : 0;
-  const int n_tiles = (p_last + 1 - k_lo + kKTile - 1) / kKTile + n_first;
-  const int skip = k_lo - n_first * kKTile;
-  auto tile_pos = [&](int t) { // tile t's first position
-    return t * kKTile + (KEPT && t < n_first ? 0 : skip);
-  };
-  // KEPT: the first logical block that a query of this block sees in its window,
-  // and its place in the ring (the cached ones behind it, at most the ring's, wrap
-  // once)
-  const int win_blk = KEPT && W > 0 ? max(p0 - W + 1, 0) / kBlockTokens : 0;
-  const int win_ring = KEPT && a.row.ring_blocks > 0
-                           ? kept_entry(a.row, max(win_blk, a.row.kept_blocks))
-                           : 0;
+  const int n_tiles = (p_last + 1 - k_lo + kKTile - 1) / kKTile;
   // keys before this position come from the cache
   const int hist_end = !HIST ? 0 : a.k ? start : INT_MAX;
 
@@ -224,19 +200,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW >= 8
     for (int j = 0; j < 4; j++) {
       r.v[j] = -1;
       if (HIST) {
-        const int p = min(tile_pos(t) + kBlockTokens * j, p_last);
-        int grp = (!KEPT && W > 0 && a.ring > 0 ? p % a.ring : p) / kBlockTokens;
-        if (KEPT && grp >= a.row.kept_blocks) {
-          if (grp < win_blk) {
-            r.v[j] = kUnseen; // not read: its table entry may be gone
-            continue;
-          }
-          if (a.row.ring_blocks > 0) {
-            grp += win_ring - max(win_blk, a.row.kept_blocks);
-            if (grp >= a.row.kept_blocks + a.row.ring_blocks)
-              grp -= a.row.ring_blocks;
-          }
-        }
+        const int p = min(k_lo + t * kKTile + kBlockTokens * j, p_last);
+        const int grp = (W > 0 && a.ring > 0 ? p % a.ring : p) / kBlockTokens;
         if (p < hist_end && grp < a.table_stride)
           r.v[j] = ((ConstI32)a.table)[(int64_t)b * a.table_stride + grp];
       }
@@ -247,7 +212,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW >= 8
     // a select chain, not an indexed access (which would put the ids in memory)
     int id = grp == 0 ? ids.v[0] : grp == 1 ? ids.v[1] : grp == 2 ? ids.v[2] : ids.v[3];
     if (id < 0 || id >= a.num_blocks) {
-      if (lane == 0 && a.dev_err && (!KEPT || id != kUnseen))
+      if (lane == 0 && a.dev_err)
         atomicOr(a.dev_err, GKV_DEVERR_BLOCK_ID);
       id = 0;
     }
@@ -257,20 +222,14 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW >= 8
   // wave 16 / NW of them. Every slot issues its loads (packed rows past the
   // prompt clamped, tiles past the last re-read), so the number of loads that
   // follow a tile's is fixed and the wait below is exact.
-  auto dma = [&](int t, int st, const Ids &ids) __attribute__((always_inline)) {
-    const int kt0 = tile_pos(t);
+  auto dma = [&](int t, int st, const Ids &ids) {
+    const int kt0 = k_lo + t * kKTile;
 #pragma unroll
     for (int i = 0; i < 16 / NW; i++) {
       const int ins = wave + i * NW;
       const int is_v = ins >> 3, grp = (ins >> 1) & 3, half = ins & 1;
       const int p = kt0 + kBlockTokens * grp; // first position of the group
-      const uint32_t dst = (is_v ? st == 0   ? lds_addr(v_st0)
-                                   : st == 1 ? lds_addr(v_st1)
-                                             : lds_addr(v_st2)
-                            : st == 0 ? lds_addr(k_st0)
-                            : st == 1 ? lds_addr(k_st1)
-                                      : lds_addr(k_st2)) +
-                           grp * 2048 + half * 1024;
+      uint16_t *dst = (is_v ? v_stage(st) : k_stage(st)) + grp * 1024 + half * 512;
       // a wave-uniform base and this lane's element offset from it. The lane
       // index is made opaque here so that the per-lane offsets are formed at
       // each load rather than hoisted out of the tile loop and kept live
@@ -280,12 +239,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW >= 8
         asm volatile("" : "+v"(lane_));
       const uint16_t *src;
       uint32_t off;
-      if (VF == 3 && half && p < hist_end) {
-        // the block's K and V scale, repeated by the lanes
-        dma4_s(a.vs + cached_block(ids, grp) / (kBlockTokens * D / 2), (lane_ & 1) * 4, dst);
-        continue;
-      }
-      if (VF != 0 && (is_v || F8) && p < hist_end) {
+      if (VF != 0 && (is_v || VF == 2) && p < hist_end) {
         // a cached block of codes: half 0 its 1 KB of codes, half 1 its
         // scales (int8 V: 16 floats, lanes 0-3; e4m3: 32 floats, lanes 0-7;
         // the other lanes repeat them)
@@ -336,17 +290,10 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW >= 8
   };
   auto v_half = [&](uint32_t bits16) -> uint32_t { return f32_half(bf16_to_f32((uint16_t)bits16)); };
   bool v_range = false; // a V beyond the fp16 range of the staged v * 2^-10
-  // positions whose V some query of the block sees
-  const int seen_lo = KEPT && W > 0 ? max(p0 - W + 1, 0) : 0;
-  const int seen_first = KEPT && W > 0 ? min(a.kept, p_last + 1) : 0;
-  auto seen = [&](int p) {
-    return !KEPT ? p <= p_last
-                 : (uint32_t)(p - seen_lo) <= (uint32_t)(p_last - seen_lo) || p < seen_first;
-  };
   auto convert_v = [&](int st, int buf, int t) {
     const uint16_t *vs = v_stage(st);
     uint16_t *vt_w = v_lds + buf * (D * kVRow);
-    const int kt0 = tile_pos(t);
+    const int kt0 = k_lo + t * kKTile;
 #pragma unroll
     for (int i = 0; i < kPieces; i++) {
       const int idx = tid + i * NT;
@@ -361,16 +308,16 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW >= 8
         // value is value(code) * scale in fp32, as the cache stands for it.
         // Slots past the block's last query position become 0.
         const uint16_t *blk = vs + (r0 >> 4) * 1024;
-        const float *scl = (const float *)(blk + 512) + (VF == 2 ? kBlockTokens : VF == 3 ? 1 : 0);
+        const float *scl = (const float *)(blk + 512) + (VF == 2 ? kBlockTokens : 0);
         const int t0 = r0 & 15;
         // (the power of two goes into the scales, and with int8 codes the mask too:
         // the products are the same bits. An unwritten e4m3 slot may hold the NaN
         // code, so there the products are masked; masking scale and code both
         // spilled the masks and took 92.5 us instead of 91.0 for 32 rows after
         // 1536 cached ones.)
-        const bool keep0 = seen(kt0 + r0), keep1 = seen(kt0 + r1);
-        const float s0 = F8 || keep0 ? scl[VF == 3 ? 0 : t0] * kVScale : 0.0f;
-        const float s1 = VF == 3 ? s0 : VF == 2 || keep1 ? scl[t0 + 1] * kVScale : 0.0f;
+        const bool keep0 = kt0 + r0 <= p_last, keep1 = kt0 + r1 <= p_last;
+        const float s0 = VF == 2 || keep0 ? scl[t0] * kVScale : 0.0f;
+        const float s1 = VF == 2 || keep1 ? scl[t0 + 1] * kVScale : 0.0f;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
           const int d = 4 * pd + j;
@@ -378,7 +325,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW >= 8
                                                   ((d & 15) * 4 + (t0 >> 2)) * 16 +
                                                   (d >> 4) * 4 + (t0 & 3));
           float v0, v1;
-          if (F8) {
+          if (VF == 2) {
             const f32x2 f = __builtin_amdgcn_cvt_pk_f32_fp8((int)c2, false); // bytes 0, 1
             v0 = keep0 ? f[0] * s0 : 0.0f;
             v1 = keep1 ? f[1] * s1 : 0.0f;
@@ -397,8 +344,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW >= 8
           // becomes 0 (their weight is 0, and 0 * NaN would not be)
           const uint16_t *blk = vs + (r0 >> 4) * 1024;
           const int t0 = r0 & 15;
-          const uint32_t keep = (seen(kt0 + r0) ? 0x0000ffffu : 0u) |
-                                (seen(kt0 + r1) ? 0xffff0000u : 0u);
+          const uint32_t keep = (kt0 + r0 <= p_last ? 0x0000ffffu : 0u) |
+                                (kt0 + r1 <= p_last ? 0xffff0000u : 0u);
 #pragma unroll
           for (int j = 0; j < 4; j++) {
             const int d = 4 * pd + j;
@@ -413,8 +360,6 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW >= 8
           for (int j = 0; j < 4; j++) {
             const uint32_t wa = x[j >> 1] >> (16 * (j & 1)), wb = y[j >> 1] >> (16 * (j & 1));
             pair[j] = (wa & 0xffffu) | (wb << 16);
-            if (KEPT)
-              pair[j] &= (seen(kt0 + r0) ? 0x0000ffffu : 0u) | (seen(kt0 + r1) ? 0xffff0000u : 0u);
           }
         }
 #pragma unroll
@@ -474,8 +419,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW >= 8
     for (int t = 0; t < kStages - 1; t++)
       dma(t, t, t == 0 ? ids0 : ids1);
   }
-  // (KEPT: sinks may be absent)
-  const float sink2 = KEPT && !a.sinks ? -INFINITY : a.sinks[h] * kLog2e;
+  const float sink2 = a.sinks[h] * kLog2e;
   float m_run[2] = {sink2, sink2}, lsum[2] = {0.0f, 0.0f};
   f32x4 o[2][4];
 #pragma unroll
@@ -492,21 +436,20 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW >= 8
   // wave's loads visible and frees the V^T buffer of tile t - 1, which takes
   // the V^T of tile t + 1. A tile's loads thus have two tiles' compute to
   // land in.
-  auto tile = [&](const int t, const int st) __attribute__((always_inline)) {
+  auto tile = [&](const int t, const int st) {
     lds_barrier();
     dma(t + kStages - 1, (st + kStages - 1) % kStages, ids_next);
     const uint16_t *ks = k_stage(st);
     const uint16_t *vt = v_lds + (t & 1) * (D * kVRow);
-    const int kt0 = tile_pos(t);
+    const int kt0 = k_lo + t * kKTile;
 #pragma unroll
     for (int s = 0; s < kKTile / 32; s++) {
       const int kb = kt0 + 32 * s; // first key of the step
       // uniform skips: every key after the last query, or (window) older
       // than the first query's window
-      // (KEPT: and not among the kept positions)
-      if (!active || kb > p_last || (W > 0 && kb + 31 <= p0 - W && (!KEPT || kb >= a.kept)))
+      if (!active || kb > p_last || (W > 0 && kb + 31 <= p0 - W))
         continue;
-      const bool need_mask = kb + 31 > p0 || (W > 0 && kb <= p_last - W && (!KEPT || kb + 31 >= a.kept));
+      const bool need_mask = kb + 31 > p0 || (W > 0 && kb <= p_last - W);
       f32x4 acc[2][2]; // [key tile][query column tile]
 #pragma unroll
       for (int kt = 0; kt < 2; kt++) {
@@ -518,7 +461,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW >= 8
         // e4m3 codes of a cached group: lane (kg, n) holds key n's dims
         // 8kg .. +7 (bytes 0-7) and 32 + 8kg .. +7 (bytes 8-15) at lane * 16;
         // turned into bf16 exactly, the K scale applied to the scores
-        const bool f8 = F8 && kb + 16 * kt < hist_end; // wave-uniform
+        const bool f8 = VF == 2 && kb + 16 * kt < hist_end; // wave-uniform
 #pragma unroll
         for (int dh = 0; dh < 2; dh++) {
           const int ki = HIST ? (2 * s + kt) * 1024 + dh * 512 + lane * 8
@@ -539,9 +482,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW >= 8
           }
         }
         if (f8) { // keys 4kg .. 4kg+3 of the group: their K scales
-          const float *kscl = (const float *)(ks + (2 * s + kt) * 1024 + 512);
-          const f32x4 ksc = VF == 3 ? f32x4{kscl[0], kscl[0], kscl[0], kscl[0]}
-                                    : *(const f32x4 *)(kscl + 4 * kg);
+          const f32x4 ksc = *(const f32x4 *)((const float *)(ks + (2 * s + kt) * 1024 + 512) + 4 * kg);
 #pragma unroll
           for (int c = 0; c < 2; c++)
             acc[kt][c] *= ksc;
@@ -565,8 +506,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW >= 8
           for (int kt = 0; kt < 2; kt++)
 #pragma unroll
             for (int r = 0; r < 4; r++)
-              if ((uint32_t)(back0 - 16 * kt - r) >= wlim &&
-                  (!KEPT || kb + 4 * kg + 16 * kt + r >= a.kept || back0 - 16 * kt - r < 0))
+              if ((uint32_t)(back0 - 16 * kt - r) >= wlim)
                 sc[4 * kt + r] = -INFINITY;
         }
 #pragma unroll
@@ -718,17 +658,17 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW >= 8
 
 } // namespace gkv
 
-template <bool HIST, int VF, bool KEPT = false>
+template <bool HIST, int VF>
 static void launch_prefill(const gkv::PrefillArgs &a, int G, dim3 g, hipStream_t s) {
   using namespace gkv;
   if (G > 4)
-    hipLaunchKernelGGL((prefill_kernel<8, HIST, VF, KEPT>), g, dim3(512), 0, s, a);
+    hipLaunchKernelGGL((prefill_kernel<8, HIST, VF>), g, dim3(512), 0, s, a);
   else if (G > 2)
-    hipLaunchKernelGGL((prefill_kernel<4, HIST, VF, KEPT>), g, dim3(256), 0, s, a);
+    hipLaunchKernelGGL((prefill_kernel<4, HIST, VF>), g, dim3(256), 0, s, a);
   else if (G > 1)
-    hipLaunchKernelGGL((prefill_kernel<2, HIST, VF, KEPT>), g, dim3(128), 0, s, a);
+    hipLaunchKernelGGL((prefill_kernel<2, HIST, VF>), g, dim3(128), 0, s, a);
   else
-    hipLaunchKernelGGL((prefill_kernel<1, HIST, VF, KEPT>), g, dim3(64), 0, s, a);
+    hipLaunchKernelGGL((prefill_kernel<1, HIST, VF>), g, dim3(64), 0, s, a);
 }
 
 // Query blocks per band of the grid order (2, or GKV_PREFILL_BAND, read
@@ -747,12 +687,12 @@ static int prefill_launch(void *stream, int32_t B, const int32_t *cu_seqlens,
                           const float *cos_tab, const float *sin_tab, const void *k,
                           const void *v, const gkv_cache_view *cache, const float *sinks,
                           int32_t window, void *out, int64_t out_stride, int32_t out_dtype,
-                          uint32_t *dev_err, bool keeps = false, int32_t kept = 0) {
+                          uint32_t *dev_err) {
   using namespace gkv;
   if (B < 0 || max_len < 0 || n_q_heads <= 0 || n_kv_heads <= 0 || window < 0 ||
       (out_dtype != GKV_F32 && out_dtype != GKV_BF16))
     return GKV_ERR_ARG;
-  if (B > 0 && (!cu_seqlens || !q || (!sinks && !keeps) || !out))
+  if (B > 0 && (!cu_seqlens || !q || !sinks || !out))
     return GKV_ERR_ARG;
   if (n_q_heads % n_kv_heads != 0 || (cos_tab == nullptr) != (sin_tab == nullptr) ||
       (k == nullptr) != (v == nullptr))
@@ -762,13 +702,7 @@ static int prefill_launch(void *stream, int32_t B, const int32_t *cu_seqlens,
     return GKV_ERR_ARG; // keys from nowhere
   if (start_pos && !cached)
     return GKV_ERR_ARG; // a history needs the cache
-  if (cached && keeps) {
-    const int st = kept_check(*cache, kept, window, true);
-    if (st != GKV_OK)
-      return st;
-    if (cache->n_kv_heads != n_kv_heads || (cache->ring > 0 && !k))
-      return GKV_ERR_ARG; // (a ring holds the history only)
-  } else if (cached) {
+  if (cached) {
     if (!cache->v || !cache->block_table || cache->table_stride <= 0 || cache->num_blocks <= 0 ||
         cache->n_kv_heads != n_kv_heads || cache->ring < 0)
       return GKV_ERR_ARG;
@@ -827,17 +761,9 @@ static int prefill_launch(void *stream, int32_t B, const int32_t *cu_seqlens,
   a.out_stride = out_stride;
   a.out_bf16 = out_dtype == GKV_BF16;
   a.dev_err = dev_err;
-  a.kept = kept;
-  a.row = KeptRow{kept / kBlockTokens, a.ring / kBlockTokens};
   hipStream_t s = (hipStream_t)stream;
   const dim3 g((unsigned)grid);
-  if (keeps && cached && cache->v_format == GKV_KV_FP8_BLOCK)
-    launch_prefill<true, 3, true>(a, G, g, s);
-  else if (keeps && cached)
-    launch_prefill<true, 0, true>(a, G, g, s);
-  else if (keeps)
-    launch_prefill<false, 0, true>(a, G, g, s);
-  else if (cached && cache->v_format == GKV_KV_FP8)
+  if (cached && cache->v_format == GKV_KV_FP8)
     launch_prefill<true, 2>(a, G, g, s);
   else if (cached && cache->v_format == GKV_V_INT8)
     launch_prefill<true, 1>(a, G, g, s);
@@ -871,19 +797,4 @@ extern "C" int gkv_prefill_paged(void *stream, int32_t B, const int32_t *cu_seql
   return prefill_launch(stream, B, cu_seqlens, start_pos, max_len, n_q_heads, cache.n_kv_heads,
                         q, q_stride, cos_tab, sin_tab, k, v, &cache, sinks, window, out,
                         out_stride, out_dtype, dev_err);
-}
-
-extern "C" int gkv_kept_prefill(void *stream, int32_t B, const int32_t *cu_seqlens,
-                                const int32_t *start_pos, int32_t max_len, int32_t n_q_heads,
-                                const float *q, int64_t q_stride, const float *cos_tab,
-                                const float *sin_tab, const void *k, const void *v,
-                                gkv_cache_view cache, int32_t kept, int32_t window,
-                                const float *sinks, void *out, int64_t out_stride,
-                                int32_t out_dtype, uint32_t *dev_err) {
-  const int st = gkv::kept_check(cache, kept, window, false);
-  if (st != GKV_OK)
-    return st;
-  return prefill_launch(stream, B, cu_seqlens, start_pos, max_len, n_q_heads, cache.n_kv_heads,
-                        q, q_stride, cos_tab, sin_tab, k, v, &cache, sinks, window, out,
-                        out_stride, out_dtype, dev_err, true, kept);
 }

@@ -169,9 +169,12 @@ def decode_bound(out, pav, qk, fmt, bf16):
 
 
 def prefill_bound(out, pav, qk, n_keys, v_max, bf16):
-    """Largest error of a prefill output: q's two bf16 pieces and the sums as in decode_bound;
-    p as one fp16 piece (2^-11, in the weight and in the sum: 2^-10; 2^-25 each where it is
-    subnormal), V staged as fp16 of v 2^-10 (2^-11, or 2^-15 where that is subnormal)."""
-    d = qk * (2.0 ** -18 + 66 * 2.0 ** -24)
+    """Largest error of a prefill output: q as one fp16 piece of its row over the power of two
+    below the row's largest element (2^-11 of an element; one below 2^-14 of that power is
+    subnormal and off by 2^-25 of it: with q and k of one distribution, as here, the few of
+    them stay within 2^-18 of the sum of |q k|), the sums as in decode_bound; p as one fp16 piece (2^-11, in the weight and in the
+    sum: 2^-10; 2^-25 each where it is subnormal), V staged as fp16 of v 2^-10 (2^-11, or 2^-15
+    where that is subnormal)."""
+    d = qk * (2.0 ** -11 + 2.0 ** -18 + 66 * 2.0 ** -24)
     e = pav * (2 * d + 2.0 ** -10 + 2.0 ** -11 + 2.0 ** -17) + 2.0 ** -15 + n_keys * 2.0 ** -25 * v_max
     return e + np.abs(out) * (2.0 ** -8 if bf16 else 2.0 ** -24)
