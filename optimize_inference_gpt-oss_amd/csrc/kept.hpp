@@ -79,10 +79,10 @@ __host__ __device__ __forceinline__ float block_scale(float amax) {
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 
-// Four e4m3 codes -> four fp16 (exact).
-__device__ __forceinline__ u32x2 codes_to_f16(uint32_t w) {
-  const f16x2 a = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false));
-  const f16x2 b = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true));
+// Four e4m3 codes -> four fp16 of code * scale, scale a power of two (1: exact).
+__device__ __forceinline__ u32x2 codes_to_f16(uint32_t w, float scale = 1.0f) {
+  const f16x2 a = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, false));
+  const f16x2 b = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, true));
   return u32x2{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b)};
 }
 

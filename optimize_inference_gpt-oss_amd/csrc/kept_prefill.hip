@@ -81,10 +81,13 @@ struct KeptPrefillArgs {
 // What a wave fetches of a tile: a 16-key piece of K or V.
 struct Piece {
   u32x4 x[2];
-  float scale; // of codes; 0: bf16
+  float scale; // of codes
   bool hist;   // a block of the cache (else packed rows)
   int p;       // its first position
 };
+
+// Keeps a uniform branch a branch (its body is not worth running for nothing).
+#define GKV_KEEP_BRANCH asm volatile("")
 
 __device__ __forceinline__ uint32_t f16_pair(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{a, b}), f16x2));
@@ -146,7 +149,8 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
   auto tile_pos = [&](int t) { return t < n_first ? t * kPTile : k_lo + (t - n_first) * kPTile; };
   const int hist_end = a.k ? start : INT_MAX;
   const int lo_blk = lo / kBlockTokens;
-  const int lo_entry = kept_entry(a.row, max(lo_blk, a.row.kept_blocks));
+  const int to_ring = kept_entry(a.row, max(lo_blk, a.row.kept_blocks)) - max(lo_blk, a.row.kept_blocks);
+  const int ring_end = a.row.kept_blocks + a.row.ring_blocks;
   const int n_waves = a.G * a.subs;
 
   // Block id of a piece of tile t (kNone: not from the cache, or seen by nobody). It
@@ -161,11 +165,12 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
       return kNone;
     int e = p / kBlockTokens;
     if (W > 0 && e >= a.row.kept_blocks) {
+      GKV_KEEP_BRANCH;
       if (e < lo_blk)
         return kNone;
       if (a.row.ring_blocks > 0) { // the blocks seen, at most the ring's, wrap once
-        e += lo_entry - max(lo_blk, a.row.kept_blocks);
-        if (e >= a.row.kept_blocks + a.row.ring_blocks)
+        e += to_ring;
+        if (e >= ring_end)
           e -= a.row.ring_blocks;
       }
     }
@@ -190,11 +195,13 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
     x.scale = 0.0f;
     x.hist = x.p < hist_end;
     if (x.hist) {
+      GKV_KEEP_BRANCH;
       const bool ok = (uint32_t)id < (uint32_t)a.num_blocks;
       bad |= !ok && id != kNone;
       const int64_t hb = (int64_t)(ok ? id : 0) * a.n_kv_heads + g;
       const char *src = is_v ? a.vc : a.kc;
       if (a.scales) {
+        GKV_KEEP_BRANCH;
         const __amdgpu_buffer_rsrc_t r = head_rsrc(src + hb * 1024, ok ? 1024 : 0);
         x.x[0] = __builtin_amdgcn_raw_buffer_load_b128(r, is_v ? (c16 * 4 + kg) * 16 : ln * 16, 0, 0);
         const __amdgpu_buffer_rsrc_t sr = head_rsrc(a.scales + 2 * hb, ok ? 8 : 0);
@@ -224,84 +231,92 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
   };
   // Converts a piece and writes it into LDS. K: key rows; V: dimension rows, the
   // tokens of each 16 in the order of the operand slots (8 i + 4 h + r at 8 h + 4 i + r).
-  // K or V beyond fp16's range (codes: where 448 scales are), a flag per wave
-  bool range = false;
-  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-  auto top = [&](uint32_t x, uint32_t y) { // the larger magnitudes, per half
-    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, x & 0x7fff7fffu),
-                                                                  __builtin_bit_cast(u16x2, y)));
-  };
-  auto note = [&](uint32_t x) { range |= __any((x & 0x7fffu) == 0x7c00u || x >> 16 == 0x7c00u); };
-  auto put_v = [&](uint16_t *dst, int blk, int d, int kg, uint32_t t01, uint32_t t23) {
-    // tokens 4kg .. 4kg+3 of dimension d
-    *(u32x2 *)(dst + d * kPRow + 16 * blk + 8 * (kg & 1) + 4 * (kg >> 1)) = u32x2{t01, t23};
-  };
-  auto store = [&](const Piece &x, int buf, int task) {
+  auto store = [&](Piece &x, int buf, int task) {
     const int blk = task & 3, ln = opaque_lane(), c16 = ln & 15, kg = ln >> 4;
-    // a cached piece with tokens that no query of the workgroup sees: what they
-    // hold, which may be anything, becomes 0
-    const bool edge = x.hist && (x.p < lo || x.p + kBlockTokens - 1 > p_last);
-    auto seen = [&](int r) {
-      const int p = x.p + r;
-      return p <= p_last && (p >= lo || p < kept);
-    };
-    if (task < 4) {
+    const bool is_v = task >= 4;
+    const bool codes = x.hist && a.scales;
+    if (x.hist && (x.p < lo || x.p + kBlockTokens - 1 > p_last)) {
+      // a cached piece with tokens that no query of the workgroup sees: what they
+      // hold, which may be anything, becomes 0
+      GKV_KEEP_BRANCH;
+      auto seen = [&](int r) {
+        const int p = x.p + r;
+        return p <= p_last && (p >= lo || p < kept);
+      };
+      if (!is_v) {
+        if (!seen(c16))
+          x.x[0] = x.x[1] = u32x4{0, 0, 0, 0};
+      } else if (codes) {
+        uint32_t keep = 0;
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+          keep |= seen(4 * kg + r) ? 0xffu << (8 * r) : 0u;
+        x.x[0] &= u32x4{keep, keep, keep, keep};
+      } else {
+        const uint32_t m01 = (seen(4 * kg) ? 0xffffu : 0u) | (seen(4 * kg + 1) ? 0xffff0000u : 0u);
+        const uint32_t m23 = (seen(4 * kg + 2) ? 0xffffu : 0u) | (seen(4 * kg + 3) ? 0xffff0000u : 0u);
+        x.x[0] &= u32x4{m01, m23, m01, m23};
+        x.x[1] &= u32x4{m01, m23, m01, m23};
+      }
+    }
+    if (!is_v) {
       u32x4 lo4, hi4;
-      if (x.hist && a.scales) {
+      if (codes) {
+        GKV_KEEP_BRANCH;
         const u32x2 y0 = codes_to_f16(x.x[0][0]), y1 = codes_to_f16(x.x[0][1]);
         const u32x2 y2 = codes_to_f16(x.x[0][2]), y3 = codes_to_f16(x.x[0][3]);
         lo4 = u32x4{y0[0], y0[1], y1[0], y1[1]};
         hi4 = u32x4{y2[0], y2[1], y3[0], y3[1]};
       } else {
-        const uint32_t keep = !edge || seen(c16) ? ~0u : 0u;
-        uint32_t most = 0;
+        GKV_KEEP_BRANCH;
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-          lo4[i] = keep & f16_pair(__uint_as_float(x.x[0][i] << 16), __uint_as_float(x.x[0][i] & 0xffff0000u));
-          hi4[i] = keep & f16_pair(__uint_as_float(x.x[1][i] << 16), __uint_as_float(x.x[1][i] & 0xffff0000u));
-          most = top(lo4[i], top(hi4[i], most));
+          lo4[i] = f16_pair(__uint_as_float(x.x[0][i] << 16), __uint_as_float(x.x[0][i] & 0xffff0000u));
+          hi4[i] = f16_pair(__uint_as_float(x.x[1][i] << 16), __uint_as_float(x.x[1][i] & 0xffff0000u));
         }
-        note(most);
       }
       uint16_t *dst = s_kv[buf][0] + (kBlockTokens * blk + c16) * kPRow + 8 * kg;
       *(u32x4 *)dst = lo4;
       *(u32x4 *)(dst + 32) = hi4;
       if (ln == 0)
-        s_ks[buf][blk] = x.hist && a.scales ? x.scale : 1.0f;
+        s_ks[buf][blk] = codes ? x.scale : 1.0f;
       return;
     }
-    uint16_t *dst = s_kv[buf][1];
-    uint32_t m01 = ~0u, m23 = ~0u;
-    if (edge) {
-      m01 = (seen(4 * kg) ? 0xffffu : 0u) | (seen(4 * kg + 1) ? 0xffff0000u : 0u);
-      m23 = (seen(4 * kg + 2) ? 0xffffu : 0u) | (seen(4 * kg + 3) ? 0xffff0000u : 0u);
-    }
-    if (x.hist && a.scales) {
-      const float s = x.scale * kPVScale;
-      note(f16_pair(448.0f * s, 0.0f));
+    // tokens 4kg .. 4kg+3 of dimension d at dst + d rows
+    uint16_t *dst = s_kv[buf][1] + 16 * blk + 8 * (kg & 1) + 4 * (kg >> 1);
+    if (codes) {
+      GKV_KEEP_BRANCH;
+      dst += c16 * kPRow;
+      const float s = __uint_as_float(uniform(__float_as_uint(x.scale * kPVScale)));
+      if ((__float_as_uint(s) & 0x7fffffu) == 0) {
+        // a power of two: the conversion applies it
+        GKV_KEEP_BRANCH;
 #pragma unroll
-      for (int nn = 0; nn < 4; nn++) {
-        const f32x2 f0 = __builtin_amdgcn_cvt_pk_f32_fp8((int)x.x[0][nn], false);
-        const f32x2 f1 = __builtin_amdgcn_cvt_pk_f32_fp8((int)x.x[0][nn], true);
-        put_v(dst, blk, c16 + 16 * nn, kg, f16_pair(f0[0] * s, f0[1] * s) & m01,
-              f16_pair(f1[0] * s, f1[1] * s) & m23);
+        for (int nn = 0; nn < 4; nn++)
+          *(u32x2 *)(dst + 16 * nn * kPRow) = codes_to_f16(x.x[0][nn], s);
+      } else {
+        GKV_KEEP_BRANCH;
+#pragma unroll
+        for (int nn = 0; nn < 4; nn++) {
+          const f32x2 f0 = __builtin_amdgcn_cvt_pk_f32_fp8((int)x.x[0][nn], false);
+          const f32x2 f1 = __builtin_amdgcn_cvt_pk_f32_fp8((int)x.x[0][nn], true);
+          *(u32x2 *)(dst + 16 * nn * kPRow) = u32x2{f16_pair(f0[0] * s, f0[1] * s), f16_pair(f1[0] * s, f1[1] * s)};
+        }
       }
     } else if (x.hist) {
-      uint32_t most = 0;
+      GKV_KEEP_BRANCH;
+      dst += c16 * kPRow;
 #pragma unroll
       for (int nn = 0; nn < 4; nn++) { // dims c + 32 (nn / 2) + 16 (nn % 2)
         const uint32_t t01 = x.x[nn / 2][2 * (nn & 1)], t23 = x.x[nn / 2][2 * (nn & 1) + 1];
-        const uint32_t f01 =
-            m01 & f16_pair(__uint_as_float(t01 << 16) * kPVScale, __uint_as_float(t01 & 0xffff0000u) * kPVScale);
-        const uint32_t f23 =
-            m23 & f16_pair(__uint_as_float(t23 << 16) * kPVScale, __uint_as_float(t23 & 0xffff0000u) * kPVScale);
-        most = top(f01, top(f23, most));
-        put_v(dst, blk, c16 + 16 * nn, kg, f01, f23);
+        *(u32x2 *)(dst + 16 * nn * kPRow) =
+            u32x2{f16_pair(__uint_as_float(t01 << 16) * kPVScale, __uint_as_float(t01 & 0xffff0000u) * kPVScale),
+                  f16_pair(__uint_as_float(t23 << 16) * kPVScale, __uint_as_float(t23 & 0xffff0000u) * kPVScale)};
       }
-      note(most);
     } else {
       // rows 4kg + i, dims 4 c .. 4 c + 3: 4 x 4 turned
-      uint32_t most = 0;
+      GKV_KEEP_BRANCH;
+      dst += 4 * c16 * kPRow;
 #pragma unroll
       for (int d = 0; d < 4; d++) {
         float f[4];
@@ -310,11 +325,8 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
           const uint32_t y = x.x[i / 2][2 * (i & 1) + d / 2];
           f[i] = __uint_as_float(d & 1 ? y & 0xffff0000u : y << 16) * kPVScale;
         }
-        const uint32_t f01 = f16_pair(f[0], f[1]), f23 = f16_pair(f[2], f[3]);
-        most = top(f01, top(f23, most));
-        put_v(dst, blk, 4 * c16 + d, kg, f01, f23);
+        *(u32x2 *)(dst + d * kPRow) = u32x2{f16_pair(f[0], f[1]), f16_pair(f[2], f[3])};
       }
-      note(most);
     }
   };
 
@@ -410,6 +422,10 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
       store(pc[i], 0, wave + i * n_waves);
   lds_barrier();
 
+  // steps (32 keys from kb on) that this wave's queries see something of: kb in
+  // [key_begin, key_end] or below kept; up to window_end some query has left them behind
+  const int key_end = active ? p_last_s : -1, key_begin = W > 0 ? p0s - W - 30 : INT_MIN;
+  const int window_end = W > 0 ? p_last_s - W : INT_MIN;
   for (int t = 0; t < n_tiles; t++) {
     const int buf = t & 1;
 #pragma unroll
@@ -425,7 +441,7 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
 #pragma unroll
     for (int s = 0; s < 2; s++) {
       const int kb = kt + 32 * s;
-      if (!active || kb > p_last_s || (W > 0 && kb + 31 <= p0s - W && kb >= kept))
+      if (kb > key_end || (kb < key_begin && kb >= kept))
         continue; // nothing of the step is seen
       f32x16 acc;
 #pragma unroll
@@ -438,7 +454,8 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
         acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kop, qv[kk], acc, 0, 0, 0);
       }
       const float c0 = qf * s_ks[buf][2 * s], c1 = qf * s_ks[buf][2 * s + 1];
-      if (kb + 31 > p0s || (W > 0 && kb <= p_last_s - W && kb + 31 >= kept)) {
+      if (kb > p0s - 31 || (kb <= window_end && kb + 31 >= kept)) {
+        GKV_KEEP_BRANCH;
         // key kb + 4 h + off is seen iff 0 <= last - off < W, or it is a kept one
         const int ln = opaque_lane(), h = ln >> 5, last = p0s + (ln & 31) - kb - 4 * h;
         const uint32_t wide = W > 0 ? (uint32_t)W : 0x80000000u;
@@ -517,8 +534,6 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
   if (a.dev_err) {
     if (bad && lane == 0)
       atomicOr(a.dev_err, GKV_DEVERR_BLOCK_ID);
-    if (range && lane == 0)
-      atomicOr(a.dev_err, GKV_DEVERR_RANGE);
   }
 
   // out = o / (l + sink's weight) / kPVScale; 0 for a row that saw nothing
@@ -529,6 +544,15 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
   const float den = fmaf(l, f, __builtin_amdgcn_exp2f(sink2 - M));
   const float scale = den == 0.0f ? 0.0f : f / den / kPVScale;
   const int q_first = q0 + kPQueries * sub; // this wave's first row of the prompt
+  if (a.dev_err) {
+    // an output that is not finite, as K and V beyond fp16 give it
+    float z = scale * 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; i++)
+      z = fmaf(o[0][i], 0.0f, fmaf(o[1][i], 0.0f, z));
+    if (__any(!(z == 0.0f) && active && q_first + n_o < L) && ln == 0)
+      atomicOr(a.dev_err, GKV_DEVERR_RANGE);
+  }
   if (!a.out_bf16) {
     if (!active || q_first + n_o >= L)
       return;
