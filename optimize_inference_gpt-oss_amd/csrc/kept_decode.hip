@@ -20,16 +20,19 @@
 // A step is two blocks (32 tokens). A wave takes the steps of one (sequence, kv
 // head), loads the next step's blocks while it computes this one's, and leaves it
 // to the other waves of its SIMD to cover the chain of matrix op, exponential,
-// matrix op: 4 waves per SIMD for codes (a step is 16 registers of data),
-// 2 for bf16 with a ring of 3 steps. Two ways to deal the steps out:
-//   whole   few steps a sequence (a window, short contexts): a (sequence, kv
-//           head) belongs to 1 .. 8 waves of one workgroup, which cut its steps and
-//           merge in LDS. One launch, no workspace.
+// matrix op: 2 steps in registers, 4 waves per SIMD (3 steps and 3 or 5 waves
+// measured the same or worse). Two ways to deal the steps out:
+//   whole   contexts and windows that are not long: a (sequence, kv head) belongs
+//           to 1 .. 8 waves of one workgroup, which cut its steps and merge in LDS.
+//           One launch, no workspace. 512 sequences of 129 .. 2049 tokens (8 kv
+//           heads, codes, 586 MB): 107 us, 5.5 TB/s; 97 windows of 4096 behind 64
+//           (411 MB): 70 us, 5.9 TB/s.
 //   ranges  the sequences laid end to end are cut into equal ranges, one per
-//           resident wave; every workgroup finds its own range from the lengths
+//           wave; every workgroup finds its own range from the lengths
 //           in its prologue. A sequence inside one range is finished there,
 //           the pieces of the others go to the workspace and a second launch
-//           merges them, a workgroup per range.
+//           merges them, a workgroup per range. 4 sequences of 129 .. 16384 tokens:
+//           18 us, where one workgroup a sequence and head takes 43.
 #include "kept.hpp"
 
 #include <algorithm>
@@ -39,7 +42,10 @@ namespace gkv {
 constexpr int kKeptAux = 2;            // nontemporal: each K/V byte is read once
 constexpr int kKeptStep = 32;          // tokens per step
 constexpr int kHeads = 8;              // query heads per kv head, at most
-constexpr int kSplitWgs = 512;         // range workgroups: two per CU (bf16: 256, one per CU)
+// Range workgroups: one per CU, two waves a SIMD. Two per CU make twice the pieces
+// and shorter ranges (us, 256 / 512 workgroups: 32 sequences of 129 .. 16384
+// tokens 55.7 / 60.4, bf16 100 / 108; 4 of them 18.4 / 20.6, 22.1 / 28.3).
+constexpr int kSplitWgs = 256;
 constexpr int kMinRangeSteps = 4;      // steps per range, at least
 constexpr int kPieceFloats = kHeads * kHeadDim;
 constexpr int kPieceMl = 2 * kHeads;   // (m, l) of a piece's heads
@@ -555,7 +561,7 @@ void kept_decode_whole_kernel(KeptDecodeArgs a) {
 
 // ---- ranges ----------------------------------------------------------------------
 
-// Range r of the T steps cut into n (n <= 4096): floor(r T / n), in 32 bits.
+// Range r of the T steps cut into n (n <= 2048): floor(r T / n), in 32 bits.
 __device__ __forceinline__ int range_begin(int r, int T, int n) {
   const uint32_t q = (uint32_t)T / (uint32_t)n, m = (uint32_t)T % (uint32_t)n;
   return (int)(r * q + r * m / (uint32_t)n);
@@ -867,11 +873,38 @@ static int64_t steps_bound(int32_t max_seq_len, int32_t kept, int32_t window) {
   return (blocks + 1) / 2;
 }
 
+// Whole sequences or ranges. A wave takes about 1 us for a step (bf16: 1.2), eight
+// share a sequence, so the longest one costs steps / 8 us whatever the rest do;
+// ranges cost a second launch and their pieces, 5 to 10 us, but no sequence is
+// longer than the others. Measured (us, whole / ranges, 8 heads, codes): 512
+// sequences of 129 .. 2049 tokens 110 / 116 (bf16 192 / 209), 16 of them 10.7 /
+// 17.0; 128 of 129 .. 4096 56 / 58, 8 of them 16.0 / 16.8 (bf16 19.1 / 18.0); 8 of
+// 129 .. 8192 26 / 19, 4 of 129 .. 16384 43 / 18. A window of 4096 behind 16: 97
+// sequences 68 / 76, 32 of them 25 / 34, 8 of them 18 / 16 (bf16 25 / 21).
+constexpr int kWholeSteps = 72;      // whole whatever the number of sequences
+constexpr int kWholeStepsMany = 144; // whole for this many (sequence, head)s
+constexpr int kWholeMany = 96;
 static bool use_whole(int32_t B, int32_t n_kv_heads, int32_t max_seq_len, int32_t kept,
                       int32_t window) {
-  (void)B;
-  (void)n_kv_heads;
-  return steps_bound(max_seq_len, kept, window) <= (window > 0 ? 160 : 16);
+  const int64_t steps = steps_bound(max_seq_len, kept, window);
+  return steps <= kWholeSteps ||
+         (steps <= kWholeStepsMany && (int64_t)B * n_kv_heads >= kWholeMany);
+}
+
+// Waves per (sequence, head) of the whole kernel. As many as take half the GPU's
+// 4096 wave slots: more leave each wave too few steps (a window of 128: 512
+// sequences 19 us with one, 32 with four) without reading faster. Contexts without a window differ
+// in length, so there a wave gets at most 16 steps and the last sequences end
+// sooner (512 sequences of 129 .. 2049 tokens: 126 us with one wave, 114, 108,
+// 110 with 2, 4, 8; bf16 226, 206, 196, 189).
+constexpr int kWholeWaves = 2048;
+static int whole_parts(int32_t B, int32_t n_kv_heads, int64_t steps, int32_t window) {
+  int parts = 1;
+  while (parts < 8 && 2 * parts <= steps &&
+         (2 * parts * (int64_t)B * n_kv_heads <= kWholeWaves ||
+          (window == 0 && steps > 16 * parts)))
+    parts *= 2;
+  return parts;
 }
 
 static int range_subs(int n_kv_heads) { return 8 / n_kv_heads; }
@@ -958,16 +991,10 @@ extern "C" int gkv_kept_decode(void *stream, int32_t B, int32_t n_q_heads, const
   if (use_whole(B, a.n_kv_heads, max_seq_len, kept, window)) {
     if (B == 0)
       return GKV_OK;
-    // waves per (sequence, head): as many as leave every wave slot of the GPU
-    // taken, at most 8 and no more than there are steps
-    const int64_t slots = 256 * (blk ? 16 : 8);
-    int parts = 1;
-    while (parts < 8 && 2 * parts * (int64_t)B * a.n_kv_heads <= slots && 2 * parts <= steps)
-      parts *= 2;
-    a.parts = parts;
-    a.heads_per_wg = std::min(8 / parts, a.n_kv_heads);
+    a.parts = whole_parts(B, a.n_kv_heads, steps, window);
+    a.heads_per_wg = std::min(8 / a.parts, a.n_kv_heads);
     const dim3 grid((unsigned)((int64_t)B * ((a.n_kv_heads + a.heads_per_wg - 1) / a.heads_per_wg)));
-    const dim3 block(64 * parts * a.heads_per_wg);
+    const dim3 block(64 * a.parts * a.heads_per_wg);
     if (blk)
       hipLaunchKernelGGL((kept_decode_whole_kernel<true, 2, 4>), grid, block, 0, s, a);
     else
@@ -981,16 +1008,16 @@ extern "C" int gkv_kept_decode(void *stream, int32_t B, int32_t n_q_heads, const
     return GKV_ERR_ARG;
   if (B == 0)
     return GKV_OK;
-  const int n_wg = blk ? kSplitWgs : kSplitWgs / 2, subs = range_subs(a.n_kv_heads);
-  a.max_ranges = n_wg * subs;
+  const int subs = range_subs(a.n_kv_heads);
+  a.max_ranges = kSplitWgs * subs;
   a.cuts = (int4 *)workspace;
   a.ws_ml = (float *)((char *)workspace + w.ml);
   a.ws_o = (float *)((char *)workspace + w.o);
   const dim3 block(64 * subs * a.n_kv_heads);
   if (blk)
-    hipLaunchKernelGGL((kept_decode_split_kernel<true, 2, 4>), dim3(n_wg), block, 0, s, a);
+    hipLaunchKernelGGL((kept_decode_split_kernel<true, 2, 4>), dim3(kSplitWgs), block, 0, s, a);
   else
-    hipLaunchKernelGGL((kept_decode_split_kernel<false, 2, 4>), dim3(n_wg), block, 0, s, a);
+    hipLaunchKernelGGL((kept_decode_split_kernel<false, 2, 4>), dim3(kSplitWgs), block, 0, s, a);
   if ((st = launch_status("kept_decode_split_kernel")))
     return st;
   hipLaunchKernelGGL(kept_decode_merge_kernel, dim3((unsigned)a.max_ranges), dim3(kMergeThreads), 0, s,
