@@ -69,7 +69,7 @@ typedef enum {
 #define GKV_DEVERR_LENGTH 2u   /* a sequence length beyond the table's capacity */
 #define GKV_DEVERR_ALIGN 4u    /* a prefill start position that is not a multiple of 16 */
 #define GKV_DEVERR_RANGE 8u    /* a V beyond the prefill's range (|v| >= 2^26: the output
-                                  holds inf there) */
+                                  holds inf there); gkv_kept_prefill: see there */
 #define GKV_DEVERR_PLAN 16u    /* gkv_decode_layer_planned was asked to reuse a plan the
                                   workspace does not hold for this call (it planned afresh) */
 
@@ -440,9 +440,9 @@ int gkv_prefill_paged(void *stream, int32_t B, const int32_t *cu_seqlens,
  *                             window / 16 + 1 (GKV_ERR_ARG otherwise).
  * gkv_pool_create_kept makes such caches; full layers of any pool in these formats
  * are the ring = 0 form. sinks: fp32 [Hq] logits, or NULL (no sink). Masked
- * positions count for nothing, whatever their slots hold; in a prefill a V that
- * is not finite reaches every row of its workgroup's 32 that is not masked off
- * it by a whole block. */
+ * positions count for nothing, whatever their slots hold; only in a prefill a V that
+ * is not finite and that some row sees reaches rows up to 62 positions away from
+ * that one too. */
 
 /* Append by whole blocks: the rows of sequence b, cu_seqlens[b] ..
  * cu_seqlens[b+1] - 1 (device int32 [B+1]; NULL: row b alone, as in a decode
@@ -473,7 +473,8 @@ int gkv_kept_append(void *stream, int32_t B, const int32_t *cu_seqlens, const in
                     int32_t kept, int32_t window, void *k_pack, void *v_pack,
                     uint32_t *dev_err);
 
-/* Bytes of workspace gkv_kept_decode needs (0: none, workspace may be NULL). */
+/* Bytes of workspace gkv_kept_decode needs for up to B sequences (0: none, workspace may
+ * be NULL). */
 size_t gkv_kept_workspace_bytes(int32_t B, int32_t n_kv_heads, int32_t max_seq_len, int32_t kept,
                                 int32_t window);
 
@@ -497,7 +498,13 @@ int gkv_kept_decode(void *stream, int32_t B, int32_t n_q_heads, const float *q, 
  * history (start_pos: multiples of 16), with gkv_prefill_paged's arguments and
  * rules: keys before start_pos[b] from the cache, those from there on from the
  * packed rows (k = v = NULL: from the cache too, ring = 0 only). On a ring,
- * append the chunk after this call. */
+ * append the chunk after this call. At most 8 query heads per kv head. q, k, v, out
+ * and the tables are 16-byte aligned, strides multiples of 4 (out_stride in bf16:
+ * of 8). The matrix cores take fp16: q is rounded to 11 bits against its row's
+ * largest element, so a score is off by at most 2^-11 sum |q k| / 8; a weight has 11
+ * bits; bf16 K is exact for magnitudes 2^-14 .. 2^16, V for 2^-4 .. 2^26, with an
+ * absolute error of at most 2^-25 and 2^-15 below that. Beyond, and where an
+ * output is not finite: GKV_DEVERR_RANGE. */
 int gkv_kept_prefill(void *stream, int32_t B, const int32_t *cu_seqlens, const int32_t *start_pos,
                      int32_t max_len, int32_t n_q_heads, const float *q, int64_t q_stride,
                      const float *cos_tab, const float *sin_tab, const void *k, const void *v,

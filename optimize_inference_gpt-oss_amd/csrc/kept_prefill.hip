@@ -16,12 +16,13 @@
 //
 // Matrix cores, 32x32 output, K = 16, all operands fp16: S^T[key][query] = K Q^T,
 // O^T[dim][query] += V^T P^T. K: e4m3 codes and bf16 magnitudes 2^-14 .. 2^16 are
-// fp16 values (below, an absolute error of 2^-25; above inf, which is flagged). q and P
+// fp16 values (below, an absolute error of 2^-25; beyond, flagged when staged). q and P
 // are rounded to fp16's 11 bits, q after a power of two that brings its row's
 // largest element into [1, 2): a score is off by at most 2^-11 sum |q k| / 8, a
 // weight by as much again as its own rounding, 2^-11; the bf16 output's is 2^-8
 // (q in two bf16 pieces, 16 bits, doubled the first product and spilled: 204 us
-// against TIME_F16 for 8 chunks of 100 .. 700 rows after 1536 cached ones). V is
+// against 172 for 8 chunks of 100 .. 700 rows after 1536 cached ones, before the
+// staging was trimmed). V is
 // staged as v * 2^-10 (exact for bf16 magnitudes 2^-4 .. 2^26, an absolute error of at
 // most 2^-15 below, inf above, which is flagged). A lane (half h, query n)
 // holds 16 scores of one query, keys 8 i + 4 h + 0..3 of the 32; these are its
@@ -138,13 +139,15 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
                       : INT_MAX;
   if (start > cap - L && q0 == 0 && tid == 0 && a.dev_err)
     atomicOr(a.dev_err, GKV_DEVERR_LENGTH);
+  if (start > INT_MAX - L)
+    start = 0; // (no such positions)
   const int p0 = start + q0, p_last = start + min(q0 + qn, L) - 1;
   const int W = a.window;
   // first position that the window of any query holds; its tile's start
   const int lo = W > 0 ? max(p0 - W + 1, 0) : 0;
   const int k_lo = lo & ~(kPTile - 1);
   const int kept = W > 0 ? a.kept : 0;
-  const int n_first = min((kept + kPTile - 1) / kPTile, k_lo / kPTile); // kept positions' tiles
+  const int n_first = min(kept / kPTile + (kept % kPTile != 0), k_lo / kPTile); // kept positions' tiles
   const int n_tiles = (p_last - k_lo) / kPTile + 1 + n_first;
   auto tile_pos = [&](int t) { return t < n_first ? t * kPTile : k_lo + (t - n_first) * kPTile; };
   const int hist_end = a.k ? start : INT_MAX;
@@ -178,7 +181,7 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
       return kNone;
     return __builtin_amdgcn_raw_buffer_load_b32(table_row, 0, 4 * e, 0);
   };
-  bool bad = false;
+  bool bad = false, range = false;
   // (lane roles: K's piece as (kg, t), V's blocks as (kg, c), V's rows as (kg, d).
   // The lane is made opaque in each use, so that the offsets are formed there and not
   // kept in registers, of which there are none to spare, through the loop.)
@@ -274,6 +277,16 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
           lo4[i] = f16_pair(__uint_as_float(x.x[0][i] << 16), __uint_as_float(x.x[0][i] & 0xffff0000u));
           hi4[i] = f16_pair(__uint_as_float(x.x[1][i] << 16), __uint_as_float(x.x[1][i] & 0xffff0000u));
         }
+        // beyond fp16: a score of -inf would count for nothing without a trace
+        typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+        u16x2 top{0, 0};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, lo4[i] & 0x7fff7fffu));
+          top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, hi4[i] & 0x7fff7fffu));
+        }
+        if (__any(((__builtin_bit_cast(uint32_t, top) + 0x04000400u) & 0x80008000u) != 0))
+          range = true;
       }
       uint16_t *dst = s_kv[buf][0] + (kBlockTokens * blk + c16) * kPRow + 8 * kg;
       *(u32x4 *)dst = lo4;
@@ -424,7 +437,7 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
 
   // steps (32 keys from kb on) that this wave's queries see something of: kb in
   // [key_begin, key_end] or below kept; up to window_end some query has left them behind
-  const int key_end = active ? p_last_s : -1, key_begin = W > 0 ? p0s - W - 30 : INT_MIN;
+  const int key_end = active ? p_last_s : -1, key_begin = W > 0 ? max(p0s - W, INT_MIN + 30) - 30 : INT_MIN;
   const int window_end = W > 0 ? p_last_s - W : INT_MIN;
   for (int t = 0; t < n_tiles; t++) {
     const int buf = t & 1;
@@ -532,8 +545,8 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
     }
   }
   if (a.dev_err) {
-    if (bad && lane == 0)
-      atomicOr(a.dev_err, GKV_DEVERR_BLOCK_ID);
+    if ((bad || range) && lane == 0)
+      atomicOr(a.dev_err, (bad ? GKV_DEVERR_BLOCK_ID : 0u) | (range ? GKV_DEVERR_RANGE : 0u));
   }
 
   // out = o / (l + sink's weight) / kPVScale; 0 for a row that saw nothing
