@@ -20,8 +20,8 @@
 // A step is two blocks (32 tokens). A wave takes the steps of one (sequence, kv
 // head), loads the next step's blocks while it computes this one's, and leaves it
 // to the other waves of its SIMD to cover the chain of matrix op, exponential,
-// matrix op: 2 steps in registers, 4 waves per SIMD (3 steps and 3 or 5 waves
-// measured the same or worse). Two ways to deal the steps out:
+// matrix op: 2 steps in registers, 4 waves per SIMD, with ranges 2 (3 or 4 steps
+// and 3 or 5 waves measured the same or worse). Two ways to deal the steps out:
 //   whole   contexts and windows that are not long: a (sequence, kv head) belongs
 //           to 1 .. 8 waves of one workgroup, which cut its steps and merge in LDS.
 //           One launch, no workspace. 512 sequences of 129 .. 2049 tokens (8 kv
@@ -927,8 +927,9 @@ static KeptWorkspace kept_workspace(int32_t n_kv_heads) {
 extern "C" size_t gkv_kept_workspace_bytes(int32_t B, int32_t n_kv_heads, int32_t max_seq_len,
                                            int32_t kept, int32_t window) {
   using namespace gkv;
+  // (what the call of any smaller batch needs too)
   if (B <= 0 || n_kv_heads <= 0 || n_kv_heads > 8 || max_seq_len < 0 || kept < 0 || window < 0 ||
-      use_whole(B, n_kv_heads, max_seq_len, kept, window))
+      steps_bound(max_seq_len, kept, window) <= kWholeSteps)
     return 0;
   return kept_workspace(n_kv_heads).total;
 }
@@ -1015,9 +1016,9 @@ extern "C" int gkv_kept_decode(void *stream, int32_t B, int32_t n_q_heads, const
   a.ws_o = (float *)((char *)workspace + w.o);
   const dim3 block(64 * subs * a.n_kv_heads);
   if (blk)
-    hipLaunchKernelGGL((kept_decode_split_kernel<true, 2, 4>), dim3(kSplitWgs), block, 0, s, a);
+    hipLaunchKernelGGL((kept_decode_split_kernel<true, 2, 2>), dim3(kSplitWgs), block, 0, s, a);
   else
-    hipLaunchKernelGGL((kept_decode_split_kernel<false, 2, 4>), dim3(kSplitWgs), block, 0, s, a);
+    hipLaunchKernelGGL((kept_decode_split_kernel<false, 2, 2>), dim3(kSplitWgs), block, 0, s, a);
   if ((st = launch_status("kept_decode_split_kernel")))
     return st;
   hipLaunchKernelGGL(kept_decode_merge_kernel, dim3((unsigned)a.max_ranges), dim3(kMergeThreads), 0, s,

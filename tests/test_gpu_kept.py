@@ -254,7 +254,7 @@ def test_decode_many_short_sequences_through_the_ranges(gkv, cuda, fmt):
     """Far more sequences than ranges' steps, many of them empty, and one long."""
     rng = np.random.default_rng(5)
     lens = list(rng.integers(0, 40, 300)) + [600]
-    run_decode(gkv, [int(x) for x in lens], 2, 1, Layout(0, 0, False), fmt, max_len=600)
+    run_decode(gkv, [int(x) for x in lens], 2, 1, Layout(0, 0, False), fmt, max_len=20000)
 
 
 @pytest.mark.parametrize("fmt", [BF16, BLOCK])
@@ -314,8 +314,9 @@ def test_decode_bad_pages_and_long_lengths(gkv, cuda):
 
 
 def run_prefill(gkv, starts, rows, Hq, Hkv, lay, fmt, sinks=True, bf16=False, seed=0, cached=True,
-                from_cache=False):
-    c = Cache(np.asarray(starts) + (rows if from_cache else 0), Hkv, lay, fmt, seed=seed)
+                from_cache=False, spread=False, scale=1.0):
+    c = Cache(np.asarray(starts) + (rows if from_cache else 0), Hkv, lay, fmt, seed=seed, spread=spread,
+              scale=scale)
     last = np.asarray(starts) + rows - 1
     c.poison(starts, last)
     rng = np.random.default_rng(seed + 3)

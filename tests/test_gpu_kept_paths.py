@@ -1,0 +1,229 @@
+"""The gkv_kept_* entry points where a call takes another way than the short ones: long
+bounds, many sequences, pools past 4 GiB, other streams, padded rows, values at the range's end."""
+import numpy as np
+import pytest
+import torch
+
+from keptcase import BF16, BLOCK, D, Cache, Layout
+from oracle import kv_oracle as O
+from test_gpu_kept import dev, run_decode, run_prefill
+
+pytestmark = pytest.mark.gpu
+
+LONG = 20000  # a bound past which the decode cuts sequences into ranges, whatever their lengths
+WIDE = 4800   # a window past it
+
+
+@pytest.mark.parametrize("fmt", [BF16, BLOCK])
+@pytest.mark.parametrize("kept,window,ring", [(0, 0, False), (16, WIDE, True), (48, WIDE, False)])
+@pytest.mark.parametrize("lens", [[1], [0, 0, 0], [0, 1, 15, 16, 17], [33, 250, 0, 64, 31, 129], [700, 3]])
+def test_ranges_of_short_sequences(gkv, cuda, fmt, kept, window, ring, lens):
+    assert gkv.kept_workspace_bytes(len(lens), 2, LONG, kept, window) > 0
+    run_decode(gkv, lens, 16, 2, Layout(kept, window, ring), fmt, seed=kept + len(lens), max_len=LONG,
+               sinks=len(lens) % 2 == 0, bf16=len(lens) == 5, spread=len(lens) == 6)
+
+
+@pytest.mark.parametrize("fmt", [BF16, BLOCK])
+@pytest.mark.parametrize("Hq,Hkv", [(64, 8), (6, 3), (7, 7), (8, 1), (5, 5), (24, 4)])
+def test_ranges_of_all_head_counts(gkv, cuda, fmt, Hq, Hkv):
+    run_decode(gkv, [40, 0, 900, 17], Hq, Hkv, Layout(0, 0, False), fmt, seed=Hq, sinks=Hq % 2 == 0, max_len=LONG)
+
+
+@pytest.mark.parametrize("fmt", [BF16, BLOCK])
+@pytest.mark.parametrize("kept,window,ring", [(0, 0, False), (16, WIDE, True), (32, WIDE, False)])
+def test_ranges_of_long_sequences(gkv, cuda, fmt, kept, window, ring):
+    run_decode(gkv, [7003, 5, 0, 5200], 8, 2, Layout(kept, window, ring), fmt, max_len=LONG)
+
+
+@pytest.mark.parametrize("fmt", [BF16, BLOCK])
+@pytest.mark.parametrize("B,Hkv,window", [(300, 8, 0), (300, 8, 32), (150, 8, 0), (70, 8, 48), (70, 5, 0), (40, 8, 0)])
+def test_many_sequences(gkv, cuda, fmt, B, Hkv, window):
+    """One, two, four and eight waves per sequence and head."""
+    lens = [int(x) for x in np.random.default_rng(B).integers(0, 90, B)]
+    run_decode(gkv, lens, Hkv, Hkv, Layout(16 if window else 0, window, bool(window)), fmt, max_len=512)
+
+
+def test_the_workspace_of_a_batch_does_for_a_smaller_one(gkv, cuda):
+    for kept, window, max_len in ((0, 0, 3000), (64, 4096, 9000), (0, 0, 2000), (16, 128, 100000)):
+        need = [gkv.kept_workspace_bytes(B, 8, max_len, kept, window) for B in (1, 11, 12, 500)]
+        assert sorted(need) == need and need[0] in (0, need[-1])
+
+
+@pytest.mark.parametrize("fmt", [BF16, BLOCK])
+@pytest.mark.parametrize("kept,window,ring", [(0, 0, False), (32, 128, True)])
+def test_prefill_of_any_scales(gkv, cuda, fmt, kept, window, ring):
+    """Block scales that are no powers of two, blocks of very different size (magnitudes
+    2^-9 .. 2^2)."""
+    run_prefill(gkv, [208, 16, 336], [70, 33, 5], 16, 2, Layout(kept, window, ring), fmt, spread=True, scale=0.125)
+
+
+HUGE = 2**31 - 16
+
+
+@pytest.mark.parametrize("kept,window", [(0, HUGE), (HUGE, 16), (HUGE, HUGE), (1 << 30, 1 << 30)])
+def test_masks_wider_than_any_sequence(gkv, cuda, kept, window):
+    """... are the causal mask."""
+    lay = Layout(0, 0, False)
+    c = Cache([96, 33], 2, lay, BLOCK)
+    view = c.device(gkv)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q = torch.randn(60, 4 * D, generator=g, device="cuda")
+    kv = [torch.randn(60, 2 * D, generator=g, device="cuda").bfloat16() for _ in "kv"]
+    cu, start = dev(np.array([0, 40, 60], np.int32)), dev(np.array([80, 32], np.int32))
+    lens = dev(np.array([96, 33], np.int32))
+    outs = []
+    for k, w in ((0, 0), (kept, window)):
+        out = torch.zeros(60, 4 * D, device="cuda")
+        gkv.kept_prefill(cu, 40, q, 4, view, out, start_pos=start, k=kv[0], v=kv[1], kept=k, window=w, dev_err=c.err)
+        one = torch.zeros(2, 4 * D, device="cuda")
+        gkv.kept_decode(q[:2], 4, lens, 96, view, one, kept=k, window=w, dev_err=c.err)
+        outs.append((out, one))
+    assert all(torch.equal(x, y) for x, y in zip(*outs)) and int(c.err.item()) == 0
+
+
+def test_prefill_leaves_other_rows_alone(gkv, cuda):
+    """Prompts without rows, rows behind the last prompt, padding between the rows."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    q = torch.randn(50, 4 * D + 4, generator=g, device="cuda")
+    k, v = (torch.randn(50, 2 * D, generator=g, device="cuda").bfloat16() for _ in "kv")
+    cu = dev(np.array([0, 0, 33, 33, 40], np.int32))
+    for dt in (torch.bfloat16, torch.float32):
+        pad = torch.full((50, 4 * D + 8), 7.0, dtype=dt, device="cuda")
+        out = torch.zeros(50, 4 * D, dtype=dt, device="cuda")
+        view = gkv.CacheView(n_kv_heads=2)
+        gkv.kept_prefill(cu, 33, q[:, :4 * D], 4, view, pad[:, :4 * D], k=k, v=v, window=16)
+        gkv.kept_prefill(cu, 33, q[:, :4 * D].contiguous(), 4, view, out, k=k, v=v, window=16)
+        assert torch.equal(pad[:40, :4 * D], out[:40])
+        assert (pad[40:] == 7).all() and (pad[:, 4 * D:] == 7).all() and (out[40:] == 0).all()
+
+
+@pytest.mark.parametrize("where", ["k", "v"])
+@pytest.mark.parametrize("x,flag", [(65280.0, False), (65536.0, True), (-1e30, True), (float("inf"), True)])
+def test_prefill_flags_values_beyond_its_range(gkv, cuda, where, x, flag):
+    x = x if where == "k" else x * 1024  # V is taken as v * 2^-10
+    k, v = torch.zeros(40, D, dtype=torch.bfloat16, device="cuda"), torch.ones(40, D, dtype=torch.bfloat16, device="cuda")
+    (k if where == "k" else v)[7, 3] = x
+    q = torch.ones(40, D, device="cuda")
+    out, err = torch.zeros(40, D, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    gkv.kept_prefill(dev(np.array([0, 40], np.int32)), 40, q, 1, gkv.CacheView(n_kv_heads=1), out, k=k, v=v,
+                     dev_err=err)
+    assert int(err.item()) == (gkv.DEVERR_RANGE if flag else 0)
+    assert torch.isfinite(out).all() or flag
+
+
+def test_a_cached_k_beyond_the_range_is_flagged(gkv, cuda):
+    c = Cache([32], 1, Layout(0, 0, False), BF16)
+    view = c.device(gkv)
+    c.dk[int(c.table[0, 1])].fill_(int(np.float32(-1e9).view(np.int32)) >> 16)
+    q, kv = torch.ones(4, D, device="cuda"), torch.zeros(4, D, dtype=torch.bfloat16, device="cuda")
+    out = torch.zeros(4, D, device="cuda")
+    gkv.kept_prefill(dev(np.array([0, 4], np.int32)), 4, q, 1, view, out, start_pos=dev(np.array([32], np.int32)),
+                     k=kv, v=kv, dev_err=c.err)
+    assert int(c.err.item()) == gkv.DEVERR_RANGE
+
+
+@pytest.mark.parametrize("fmt,blocks", [(BF16, 265000), (BLOCK, 530000)])
+def test_a_pool_past_32_bits(gkv, cuda, fmt, blocks):
+    """Blocks beyond 4 GiB of K: append, decode (whole and ranges), prefill and copies give what
+    they give at the pool's start."""
+    Hq, Hkv, B, n = 16, 8, 2, 40
+    dt, el = (torch.int16, 1024) if fmt == BF16 else (torch.uint8, 1024)
+    ids = np.arange(B * n).reshape(B, n).astype(np.int32)
+    pools = []
+    for nb, table in ((2 * B * n, ids), (blocks, blocks - 1 - ids)):
+        k, v = (torch.empty(nb, Hkv, el, dtype=dt, device="cuda") for _ in "kv")
+        s = torch.empty(nb, Hkv, 2, device="cuda") if fmt == BLOCK else None
+        t = dev(np.ascontiguousarray(table))
+        pools.append((gkv.cache_view(k, v, t, Hkv, v_scale=s, v_format=fmt), k, v, s, t))
+    assert pools[1][1].nbytes > 2**32
+    g = torch.Generator(device="cuda").manual_seed(5)
+    lens, rows = np.array([515, 300], np.int32), np.array([400, 300], np.int32)
+    qkv = torch.randn(int(rows.sum()), (Hq + 2 * Hkv) * D, generator=g, device="cuda")
+    cos, sin = (dev(x) for x in O.rope_table(LONG))
+    cu = dev(np.concatenate([[0], np.cumsum(rows)]).astype(np.int32))
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    ws = torch.zeros(gkv.kept_workspace_bytes(B, Hkv, LONG), dtype=torch.uint8, device="cuda")
+
+    def attention(view):
+        res = []
+        for bound in (600, LONG):
+            out = torch.zeros(B, Hq * D, device="cuda")
+            gkv.kept_decode(qkv[:B], Hq, dev(lens), bound, view, out, cos_tab=cos, sin_tab=sin, workspace=ws,
+                            dev_err=err)
+            res.append(out)
+        out = torch.zeros(6, Hq * D, device="cuda")
+        gkv.kept_prefill(dev(np.array([0, 3, 6], np.int32)), 3, qkv[:6], Hq, view, out,
+                         start_pos=dev(np.array([496, 288], np.int32)), cos_tab=cos, sin_tab=sin, dev_err=err)
+        return res + [out]
+
+    got = []
+    for view, *_ in pools:
+        # (the first sequence's older tokens in a call of their own: a block is continued)
+        gkv.kept_append(qkv[:115], Hq, cos, sin, dev(np.array([115, 0], np.int32)), view, max_rows=115,
+                        cu_seqlens=dev(np.array([0, 115, 115], np.int32)), dev_err=err)
+        gkv.kept_append(qkv, Hq, cos, sin, dev(lens), view, max_rows=400, cu_seqlens=cu, dev_err=err)
+        got.append(attention(view))
+    assert all(torch.equal(x, y) for x, y in zip(*got)) and all(torch.isfinite(x).all() for x in got[0])
+    # far blocks to near places of the same pool
+    view, _, _, _, table = pools[1]
+    near = dev(ids.reshape(-1))
+    gkv.copy_blocks([view], table.reshape(-1), near, dev_err=err)
+    view.block_table = near.data_ptr()
+    assert all(torch.equal(x, y) for x, y in zip(got[0], attention(view)))
+    assert int(err.item()) == 0
+
+
+@pytest.mark.parametrize("fmt", [BF16, BLOCK])
+def test_two_streams_with_workspaces_of_their_own(gkv, cuda, fmt):
+    lay = Layout(0, 0, False)
+    c = Cache([5000, 900, 2600], 2, lay, fmt)
+    view = c.device(gkv)
+    g = torch.Generator(device="cuda").manual_seed(6)
+    q = [torch.randn(3, 4 * D, generator=g, device="cuda") for _ in range(2)]
+    lens = [dev(np.array(x, np.int32)) for x in ([5000, 900, 2600], [3000, 1, 2599])]
+    ws = [torch.zeros(gkv.kept_workspace_bytes(3, 2, LONG), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    out = [torch.zeros(3, 4 * D, device="cuda") for _ in range(4)]
+    for i in range(2):
+        gkv.kept_decode(q[i], 4, lens[i], LONG, view, out[i], workspace=ws[i], dev_err=c.err)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            gkv.kept_decode(q[i], 4, lens[i], LONG, view, out[2 + i], workspace=ws[i], dev_err=c.err, stream=s)
+    torch.cuda.synchronize()
+    assert torch.equal(out[0], out[2]) and torch.equal(out[1], out[3]) and int(c.err.item()) == 0
+
+
+@pytest.mark.parametrize("fmt", [BF16, BLOCK])
+def test_captured_ranges_share_a_workspace_in_order(gkv, cuda, fmt):
+    """Two captured calls of one workspace, replayed in turn with lengths that change."""
+    c = Cache([4000, 900], 1, Layout(0, 0, False), fmt)
+    view = c.device(gkv)
+    q = torch.randn(2, 4 * D, generator=torch.Generator(device="cuda").manual_seed(7), device="cuda")
+    now = torch.zeros(2, dtype=torch.int32, device="cuda")
+    ws = torch.zeros(gkv.kept_workspace_bytes(2, 1, LONG), dtype=torch.uint8, device="cuda")
+    outs = [torch.zeros(2, 4 * D, device="cuda") for _ in range(3)]
+
+    def call(i):
+        gkv.kept_decode(qs[i], 4, now, LONG, view, outs[i], workspace=ws, dev_err=c.err)
+
+    qs = [q, q * 0.5]
+    call(0)
+    torch.cuda.synchronize()
+    graphs = []
+    for i in range(2):
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            call(i)
+        graphs.append(graph)
+    for lens in ([4000, 900], [1, 0], [2500, 64], [0, 0]):
+        now.copy_(dev(np.array(lens, np.int32)))
+        for i in (0, 1, 0):
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            got = outs[i].clone()
+            gkv.kept_decode(qs[i], 4, now, LONG, view, outs[2], workspace=ws, dev_err=c.err)
+            assert torch.equal(got, outs[2])
+    assert int(c.err.item()) == 0

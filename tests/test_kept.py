@@ -89,8 +89,8 @@ def test_nothing_to_do(gkv):
     (dict(stride=64 * 64 - 4), "ARG"), (dict(stride=64 * 64 + 2), "ARG"), (dict(out_stride=64 * 64 - 4), "ARG"),
     (dict(out_stride=64 * 64 + 2), "ARG"), (dict(q=FAKE + 4), "ARG"), (dict(out=FAKE + 8), "ARG"),
     (dict(out=FAKE + 4, dtype=1), "ARG"), (dict(hq=72), "UNSUPPORTED"),
-    (dict(max_len=2000, ws=None), "WORKSPACE"), (dict(max_len=2000, ws_bytes=1000), "WORKSPACE"),
-    (dict(max_len=2000, ws=FAKE + 8), "ARG"), (dict(B=1 << 30, max_len=1 << 20), "UNSUPPORTED")])
+    (dict(max_len=20000, ws=None), "WORKSPACE"), (dict(max_len=20000, ws_bytes=1000), "WORKSPACE"),
+    (dict(max_len=20000, ws=FAKE + 8), "ARG"), (dict(B=1 << 30, max_len=1 << 20), "UNSUPPORTED")])
 def test_decode_refusals(gkv, bad, why):
     assert decode(gkv, **bad) == getattr(gkv, "GKV_ERR_" + why)
 
