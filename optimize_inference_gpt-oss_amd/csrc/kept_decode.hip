@@ -15,7 +15,9 @@
 // stream costs no scale loads per token. Against codes q is split into fp16 pieces
 // (e4m3 values are fp16 values; 22 bits of q, scaled by a power of two per head so
 // that no range is lost), against bf16 K into bf16 pieces (16 bits); p always into
-// bf16 pieces (its range is that of exp2).
+// bf16 pieces (its range is that of exp2). Two bf16 pieces leave up to 2^-18 of a
+// value, 2^-9 of a bf16 output's own rounding; an fp32 output takes three, the
+// third through matrix ops of its own (FINE).
 //
 // A step is two blocks (32 tokens). A wave takes the steps of one (sequence, kv
 // head), loads the next step's blocks while it computes this one's, and leaves it
@@ -146,8 +148,8 @@ typedef const __attribute__((address_space(4))) int32_t *ScalarI32;
 typedef const __attribute__((address_space(4))) f32x2 *ScalarF2;
 
 // Steps s0 .. s1 - 1 of sequence b for kv head g, by one wave. R: steps of data in
-// registers.
-template <bool BLK, int R>
+// registers. FINE: three bf16 pieces where two would do for a bf16 output.
+template <bool BLK, int R, bool FINE>
 __device__ __forceinline__ State attend(const KeptDecodeArgs &a, int b, int g, const Span &sp,
                                         int s0, int s1) {
   constexpr int D = kHeadDim;
@@ -267,7 +269,7 @@ __device__ __forceinline__ State attend(const KeptDecodeArgs &a, int b, int g, c
       qb[i] *= qf;
     }
   }
-  u32x4 q0, q1;
+  u32x4 q0, q1, q2, q3; // (q2, q3: the third pieces, bf16 K and FINE)
   {
     typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
     if (BLK) {
@@ -290,9 +292,24 @@ __device__ __forceinline__ State attend(const KeptDecodeArgs &a, int b, int g, c
       }
       q0 = __builtin_bit_cast(u32x4, x);
       q1 = __builtin_bit_cast(u32x4, y);
+      if (FINE) {
+        auto third = [&](float f) {
+          const __bf16 h = (__bf16)f;
+          const float r = f - (float)h;
+          const __bf16 m = (__bf16)r;
+          return low ? (__bf16)0.0f : (__bf16)(r - (float)m);
+        };
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          x[i] = third(qa[i]);
+          y[i] = third(qb[i]);
+        }
+        q2 = __builtin_bit_cast(u32x4, x);
+        q3 = __builtin_bit_cast(u32x4, y);
+      }
     }
     if (!head_ok)
-      q0 = q1 = u32x4{0, 0, 0, 0};
+      q0 = q1 = q2 = q3 = u32x4{0, 0, 0, 0};
   }
 
   State st;
@@ -327,6 +344,12 @@ __device__ __forceinline__ State attend(const KeptDecodeArgs &a, int b, int g, c
                                                          __builtin_bit_cast(bf16x8, q0), acc[j], 0, 0, 0);
         acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x.k[2 * j + 1]),
                                                          __builtin_bit_cast(bf16x8, q1), acc[j], 0, 0, 0);
+        if (FINE) {
+          acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x.k[2 * j]),
+                                                           __builtin_bit_cast(bf16x8, q2), acc[j], 0, 0, 0);
+          acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, x.k[2 * j + 1]),
+                                                           __builtin_bit_cast(bf16x8, q3), acc[j], 0, 0, 0);
+        }
       }
     }
     float t[4];
@@ -402,16 +425,23 @@ __device__ __forceinline__ State attend(const KeptDecodeArgs &a, int b, int g, c
     }
     // p in bf16 and what that leaves, for the 4 tokens; the columns below 8 need
     // the first of both blocks, those above the second
-    uint32_t hi[2], lo[2], w0[2], w1[2];
+    uint32_t hi[2], lo[2], w0[2], w1[2], t0[2], t1[2];
 #pragma unroll
     for (int k = 0; k < 2; k++) {
       const float x0 = p[2 * k], x1 = p[2 * k + 1];
       hi[k] = f32x2_to_bf16_rne(x0, x1);
-      lo[k] = f32x2_to_bf16_rne(x0 - __uint_as_float(hi[k] << 16),
-                                x1 - __uint_as_float(hi[k] & 0xffff0000u));
+      const float r0 = x0 - __uint_as_float(hi[k] << 16), r1 = x1 - __uint_as_float(hi[k] & 0xffff0000u);
+      lo[k] = f32x2_to_bf16_rne(r0, r1);
       const uint32_t got = __float_as_uint(swap8(__uint_as_float(low ? hi[k] : lo[k])));
       w0[k] = low ? got : hi[k];
       w1[k] = low ? lo[k] : got;
+      if (FINE) { // the third of both blocks in the columns below 8
+        const uint32_t th = f32x2_to_bf16_rne(r0 - __uint_as_float(lo[k] << 16),
+                                              r1 - __uint_as_float(lo[k] & 0xffff0000u));
+        const uint32_t from = __float_as_uint(swap8(__uint_as_float(th)));
+        t0[k] = low ? 0 : th;
+        t1[k] = low ? 0 : from;
+      }
     }
     const bf16x8 pw = __builtin_bit_cast(bf16x8, u32x4{w0[0], w0[1], w1[0], w1[1]});
 #pragma unroll
@@ -428,6 +458,10 @@ __device__ __forceinline__ State attend(const KeptDecodeArgs &a, int b, int g, c
       }
       st.o[nn] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w), pw,
                                                          st.o[nn], 0, 0, 0);
+      if (FINE)
+        st.o[nn] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            __builtin_bit_cast(bf16x8, w), __builtin_bit_cast(bf16x8, u32x4{t0[0], t0[1], t1[0], t1[1]}),
+            st.o[nn], 0, 0, 0);
     }
   };
 
@@ -489,7 +523,7 @@ __device__ __forceinline__ void put_zeros(const KeptDecodeArgs &a, int64_t at, i
 
 // ---- whole: one workgroup holds every step of its (sequence, kv head)s --------------
 
-template <bool BLK, int R, int WPE>
+template <bool BLK, int R, int WPE, bool FINE>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(WPE)))
 void kept_decode_whole_kernel(KeptDecodeArgs a) {
   __shared__ float s_o[8][kPieceFloats];
@@ -515,7 +549,7 @@ void kept_decode_whole_kernel(KeptDecodeArgs a) {
   if (ok) {
     const int s0 = part * n / a.parts, s1 = (part + 1) * n / a.parts;
     if (s0 < s1) {
-      st = attend<BLK, R>(a, b, g, sp, s0, s1);
+      st = attend<BLK, R, FINE>(a, b, g, sp, s0, s1);
     } else {
       st.m = kLowest;
       st.l = 0.0f;
@@ -572,7 +606,7 @@ __device__ __forceinline__ int range_of(int p, int T, int n) {
   return (int)(((int64_t)(p + 1) * n - 1) / T);
 }
 
-template <bool BLK, int R, int WPE>
+template <bool BLK, int R, int WPE, bool FINE>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(WPE)))
 void kept_decode_split_kernel(KeptDecodeArgs a) {
   __shared__ int s_wave[8];
@@ -646,7 +680,7 @@ void kept_decode_split_kernel(KeptDecodeArgs a) {
     const int m = span_steps(sp);
     const int s0 = max(rs - cb, 0), s1 = min(re - cb, m);
     if (s0 < s1) {
-      const State st = attend<BLK, R>(a, b, g, sp, s0, s1);
+      const State st = attend<BLK, R, FINE>(a, b, g, sp, s0, s1);
       if (s0 == 0 && s1 == m) {
         put_whole(a, b, g, st);
       } else {
@@ -996,10 +1030,14 @@ extern "C" int gkv_kept_decode(void *stream, int32_t B, int32_t n_q_heads, const
     a.heads_per_wg = std::min(8 / a.parts, a.n_kv_heads);
     const dim3 grid((unsigned)((int64_t)B * ((a.n_kv_heads + a.heads_per_wg - 1) / a.heads_per_wg)));
     const dim3 block(64 * a.parts * a.heads_per_wg);
-    if (blk)
-      hipLaunchKernelGGL((kept_decode_whole_kernel<true, 2, 4>), grid, block, 0, s, a);
+    if (blk && a.out_bf16)
+      hipLaunchKernelGGL((kept_decode_whole_kernel<true, 2, 4, false>), grid, block, 0, s, a);
+    else if (blk)
+      hipLaunchKernelGGL((kept_decode_whole_kernel<true, 2, 4, true>), grid, block, 0, s, a);
+    else if (a.out_bf16)
+      hipLaunchKernelGGL((kept_decode_whole_kernel<false, 2, 4, false>), grid, block, 0, s, a);
     else
-      hipLaunchKernelGGL((kept_decode_whole_kernel<false, 2, 4>), grid, block, 0, s, a);
+      hipLaunchKernelGGL((kept_decode_whole_kernel<false, 2, 4, true>), grid, block, 0, s, a);
     return launch_status("kept_decode_whole_kernel");
   }
   const KeptWorkspace w = kept_workspace(a.n_kv_heads);
@@ -1015,10 +1053,14 @@ extern "C" int gkv_kept_decode(void *stream, int32_t B, int32_t n_q_heads, const
   a.ws_ml = (float *)((char *)workspace + w.ml);
   a.ws_o = (float *)((char *)workspace + w.o);
   const dim3 block(64 * subs * a.n_kv_heads);
-  if (blk)
-    hipLaunchKernelGGL((kept_decode_split_kernel<true, 2, 2>), dim3(kSplitWgs), block, 0, s, a);
+  if (blk && a.out_bf16)
+    hipLaunchKernelGGL((kept_decode_split_kernel<true, 2, 2, false>), dim3(kSplitWgs), block, 0, s, a);
+  else if (blk)
+    hipLaunchKernelGGL((kept_decode_split_kernel<true, 2, 2, true>), dim3(kSplitWgs), block, 0, s, a);
+  else if (a.out_bf16)
+    hipLaunchKernelGGL((kept_decode_split_kernel<false, 2, 2, false>), dim3(kSplitWgs), block, 0, s, a);
   else
-    hipLaunchKernelGGL((kept_decode_split_kernel<false, 2, 2>), dim3(kSplitWgs), block, 0, s, a);
+    hipLaunchKernelGGL((kept_decode_split_kernel<false, 2, 2, true>), dim3(kSplitWgs), block, 0, s, a);
   if ((st = launch_status("kept_decode_split_kernel")))
     return st;
   hipLaunchKernelGGL(kept_decode_merge_kernel, dim3((unsigned)a.max_ranges), dim3(kMergeThreads), 0, s,

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from keptcase import BF16, BLOCK, D, Cache, Layout
+from keptcase import BF16, BLOCK, D, Cache, Layout, attend
 from oracle import kv_oracle as O
 from test_gpu_kept import dev, run_decode, run_prefill
 
@@ -227,3 +227,25 @@ def test_captured_ranges_share_a_workspace_in_order(gkv, cuda, fmt):
             gkv.kept_decode(qs[i], 4, now, LONG, view, outs[2], workspace=ws, dev_err=c.err)
             assert torch.equal(got, outs[2])
     assert int(c.err.item()) == 0
+
+
+@pytest.mark.parametrize("max_len", [64, LONG])
+@pytest.mark.parametrize("fmt", [BF16, BLOCK])
+def test_fp32_outputs_keep_more_than_two_bf16_pieces(gkv, cuda, fmt, max_len):
+    """Two positions, scores near 0. In units of 2^-24: the scores' sums 70 of sum |q k|, their
+    exponent's argument 1, exp2 and its place in both sums 4, the sum 2, six products and
+    their sums 8, joining the pieces 1, the quotient and its product 2, q's pieces below
+    these: 24 with the rest. Two bf16 pieces of a weight leave up to 2^-18 of it."""
+    lay = Layout(0, 0, False)
+    c = Cache([2] * 40, 2, lay, fmt, seed=9)
+    view = c.device(gkv)
+    q = (np.random.default_rng(9).standard_normal((40, 16, D)) / 256).astype(np.float32)
+    out = torch.zeros(40, 16 * D, device="cuda")
+    ws = torch.zeros(max(16, gkv.kept_workspace_bytes(40, 2, max_len)), dtype=torch.uint8, device="cuda")
+    gkv.kept_decode(dev(q.reshape(40, -1)), 16, dev(np.full(40, 2, np.int32)), max_len, view, out, workspace=ws,
+                    dev_err=c.err)
+    got = out.cpu().numpy().reshape(40, 16, D)
+    for b in range(40):
+        want, pav, qk = attend(q[b:b + 1].astype(np.float64), *c.kv[b], np.ones((1, 2), bool), None)
+        bound = pav * (2 * qk * 70 + 24) * 2.0 ** -24
+        assert (np.abs(got[b] - want[0]) <= bound[0]).all()
