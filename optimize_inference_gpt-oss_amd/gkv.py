@@ -234,9 +234,11 @@ def hip_memcpy_d2d(dst: int, src: int, nbytes: int) -> None:
 
 
 def stream_handle(stream=None) -> int | None:
+    if stream is not None:
+        return stream.cuda_stream
     import torch
-    s = stream if stream is not None else torch.cuda.current_stream()
-    return s.cuda_stream
+    # the handle of torch.cuda.current_stream(), without the 2.5 us of making its object
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def rope_table(n_pos: int, **overrides):

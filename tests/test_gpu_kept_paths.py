@@ -249,3 +249,11 @@ def test_fp32_outputs_keep_more_than_two_bf16_pieces(gkv, cuda, fmt, max_len):
         want, pav, qk = attend(q[b:b + 1].astype(np.float64), *c.kv[b], np.ones((1, 2), bool), None)
         bound = pav * (2 * qk * 70 + 24) * 2.0 ** -24
         assert (np.abs(got[b] - want[0]) <= bound[0]).all()
+
+
+def test_calls_go_to_the_current_stream(gkv, cuda):
+    s = torch.cuda.Stream()
+    assert gkv.stream_handle() == torch.cuda.current_stream().cuda_stream
+    with torch.cuda.stream(s):
+        assert gkv.stream_handle() == s.cuda_stream
+    assert gkv.stream_handle(s) == s.cuda_stream
