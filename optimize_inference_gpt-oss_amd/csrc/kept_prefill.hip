@@ -389,18 +389,24 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
       if (wave + i * n_waves < 8)
         fetch(pc[i], 0, wave + i * n_waves, ids0[i]);
     __builtin_amdgcn_sched_barrier(0);
+    if (a.cos_tab) {
+      // x cos -/+ other sin: the sine's sign bit is flipped below c = 8, so that both
+      // halves run the same instructions (and round as rope_first and rope_second do)
+      const uint32_t flip = c < 8 ? 0x80000000u : 0u;
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const float x = y[i][k], sine = __uint_as_float(__float_as_uint(sn[i][k]) ^ flip);
+          y[i][k] = rope_second(swap8(x), x, cs[i][k], sine);
+        }
+    }
 #pragma unroll
     for (int i = 0; i < 8; i++) {
       float mx = 0.0f;
 #pragma unroll
-      for (int k = 0; k < 4; k++) {
-        if (a.cos_tab) {
-          const float x = y[i][k], other = swap8(x);
-          y[i][k] = c < 8 ? rope_first(x, other, cs[i][k], sn[i][k])
-                          : rope_second(other, x, cs[i][k], sn[i][k]);
-        }
+      for (int k = 0; k < 4; k++)
         mx = fmaxf(mx, fabsf(y[i][k]));
-      }
       // the row's largest element, over its 16 lanes
       mx = fmaxf(mx, swap8(mx));
       mx = fmaxf(mx, row_rotate<4>(mx));
@@ -460,6 +466,9 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
 #pragma unroll
       for (int i = 0; i < 16; i++)
         acc[i] = 0.0f;
+      // a wave in its step goes before those that stage (8 chunks after 1536 cached
+      // tokens 162 -> 156 us)
+      __builtin_amdgcn_s_setprio(1);
       const uint16_t *krow = s_kv[buf][0] + 32 * s * kPRow + operand;
 #pragma unroll
       for (int kk = 0; kk < 4; kk++) {
@@ -535,6 +544,7 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
           o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vop, p[ks], o[dt], 0, 0, 0);
         }
       }
+      __builtin_amdgcn_s_setprio(0);
     }
     if (t + 1 < n_tiles) {
 #pragma unroll
