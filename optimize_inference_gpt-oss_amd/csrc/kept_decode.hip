@@ -42,7 +42,6 @@
 namespace gkv {
 
 constexpr int kKeptAux = 2;            // nontemporal: each K/V byte is read once
-constexpr int kKeptStep = 32;          // tokens per step
 constexpr int kHeads = 8;              // query heads per kv head, at most
 // Range workgroups: one per CU, two waves a SIMD. Two per CU make twice the pieces
 // and shorter ranges (us, 256 / 512 workgroups: 32 sequences of 129 .. 16384

@@ -39,6 +39,9 @@
 // per workgroup. Kept positions' tiles come first, then the window's; blocks that
 // no query of the workgroup sees are not read.
 //
+// Few workgroups (at most one per CU): sixteen waves, two groups of eight that take
+// the tiles in turn with LDS buffers of their own and join their sums at the end.
+//
 // Running maximum as in the decode: it moves only when a lane's weights sum to
 // more than 2^8 (or to a NaN), the weights are then formed again.
 #include "kept.hpp"
@@ -57,6 +60,14 @@ constexpr int kPQueries = 32;           // queries per wave
 constexpr float kPVScale = 0x1p-10f;    // V is staged as fp16 of v * kPVScale
 constexpr float kPQScale = 0.125f * kLog2e;
 constexpr float kPLowest = -1e30f;      // the running maximum before any score (log2 units)
+// Grids of at most one workgroup per CU get two groups of waves a workgroup: a CU's
+// SIMDs then hold four waves, as with two workgroups. Where two fit, a second group only
+// takes the other's place, and a single tile cannot be split. Measured (us, one group /
+// two, 8 kv heads, codes): one prompt of 32 rows 9.6 / 10.2, of 200 13.3 / 12.8, of 1024
+// 38.5 / 32.6; 512 rows after 30000 738 / 591; 8 chunks of up to 128 after 2048 with a
+// window of 256 19.8 / 18.5; 416 workgroups (2 of up to 800 after 4096) 171 / 187.
+constexpr int64_t kPFewWgs = 256;
+constexpr int kPShort = 128; // rows of a prompt without a history that stay with one group
 constexpr int kPBand = 2;               // query blocks per band of the grid order
 
 struct KeptPrefillArgs {
@@ -100,14 +111,15 @@ __device__ __forceinline__ float row_rotate(float x) {
   return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), 0x120 + N, 0xf, 0xf, false));
 }
 
-// TASKS: pieces a wave fetches of each tile (1 with eight waves, else 2).
-template <int TASKS>
-__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(TASKS == 1 ? 4 : 2)))
+// TASKS: pieces a wave fetches of each tile (1 with eight waves, else 2). GROUPS:
+// groups of eight waves that take the tiles in turn (2: TASKS is 1).
+template <int TASKS, int GROUPS>
+__global__ __launch_bounds__(512 * GROUPS) __attribute__((amdgpu_waves_per_eu(TASKS == 1 ? 4 : 2)))
 void kept_prefill_kernel(KeptPrefillArgs a) {
   constexpr int D = kHeadDim;
-  __shared__ __attribute__((aligned(16))) uint16_t s_kv[2][2][kPTile * kPRow]; // [buffer][K, V]
+  __shared__ __attribute__((aligned(16))) uint16_t s_kv_all[GROUPS][2][2][kPTile * kPRow]; // [][buffer][K, V]
   __shared__ __attribute__((aligned(16))) uint16_t s_q[8][kPQueries * kPRow]; // a wave's rows: q, then the output
-  __shared__ float s_ks[2][4]; // K scale of each block of a tile
+  __shared__ float s_ks_all[GROUPS][2][4]; // K scale of each block of a tile
 
   // Grid order: kv head fastest (the workgroups of a head on one XCD share its
   // K/V in that L2), bands of query blocks longest first, a prompt's blocks of a band
@@ -124,7 +136,10 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
   const int qn = kPQueries * a.subs, q0 = qb * qn; // the block's queries
   if (q0 >= L)
     return;
-  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int group = GROUPS > 1 ? uniform(tid >> 9) : 0, wave = uniform((tid >> 6) & 7);
+  auto &s_kv = s_kv_all[group];
+  auto &s_ks = s_ks_all[group];
   const int n = lane & 31, h = lane >> 5;
   int start = a.start ? uniform(a.start[b]) : 0;
   if (start < 0 || start % kBlockTokens != 0) {
@@ -351,8 +366,8 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
     const int task = wave + i * n_waves;
     ids0[i] = ids[i] = kNone;
     if (task < 8) {
-      ids0[i] = id_of(0, task);
-      ids[i] = id_of(1, task);
+      ids0[i] = id_of(group, task);
+      ids[i] = id_of(group + GROUPS, task);
     }
   }
 
@@ -371,10 +386,12 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
   float qf; // what the scores of this lane's query are to be multiplied with
   {
     const int r4 = lane >> 4, c = lane & 15;
-    f32x4 y[8], cs[8], sn[8];
+    constexpr int kRows = 8 / GROUPS; // quads of rows (the groups share a wave's rows)
+    const int i0 = kRows * group;
+    f32x4 y[kRows], cs[kRows], sn[kRows];
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const int j = min(q0 + kPQueries * sub + 4 * i + r4, L - 1);
+    for (int i = 0; i < kRows; i++) {
+      const int j = min(q0 + kPQueries * sub + 4 * (i0 + i) + r4, L - 1);
       y[i] = *(const f32x4 *)(a.q + (int64_t)(row0 + j) * a.q_stride + head * D + 4 * c);
       if (a.cos_tab) {
         const int64_t at = (int64_t)min(start + j, cap - 1) * (D / 2) + 4 * (c & 7);
@@ -387,14 +404,14 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
 #pragma unroll
     for (int i = 0; i < TASKS; i++)
       if (wave + i * n_waves < 8)
-        fetch(pc[i], 0, wave + i * n_waves, ids0[i]);
+        fetch(pc[i], group, wave + i * n_waves, ids0[i]);
     __builtin_amdgcn_sched_barrier(0);
     if (a.cos_tab) {
       // x cos -/+ other sin: the sine's sign bit is flipped below c = 8, so that both
       // halves run the same instructions (and round as rope_first and rope_second do)
       const uint32_t flip = c < 8 ? 0x80000000u : 0u;
 #pragma unroll
-      for (int i = 0; i < 8; i++)
+      for (int i = 0; i < kRows; i++)
 #pragma unroll
         for (int k = 0; k < 4; k++) {
           const float x = y[i][k], sine = __uint_as_float(__float_as_uint(sn[i][k]) ^ flip);
@@ -402,7 +419,7 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
         }
     }
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
+    for (int i = 0; i < kRows; i++) {
       float mx = 0.0f;
 #pragma unroll
       for (int k = 0; k < 4; k++)
@@ -415,13 +432,16 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
       // q * 2^-e, its largest element in [1, 2)
       const int e = min(max((int)(__float_as_uint(mx) >> 23), 27), 227);
       const float down = __uint_as_float((uint32_t)(254 - e) << 23);
-      *(u32x2 *)(sq + (4 * i + r4) * kPRow + 4 * c) =
+      *(u32x2 *)(sq + (4 * (i0 + i) + r4) * kPRow + 4 * c) =
           u32x2{f16_pair(y[i][0] * down, y[i][1] * down), f16_pair(y[i][2] * down, y[i][3] * down)};
       if (c == 0)
-        *(float *)(sq + (4 * i + r4) * kPRow + D) =
+        *(float *)(sq + (4 * (i0 + i) + r4) * kPRow + D) =
             kPQScale * __uint_as_float((uint32_t)e << 23); // (in the row's padding)
     }
-    __builtin_amdgcn_wave_barrier();
+    if (GROUPS > 1)
+      lds_barrier();
+    else
+      __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int kk = 0; kk < 4; kk++)
       qv[kk] = *(const f16x8 *)(sq + n * kPRow + 8 * h + 16 * kk);
@@ -445,14 +465,13 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
   // [key_begin, key_end] or below kept; up to window_end some query has left them behind
   const int key_end = active ? p_last_s : -1, key_begin = W > 0 ? max(p0s - W, INT_MIN + 30) - 30 : INT_MIN;
   const int window_end = W > 0 ? p_last_s - W : INT_MIN;
-  for (int t = 0; t < n_tiles; t++) {
-    const int buf = t & 1;
+  for (int t = group, buf = 0; t - group < n_tiles; t += GROUPS, buf ^= 1) {
 #pragma unroll
     for (int i = 0; i < TASKS; i++) {
       const int task = wave + i * n_waves;
-      if (task < 8 && t + 1 < n_tiles) {
-        fetch(pc[i], t + 1, task, ids[i]);
-        ids[i] = id_of(t + 2, task);
+      if (task < 8 && t + GROUPS < n_tiles) {
+        fetch(pc[i], t + GROUPS, task, ids[i]);
+        ids[i] = id_of(t + 2 * GROUPS, task);
       }
     }
     __builtin_amdgcn_sched_barrier(0); // (the loads stay in front of the compute)
@@ -460,7 +479,7 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
 #pragma unroll
     for (int s = 0; s < 2; s++) {
       const int kb = kt + 32 * s;
-      if (kb > key_end || (kb < key_begin && kb >= kept))
+      if ((GROUPS > 1 && t >= n_tiles) || kb > key_end || (kb < key_begin && kb >= kept))
         continue; // nothing of the step is seen
       f32x16 acc;
 #pragma unroll
@@ -546,10 +565,10 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
       }
       __builtin_amdgcn_s_setprio(0);
     }
-    if (t + 1 < n_tiles) {
+    if (t - group + GROUPS < n_tiles) { // (the same for both groups)
 #pragma unroll
       for (int i = 0; i < TASKS; i++)
-        if (wave + i * n_waves < 8)
+        if (wave + i * n_waves < 8 && t + GROUPS < n_tiles)
           store(pc[i], buf ^ 1, wave + i * n_waves);
       lds_barrier();
     }
@@ -557,6 +576,34 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
   if (a.dev_err) {
     if ((bad || range) && lane == 0)
       atomicOr(a.dev_err, (bad ? GKV_DEVERR_BLOCK_ID : 0u) | (range ? GKV_DEVERR_RANGE : 0u));
+  }
+
+  if (GROUPS > 1) {
+    // the second group's sums to the first, through the tiles' place
+    static_assert(GROUPS == 1 || 8 * 34 * 64 * 4 <= sizeof(s_kv_all), "a group's sums fit");
+    float *sums = (float *)s_kv_all + wave * 34 * 64 + lane;
+    lds_barrier();
+    if (group == 1) {
+      sums[0] = m;
+      sums[64] = l;
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        sums[64 * (2 + i)] = o[0][i];
+        sums[64 * (18 + i)] = o[1][i];
+      }
+    }
+    lds_barrier();
+    if (group == 1)
+      return;
+    const float m1 = sums[0], mm = fmaxf(m, m1);
+    const float f0 = __builtin_amdgcn_exp2f(m - mm), f1 = __builtin_amdgcn_exp2f(m1 - mm);
+    m = mm;
+    l = fmaf(sums[64], f1, l * f0);
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      o[0][i] = fmaf(sums[64 * (2 + i)], f1, o[0][i] * f0);
+      o[1][i] = fmaf(sums[64 * (18 + i)], f1, o[1][i] * f0);
+    }
   }
 
   // out = o / (l + sink's weight) / kPVScale; 0 for a row that saw nothing
@@ -680,9 +727,11 @@ extern "C" int gkv_kept_prefill(void *stream, int32_t B, const int32_t *cu_seqle
   a.out_bf16 = out_dtype == GKV_BF16;
   a.dev_err = dev_err;
   const dim3 block(64 * G * a.subs);
-  if (G * a.subs == 8)
-    hipLaunchKernelGGL((kept_prefill_kernel<1>), dim3((unsigned)grid), block, 0, (hipStream_t)stream, a);
+  if (G * a.subs == 8 && grid <= kPFewWgs && (start_pos || max_len > kPShort))
+    hipLaunchKernelGGL((kept_prefill_kernel<1, 2>), dim3((unsigned)grid), dim3(1024), 0, (hipStream_t)stream, a);
+  else if (G * a.subs == 8)
+    hipLaunchKernelGGL((kept_prefill_kernel<1, 1>), dim3((unsigned)grid), block, 0, (hipStream_t)stream, a);
   else
-    hipLaunchKernelGGL((kept_prefill_kernel<2>), dim3((unsigned)grid), block, 0, (hipStream_t)stream, a);
+    hipLaunchKernelGGL((kept_prefill_kernel<2, 1>), dim3((unsigned)grid), block, 0, (hipStream_t)stream, a);
   return launch_status("kept_prefill_kernel");
 }

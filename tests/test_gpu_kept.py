@@ -314,7 +314,7 @@ def test_decode_bad_pages_and_long_lengths(gkv, cuda):
 
 
 def run_prefill(gkv, starts, rows, Hq, Hkv, lay, fmt, sinks=True, bf16=False, seed=0, cached=True,
-                from_cache=False, spread=False, scale=1.0):
+                from_cache=False, spread=False, scale=1.0, max_len=None):
     c = Cache(np.asarray(starts) + (rows if from_cache else 0), Hkv, lay, fmt, seed=seed, spread=spread,
               scale=scale)
     last = np.asarray(starts) + rows - 1
@@ -331,7 +331,7 @@ def run_prefill(gkv, starts, rows, Hq, Hkv, lay, fmt, sinks=True, bf16=False, se
         view = gkv.CacheView(n_kv_heads=Hkv)
     out = torch.full((n, Hq * D), float("nan"), dtype=torch.bfloat16 if bf16 else torch.float32, device="cuda")
     cu = np.concatenate([[0], np.cumsum(rows)]).astype(np.int32)
-    gkv.kept_prefill(dev(cu), max(rows), dev(qkv), Hq, view, out,
+    gkv.kept_prefill(dev(cu), max_len or max(rows), dev(qkv), Hq, view, out,
                      start_pos=dev(np.asarray(starts, np.int32)) if cached else None,
                      k=None if from_cache else dev(kb.view(np.int16)),
                      v=None if from_cache else dev(vb.view(np.int16)),

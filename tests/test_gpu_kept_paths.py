@@ -57,6 +57,18 @@ def test_prefill_of_any_scales(gkv, cuda, fmt, kept, window, ring):
     run_prefill(gkv, [208, 16, 336], [70, 33, 5], 16, 2, Layout(kept, window, ring), fmt, spread=True, scale=0.125)
 
 
+@pytest.mark.parametrize("fmt", [BF16, BLOCK])
+@pytest.mark.parametrize("kept,window,ring", [(0, 0, False), (16, 32, True), (0, 16, True), (96, 48, True),
+                                              (32, 256, False)])
+@pytest.mark.parametrize("Hq,Hkv", [(16, 2), (4, 2), (4, 1)])
+@pytest.mark.parametrize("max_len", [130, 20000])
+def test_prefill_in_one_and_two_groups(gkv, cuda, fmt, kept, window, ring, Hq, Hkv, max_len):
+    """Few workgroups split their tiles between two groups of waves, many do not (the bound of
+    the lengths decides)."""
+    run_prefill(gkv, [0, 16, 208, 336, 48, 1024], [5, 33, 70, 16, 130, 40], Hq, Hkv, Layout(kept, window, ring), fmt,
+                sinks=Hq % 8 == 0, seed=kept, bf16=Hq == 4, max_len=max_len)
+
+
 HUGE = 2**31 - 16
 
 
