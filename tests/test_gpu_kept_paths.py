@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from keptcase import BF16, BLOCK, D, Cache, Layout, attend
+from keptcase import BF16, BLOCK, D, Cache, Layout, attend, decode_bound, prefill_bound
 from oracle import kv_oracle as O
 from test_gpu_kept import dev, run_decode, run_prefill
 
@@ -269,3 +269,56 @@ def test_calls_go_to_the_current_stream(gkv, cuda):
     with torch.cuda.stream(s):
         assert gkv.stream_handle() == s.cuda_stream
     assert gkv.stream_handle(s) == s.cuda_stream
+
+
+@pytest.mark.parametrize("fmt", [BF16, BLOCK])
+@pytest.mark.parametrize("max_len", [64, LONG])
+def test_far_more_sequences_than_workgroups(gkv, cuda, fmt, max_len):
+    """70001 sequences that read the same two blocks, every seventh of them empty."""
+    B = 70001
+    c = Cache([20], 1, Layout(0, 0, False), fmt, seed=3)
+    view = c.device(gkv)
+    table = c.dt[:, :2].repeat(B, 1).contiguous()
+    view.block_table, view.table_stride = table.data_ptr(), 2
+    q = torch.randn(1, 2 * D, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").repeat(B, 1)
+    lens = torch.full((B,), 20, dtype=torch.int32, device="cuda")
+    lens[::7] = 0
+    out = torch.full((B, 2 * D), 7.0, device="cuda")
+    ws = torch.zeros(max(16, gkv.kept_workspace_bytes(B, 1, max_len)), dtype=torch.uint8, device="cuda")
+    gkv.kept_decode(q, 2, lens, max_len, view, out, workspace=ws, dev_err=c.err)
+    assert int(c.err.item()) == 0
+    empty = lens == 0
+    assert (out[empty] == 0).all() and (out[~empty] == out[1]).all()
+    want, pav, qk = attend(q[:1].cpu().numpy().reshape(1, 2, D).astype(np.float64), *c.kv[0], np.ones((1, 20), bool), None)
+    assert (np.abs(out[1].cpu().numpy().reshape(2, D) - want[0]) <= decode_bound(want, pav, qk, fmt, False)[0]).all()
+
+
+@pytest.mark.parametrize("fmt", [BF16, BLOCK])
+@pytest.mark.parametrize("max_len", [3, 20000])
+def test_a_million_tokens(gkv, cuda, fmt, max_len):
+    """... of one block, which every table entry names: attention over that block. In the
+    prefill a lane's sums take 32768 steps, 2^-24 of themselves each; the rows' own keys are
+    zeros."""
+    n = 65536
+    c = Cache([16], 1, Layout(0, 0, False), fmt, seed=3)
+    view = c.device(gkv)
+    table = c.dt[:, :1].repeat(1, n + 1).contiguous()
+    view.block_table, view.table_stride = table.data_ptr(), n + 1
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q = torch.randn(3, 4 * D, generator=g, device="cuda")
+    k, v = c.kv[0]
+    want, pav, qk = attend(q.cpu().numpy().reshape(3, 4, D).astype(np.float64), k, v, np.ones((3, 16), bool), None)
+    out = torch.zeros(1, 4 * D, device="cuda")
+    ws = torch.zeros(gkv.kept_workspace_bytes(1, 1, 16 * n), dtype=torch.uint8, device="cuda")
+    gkv.kept_decode(q[:1], 4, dev(np.array([16 * n], np.int32)), 16 * n, view, out, workspace=ws, dev_err=c.err)
+    bound = decode_bound(want, pav, qk, fmt, False)
+    assert (np.abs(out.cpu().numpy().reshape(4, D) - want[0]) <= bound[0]).all()
+    out = torch.zeros(3, 4 * D, device="cuda")
+    zero = torch.zeros(3, D, dtype=torch.bfloat16, device="cuda")
+    gkv.kept_prefill(dev(np.array([0, 3], np.int32)), max_len, q, 4, view, out, start_pos=dev(np.array([16 * n], np.int32)),
+                     k=zero, v=zero, dev_err=c.err)
+    # (3 own keys of score 0 beside 2^20 of at least -max |score|)
+    top = np.abs(np.einsum("nhd,td->nht", q.cpu().numpy().reshape(3, 4, D).astype(np.float64), k[:, 0])).max() / 8
+    own = 3 * np.exp(top) / 2 ** 20
+    bound = prefill_bound(want, pav, qk, 16, np.abs(v).max(), False) + pav * (2 * 32768 * 2.0 ** -24) + np.abs(want) * own
+    assert (np.abs(out.cpu().numpy().reshape(3, 4, D) - want) <= bound).all() and int(c.err.item()) == 0
