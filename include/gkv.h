@@ -498,7 +498,8 @@ int gkv_kept_decode(void *stream, int32_t B, int32_t n_q_heads, const float *q, 
  * history (start_pos: multiples of 16), with gkv_prefill_paged's arguments and
  * rules: keys before start_pos[b] from the cache, those from there on from the
  * packed rows (k = v = NULL: from the cache too, ring = 0 only). On a ring,
- * append the chunk after this call. At most 8 query heads per kv head. q, k, v, out
+ * append the chunk after this call. The tokens of a block whose id lies outside the
+ * pool count for nothing (GKV_DEVERR_BLOCK_ID). At most 8 query heads per kv head. q, k, v, out
  * and the tables are 16-byte aligned, strides multiples of 4 (out_stride in bf16:
  * of 8). The matrix cores take fp16: q is rounded to 11 bits against its row's
  * largest element, so a score is off by at most 2^-11 sum |q k| / 8; a weight has 11

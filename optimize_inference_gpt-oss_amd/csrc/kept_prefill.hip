@@ -95,6 +95,7 @@ struct Piece {
   u32x4 x[2];
   float scale; // of codes
   bool hist;   // a block of the cache (else packed rows)
+  bool miss;   // ... that is not there, or that nobody sees
   int p;       // its first position
 };
 
@@ -119,7 +120,7 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
   constexpr int D = kHeadDim;
   __shared__ __attribute__((aligned(16))) uint16_t s_kv_all[GROUPS][2][2][kPTile * kPRow]; // [][buffer][K, V]
   __shared__ __attribute__((aligned(16))) uint16_t s_q[8][kPQueries * kPRow]; // a wave's rows: q, then the output
-  __shared__ float s_ks_all[GROUPS][2][4]; // K scale of each block of a tile
+  __shared__ float s_ks_all[GROUPS][2][4]; // K scale of each block of a tile, negative: it is not there
 
   // Grid order: kv head fastest (the workgroups of a head on one XCD share its
   // K/V in that L2), bands of query blocks longest first, a prompt's blocks of a band
@@ -212,10 +213,12 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
     x.p = tile_pos(t) + kBlockTokens * (task & 3);
     x.scale = 0.0f;
     x.hist = x.p < hist_end;
+    x.miss = false;
     if (x.hist) {
       GKV_KEEP_BRANCH;
       const bool ok = (uint32_t)id < (uint32_t)a.num_blocks;
       bad |= !ok && id != kNone;
+      x.miss = !ok;
       const int64_t hb = (int64_t)(ok ? id : 0) * a.n_kv_heads + g;
       const char *src = is_v ? a.vc : a.kc;
       if (a.scales) {
@@ -306,8 +309,9 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
       uint16_t *dst = s_kv[buf][0] + (kBlockTokens * blk + c16) * kPRow + 8 * kg;
       *(u32x4 *)dst = lo4;
       *(u32x4 *)(dst + 32) = hi4;
-      if (ln == 0)
-        s_ks[buf][blk] = codes ? x.scale : 1.0f;
+      if (ln == 0) {
+        s_ks[buf][blk] = x.miss ? -1.0f : codes ? x.scale : 1.0f;
+      }
       return;
     }
     // tokens 4kg .. 4kg+3 of dimension d at dst + d rows
@@ -495,8 +499,17 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
         acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kop, qv[kk], acc, 0, 0, 0);
       }
       const float c0 = qf * s_ks[buf][2 * s], c1 = qf * s_ks[buf][2 * s + 1];
-      if (kb > p0s - 31 || (kb <= window_end && kb + 31 >= kept)) {
+      const bool gone = __any(fminf(c0, c1) < 0.0f);
+      if (kb > p0s - 31 || (kb <= window_end && kb + 31 >= kept) || gone) {
         GKV_KEEP_BRANCH;
+        // a missing block's tokens count for nothing (their V is 0)
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+          if ((j ? c1 : c0) < 0.0f) {
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+              acc[8 * j + i] = -INFINITY;
+          }
         // key kb + 4 h + off is seen iff 0 <= last - off < W, or it is a kept one
         const int ln = opaque_lane(), h = ln >> 5, last = p0s + (ln & 31) - kb - 4 * h;
         const uint32_t wide = W > 0 ? (uint32_t)W : 0x80000000u;

@@ -322,3 +322,49 @@ def test_a_million_tokens(gkv, cuda, fmt, max_len):
     own = 3 * np.exp(top) / 2 ** 20
     bound = prefill_bound(want, pav, qk, 16, np.abs(v).max(), False) + pav * (2 * 32768 * 2.0 ** -24) + np.abs(want) * own
     assert (np.abs(out.cpu().numpy().reshape(3, 4, D) - want) <= bound).all() and int(c.err.item()) == 0
+
+
+@pytest.mark.parametrize("fmt", [BF16, BLOCK])
+@pytest.mark.parametrize("kept,window,ring", [(0, 0, False), (32, 64, False), (16, 128, True)])
+@pytest.mark.parametrize("max_len", [70, 20000])
+@pytest.mark.parametrize("Hq,Hkv", [(8, 1), (3, 1)])
+def test_prefill_masks_missing_blocks(gkv, cuda, fmt, kept, window, ring, max_len, Hq, Hkv):
+    """Blocks whose ids lie outside the pool are flagged, and their tokens count for nothing."""
+    lay = Layout(kept, window, ring)
+    starts, rows = [208, 64], [70, 40]
+    c = Cache(starts, Hkv, lay, fmt, seed=8)
+    gone = [np.zeros(s, bool) for s in starts]
+    for b, blocks in enumerate(([0, 5, 8, 9, 12], [1, 3])):
+        for j in blocks:
+            c.table[b, lay.entry(j)] = [-1, c.nb, 2**31 - 1][j % 3]
+        for j in range(starts[b] // 16):  # (on a ring a place is several blocks', the last one counts)
+            gone[b][16 * j:16 * j + 16] = lay.entry(j) in [lay.entry(i) for i in blocks]
+    view = c.device(gkv)
+    rng = np.random.default_rng(8)
+    q = rng.standard_normal((110, Hq, D)).astype(np.float32)
+    kv = [torch.from_numpy(rng.standard_normal((110, Hkv, D)).astype(np.float32)).bfloat16() for _ in "kv"]
+    out = torch.zeros(110, Hq * D, device="cuda")
+    cu = np.array([0, 70, 110], np.int32)
+    gkv.kept_prefill(dev(cu), max_len, dev(q.reshape(110, -1)), Hq, view, out, start_pos=dev(np.array(starts, np.int32)),
+                     k=kv[0].cuda(), v=kv[1].cuda(), kept=kept, window=window, dev_err=c.err)
+    assert int(c.err.item()) == gkv.DEVERR_BLOCK_ID
+    got = out.cpu().numpy().reshape(110, Hq, D)
+    for b in range(2):
+        r = slice(cu[b], cu[b + 1])
+        k, v = (np.concatenate([np.nan_to_num(x), y[r].double().numpy()]) for x, y in zip(c.kv[b], kv))
+        t = np.arange(len(k))
+        ok = np.stack([lay.sees(p, t) for p in range(starts[b], starts[b] + rows[b])])
+        ok[:, :starts[b]] &= ~gone[b]
+        want, pav, qk = attend(q[r].astype(np.float64), k, v, ok, None)
+        assert (np.abs(got[r] - want) <= prefill_bound(want, pav, qk, len(k), np.abs(v).max(), False)).all()
+
+
+def test_prefill_of_nothing_but_missing_blocks_is_zero(gkv, cuda):
+    c = Cache([80], 1, Layout(0, 0, False), BLOCK)
+    c.table[:] = -1
+    view = c.device(gkv)
+    for max_len in (40, 20000):
+        out = torch.full((40, 2 * D), 7.0, device="cuda")
+        gkv.kept_prefill(dev(np.array([0, 40], np.int32)), max_len, torch.ones(40, 2 * D, device="cuda"), 2, view, out,
+                         start_pos=dev(np.array([32], np.int32)), dev_err=c.err)
+        assert (out == 0).all() and int(c.err.item()) == gkv.DEVERR_BLOCK_ID
