@@ -5,9 +5,12 @@
 // and (window 0, or t < kept, or t > start + j - window). Positions before start come
 // from the cache, the others from the packed bf16 rows. 4 * 64 operations a
 // query head, row and position seen, against 256 bytes of K and V that 8 heads
-// and 32 rows or more share: bound by the vector instructions of the softmax (16
-// exponentials a lane and 32 x 32 scores, at a quarter of the rate of the 36 others)
-// beside 8 matrix ops of 32 cycles.
+// and 32 rows or more share: bound by the issue of vector and matrix instructions (32
+// keys a wave: 57 vector instructions, 16 of them exponentials, about 45 for
+// staging, queries and masks, and 8 matrix ops of 32 cycles). Counted for 8 chunks
+// after 1536 cached tokens (157 us): vector units busy 56% of the time, matrix units
+// 30%, LDS about 45%; what is left is the chain of one wave, which the three others
+// of its SIMD do not cover to the end.
 //
 // Work: one workgroup per (prompt, kv head, block of queries), eight waves (or
 // the largest multiple of the group's heads below): wave = (32 queries, query head),
