@@ -368,3 +368,10 @@ def test_prefill_of_nothing_but_missing_blocks_is_zero(gkv, cuda):
         gkv.kept_prefill(dev(np.array([0, 40], np.int32)), max_len, torch.ones(40, 2 * D, device="cuda"), 2, view, out,
                          start_pos=dev(np.array([32], np.int32)), dev_err=c.err)
         assert (out == 0).all() and int(c.err.item()) == gkv.DEVERR_BLOCK_ID
+
+
+@pytest.mark.parametrize("fmt", [BF16, BLOCK])
+@pytest.mark.parametrize("Hq,Hkv", [(40, 8), (6, 1), (14, 2), (64, 8)])
+@pytest.mark.parametrize("kept,window,ring", [(0, 0, False), (16, 64, True)])
+def test_prefill_of_all_group_sizes(gkv, cuda, fmt, Hq, Hkv, kept, window, ring):
+    run_prefill(gkv, [128, 0, 320], [33, 1, 48], Hq, Hkv, Layout(kept, window, ring), fmt, sinks=Hq % 4 == 0, seed=Hq)
