@@ -503,9 +503,11 @@ int gkv_kept_decode(void *stream, int32_t B, int32_t n_q_heads, const float *q, 
  * and the tables are 16-byte aligned, strides multiples of 4 (out_stride in bf16:
  * of 8). The matrix cores take fp16: q is rounded to 11 bits against its row's
  * largest element, so a score is off by at most 2^-11 sum |q k| / 8; a weight has 11
- * bits; bf16 K is exact for magnitudes 2^-14 .. 2^16, V for 2^-4 .. 2^26, with an
- * absolute error of at most 2^-25 and 2^-15 below that. Beyond, and where an
- * output is not finite: GKV_DEVERR_RANGE. */
+ * bits down to 2^-22 of the row's largest key's (15 nats; the sink's, in fp32, does
+ * not count), and is off by at most 2^-33 of that one's below; bf16 K is exact for
+ * magnitudes 2^-14 .. 2^16, V for 2^-4 .. 2^26, with an absolute error of at most
+ * 2^-25 and 2^-15 below that. Beyond, and where an output is not finite:
+ * GKV_DEVERR_RANGE. */
 int gkv_kept_prefill(void *stream, int32_t B, const int32_t *cu_seqlens, const int32_t *start_pos,
                      int32_t max_len, int32_t n_q_heads, const float *q, int64_t q_stride,
                      const float *cos_tab, const float *sin_tab, const void *k, const void *v,

@@ -22,7 +22,7 @@
 // fp16 values (below, an absolute error of 2^-25; beyond, flagged when staged). q and P
 // are rounded to fp16's 11 bits, q after a power of two that brings its row's
 // largest element into [1, 2): a score is off by at most 2^-11 sum |q k| / 8, a
-// weight by as much again as its own rounding, 2^-11; the bf16 output's is 2^-8
+// weight by its own rounding, 2^-11, beside it; the bf16 output's is 2^-8
 // (q in two bf16 pieces, 16 bits, doubled the first product and spilled: 204 us
 // against 172 for 8 chunks of 100 .. 700 rows after 1536 cached ones, before the
 // staging was trimmed). V is
@@ -45,8 +45,13 @@
 // Few workgroups (at most one per CU): sixteen waves, two groups of eight that take
 // the tiles in turn with LDS buffers of their own and join their sums at the end.
 //
-// Running maximum as in the decode: it moves only when a lane's weights sum to
-// more than 2^8 (or to a NaN), the weights are then formed again.
+// Weights are taken against a reference that moves only when a lane's 16 of a step sum to
+// more than 2^15 (or to a NaN); it then goes 8 bits below the largest score met, and the
+// weights are formed again. fp16 holds them in 11 bits from 2^-14 to 2^16, so that
+// a weight has them down to 2^-22 of a row's largest and is 0 only below 2^-33 of it: a
+// first key that takes nearly all the weight leaves the others theirs. (The reference
+// starts below every score, not at the sink, which joins at the end in fp32: against a
+// sink 18 nats above the scores the weights would all be 0.)
 #include "kept.hpp"
 #include "lds_dma.hpp"
 
@@ -62,7 +67,9 @@ constexpr int kPRow = kPTile + 8;       // 16-bit values per LDS row (a key's di
 constexpr int kPQueries = 32;           // queries per wave
 constexpr float kPVScale = 0x1p-10f;    // V is staged as fp16 of v * kPVScale
 constexpr float kPQScale = 0.125f * kLog2e;
-constexpr float kPLowest = -1e30f;      // the running maximum before any score (log2 units)
+constexpr float kPLowest = -1e30f;      // the weights' reference before any score (log2 units)
+constexpr float kPLift = 8.0f;          // bits from the reference up to the largest score, when it moves
+constexpr float kPSum = 32768.0f;       // a lane's weights of a step, at most: none reaches fp16's end
 // Grids of at most one workgroup per CU get two groups of waves a workgroup: a CU's
 // SIMDs then hold four waves, as with two workgroups. Where two fit, a second group only
 // takes the other's place, and a single tile cannot be split. Measured (us, one group /
@@ -456,7 +463,7 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
   }
   const int operand = n * kPRow + 8 * h; // this lane's place in an operand's rows
   const float sink2 = a.sinks && active ? a.sinks[head] * kLog2e : -INFINITY;
-  float m = fmaxf(sink2, kPLowest), l = 0.0f;
+  float m = kPLowest, l = 0.0f;
   f32x16 o[2];
 #pragma unroll
   for (int i = 0; i < 16; i++)
@@ -549,7 +556,7 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
         p[1] = __builtin_bit_cast(f16x8, u32x4{x[4], x[5], x[6], x[7]});
       };
       weights(m);
-      if (__any(!(sum <= 256.0f))) {
+      if (__any(!(sum <= kPSum))) {
         float m0 = acc[0], m1 = acc[8];
 #pragma unroll
         for (int i = 1; i < 8; i++) {
@@ -558,7 +565,7 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
         }
         float mx = fmaxf(m0 * d0, m1 * d1);
         mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const float mn = fmaxf(m, mx);
+        const float mn = fmaxf(m, mx - kPLift);
         const float f = __builtin_amdgcn_exp2f(m - mn);
         m = mn;
         l *= f;
