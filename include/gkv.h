@@ -601,7 +601,10 @@ int gkv_pool_create_kept(const gkv_pool_config *cfg, int32_t kept, gkv_pool **ou
 int gkv_pool_destroy(gkv_pool *pool);
 /* Takes a free sequence id (its length starts at 0). */
 int gkv_pool_seq_alloc(gkv_pool *pool, int32_t *seq_id);
-/* Makes room for seq_len tokens of seq_id (allocating blocks; never shrinks). */
+/* Makes room for seq_len tokens of seq_id (allocating blocks; never shrinks).
+ * In a pool with window layers the last call's seq_len is also taken for the sequence's
+ * length, by which gkv_pool_seq_fork and gkv_pool_seq_trim know what its rings
+ * hold: where room was made ahead, call it again with the tokens that are there. */
 int gkv_pool_seq_reserve(gkv_pool *pool, int32_t seq_id, int32_t seq_len);
 /* Returns the sequence's blocks to the free list (those that no other
  * sequence holds). */
@@ -610,20 +613,23 @@ int gkv_pool_seq_free(gkv_pool *pool, int32_t seq_id);
  * blocks are shared (freed with their last holder), the partly filled last one
  * and the window layers' rings are copied, on stream, at once. The tokens are
  * already appended (their kernels queued before this call on the same stream), and
- * both sequences append behind their own lengths only. Window layers: a ring
- * holds what it holds, so there n_tokens is the parent's length.
- * GKV_ERR_CAPACITY (no sequence id, no block left) and GKV_ERR_ARG (more tokens
- * than the parent has room for) take nothing. The child's table entries
+ * both sequences append behind their own lengths only. Window layers: a ring holds
+ * the parent's last tokens, so n_tokens is the parent's length or little less; a fork
+ * whose next token would see one that the ring no longer holds is refused
+ * (GKV_ERR_ARG; the parent's length: see gkv_pool_seq_reserve). To share a prefix that
+ * ends earlier, keep a sequence that ends with it and fork that one.
+ * GKV_ERR_CAPACITY (no sequence id, no block left) and GKV_ERR_ARG (that, or more
+ * tokens than the parent has room for) take nothing. The child's table entries
  * reach the device with the next gkv_pool_sync. */
 int gkv_pool_seq_fork(gkv_pool *pool, int32_t parent, int32_t n_tokens, void *stream,
                       int32_t *child);
 /* Cuts the sequence back to n_tokens: returns the full layers' blocks behind
  * them. A partly filled last block that other sequences hold is replaced by a
  * copy (on stream), as appends go on in it; GKV_ERR_CAPACITY if that needs
- * a block and none is left (nothing is taken then). The rings stay: what the
- * dropped tokens overwrote is gone (on a ring of window + 16 slots nothing
- * that is seen, if n_tokens does not go back behind the start of the block
- * that was begun last). */
+ * a block and none is left (nothing is taken then). The rings stay, and what the
+ * dropped tokens overwrote is gone: GKV_ERR_ARG, and nothing happens, if the next token
+ * would see any of it (on a ring of window + 16 slots it never does while n_tokens does
+ * not go back behind the start of the block that was begun last). */
 int gkv_pool_seq_trim(gkv_pool *pool, int32_t seq_id, int32_t n_tokens, void *stream);
 /* Moves the full layers' blocks in use to the ids 0 .. n - 1 (n in *n_used, which
  * may be NULL): one launch per 32 layers copies what lies behind, on stream, and

@@ -50,6 +50,7 @@ struct gkv_pool {
   int table_stride = 0; // full-table entries per sequence
   int ring_blocks = 0;  // window layers' table entries per sequence: W / 16, or kept / 16 + W / 16 + 1
   int ring = 0;         // slots of the window layers' ring: W, or W + 16
+  int kept = 0;         // positions before it that stay
   int64_t num_blocks = 0, num_ring_blocks = 0;
   std::vector<void *> k_full, v_full, k_ring, v_ring;
   std::vector<void *> s_full, s_ring; // fp32 V scales (int8 V only)
@@ -58,6 +59,12 @@ struct gkv_pool {
   std::vector<int32_t> free_blocks; // stack; back() is handed out next
   std::vector<int32_t> refs;        // per block: the sequences that hold it
   std::vector<int32_t> seq_blocks;  // blocks held per sequence
+  // What the window layers' rings hold, for forks and trims that go back: units of
+  // `unit` tokens (16; 1 in a ring of W slots, where a token takes another's place alone),
+  // per sequence the unit in each place when it was forked or last trimmed, its length then,
+  // and its length now by the last reserve.
+  int unit = 1, units = 0;
+  std::vector<int32_t> ring_units, seq_base, seq_len;
   std::vector<char> seq_live;
   std::vector<int32_t> free_seqs;
   int64_t device_bytes = 0;
@@ -135,6 +142,40 @@ struct gkv_pool {
     return v;
   }
 
+  // The unit that place e of a sequence's ring holds when the sequence is len tokens long:
+  // the last one appended there since its base, or what was there then.
+  int32_t ring_unit(int32_t seq, int32_t e, int32_t len) const {
+    const int32_t kept_units = kept / unit, last = (len - 1) / unit, back = last - kept_units - e;
+    if (len > seq_base[seq] && back >= 0) {
+      const int32_t u = last - back % units;
+      if (u >= seq_base[seq] / unit)
+        return u;
+    }
+    return ring_units[(size_t)seq * units + e];
+  }
+
+  // Whether the rings of a sequence of len tokens hold what the token behind its
+  // first n sees of them: positions max(n - W + 1, kept) .. n - 1.
+  bool ring_holds(int32_t seq, int32_t n, int32_t len) const {
+    const int32_t first = std::max({n - cfg.window + 1, kept, 0});
+    if (n_window == 0 || first >= n)
+      return true;
+    for (int32_t u = first / unit; u <= (n - 1) / unit; u++)
+      if (ring_unit(seq, (u - kept / unit) % units, len) != u)
+        return false;
+    return true;
+  }
+
+  // Sequence `to` goes on at n tokens, with the rings of `from` (a sequence of len).
+  void ring_rebase(int32_t to, int32_t from, int32_t n, int32_t len) {
+    if (to == from && n >= seq_len[to])
+      return; // (nothing dropped)
+    if (n_window > 0)
+      for (int32_t e = 0; e < units; e++)
+        ring_units[(size_t)to * units + e] = ring_unit(from, e, len);
+    seq_base[to] = seq_len[to] = n;
+  }
+
   // Copies blocks {src, dst} in every full (or window) layer, on stream: one
   // launch per 32 layers. The ids travel as kernel arguments, or, many of
   // them, through a staging buffer.
@@ -204,6 +245,7 @@ static int pool_create(const gkv_pool_config *cfg, int32_t kept, int32_t slack, 
   }
   p->table_stride = (c.max_seq_len + kBT - 1) / kBT;
   p->ring = c.window > 0 ? c.window + slack : 0;
+  p->kept = kept;
   p->ring_blocks = c.window > 0 ? (kept + c.window + slack) / kBT : 0;
   p->num_ring_blocks = (int64_t)c.max_seqs * p->ring_blocks;
   const int64_t bpl = bb.k + bb.v + bb.s;
@@ -288,6 +330,11 @@ static int pool_create(const gkv_pool_config *cfg, int32_t kept, int32_t slack, 
   std::copy(ring_ids.begin(), ring_ids.end(), p->h_ring_table.begin());
   p->refs.assign(p->num_blocks, 0);
   p->seq_blocks.assign(c.max_seqs, 0);
+  p->unit = slack > 0 ? kBT : 1;
+  p->units = p->ring / p->unit;
+  p->ring_units.assign((size_t)c.max_seqs * p->units, -1);
+  p->seq_base.assign(c.max_seqs, 0);
+  p->seq_len.assign(c.max_seqs, 0);
   p->seq_live.assign(c.max_seqs, 0);
   p->free_seqs.resize(c.max_seqs);
   for (int s = 0; s < c.max_seqs; s++)
@@ -340,6 +387,8 @@ extern "C" int gkv_pool_seq_alloc(gkv_pool *pool, int32_t *seq_id) {
   pool->free_seqs.pop_back();
   pool->seq_live[s] = 1;
   pool->seq_blocks[s] = 0;
+  pool->seq_base[s] = pool->seq_len[s] = 0;
+  std::fill_n(pool->ring_units.begin() + (size_t)s * pool->units, pool->units, -1);
   *seq_id = s;
   return GKV_OK;
 }
@@ -349,14 +398,21 @@ extern "C" int gkv_pool_seq_reserve(gkv_pool *pool, int32_t seq_id, int32_t seq_
     return GKV_ERR_ARG;
   if (seq_id < 0 || seq_id >= pool->cfg.max_seqs || !pool->seq_live[seq_id])
     return GKV_ERR_BLOCK;
-  if (pool->n_full == 0)
-    return seq_len <= pool->cfg.max_seq_len ? GKV_OK : GKV_ERR_CAPACITY;
+  const int32_t len = std::max(seq_len, pool->seq_base[seq_id]);
+  if (pool->n_full == 0) {
+    if (seq_len > pool->cfg.max_seq_len)
+      return GKV_ERR_CAPACITY;
+    pool->seq_len[seq_id] = len;
+    return GKV_OK;
+  }
   const int32_t need = (seq_len + kBT - 1) / kBT;
   if (need > pool->table_stride)
     return GKV_ERR_CAPACITY;
   const int32_t have = pool->seq_blocks[seq_id];
-  if (need <= have)
+  if (need <= have) {
+    pool->seq_len[seq_id] = len;
     return GKV_OK;
+  }
   if ((int64_t)(need - have) > (int64_t)pool->free_blocks.size())
     return GKV_ERR_CAPACITY; // nothing taken: all or none
   const size_t base = (size_t)seq_id * pool->table_stride;
@@ -368,6 +424,7 @@ extern "C" int gkv_pool_seq_reserve(gkv_pool *pool, int32_t seq_id, int32_t seq_
     pool->pending.push_back(int2{(int)(base + j), row[j]});
   }
   pool->seq_blocks[seq_id] = need;
+  pool->seq_len[seq_id] = len;
   return GKV_OK;
 }
 
@@ -406,6 +463,9 @@ extern "C" int gkv_pool_seq_fork(gkv_pool *pool, int32_t parent, int32_t n_token
   if (n_tokens > pool->cfg.max_seq_len ||
       (pool->n_full > 0 && shared + part > pool->seq_blocks[parent]))
     return GKV_ERR_ARG; // more tokens than the parent holds
+  const int32_t len = std::max(pool->seq_len[parent], n_tokens);
+  if (!pool->ring_holds(parent, n_tokens, len))
+    return GKV_ERR_ARG; // the child's next token would see what the parent's later ones replaced
   const bool full = pool->n_full > 0;
   if (pool->free_seqs.empty() || (full && part && pool->free_blocks.empty()))
     return GKV_ERR_CAPACITY;
@@ -448,6 +508,7 @@ extern "C" int gkv_pool_seq_fork(gkv_pool *pool, int32_t parent, int32_t n_token
   }
   pool->free_seqs.pop_back();
   pool->seq_live[id] = 1;
+  pool->ring_rebase(id, parent, n_tokens, len);
   *child = id;
   return GKV_OK;
 } catch (const std::exception &) {
@@ -460,8 +521,13 @@ extern "C" int gkv_pool_seq_trim(gkv_pool *pool, int32_t seq_id, int32_t n_token
     return GKV_ERR_ARG;
   if (seq_id < 0 || seq_id >= pool->cfg.max_seqs || !pool->seq_live[seq_id])
     return GKV_ERR_BLOCK;
-  if (pool->n_full == 0)
+  const int32_t len = std::max(pool->seq_len[seq_id], n_tokens);
+  if (!pool->ring_holds(seq_id, n_tokens, len))
+    return GKV_ERR_ARG; // the next token would see what the dropped ones replaced
+  if (pool->n_full == 0) {
+    pool->ring_rebase(seq_id, seq_id, n_tokens, len);
     return GKV_OK;
+  }
   const int32_t have = pool->seq_blocks[seq_id], keep = n_tokens / kBT + (n_tokens % kBT != 0);
   if (keep > have)
     return GKV_ERR_ARG;
@@ -496,6 +562,7 @@ extern "C" int gkv_pool_seq_trim(gkv_pool *pool, int32_t seq_id, int32_t n_token
     pool->pending.push_back(int2{(int)(base + keep - 1), own});
   }
   pool->seq_blocks[seq_id] = keep;
+  pool->ring_rebase(seq_id, seq_id, n_tokens, len);
   return GKV_OK;
 } catch (const std::exception &) {
   return GKV_ERR_CAPACITY; // out of host memory
