@@ -89,7 +89,8 @@ typedef enum { GKV_F32 = 0, GKV_BF16 = 1 } gkv_dtype;
  * scale of K and one of V per BLOCK of 16 tokens and head (129 bytes a token and
  * head for K and V together, against 136): for the gkv_kept_* entry points,
  * gkv_copy_blocks and the pool; the other kernels refuse it. Readers take any
- * finite scale >= 0; gkv_kept_append writes powers of two (see there). */
+ * finite scale >= 0 (what sees a block with a NaN for a scale gives NaN);
+ * gkv_kept_append writes powers of two (see there). */
 typedef enum {
   GKV_V_BF16 = 0,
   GKV_V_INT8 = 1,

@@ -355,8 +355,6 @@ __device__ __forceinline__ State attend(const KeptDecodeArgs &a, int b, int g, c
 #pragma unroll
     for (int r = 0; r < 4; r++)
       t[r] = (low ? acc[1][r] : acc[0][r]) + swap8(low ? acc[0][r] : acc[1][r]);
-    // the scale of this lane's block (never 0: a masked score of -inf stays one)
-    const float c = BLK ? fmaxf(qf * (low ? x.sc[1][0] : x.sc[0][0]), 1e-37f) : 1.0f;
     // The tokens of the block that are seen: all but in a sequence's last block
     // and in a window's first. The others get weight 0, and their values (never
     // written, or no longer seen) become 0.
@@ -384,7 +382,7 @@ __device__ __forceinline__ State attend(const KeptDecodeArgs &a, int b, int g, c
           for (int nn = 0; nn < 4; nn++)
             x.v[j][nn] &= keep;
           if (hi == 0)
-            x.sc[j][1] = 0.0f; // (a missing block's scale is another block's)
+            x.sc[j] = f32x2{0.0f, 0.0f}; // (a missing block's scales are another block's)
         } else {
           const uint32_t m0 = (keep & 0xffu ? 0xffffu : 0u) | (keep & 0xff00u ? 0xffff0000u : 0u);
           const uint32_t m1 =
@@ -397,6 +395,10 @@ __device__ __forceinline__ State attend(const KeptDecodeArgs &a, int b, int g, c
         }
       }
     }
+    // the scale of this lane's block (never 0: a masked score of -inf stays one; a NaN
+    // stays a NaN)
+    const float c =
+        BLK ? __builtin_elementwise_maximum(qf * (low ? x.sc[1][0] : x.sc[0][0]), 1e-37f) : 1.0f;
     float mx = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * c;
     // The running maximum moves only when a score passes it by more than 8
     // (weights stay below 2^8); the test needs no cross-lane maximum, only the

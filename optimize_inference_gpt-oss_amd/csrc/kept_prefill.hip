@@ -298,6 +298,12 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
         const u32x2 y2 = codes_to_f16(x.x[0][2]), y3 = codes_to_f16(x.x[0][3]);
         lo4 = u32x4{y0[0], y0[1], y1[0], y1[1]};
         hi4 = u32x4{y2[0], y2[1], y3[0], y3[1]};
+        // a scale that is not finite makes its block NaN, for the rows that see it
+        if (!(x.scale < INFINITY)) {
+          GKV_KEEP_BRANCH;
+          lo4 = hi4 = u32x4{0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u};
+          x.scale = 1.0f;
+        }
       } else {
         GKV_KEEP_BRANCH;
 #pragma unroll
