@@ -463,7 +463,7 @@ int gkv_prefill_paged(void *stream, int32_t B, const int32_t *cu_seqlens,
  * it continues stay as they are. On a ring, blocks that later ones of the same call
  * replace are not stored. max_rows: host bound of the rows of a sequence (a
  * sequence with more sets GKV_DEVERR_LENGTH and its further blocks are not
- * stored). A block beyond the table row: GKV_DEVERR_LENGTH, not stored. k_pack,
+ * stored; 0: nothing is done). A block beyond the table row: GKV_DEVERR_LENGTH, not stored. k_pack,
  * v_pack: NULL, or bf16 [rows][Hkv][64] as gkv_kv_append's (cache.k = cache.v =
  * NULL: packed rows only). Two sequences of one call must not share a block
  * that either appends to. B <= 65535. qkv, tables and packed rows are 16-byte
@@ -499,7 +499,9 @@ int gkv_kept_decode(void *stream, int32_t B, int32_t n_q_heads, const float *q, 
  * history (start_pos: multiples of 16), with gkv_prefill_paged's arguments and
  * rules: keys before start_pos[b] from the cache, those from there on from the
  * packed rows (k = v = NULL: from the cache too, ring = 0 only). On a ring,
- * append the chunk after this call. The tokens of a block whose id lies outside the
+ * append the chunk after this call. A prompt of more than max_len rows sets
+ * GKV_DEVERR_LENGTH, and rows past the bound may be left unwritten (max_len = 0: nothing is
+ * done). The tokens of a block whose id lies outside the
  * pool count for nothing (GKV_DEVERR_BLOCK_ID). At most 8 query heads per kv head. q, k, v, out
  * and the tables are 16-byte aligned, strides multiples of 4 (out_stride in bf16:
  * of 8). The matrix cores take fp16: q is rounded to 11 bits against its row's

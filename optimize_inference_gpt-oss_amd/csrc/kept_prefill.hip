@@ -93,7 +93,7 @@ struct KeptPrefillArgs {
   int table_stride, num_blocks;
   KeptRow row;
   const float *sinks;
-  int B, G, n_kv_heads, subs, kept, window, n_qblocks, band;
+  int B, G, n_kv_heads, subs, kept, window, max_len, n_qblocks, band;
   void *out;
   int64_t out_stride;
   int out_bf16;
@@ -163,7 +163,8 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
   const int cap = a.kc && a.row.ring_blocks == 0
                       ? (int)min((int64_t)a.table_stride * kBlockTokens, (int64_t)INT_MAX)
                       : INT_MAX;
-  if (start > cap - L && q0 == 0 && tid == 0 && a.dev_err)
+  // (the grid covers max_len rows)
+  if ((start > cap - L || L > a.max_len) && q0 == 0 && tid == 0 && a.dev_err)
     atomicOr(a.dev_err, GKV_DEVERR_LENGTH);
   if (start > INT_MAX - L)
     start = 0; // (no such positions)
@@ -751,6 +752,7 @@ extern "C" int gkv_kept_prefill(void *stream, int32_t B, const int32_t *cu_seqle
   a.n_kv_heads = cache.n_kv_heads;
   a.kept = kept;
   a.window = window;
+  a.max_len = max_len;
   a.out = out;
   a.out_stride = out_stride;
   a.out_bf16 = out_dtype == GKV_BF16;
