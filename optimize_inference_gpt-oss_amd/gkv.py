@@ -165,6 +165,7 @@ SIGNATURES = {
 }
 
 _lib = None
+_torch = None  # the module, where there is one
 
 
 class GkvError(RuntimeError):
@@ -176,14 +177,15 @@ class GkvError(RuntimeError):
 
 def lib():
     """Load libgkv.so; raises if it has not been built."""
-    global _lib
+    global _lib, _torch
     if _lib is None:
         # One HIP runtime per process: torch ships its own libamdhip64.so.7;
         # loading it first makes libgkv.so bind to that same runtime (its
         # NEEDED soname is already satisfied), so torch streams and device
         # pointers are valid in both.
         try:
-            import torch  # noqa: F401
+            import torch
+            _torch = torch
         except ImportError:
             pass
         if not os.path.exists(LIB_PATH):
@@ -446,15 +448,74 @@ def prefill_paged(cu_seqlens, max_len, q, cache: CacheView, sinks, out, start_po
     check("gkv_prefill_paged", st)
 
 
+# What the kept-token calls and copy_blocks ask of the tensors whose addresses they hand over
+# (ValueError otherwise). Calls of a few microseconds: no check that would not catch a mistake.
+
+
+def _refuse(what, want):
+    raise ValueError(f"{what}: {want}")
+
+
+def _ints(t, what):
+    """Address of lengths, offsets or block ids."""
+    if t.dtype is not _torch.int32 or not t.is_contiguous():
+        _refuse(what, "not contiguous int32")
+    if not t.is_cuda and not t.is_pinned():
+        _refuse(what, "not in GPU memory")
+    return t.data_ptr()
+
+
+def _floats(t, what):
+    """Address of a table or of sinks, which may be None."""
+    if t is None:
+        return None
+    if t.dtype is not _torch.float32:
+        _refuse(what, "not fp32")
+    return t.data_ptr()
+
+
+def _packed(t, what):
+    """Address of packed bf16 rows (or their bits as int16), which may be None."""
+    if t is None:
+        return None
+    if t.dtype.itemsize != 2 or t.dtype is _torch.float16 or not t.is_contiguous():
+        _refuse(what, "not contiguous bf16")
+    return t.data_ptr()
+
+
+def _row_stride(t, what):
+    """Row stride of fp32 rows."""
+    strides = t.stride()
+    if t.dtype is not _torch.float32 or strides[-1] != 1:
+        _refuse(what, "not rows of contiguous fp32")
+    return strides[0]
+
+
+def _out_rows(t):
+    """Row stride and gkv_dtype of an output."""
+    strides, dtype = t.stride(), t.dtype
+    if strides[-1] != 1:
+        _refuse("out", "not rows of contiguous elements")
+    if dtype is _torch.bfloat16:
+        return strides[0], BF16
+    if dtype is not _torch.float32:
+        _refuse("out", "neither fp32 nor bf16")
+    return strides[0], F32
+
+
 def kept_append(qkv, n_q_heads, cos_tab, sin_tab, seq_lens, view: CacheView, kept=0, window=0,
                 cu_seqlens=None, max_rows=1, k_pack=None, v_pack=None, dev_err=None, stream=None):
     """gkv_kept_append: the rows cu_seqlens[b] .. cu_seqlens[b+1]-1 (None: row b) as the last
     positions of sequence b, seq_lens[b] tokens long with them, into whole blocks of bf16, or
-    of e4m3 codes with one scale per block and head."""
-    st = lib().gkv_kept_append(stream_handle(stream), seq_lens.shape[0], ptr(cu_seqlens),
-                               ptr(seq_lens), max_rows, ptr(qkv), qkv.stride(0), n_q_heads,
-                               ptr(cos_tab), ptr(sin_tab), view, kept, window, ptr(k_pack),
-                               ptr(v_pack), ptr(dev_err))
+    of e4m3 codes with one scale per block and head. int32 lengths, fp32 rows and tables, packed
+    rows of bf16 or its bits; ValueError otherwise."""
+    L = lib()
+    st = L.gkv_kept_append(stream_handle(stream), seq_lens.shape[0],
+                           None if cu_seqlens is None else _ints(cu_seqlens, "cu_seqlens"),
+                           _ints(seq_lens, "seq_lens"), max_rows, qkv.data_ptr(),
+                           _row_stride(qkv, "qkv"), n_q_heads, _floats(cos_tab, "cos_tab"),
+                           _floats(sin_tab, "sin_tab"), view, kept, window,
+                           _packed(k_pack, "k_pack"), _packed(v_pack, "v_pack"), ptr(dev_err))
     check("gkv_kept_append", st)
 
 
@@ -465,14 +526,16 @@ def kept_workspace_bytes(B, n_kv_heads, max_seq_len, kept=0, window=0) -> int:
 def kept_decode(q, n_q_heads, seq_lens, max_seq_len, view: CacheView, out, sinks=None, kept=0,
                 window=0, cos_tab=None, sin_tab=None, workspace=None, dev_err=None, stream=None):
     """gkv_kept_decode: one query per sequence, which sees the first `kept` positions and
-    the last `window` (window 0: all)."""
-    import torch
-    out_dtype = BF16 if out.dtype == torch.bfloat16 else F32
+    the last `window` (window 0: all). int32 lengths, fp32 queries, sinks and tables, out in
+    fp32 or bf16; ValueError otherwise."""
+    L = lib()
+    out_stride, out_dtype = _out_rows(out)
     ws_bytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
-    st = lib().gkv_kept_decode(stream_handle(stream), q.shape[0], n_q_heads, ptr(q), q.stride(0),
-                               ptr(cos_tab), ptr(sin_tab), ptr(seq_lens), max_seq_len, view, kept,
-                               window, ptr(sinks), ptr(workspace), ws_bytes, ptr(out),
-                               out.stride(0), out_dtype, ptr(dev_err))
+    st = L.gkv_kept_decode(stream_handle(stream), q.shape[0], n_q_heads, q.data_ptr(),
+                           _row_stride(q, "q"), _floats(cos_tab, "cos_tab"),
+                           _floats(sin_tab, "sin_tab"), _ints(seq_lens, "seq_lens"), max_seq_len,
+                           view, kept, window, _floats(sinks, "sinks"), ptr(workspace), ws_bytes,
+                           out.data_ptr(), out_stride, out_dtype, ptr(dev_err))
     check("gkv_kept_decode", st)
 
 
@@ -480,13 +543,18 @@ def kept_prefill(cu_seqlens, max_len, q, n_q_heads, view: CacheView, out, start_
                  v=None, sinks=None, kept=0, window=0, cos_tab=None, sin_tab=None, dev_err=None,
                  stream=None):
     """gkv_kept_prefill: prompts (a view without a cache: CacheView(n_kv_heads=...)), or chunks
-    continuing the sequences in `view`, with the mask of kept_decode."""
-    import torch
-    out_dtype = BF16 if out.dtype == torch.bfloat16 else F32
-    st = lib().gkv_kept_prefill(stream_handle(stream), cu_seqlens.shape[0] - 1, ptr(cu_seqlens),
-                                ptr(start_pos), max_len, n_q_heads, ptr(q), q.stride(0),
-                                ptr(cos_tab), ptr(sin_tab), ptr(k), ptr(v), view, kept, window,
-                                ptr(sinks), ptr(out), out.stride(0), out_dtype, ptr(dev_err))
+    continuing the sequences in `view`, with the mask of kept_decode. The types of kept_decode,
+    packed rows of bf16 or its bits; ValueError otherwise."""
+    L = lib()
+    out_stride, out_dtype = _out_rows(out)
+    st = L.gkv_kept_prefill(stream_handle(stream), cu_seqlens.shape[0] - 1,
+                            _ints(cu_seqlens, "cu_seqlens"),
+                            None if start_pos is None else _ints(start_pos, "start_pos"), max_len,
+                            n_q_heads, q.data_ptr(), _row_stride(q, "q"),
+                            _floats(cos_tab, "cos_tab"), _floats(sin_tab, "sin_tab"),
+                            _packed(k, "k"), _packed(v, "v"), view, kept, window,
+                            _floats(sinks, "sinks"), out.data_ptr(), out_stride, out_dtype,
+                            ptr(dev_err))
     check("gkv_kept_prefill", st)
 
 
@@ -496,14 +564,15 @@ def cache_views(views):
 
 
 def copy_blocks(views, src, dst, dev_err=None, stream=None):
-    """gkv_copy_blocks: block src[i] to dst[i] (int32 device tensors) in every view (a
-    cache_views array, or a list of CacheView)."""
+    """gkv_copy_blocks: block src[i] to dst[i] (contiguous int32 device tensors; ValueError
+    otherwise) in every view (a cache_views array, or a list of CacheView)."""
+    L = lib()
     if not isinstance(views, ctypes.Array):
         views = cache_views(views)
     if src.shape != dst.shape:
         raise ValueError("src and dst differ in length")
-    st = lib().gkv_copy_blocks(stream_handle(stream), views, len(views), src.numel(), ptr(src),
-                               ptr(dst), ptr(dev_err))
+    st = L.gkv_copy_blocks(stream_handle(stream), views, len(views), src.numel(),
+                           _ints(src, "src"), _ints(dst, "dst"), ptr(dev_err))
     check("gkv_copy_blocks", st)
 
 
