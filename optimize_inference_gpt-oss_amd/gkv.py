@@ -239,8 +239,12 @@ def stream_handle(stream=None) -> int | None:
     if stream is not None:
         return stream.cuda_stream
     import torch
-    # the handle of torch.cuda.current_stream(), without the 2.5 us of making its object
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    # the handle of torch.cuda.current_stream(), without the 2.5 us of making its object where
+    # this torch hands it out (the function is not a public one)
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    if raw is None:
+        return torch.cuda.current_stream().cuda_stream
+    return raw(torch.cuda.current_device())
 
 
 def rope_table(n_pos: int, **overrides):

@@ -1,4 +1,5 @@
-"""What the Python binding of the kept-token entry points refuses before any pointer is handed over."""
+"""What the Python binding of the kept-token entry points refuses before any pointer is handed over,
+and where it takes its stream from."""
 from types import SimpleNamespace
 
 import pytest
@@ -70,3 +71,11 @@ def test_refused_tensors(gkv, monkeypatch, call, bad):
 def test_host_memory_is_refused(gkv, call):
     with pytest.raises(ValueError, match="not in GPU memory"):
         call(gkv)
+
+
+def test_the_current_stream_by_the_public_way(gkv, monkeypatch):
+    """A torch without the private function."""
+    monkeypatch.delattr(torch._C, "_cuda_getCurrentRawStream", raising=False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda: SimpleNamespace(cuda_stream=0x70))
+    assert gkv.stream_handle() == 0x70
+    assert gkv.stream_handle(SimpleNamespace(cuda_stream=0x80)) == 0x80
