@@ -519,7 +519,7 @@ int gkv_kept_prefill(void *stream, int32_t B, const int32_t *cu_seqlens, const i
 
 /* Copies block src[i] to block dst[i] (device int32 [n_pairs]) in every one of
  * n_views caches (host array; any format, K, V and scales; the block tables are
- * not used), all in one launch per 32 views. The targets are distinct and no
+ * not used), all in one launch per 32 views (fewer from 2^18 pairs on). The targets are distinct and no
  * target is a source. An id outside a cache sets GKV_DEVERR_BLOCK_ID and is not
  * copied there. No counterpart in the reference. */
 int gkv_copy_blocks(void *stream, const gkv_cache_view *views, int32_t n_views, int32_t n_pairs,

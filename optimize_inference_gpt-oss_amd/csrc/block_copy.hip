@@ -12,7 +12,6 @@
 #include "block_copy.hpp"
 
 #include <algorithm>
-#include <climits>
 #include <type_traits>
 
 namespace gkv {
@@ -21,6 +20,7 @@ constexpr int kCopyThreads = 256;
 constexpr int kCopyViews = 32;  // layers per launch (their pointers are kernel arguments)
 constexpr int kCopySpread = 1024; // workgroups up to which pairs are cut into parts
 constexpr int kCopyParts = 4;
+constexpr int kCopyGrid = 1 << 23; // workgroups per launch, at most (a launch takes 2^32 threads)
 
 struct CopyLayer {
   char *k, *v, *s;
@@ -110,12 +110,12 @@ int block_bytes(int n_kv_heads, int v_format, BlockBytes *out) {
 int copy_blocks(hipStream_t stream, const gkv_cache_view *views, int32_t n_views, int32_t n_pairs,
                 const int32_t *src, const int32_t *dst, int stride, const int2 *host_pairs,
                 uint32_t *dev_err) {
-  for (int v0 = 0; v0 < n_views; v0 += kCopyViews) {
+  // (as many layers a launch as its grid takes; more pairs than that in several launches)
+  const int most = std::min(n_pairs, kCopyGrid);
+  const int views_at_once = std::min(kCopyViews, kCopyGrid / most);
+  for (int v0 = 0; v0 < n_views; v0 += views_at_once) {
     CopyArgs a{};
-    a.n_layers = std::min(kCopyViews, n_views - v0);
-    a.n_pairs = n_pairs;
-    a.src = src;
-    a.dst = dst;
+    a.n_layers = std::min(views_at_once, n_views - v0);
     a.stride = stride;
     a.dev_err = dev_err;
     for (int i = 0; i < a.n_layers; i++) {
@@ -128,21 +128,24 @@ int copy_blocks(hipStream_t stream, const gkv_cache_view *views, int32_t n_views
                              (uint32_t)b.k,       (uint32_t)b.v,       (uint32_t)b.s,
                              c.num_blocks};
     }
-    const int64_t items = (int64_t)a.n_layers * n_pairs;
-    a.parts = items * kCopyParts <= kCopySpread ? kCopyParts : 1;
-    if (items * a.parts > INT_MAX)
-      return GKV_ERR_ARG;
-    const dim3 grid((unsigned)(items * a.parts)), block(kCopyThreads);
-    if (host_pairs) {
-      InlinePairs in{};
-      std::copy(host_pairs, host_pairs + n_pairs, in.p);
-      hipLaunchKernelGGL((copy_blocks_kernel<InlinePairs>), grid, block, 0, stream, a, in);
-    } else {
-      hipLaunchKernelGGL((copy_blocks_kernel<NoPairs>), grid, block, 0, stream, a, NoPairs{});
+    for (int64_t p0 = 0; p0 < n_pairs; p0 += most) {
+      a.n_pairs = (int)std::min<int64_t>(most, n_pairs - p0);
+      a.src = src ? src + p0 * stride : nullptr;
+      a.dst = dst ? dst + p0 * stride : nullptr;
+      const int items = a.n_layers * a.n_pairs;
+      a.parts = items <= kCopySpread / kCopyParts ? kCopyParts : 1;
+      const dim3 grid((unsigned)(items * a.parts)), block(kCopyThreads);
+      if (host_pairs) {
+        InlinePairs in{};
+        std::copy(host_pairs, host_pairs + n_pairs, in.p);
+        hipLaunchKernelGGL((copy_blocks_kernel<InlinePairs>), grid, block, 0, stream, a, in);
+      } else {
+        hipLaunchKernelGGL((copy_blocks_kernel<NoPairs>), grid, block, 0, stream, a, NoPairs{});
+      }
+      const int st = launch_status("copy_blocks_kernel");
+      if (st != GKV_OK)
+        return st;
     }
-    const int st = launch_status("copy_blocks_kernel");
-    if (st != GKV_OK)
-      return st;
   }
   return GKV_OK;
 }

@@ -34,3 +34,45 @@ def test_prefill_flags_prompts_longer_than_the_bound(gkv, cuda, Hq, Hkv, rows, b
     for b, m in enumerate(rows):
         r = slice(cu[b], cu[b] + min(m, bound))
         assert torch.allclose(outs[0][r], outs[1][r], rtol=0, atol=tol)
+
+
+def test_prefill_under_a_bound_of_more_workgroups_than_a_grid_row(gkv, cuda):
+    """300 prompts of a few rows, the bound 131072 rows: ten million workgroups, nearly all empty."""
+    B, Hkv = 300, 8
+    rng = np.random.default_rng(3)
+    rows = rng.integers(0, 4, B)
+    n = int(rows.sum())
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q = torch.randn(n, 8 * Hkv * D, generator=g, device="cuda")
+    k, v = (torch.randn(n, Hkv * D, generator=g, device="cuda").bfloat16() for _ in "kv")
+    cu = dev(np.concatenate([[0], np.cumsum(rows)]).astype(np.int32))
+    outs = []
+    for m in (4, 131072):
+        out, err = torch.zeros(n, 8 * Hkv * D, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+        gkv.kept_prefill(cu, m, q, 8 * Hkv, gkv.CacheView(n_kv_heads=Hkv), out, k=k, v=v, dev_err=err)
+        assert int(err.item()) == 0
+        outs.append(out)
+    assert torch.equal(*outs) and outs[0].abs().sum(1).min() > 0
+
+
+@pytest.mark.parametrize("views,pairs", [(32, 600001), (3, 9000000)])
+def test_copies_of_more_blocks_than_a_launch_takes(gkv, cuda, views, pairs):
+    """Ids outside the cache but for the first, the middle and the last pair."""
+    nb = 8
+    g = torch.Generator(device="cuda").manual_seed(4)
+    caches = [[torch.randint(0, 256, (nb, m), dtype=torch.uint8, device="cuda", generator=g) for m in (1024, 1024, 8)]
+              for _ in range(views)]
+    src = torch.full((pairs,), -1, dtype=torch.int32, device="cuda")
+    dst = torch.zeros(pairs, dtype=torch.int32, device="cuda")
+    for i, (s, d) in zip((0, pairs // 2, pairs - 1), ((1, 2), (3, 4), (7, 6))):
+        src[i], dst[i] = s, d
+    want = [[x.clone() for x in c] for c in caches]
+    for c in want:
+        for x in c:
+            x[[2, 4, 6]] = x[[1, 3, 7]]
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    arr = gkv.cache_views([gkv.CacheView(c[0].data_ptr(), c[1].data_ptr(), None, 0, nb, 1, 0, c[2].data_ptr(),
+                                         gkv.KV_FP8_BLOCK) for c in caches])
+    gkv.copy_blocks(arr, src, dst, dev_err=err)
+    assert int(err.item()) == gkv.DEVERR_BLOCK_ID
+    assert all(torch.equal(x, y) for c, w in zip(caches, want) for x, y in zip(c, w))
