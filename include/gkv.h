@@ -466,7 +466,7 @@ int gkv_prefill_paged(void *stream, int32_t B, const int32_t *cu_seqlens,
  * stored; 0: nothing is done). A block beyond the table row: GKV_DEVERR_LENGTH, not stored. k_pack,
  * v_pack: NULL, or bf16 [rows][Hkv][64] as gkv_kv_append's (cache.k = cache.v =
  * NULL: packed rows only). Two sequences of one call must not share a block
- * that either appends to. B <= 65535. qkv, tables and packed rows are 16-byte
+ * that either appends to. B <= 65535, max_rows < 2^28 - 30. qkv, tables and packed rows are 16-byte
  * aligned, row_stride is a multiple of 4. */
 int gkv_kept_append(void *stream, int32_t B, const int32_t *cu_seqlens, const int32_t *seq_lens,
                     int32_t max_rows, const float *qkv, int64_t row_stride, int32_t n_q_heads,
@@ -485,7 +485,7 @@ size_t gkv_kept_workspace_bytes(int32_t B, int32_t n_kv_heads, int32_t max_seq_l
  * tables cover (a longer sequence, or one past the table row, sets
  * GKV_DEVERR_LENGTH and is taken at the bound). A sequence of length 0 gets
  * zeros; so does a head that sees nothing (every block id bad, no sink). At most 8
- * kv heads and 8 query heads per kv head. Calls that may overlap need
+ * kv heads, 8 query heads per kv head, and about a million sequences. Calls that may overlap need
  * workspaces of their own. Rows are 16-byte aligned (out in bf16: 8-byte), their
  * strides multiples of 4. */
 int gkv_kept_decode(void *stream, int32_t B, int32_t n_q_heads, const float *q, int64_t q_stride,

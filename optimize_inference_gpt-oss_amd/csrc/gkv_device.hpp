@@ -74,5 +74,10 @@ namespace gkv {
 // Host side: turns the launch status into a gkv_status, keeping the HIP error
 // text for gkv_last_error() (thread-local).
 int hip_status(hipError_t e, const char *where);
+// Whether a grid's first axis fits a launch, which counts it in threads, in 32 bits, and drops
+// what goes beyond without an error.
+inline bool grid_fits(int64_t workgroups, int64_t threads) {
+  return workgroups * threads < ((int64_t)1 << 32);
+}
 inline int launch_status(const char *where) { return hip_status(hipGetLastError(), where); }
 } // namespace gkv

@@ -353,6 +353,10 @@ extern "C" int gkv_kept_append(void *stream, int32_t B, const int32_t *cu_seqlen
     return GKV_ERR_UNSUPPORTED; // a grid row per sequence
   if (cu_seqlens == nullptr && max_rows > 1)
     return GKV_ERR_ARG;
+  // blocks that max_rows consecutive positions can touch
+  const int64_t blocks = (max_rows + (int64_t)kBlockTokens - 2) / kBlockTokens + 1;
+  if (!grid_fits(blocks, 64 * kAppendWaves))
+    return GKV_ERR_UNSUPPORTED;
   if (B == 0 || max_rows == 0 || (!to_cache && !k_pack && !v_pack))
     return GKV_OK;
   KeptAppendArgs a;
@@ -376,9 +380,7 @@ extern "C" int gkv_kept_append(void *stream, int32_t B, const int32_t *cu_seqlen
   a.v_pack = (uint16_t *)v_pack;
   a.dev_err = dev_err;
   const int waves = std::min(kAppendWaves, a.n_kv_heads);
-  // blocks that max_rows consecutive positions can touch
-  const dim3 grid((unsigned)((max_rows + (int64_t)kBlockTokens - 2) / kBlockTokens + 1), B,
-                  (unsigned)((a.n_kv_heads + waves - 1) / waves));
+  const dim3 grid((unsigned)blocks, B, (unsigned)((a.n_kv_heads + waves - 1) / waves));
   const dim3 block(64 * waves);
   if (to_cache && cache.v_format == GKV_KV_FP8_BLOCK)
     hipLaunchKernelGGL((kept_append_kernel<true>), grid, block, 0, (hipStream_t)stream, a);

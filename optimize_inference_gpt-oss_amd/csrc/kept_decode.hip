@@ -1029,8 +1029,10 @@ extern "C" int gkv_kept_decode(void *stream, int32_t B, int32_t n_q_heads, const
       return GKV_OK;
     a.parts = whole_parts(B, a.n_kv_heads, steps, window);
     a.heads_per_wg = std::min(8 / a.parts, a.n_kv_heads);
-    const dim3 grid((unsigned)((int64_t)B * ((a.n_kv_heads + a.heads_per_wg - 1) / a.heads_per_wg)));
-    const dim3 block(64 * a.parts * a.heads_per_wg);
+    const int64_t wgs = (int64_t)B * ((a.n_kv_heads + a.heads_per_wg - 1) / a.heads_per_wg);
+    const dim3 grid((unsigned)wgs), block(64 * a.parts * a.heads_per_wg);
+    if (!grid_fits(wgs, block.x))
+      return GKV_ERR_UNSUPPORTED;
     if (blk && a.out_bf16)
       hipLaunchKernelGGL((kept_decode_whole_kernel<true, 2, 4, false>), grid, block, 0, s, a);
     else if (blk)
