@@ -79,5 +79,6 @@ int hip_status(hipError_t e, const char *where);
 inline bool grid_fits(int64_t workgroups, int64_t threads) {
   return workgroups * threads < ((int64_t)1 << 32);
 }
+constexpr int kGridRow = 1 << 22; // workgroups (of up to 512 threads) in a row of a grid of several
 inline int launch_status(const char *where) { return hip_status(hipGetLastError(), where); }
 } // namespace gkv

@@ -79,7 +79,6 @@ constexpr float kPSum = 32768.0f;       // a lane's weights of a step, at most: 
 constexpr int64_t kPFewWgs = 256;
 constexpr int kPShort = 128; // rows of a prompt without a history that stay with one group
 constexpr int kPBand = 2;               // query blocks per band of the grid order
-constexpr int kPGridX = 1 << 22;        // workgroups in a row of the grid (a row takes 2^32 threads)
 
 struct KeptPrefillArgs {
   const int32_t *cu, *start;
@@ -136,7 +135,7 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
   // Grid order: kv head fastest (the workgroups of a head on one XCD share its
   // K/V in that L2), bands of query blocks longest first, a prompt's blocks of a band
   // together.
-  int id = blockIdx.y * kPGridX + blockIdx.x;
+  int id = blockIdx.y * kGridRow + blockIdx.x;
   const int g = id % a.n_kv_heads;
   id /= a.n_kv_heads;
   const int band = id / (a.B * a.band), w = id - band * (a.B * a.band);
@@ -759,7 +758,7 @@ extern "C" int gkv_kept_prefill(void *stream, int32_t B, const int32_t *cu_seqle
   a.out_bf16 = out_dtype == GKV_BF16;
   a.dev_err = dev_err;
   const dim3 block(64 * G * a.subs);
-  const dim3 rows((unsigned)std::min<int64_t>(grid, kPGridX), (unsigned)((grid + kPGridX - 1) / kPGridX));
+  const dim3 rows((unsigned)std::min<int64_t>(grid, kGridRow), (unsigned)((grid + kGridRow - 1) / kGridRow));
   if (G * a.subs == 8 && grid <= kPFewWgs && (start_pos || max_len > kPShort))
     hipLaunchKernelGGL((kept_prefill_kernel<1, 2>), rows, dim3(1024), 0, (hipStream_t)stream, a);
   else if (G * a.subs == 8)

@@ -131,7 +131,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW >= 8
   // share their K/V tiles in its L2 (a band's blocks see nearly the same
   // keys), while the longest blocks still start first. Ids past the first
   // query block (the last band's padding) exit at once.
-  int id = blockIdx.x;
+  int id = blockIdx.y * kGridRow + blockIdx.x;
   const int g = id % a.n_kv_heads;
   id /= a.n_kv_heads;
   const int band = id / (a.B * a.band), w = id - band * (a.B * a.band);
@@ -726,7 +726,7 @@ static int prefill_launch(void *stream, int32_t B, const int32_t *cu_seqlens,
   if (((uintptr_t)k | (uintptr_t)v | (uintptr_t)q | (uintptr_t)cos_tab | (uintptr_t)sin_tab) %
           16 != 0)
     return GKV_ERR_ARG; // 16-byte vector loads
-  const int n_qblocks = (max_len + kQBlock - 1) / kQBlock;
+  const int n_qblocks = (int)(((int64_t)max_len + kQBlock - 1) / kQBlock);
   const int band = std::min(query_band(), std::max(n_qblocks, 1));
   const int64_t grid = (int64_t)((n_qblocks + band - 1) / band) * band * B * n_kv_heads;
   if (grid == 0)
@@ -762,7 +762,7 @@ static int prefill_launch(void *stream, int32_t B, const int32_t *cu_seqlens,
   a.out_bf16 = out_dtype == GKV_BF16;
   a.dev_err = dev_err;
   hipStream_t s = (hipStream_t)stream;
-  const dim3 g((unsigned)grid);
+  const dim3 g((unsigned)std::min<int64_t>(grid, kGridRow), (unsigned)((grid + kGridRow - 1) / kGridRow));
   if (cached && cache->v_format == GKV_KV_FP8)
     launch_prefill<true, 2>(a, G, g, s);
   else if (cached && cache->v_format == GKV_V_INT8)
