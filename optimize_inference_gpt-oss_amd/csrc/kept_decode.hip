@@ -141,7 +141,7 @@ struct StepData {
   f32x2 sc[2];   // per block: K scale, V scale (wave-uniform)
   uint32_t miss; // bit j: block j is not there (padding, or an id outside the pool)
 };
-constexpr int kNoBlock = INT32_MIN; // the id of a step's missing second block
+constexpr int kNoBlock = -1; // the id of a step's missing second block
 
 typedef const __attribute__((address_space(4))) int32_t *ScalarI32;
 typedef const __attribute__((address_space(4))) f32x2 *ScalarF2;
@@ -196,13 +196,14 @@ __device__ __forceinline__ State attend(const KeptDecodeArgs &a, int b, int g, c
   const char *k_head = a.kc + g * kHeadBytes, *v_head = a.vc + g * kHeadBytes;
   const char *s_head = (const char *)a.scales + g * 8;
   const uint32_t stride = (uint32_t)a.n_kv_heads * kHeadBytes; // bytes of a block
-  auto load = [&](StepData<BLK> &x, int2 ids) {
+  auto load = [&](StepData<BLK> &x, int2 ids, int s) {
     x.miss = 0;
+    const bool first = s < s1, second = first && 2 * s + 1 < sp.n_blocks; // which there are
 #pragma unroll
     for (int j = 0; j < 2; j++) {
       const int id = uniform(j ? ids.y : ids.x);
       const bool ok = (uint32_t)id < (uint32_t)a.num_blocks;
-      bad |= !ok && id != kNoBlock;
+      bad |= !ok && (j ? second : first);
       x.miss |= ok ? 0u : 1u << j;
       const uint64_t off = (uint64_t)(ok ? (uint32_t)id : 0u) * stride;
       // a missing block reads nothing: its resource covers 0 bytes
@@ -228,7 +229,7 @@ __device__ __forceinline__ State attend(const KeptDecodeArgs &a, int b, int g, c
 #pragma unroll
   for (int i = 0; i < R - 1; i++) {
     const int2 next = ids_of(s0 + i + 1);
-    load(buf[i], ids);
+    load(buf[i], ids, s0 + i);
     ids = next;
   }
 
@@ -472,7 +473,7 @@ __device__ __forceinline__ State attend(const KeptDecodeArgs &a, int b, int g, c
       if (s + r >= s1)
         break;
       const int2 next = ids_of(s + r + R);
-      load(buf[(r + R - 1) % R], ids);
+      load(buf[(r + R - 1) % R], ids, s + r + R - 1);
       ids = next;
       compute(buf[r], s + r);
     }

@@ -183,10 +183,10 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
   const int ring_end = a.row.kept_blocks + a.row.ring_blocks;
   const int n_waves = a.G * a.subs;
 
-  // Block id of a piece of tile t (kNone: not from the cache, or seen by nobody). It
+  // Block id of a piece of tile t (kNone: not from the cache, or seen by nobody; outside any pool). It
   // and the scales come through vector loads: a scalar load in flight would
   // hold up the wait for every LDS read behind it.
-  constexpr int kNone = INT_MIN;
+  constexpr int kNone = -1;
   const __amdgpu_buffer_rsrc_t table_row =
       head_rsrc(a.table + (int64_t)b * a.table_stride, a.table ? 4 * a.table_stride : 0);
   auto id_of = [&](int t, int task) -> int {
@@ -228,7 +228,12 @@ void kept_prefill_kernel(KeptPrefillArgs a) {
     if (x.hist) {
       GKV_KEEP_BRANCH;
       const bool ok = (uint32_t)id < (uint32_t)a.num_blocks;
-      bad |= !ok && id != kNone;
+      if (!ok) { // flagged if id_of read it (its conditions)
+        GKV_KEEP_BRANCH;
+        const int e = x.p / kBlockTokens;
+        bad |= x.p <= p_last && (W == 0 || e < a.row.kept_blocks || e >= lo_blk) &&
+               (a.row.ring_blocks > 0 || e < a.table_stride);
+      }
       x.miss = !ok;
       const int64_t hb = (int64_t)(ok ? id : 0) * a.n_kv_heads + g;
       const char *src = is_v ? a.vc : a.kc;

@@ -24,6 +24,29 @@ def leave_first_block(c):
         c.s[0] = np.nan
 
 
+@pytest.mark.parametrize("bad", [-2**31, 2**31 - 1, -1])
+@pytest.mark.parametrize("kept,window,ring", [(0, 0, False), (16, 64, True), (16, 64, False)])
+@pytest.mark.parametrize("max_len", [100, 20000])
+def test_any_id_outside_the_pool_is_flagged(gkv, cuda, bad, kept, window, ring, max_len):
+    """Of a block that is seen, by the decode and the prefill; of one that nothing sees it is not."""
+    lay = Layout(kept, window, ring)
+    for lose, flag in ((5, gkv.DEVERR_BLOCK_ID), (1 if window and not ring else None, 0)):
+        c = Cache([96], 1, lay, BLOCK)
+        if lose is not None:
+            c.table[0, lay.entry(lose)] = bad
+        view = c.device(gkv)
+        q = torch.ones(3, D, device="cuda")
+        ws = torch.zeros(max(16, gkv.kept_workspace_bytes(1, 1, max_len, kept, window)), dtype=torch.uint8, device="cuda")
+        out, kv = torch.zeros(3, D, device="cuda"), torch.zeros(3, D, dtype=torch.bfloat16, device="cuda")
+        gkv.kept_decode(q[:1], 1, dev(np.array([96], np.int32)), max_len, view, out[:1], kept=kept, window=window,
+                        workspace=ws, dev_err=c.err)
+        assert int(c.err.item()) == flag
+        c.err.zero_()
+        gkv.kept_prefill(dev(np.array([0, 3], np.int32)), max_len, q, 1, view, out, start_pos=dev(np.array([96], np.int32)),
+                         k=kv, v=kv, kept=kept, window=window, dev_err=c.err)
+        assert int(c.err.item()) == flag
+
+
 @pytest.mark.parametrize("fmt", [BF16, BLOCK])
 @pytest.mark.parametrize("kept,window,ring", [(0, 0, False), (16, 64, False), (32, 64, True), (0, 1600, True),
                                               (48, 1616, False)])
