@@ -714,8 +714,8 @@ extern "C" int gkv_kept_prefill(void *stream, int32_t B, const int32_t *cu_seqle
   if ((!k && !cached) || (start_pos && !cached) || (cached && cache.ring > 0 && !k))
     return GKV_ERR_ARG; // keys from nowhere; a history needs the cache; a ring holds the history only
   const int G = n_q_heads / cache.n_kv_heads;
-  if (G > 8 || cache.n_kv_heads > (1 << 20))
-    return GKV_ERR_UNSUPPORTED;
+  if (G > 8 || cache.n_kv_heads >= (1 << 20))
+    return GKV_ERR_UNSUPPORTED; // (16 packed rows take less than 2^31 bytes)
   if (q_stride < (int64_t)n_q_heads * kHeadDim || out_stride < (int64_t)n_q_heads * kHeadDim ||
       q_stride % 4 != 0 || out_stride % (out_dtype == GKV_BF16 ? 8 : 4) != 0)
     return GKV_ERR_ARG;
