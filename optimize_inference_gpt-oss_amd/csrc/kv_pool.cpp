@@ -29,7 +29,7 @@
 #include <cstdint>
 #include <cstring>
 #include <exception>
-#include <new>
+#include <memory>
 #include <numeric>
 #include <random>
 #include <vector>
@@ -95,6 +95,12 @@ struct gkv_pool {
       stage_done[i] = nullptr;
     }
     stage_cap = 0;
+  }
+
+  // Room for n more changed entries, made before a call takes anything.
+  void make_room(size_t n) {
+    if (pending.size() + n > pending.capacity())
+      pending.reserve(std::max(pending.size() + n, 2 * pending.capacity()));
   }
 
   // The staging buffer for the next n pairs (grown if need be), free to be
@@ -219,7 +225,7 @@ struct gkv_pool {
   }
 };
 
-static int pool_create(const gkv_pool_config *cfg, int32_t kept, int32_t slack, gkv_pool **out) {
+static int pool_create(const gkv_pool_config *cfg, int32_t kept, int32_t slack, gkv_pool **out) try {
   if (!cfg || !out)
     return GKV_ERR_ARG;
   *out = nullptr;
@@ -232,9 +238,7 @@ static int pool_create(const gkv_pool_config *cfg, int32_t kept, int32_t slack, 
   gkv::BlockBytes bb;
   if (c.n_kv_heads > 65536 || gkv::block_bytes(c.n_kv_heads, c.v_format, &bb) != GKV_OK)
     return GKV_ERR_ARG;
-  gkv_pool *p = new (std::nothrow) gkv_pool();
-  if (!p)
-    return GKV_ERR_CAPACITY;
+  std::unique_ptr<gkv_pool> p(new gkv_pool());
   p->cfg = c;
   p->layer_index.resize(c.n_layers);
   p->layer_is_window.resize(c.n_layers);
@@ -258,22 +262,16 @@ static int pool_create(const gkv_pool_config *cfg, int32_t kept, int32_t slack, 
     int64_t budget = c.bytes_budget;
     if (budget == 0) {
       size_t free_b = 0, total_b = 0;
-      if (hipMemGetInfo(&free_b, &total_b) != hipSuccess) {
-        delete p;
+      if (hipMemGetInfo(&free_b, &total_b) != hipSuccess)
         return GKV_ERR_HIP;
-      }
       budget = (int64_t)(0.9 * (double)free_b);
     }
     nb = (budget - ring_bytes - table_bytes) / (bpl * p->n_full);
-    if (nb <= 0) {
-      delete p;
+    if (nb <= 0)
       return GKV_ERR_CAPACITY;
-    }
   }
-  if (nb > INT32_MAX || p->num_ring_blocks > INT32_MAX) {
-    delete p;
+  if (nb > INT32_MAX || p->num_ring_blocks > INT32_MAX)
     return GKV_ERR_CAPACITY;
-  }
   p->num_blocks = p->n_full > 0 ? nb : 0;
 
   auto dev_alloc = [&](void **ptr, int64_t bytes) -> bool {
@@ -308,10 +306,8 @@ static int pool_create(const gkv_pool_config *cfg, int32_t kept, int32_t slack, 
   ok = ok && dev_alloc((void **)&p->d_table, (int64_t)c.max_seqs * p->table_stride * 4);
   if (ok && p->ring_blocks > 0)
     ok = dev_alloc((void **)&p->d_ring_table, (int64_t)c.max_seqs * p->ring_blocks * 4);
-  if (!ok) {
-    delete p;
+  if (!ok)
     return GKV_ERR_CAPACITY;
-  }
 
   // Unassigned table entries are -1: a kernel that meets one flags it.
   p->h_table.assign((size_t)c.max_seqs * p->table_stride, -1);
@@ -339,12 +335,12 @@ static int pool_create(const gkv_pool_config *cfg, int32_t kept, int32_t slack, 
   p->free_seqs.resize(c.max_seqs);
   for (int s = 0; s < c.max_seqs; s++)
     p->free_seqs[s] = c.max_seqs - 1 - s;
-  if (gkv_pool_sync(p, nullptr) != GKV_OK || hipDeviceSynchronize() != hipSuccess) {
-    delete p;
+  if (gkv_pool_sync(p.get(), nullptr) != GKV_OK || hipDeviceSynchronize() != hipSuccess)
     return GKV_ERR_HIP;
-  }
-  *out = p;
+  *out = p.release();
   return GKV_OK;
+} catch (const std::exception &) {
+  return GKV_ERR_CAPACITY; // out of host memory
 }
 
 extern "C" int gkv_pool_create(const gkv_pool_config *cfg, gkv_pool **out) {
@@ -393,7 +389,7 @@ extern "C" int gkv_pool_seq_alloc(gkv_pool *pool, int32_t *seq_id) {
   return GKV_OK;
 }
 
-extern "C" int gkv_pool_seq_reserve(gkv_pool *pool, int32_t seq_id, int32_t seq_len) {
+extern "C" int gkv_pool_seq_reserve(gkv_pool *pool, int32_t seq_id, int32_t seq_len) try {
   if (!pool || seq_len < 0)
     return GKV_ERR_ARG;
   if (seq_id < 0 || seq_id >= pool->cfg.max_seqs || !pool->seq_live[seq_id])
@@ -415,6 +411,7 @@ extern "C" int gkv_pool_seq_reserve(gkv_pool *pool, int32_t seq_id, int32_t seq_
   }
   if ((int64_t)(need - have) > (int64_t)pool->free_blocks.size())
     return GKV_ERR_CAPACITY; // nothing taken: all or none
+  pool->make_room(need - have);
   const size_t base = (size_t)seq_id * pool->table_stride;
   int32_t *row = &pool->h_table[base];
   for (int32_t j = have; j < need; j++) {
@@ -426,15 +423,18 @@ extern "C" int gkv_pool_seq_reserve(gkv_pool *pool, int32_t seq_id, int32_t seq_
   pool->seq_blocks[seq_id] = need;
   pool->seq_len[seq_id] = len;
   return GKV_OK;
+} catch (const std::exception &) {
+  return GKV_ERR_CAPACITY; // out of host memory
 }
 
-extern "C" int gkv_pool_seq_free(gkv_pool *pool, int32_t seq_id) {
+extern "C" int gkv_pool_seq_free(gkv_pool *pool, int32_t seq_id) try {
   if (!pool)
     return GKV_ERR_ARG;
   if (seq_id < 0 || seq_id >= pool->cfg.max_seqs || !pool->seq_live[seq_id])
     return GKV_ERR_BLOCK;
   const size_t base = (size_t)seq_id * pool->table_stride;
   int32_t *row = &pool->h_table[base];
+  pool->make_room(pool->seq_blocks[seq_id]);
   for (int32_t j = pool->seq_blocks[seq_id] - 1; j >= 0; j--) {
     if (--pool->refs[row[j]] == 0) // (the capacity for every block is there)
       pool->free_blocks.push_back(row[j]);
@@ -445,6 +445,8 @@ extern "C" int gkv_pool_seq_free(gkv_pool *pool, int32_t seq_id) {
   pool->seq_live[seq_id] = 0;
   pool->free_seqs.push_back(seq_id);
   return GKV_OK;
+} catch (const std::exception &) {
+  return GKV_ERR_CAPACITY; // out of host memory
 }
 
 // ---- sharing, trimming, compacting ---------------------------------------------
@@ -472,7 +474,7 @@ extern "C" int gkv_pool_seq_fork(gkv_pool *pool, int32_t parent, int32_t n_token
   const int32_t id = pool->free_seqs.back();
   const size_t from = (size_t)parent * pool->table_stride, to = (size_t)id * pool->table_stride;
   if (full)
-    pool->pending.reserve(pool->pending.size() + shared + part);
+    pool->make_room(shared + part);
   hipStream_t s = (hipStream_t)stream;
   if (full && part) {
     const int st = pool->copy({int2{pool->h_table[from + shared], pool->free_blocks.back()}}, false, s);
@@ -533,7 +535,7 @@ extern "C" int gkv_pool_seq_trim(gkv_pool *pool, int32_t seq_id, int32_t n_token
     return GKV_ERR_ARG;
   const size_t base = (size_t)seq_id * pool->table_stride;
   int32_t *row = &pool->h_table[base];
-  pool->pending.reserve(pool->pending.size() + (have - keep) + 1);
+  pool->make_room((have - keep) + 1);
   // appends go on inside the last block: it has to be this sequence's own
   int32_t own = -1;
   if (n_tokens % kBT != 0 && pool->refs[row[keep - 1]] > 1) {
@@ -589,7 +591,7 @@ extern "C" int gkv_pool_compact(gkv_pool *pool, void *stream, int64_t *n_used) t
   size_t entries = 0;
   for (int32_t q = 0; q < pool->cfg.max_seqs; q++)
     entries += pool->seq_blocks[q];
-  pool->pending.reserve(pool->pending.size() + (moves.empty() ? 0 : entries));
+  pool->make_room(moves.empty() ? 0 : entries);
   const int st = pool->copy(moves, false, (hipStream_t)stream);
   if (st != GKV_OK)
     return st;
