@@ -428,6 +428,9 @@ int gkv_prefill_paged(void *stream, int32_t B, const int32_t *cu_seqlens,
  * t > p - window): a sliding window and the first tokens, which stay visible
  * however far the sequence runs; window = 0: every t <= p (kept is then
  * ignored). kept and window are multiples of 16 (GKV_ERR_UNSUPPORTED otherwise).
+ * Positions are a sequence's own throughout: kept tokens keep theirs, and the distance
+ * that RoPE sees from them grows with the sequence (nothing is numbered anew inside
+ * the cache), as far as the caller's angle tables go.
  * No counterpart in the reference. The cache holds whole blocks, in the formats
  * GKV_V_BF16 and GKV_KV_FP8_BLOCK (the others: GKV_ERR_UNSUPPORTED):
  *   cache.ring = 0            logical block j (positions 16 j .. 16 j + 15) is entry
@@ -483,7 +486,9 @@ size_t gkv_kept_workspace_bytes(int32_t B, int32_t n_kv_heads, int32_t max_seq_l
  * its own token already appended. q, cos_tab / sin_tab, out as in
  * gkv_decode_attention; max_seq_len: host bound of seq_lens, which the angle
  * tables cover (a longer sequence, or one past the table row, sets
- * GKV_DEVERR_LENGTH and is taken at the bound). A sequence of length 0 gets
+ * GKV_DEVERR_LENGTH and is taken at the bound). The bound also picks the form: one far
+ * above the lengths may cost short sequences a second launch (16 of 129 .. 2049 tokens 17 us
+ * instead of 11). A sequence of length 0 gets
  * zeros; so does a head that sees nothing (every block id bad, no sink). At most 8
  * kv heads, 8 query heads per kv head, and about a million sequences. Calls that may overlap need
  * workspaces of their own. Rows are 16-byte aligned (out in bf16: 8-byte), their
@@ -634,6 +639,10 @@ int gkv_pool_seq_fork(gkv_pool *pool, int32_t parent, int32_t n_tokens, void *st
  * would see any of it (on a ring of window + 16 slots it never does while n_tokens does
  * not go back behind the start of the block that was begun last). */
 int gkv_pool_seq_trim(gkv_pool *pool, int32_t seq_id, int32_t n_tokens, void *stream);
+/* (Fork, trim and compact queue their copies on stream at once, and the tables follow with the
+ * next gkv_pool_sync. Queue no append between the two: behind a compaction any sequence's
+ * would go to a block's old place and be lost; behind a trim the sequence's own would go to
+ * the block that others hold.) */
 /* Moves the full layers' blocks in use to the ids 0 .. n - 1 (n in *n_used, which
  * may be NULL): one launch per 32 layers copies what lies behind, on stream, and
  * the next gkv_pool_sync brings the tables; a kernel queued between the two

@@ -596,6 +596,9 @@ void kept_decode_whole_kernel(KeptDecodeArgs a) {
 }
 
 // ---- ranges ----------------------------------------------------------------------
+//
+// (About 30 scalar registers of the prologue and the loop over sequences wait in lanes of a
+// vector register while a wave is in its steps; nothing goes to memory.)
 
 // Range r of the T steps cut into n (n <= 2048): floor(r T / n), in 32 bits.
 __device__ __forceinline__ int range_begin(int r, int T, int n) {

@@ -8,8 +8,8 @@
 // and 32 rows or more share: bound by the issue of vector and matrix instructions (32
 // keys a wave: 57 vector instructions, 16 of them exponentials, about 45 for
 // staging, queries and masks, and 8 matrix ops of 32 cycles). Counted for 8 chunks
-// after 1536 cached tokens (157 us): vector units busy 56% of the time, matrix units
-// 30%, LDS about 45%; what is left is the chain of one wave, which the three others
+// after 1536 cached tokens (159 us): vector units busy 57% of the time, matrix units
+// 28%, LDS about 45%; what is left is the chain of one wave, which the three others
 // of its SIMD do not cover to the end.
 //
 // Work: one workgroup per (prompt, kv head, block of queries), eight waves (or
@@ -51,7 +51,10 @@
 // a weight has them down to 2^-22 of a row's largest and is 0 only below 2^-33 of it: a
 // first key that takes nearly all the weight leaves the others theirs. (The reference
 // starts below every score, not at the sink, which joins at the end in fp32: against a
-// sink 18 nats above the scores the weights would all be 0.)
+// sink 18 nats above the scores the weights would all be 0. It costs a row's first step
+// a second forming of its weights: 8 chunks after 1536 cached tokens 156 -> 160 us, 12
+// prompts with a window of 128 106.5 -> 109. References 10 and 12 bits below the largest score
+// move more often: 166 and 174, 111 and 119.)
 #include "kept.hpp"
 #include "lds_dma.hpp"
 
@@ -75,7 +78,9 @@ constexpr float kPSum = 32768.0f;       // a lane's weights of a step, at most: 
 // takes the other's place, and a single tile cannot be split. Measured (us, one group /
 // two, 8 kv heads, codes): one prompt of 32 rows 9.6 / 10.2, of 200 13.3 / 12.8, of 1024
 // 38.5 / 32.6; 512 rows after 30000 738 / 591; 8 chunks of up to 128 after 2048 with a
-// window of 256 19.8 / 18.5; 416 workgroups (2 of up to 800 after 4096) 171 / 187.
+// window of 256 19.8 / 18.5; 416 workgroups (2 of up to 800 after 4096) 171 / 187. How much
+// history a chunk has the host does not know: 16 to 64 rows after 16 cached ones 8.6 / 10.0,
+// after 128 12.0 / 12.1, after 512 23.2 / 20.6, after 2048 64.6 / 52.3.
 constexpr int64_t kPFewWgs = 256;
 constexpr int kPShort = 128; // rows of a prompt without a history that stay with one group
 constexpr int kPBand = 2;               // query blocks per band of the grid order
