@@ -620,12 +620,15 @@ class Pool:
         return lib().gkv_pool_seq_free(self.h, seq)
 
     def fork(self, parent: int, n_tokens: int, stream=None) -> int:
+        """gkv_pool_seq_fork: a new sequence of parent's first n_tokens (with window layers: as far
+        back as the rings hold, by the lengths last reserved; GkvError beyond)."""
         s = _i32()
         check("gkv_pool_seq_fork", lib().gkv_pool_seq_fork(self.h, parent, n_tokens,
                                                            stream_handle(stream), ctypes.byref(s)))
         return s.value
 
     def trim(self, seq: int, n_tokens: int, stream=None):
+        """gkv_pool_seq_trim: cuts seq back to n_tokens (with window layers as fork does)."""
         check("gkv_pool_seq_trim", lib().gkv_pool_seq_trim(self.h, seq, n_tokens,
                                                            stream_handle(stream)))
 
