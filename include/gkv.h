@@ -72,6 +72,8 @@ typedef enum {
                                   holds inf there); gkv_kept_prefill: see there */
 #define GKV_DEVERR_PLAN 16u    /* gkv_decode_layer_planned was asked to reuse a plan the
                                   workspace does not hold for this call (it planned afresh) */
+#define GKV_DEVERR_CAPACITY 32u /* gkv_tables_resize: too few free blocks, or more new rows than
+                                  max_rows (nothing was changed) */
 
 typedef enum { GKV_F32 = 0, GKV_BF16 = 1 } gkv_dtype;
 
@@ -529,6 +531,132 @@ int gkv_kept_prefill(void *stream, int32_t B, const int32_t *cu_seqlens, const i
  * copied there. No counterpart in the reference. */
 int gkv_copy_blocks(void *stream, const gkv_cache_view *views, int32_t n_views, int32_t n_pairs,
                     const int32_t *src, const int32_t *dst, uint32_t *dev_err);
+
+/* ---- Sequences that share their first blocks ------------------------------ */
+
+/* Bytes of workspace that gkv_shared_decode needs for these sizes (0: none; workspace may be
+ * NULL then). */
+size_t gkv_shared_workspace_bytes(int32_t B, int32_t n_groups, int32_t n_q_heads,
+                                  int32_t n_kv_heads, int32_t max_shared_blocks, int32_t max_own);
+
+/* Decode attention for samples and beams of one prompt, or a batch behind one system prompt:
+ * gkv_kept_decode's (window 0: every cached position is seen; the same formats, arguments,
+ * bounds and results, up to rounding), which reads the blocks that a group's sequences share
+ * once for all of them. No counterpart in the reference.
+ *   cu_groups      device int32 [n_groups + 1]: group g is the sequences cu_groups[g] ..
+ *                  cu_groups[g + 1] - 1, in order, groups of any size (0, 1: nothing gained). A
+ *                  sequence in no group is read on its own.
+ *   shared_blocks  device int32 [n_groups]: the first shared_blocks[g] blocks (16 positions each,
+ *                  all full) are the same for the whole group, and are read through
+ *                  the table row of the group's first sequence; the other rows' entries
+ *                  there are not looked at (one more than a table row has is taken at the row's
+ *                  length: GKV_DEVERR_LENGTH). A sequence that ends before them is read on
+ *                  its own, through its own row. gkv_tables_reorder counts them; forks of the
+ *                  pool share what gkv_pool_seq_fork was given, in full blocks.
+ *   max_shared_blocks, max_own   what the largest shared_blocks and the most tokens behind
+ *                  them are about: they size the grids and the workspace, and more or less of
+ *                  either changes the time only
+ *   q, cos_tab / sin_tab, seq_lens, max_seq_len, sinks (NULL: none), out   as in
+ *                  gkv_kept_decode; the new tokens are appended
+ * A window layer of such sequences reads its window only: gkv_kept_decode. Results do not
+ * depend on the order in which workgroups run. For bf16 outputs, weights of shared tokens
+ * are rounded to bf16 (each off by at most 2^-8 of itself), and q against e4m3 codes to 11 bits.
+ * Calls that may overlap need workspaces of their own. */
+int gkv_shared_decode(void *stream, int32_t B, int32_t n_groups, const int32_t *cu_groups,
+                      const int32_t *shared_blocks, int32_t max_shared_blocks, int32_t max_own,
+                      int32_t n_q_heads, const float *q, int64_t q_stride, const float *cos_tab,
+                      const float *sin_tab, const int32_t *seq_lens, int32_t max_seq_len,
+                      gkv_cache_view cache, const float *sinks, void *workspace,
+                      size_t workspace_bytes, void *out, int64_t out_stride, int32_t out_dtype,
+                      uint32_t *dev_err);
+
+/* ---- Beam search ------------------------------------------------------------ */
+
+/* Bytes of workspace that gkv_beam_select needs for up to n_requests requests of up to n_beams
+ * beams. */
+size_t gkv_beam_workspace_bytes(int32_t n_requests, int32_t n_beams, int32_t vocab,
+                                int32_t n_out);
+
+/* The n_out best continuations of every request's beams. Beam k of request r is row
+ * r * n_beams + k of
+ *   logits      fp32 or bf16 (gkv_dtype) [rows][row_stride], any alignment of its elements
+ *   cum_scores  fp32 [rows]: the sum of the beam's log-probabilities (-inf: a place without
+ *               a beam, whose logits are not read)
+ *   done        NULL, or int32 [rows], not 0: the beam has ended, its logits are not read, and its
+ *               one continuation is the token eos at the score that it has
+ * and its continuation by token t scores cum_scores + logit[t] - log sum exp(logits). The n_out
+ * largest logits of every beam (of equal ones the lower token) compete, best score
+ * first, equal scores by the lower beam, then the lower token (scores of -inf too, where too few
+ * others are there; formed and compared in 64 bits):
+ *   scores      fp32 [n_requests][n_out]
+ *   parents     int32 [n_requests][n_out]: the row continued, r * n_beams + k
+ *   tokens      int32 [n_requests][n_out]
+ *   done_out    NULL, or int32 [n_requests][n_out]: 1 where the token is eos or the beam had ended
+ * With n_out = n_beams, scores, done_out and parents are the next step's cum_scores and done and
+ * gkv_tables_reorder's parents (of groups of n_beams). eos < 0: no token ends a beam (done NULL).
+ * n_out <= 64 and vocab, n_beams <= 64, fewer than 2^23 rows (GKV_ERR_UNSUPPORTED). A logit
+ * that is NaN counts as -inf, one of +inf as the largest fp32 number, cum_scores the same:
+ * GKV_DEVERR_RANGE. Inputs and outputs do not overlap. No counterpart in the reference. */
+int gkv_beam_select(void *stream, int32_t n_requests, int32_t n_beams, int32_t vocab,
+                    const void *logits, int64_t row_stride, int32_t logits_dtype,
+                    const float *cum_scores, const int32_t *done, int32_t eos, int32_t n_out,
+                    float *scores, int32_t *parents, int32_t *tokens, int32_t *done_out,
+                    void *workspace, size_t workspace_bytes, uint32_t *dev_err);
+
+/* ---- Block tables on the GPU ------------------------------------------------- */
+
+/* Block tables that the GPU itself keeps, without the host (which gkv_pool_* needs): for steps
+ * that are captured into a graph, and for beams, whose rows move with every token. All arrays are
+ * the caller's, in device memory; the caches are too (num_blocks blocks, any format, any number of
+ * layers under one table; window layers read it as the ring = 0 form of gkv_kept_*).
+ *   table  int32 [n_seqs][table_stride]: row s holds ceil(lens[s] / 16) blocks, -1 behind them
+ *   lens   int32 [n_seqs]: tokens of each sequence (0: an idle place): the seq_lens of
+ *          the appends and attention
+ *   refs   int32 [num_blocks]: how many table entries hold the block (0: free)
+ * No counterpart in the reference. */
+typedef struct {
+  int32_t *table;
+  int32_t *lens;
+  int32_t *refs;
+  int32_t table_stride;
+  int32_t n_seqs;
+  int32_t num_blocks;
+} gkv_tables;
+
+/* Empty rows, all blocks free. */
+int gkv_tables_init(void *stream, gkv_tables tables);
+
+/* Bytes of workspace that gkv_tables_resize needs (also for fewer sequences or blocks). */
+size_t gkv_tables_workspace_bytes(int32_t n_seqs, int32_t num_blocks);
+
+/* Gives every sequence the length new_lens[s] (device int32 [n_seqs]): takes the blocks that it
+ * lacks, gives back those it has too many (free from the next call on). Blocks are taken in
+ * the order of the sequences, the lowest free ids first. A sequence that grows inside a
+ * partly filled block that other entries hold gets one of its own there (all of its holders do
+ * that grow in the call); copy_src[s], copy_dst[s] (NULL both: the caller shares no blocks) name
+ * the copy, 0 and 0 where there is none: pairs for gkv_copy_blocks, before anything is appended.
+ * The new rows, sequence after sequence (row r is what gkv_kv_append and the others call row r):
+ *   cu_rows   NULL, or int32 [n_seqs + 1]: sequence s has the rows cu_rows[s] .. cu_rows[s+1] - 1
+ *   row_seq, row_pos   NULL, or int32 [max_rows]: the row's sequence and position
+ *   row_slot  NULL, or int64 [max_rows]: its place in the pool, block * 16 + position % 16
+ * rows behind the last one are left as they were. Too few free blocks, or more new rows than
+ * max_rows (of no account without the row arrays): GKV_DEVERR_CAPACITY, and nothing
+ * changes (cu_rows and the pairs are 0). A length below 0 or beyond a row: GKV_DEVERR_LENGTH, and
+ * that sequence stays as it is. new_lens may be lens itself (nothing happens). */
+int gkv_tables_resize(void *stream, gkv_tables tables, const int32_t *new_lens, int32_t *copy_src,
+                      int32_t *copy_dst, int32_t max_rows, int32_t *cu_rows, int32_t *row_seq,
+                      int32_t *row_pos, int64_t *row_slot, void *workspace,
+                      size_t workspace_bytes, uint32_t *dev_err);
+
+/* Rows follow their parents, in place: sequence s becomes what parents[s] was (device int32
+ * [n_seqs]; -1: empty), its blocks shared with all others that hold them, blocks that nobody
+ * holds any more free. Parents lie in the sequence's own group of group_size sequences (0 ..
+ * group_size - 1 the first; n_seqs is a multiple of it, group_size <= 2048); one outside:
+ * GKV_DEVERR_BLOCK_ID, and the sequence stays. shared_blocks: NULL, or int32
+ * [n_seqs / group_size]: the leading full blocks that all rows of the group now
+ * have in common (gkv_shared_decode's). */
+int gkv_tables_reorder(void *stream, gkv_tables tables, int32_t group_size,
+                       const int32_t *parents, int32_t *shared_blocks, uint32_t *dev_err);
 
 /* ---- Exact path (fp32 caches, bit for bit with the CPU forward) ---------- */
 

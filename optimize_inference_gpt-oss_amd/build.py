@@ -33,6 +33,9 @@ SOURCES = [
     "kept_append.hip",
     "kept_decode.hip",
     "kept_prefill.hip",
+    "shared_decode.hip",
+    "beam_select.hip",
+    "block_tables.hip",
     "rope_table.cpp",
     "kv_pool.cpp",
     "capi.cpp",

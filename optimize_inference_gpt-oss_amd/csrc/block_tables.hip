@@ -1,0 +1,456 @@
+// Block tables kept on the GPU: blocks taken and given back by the sequences' lengths, rows
+// that follow the chosen parents, and the map of new rows to slots.
+//
+// The state is the table, the lengths and, per block, how many table entries hold it (0: free);
+// a length says which entries a row holds (ceil(len / 16)). Blocks are shared freely by a
+// reorder; a row that goes on inside a block that others hold gets one of its own from the next
+// resize, which names the copy.
+//
+// The n-th block that a call takes is the n-th lowest free id: that needs no list of
+// free blocks, whose order would depend on who gave back first, and keeps the pool's low end dense.
+// All of it is whole numbers and sums, so results do not depend on the order of the atomics.
+// Everything here moves kilobytes: latency bounds it, and launches and dependent loads are
+// what is counted.
+#include "gkv_device.hpp"
+
+#include <algorithm>
+
+namespace gkv {
+
+constexpr int kTableThreads = 1024;
+
+struct TablesArgs {
+  int32_t *table, *lens, *refs;
+  int stride, n_seqs, num_blocks;
+  uint32_t *dev_err;
+};
+
+__device__ __forceinline__ void flag(uint32_t *dev_err, uint32_t bit) {
+  if (dev_err)
+    atomicOr(dev_err, bit);
+}
+
+__device__ __forceinline__ int blocks_of(int len) { return (int)(((uint32_t)len + 15u) / 16u); }
+
+// A row's length as far as its row goes (a length that no row can have counts as 0).
+__device__ __forceinline__ int sane(int len, int stride) {
+  return len < 0 || blocks_of(len) > stride ? 0 : len;
+}
+
+// ---- init ---------------------------------------------------------------------------
+
+__global__ __launch_bounds__(256) void tables_init_kernel(TablesArgs a) {
+  const int64_t n = (int64_t)a.n_seqs * a.stride, step = (int64_t)gridDim.x * 256;
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  for (int64_t i = t; i < n; i += step)
+    a.table[i] = -1;
+  for (int64_t i = t; i < a.n_seqs; i += step)
+    a.lens[i] = 0;
+  for (int64_t i = t; i < a.num_blocks; i += step)
+    a.refs[i] = 0;
+}
+
+// ---- resize ---------------------------------------------------------------------------
+
+struct ResizeArgs {
+  TablesArgs t;
+  const int32_t *new_lens;
+  int32_t *copy_src, *copy_dst;
+  int max_rows;
+  int32_t *cu_rows, *row_seq, *row_pos;
+  int64_t *row_slot;
+  // left by the plan for the second launch
+  int32_t *ok;    // 1: the call is carried out
+  int32_t *old;   // [n_seqs] lengths before the call; -1: the row is left as it is
+  int32_t *first; // [n_seqs] place of its first taken block among all; bit 31: that one replaces
+                  // the partly filled block that others hold
+  int32_t *cu;    // [n_seqs + 1] new rows before each sequence
+  int32_t *ids;   // [num_blocks] the blocks taken
+};
+
+// Sum over the workgroup of the values before this thread's, and of all.
+__device__ __forceinline__ int64_t scan_before(int64_t x, int64_t *s_wave, int64_t &total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n_waves = blockDim.x >> 6;
+  int64_t incl = x;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int64_t v = __shfl_up(incl, off, 64);
+    if (lane >= off)
+      incl += v;
+  }
+  __syncthreads(); // (s_wave may still be read for the scan before)
+  if (lane == 63)
+    s_wave[wave] = incl;
+  __syncthreads();
+  int64_t before = 0;
+  total = 0;
+  for (int w = 0; w < n_waves; w++) {
+    const int64_t v = s_wave[w];
+    before += w < wave ? v : 0;
+    total += v;
+  }
+  return before + incl - x;
+}
+
+// What a resize does to one row.
+struct RowPlan {
+  int old, now;
+  bool split;  // the block at its end is held by others too
+  int take, rows;
+};
+
+__device__ __forceinline__ RowPlan row_plan(const ResizeArgs &a, int s) {
+  const TablesArgs &t = a.t;
+  RowPlan p{};
+  const int len = t.lens[s], want = a.new_lens[s];
+  p.old = sane(len, t.stride);
+  p.now = want;
+  if (p.old != len || want < 0 || blocks_of(want) > t.stride) {
+    flag(t.dev_err, GKV_DEVERR_LENGTH);
+    p.old = -1; // left as it is
+    return p;
+  }
+  if (want > p.old) {
+    if (p.old % kBlockTokens != 0) {
+      const int id = t.table[(int64_t)s * t.stride + p.old / kBlockTokens];
+      p.split = (uint32_t)id < (uint32_t)t.num_blocks && t.refs[id] > 1;
+    }
+    p.take = (p.split ? 1 : 0) + blocks_of(want) - blocks_of(p.old);
+    p.rows = want - p.old;
+  }
+  return p;
+}
+
+// One workgroup: what each row takes, where its rows begin, and the ids of the blocks; the
+// lengths, if there is room for all.
+constexpr int kRefsEach = 16; // holders a thread looks at in one go
+__global__ __launch_bounds__(kTableThreads) void tables_plan_kernel(ResizeArgs a) {
+  __shared__ int64_t s_wave[kTableThreads / 64];
+  const TablesArgs &t = a.t;
+  const int tid = threadIdx.x;
+  int64_t need = 0, rows = 0;
+  for (int s0 = 0; s0 < t.n_seqs; s0 += kTableThreads) {
+    const int s = s0 + tid;
+    RowPlan p{};
+    if (s < t.n_seqs)
+      p = row_plan(a, s);
+    int64_t all, all_rows;
+    const int64_t at = need + scan_before(p.take, s_wave, all);
+    const int64_t row = rows + scan_before(p.rows, s_wave, all_rows);
+    if (s < t.n_seqs) {
+      a.old[s] = p.old;
+      a.first[s] = (int)(at & 0x7fffffff) | (p.split ? (int)0x80000000u : 0);
+      a.cu[s] = (int)row;
+    }
+    need += all;
+    rows += all_rows;
+  }
+  bool ok = need <= t.num_blocks && rows <= a.max_rows;
+  // the lowest free ids, as many as are needed
+  int64_t found = 0;
+  const int n_tiles = (t.num_blocks + kTableThreads * kRefsEach - 1) / (kTableThreads * kRefsEach);
+  for (int k = 0; ok && k < n_tiles && found < need; k++) {
+    const int64_t base = ((int64_t)k * kTableThreads + tid) * kRefsEach;
+    uint32_t free = 0;
+#pragma unroll
+    for (int i = 0; i < kRefsEach; i++)
+      if (base + i < t.num_blocks && t.refs[base + i] == 0)
+        free |= 1u << i;
+    int64_t all;
+    int64_t at = found + scan_before(__popc(free), s_wave, all);
+    for (; free != 0 && at < need; free &= free - 1)
+      a.ids[at++] = (int)base + __ffs(free) - 1;
+    found += all;
+  }
+  ok = ok && found >= need;
+  if (tid == 0) {
+    *a.ok = ok;
+    a.cu[t.n_seqs] = (int)rows;
+    if (!ok)
+      flag(t.dev_err, GKV_DEVERR_CAPACITY);
+  }
+  __syncthreads();
+  for (int s = tid; s <= t.n_seqs; s += kTableThreads)
+    if (a.cu_rows)
+      a.cu_rows[s] = ok ? a.cu[s] : 0;
+  if (ok)
+    for (int s = tid; s < t.n_seqs; s += kTableThreads)
+      if (a.old[s] >= 0)
+        t.lens[s] = a.new_lens[s];
+}
+
+// The sequence that new row r belongs to: the last s with cu[s] <= r, in 0 .. n - 1.
+__device__ __forceinline__ int sequence_of(const int32_t *cu, int n, int r) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (int)(((uint32_t)lo + (uint32_t)hi) / 2);
+    if (cu[mid] <= r)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+// A wave per sequence: its entries, their holders and its copy; behind those, a thread per new
+// row: its sequence, position and slot, from the plan alone.
+__global__ __launch_bounds__(256) void tables_apply_kernel(ResizeArgs a, int seq_wgs) {
+  const TablesArgs &t = a.t;
+  const bool ok = *a.ok != 0;
+  if ((int)blockIdx.x < seq_wgs) {
+    const int s = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (s >= t.n_seqs)
+      return;
+    int src = 0, dst = 0;
+    const int old = a.old[s];
+    if (ok && old >= 0) {
+      int32_t *row = t.table + (int64_t)s * t.stride;
+      const int have = blocks_of(old), want = blocks_of(a.new_lens[s]);
+      const bool split = a.first[s] < 0;
+      int at = a.first[s] & 0x7fffffff;
+      if (split) {
+        if (lane == 0) {
+          src = row[have - 1];
+          dst = a.ids[at];
+          row[have - 1] = dst;
+          atomicSub(t.refs + src, 1);
+          t.refs[dst] = 1;
+        }
+        at++;
+      }
+      for (int j = have + lane; j < want; j += 64) {
+        const int id = a.ids[at + j - have];
+        row[j] = id;
+        t.refs[id] = 1;
+      }
+      for (int j = want + lane; j < have; j += 64) {
+        const int id = row[j];
+        row[j] = -1;
+        if ((uint32_t)id < (uint32_t)t.num_blocks)
+          atomicSub(t.refs + id, 1);
+        else
+          flag(t.dev_err, GKV_DEVERR_BLOCK_ID);
+      }
+    }
+    if (lane == 0 && a.copy_src) {
+      a.copy_src[s] = src;
+      a.copy_dst[s] = dst;
+    }
+    return;
+  }
+  const int64_t r = (int64_t)((int)blockIdx.x - seq_wgs) * 256 + threadIdx.x;
+  if (!ok || r >= a.cu[t.n_seqs])
+    return;
+  const int s = sequence_of(a.cu, t.n_seqs, (int)r);
+  const int pos = a.old[s] + (int)r - a.cu[s];
+  if (a.row_seq)
+    a.row_seq[r] = s;
+  if (a.row_pos)
+    a.row_pos[r] = pos;
+  if (a.row_slot) {
+    const int have = blocks_of(a.old[s]), j = pos / kBlockTokens, at = a.first[s] & 0x7fffffff;
+    const bool split = a.first[s] < 0;
+    int id;
+    if (j >= have)
+      id = a.ids[at + (split ? 1 : 0) + j - have];
+    else
+      id = split ? a.ids[at] : t.table[(int64_t)s * t.stride + j];
+    a.row_slot[r] = (int64_t)id * kBlockTokens + pos % kBlockTokens;
+  }
+}
+
+// ---- reorder ----------------------------------------------------------------------------
+
+struct ReorderArgs {
+  TablesArgs t;
+  const int32_t *parents;
+  int per;             // rows of a group
+  int width;           // columns of a tile
+  int32_t *shared;     // NULL, or per group the leading blocks that all its rows hold
+};
+
+// One workgroup per group, tile of columns after tile: the rows' entries go to LDS, and each
+// row takes its parent's from there, so it works in place. Holders change only
+// where the entry does (rows of a beam search share most of their blocks).
+constexpr int kTileEntries = 1 << 13;
+__global__ __launch_bounds__(kTableThreads) void tables_reorder_kernel(ReorderArgs a) {
+  extern __shared__ int32_t s_mem[];
+  const TablesArgs &t = a.t;
+  int32_t *s_tile = s_mem, *s_parent = s_mem + a.per * a.width, *s_len = s_parent + a.per;
+  __shared__ int s_max, s_min, s_first;
+  const int tid = threadIdx.x, base = blockIdx.x * a.per;
+  if (tid == 0) {
+    s_max = 0;
+    s_min = INT32_MAX;
+    s_first = INT32_MAX;
+  }
+  __syncthreads();
+  for (int i = tid; i < a.per; i += kTableThreads) {
+    int p = a.parents[base + i];
+    if (p != -1 && (p < base || p >= base + a.per)) {
+      flag(t.dev_err, GKV_DEVERR_BLOCK_ID);
+      p = base + i;
+    }
+    s_parent[i] = p < 0 ? -1 : p - base;
+    const int len = t.lens[base + i];
+    s_len[i] = sane(len, t.stride);
+    if (s_len[i] != len)
+      flag(t.dev_err, GKV_DEVERR_LENGTH);
+    atomicMax(&s_max, blocks_of(s_len[i]));
+  }
+  __syncthreads();
+  const int cols = s_max;
+  for (int c0 = 0; c0 < cols; c0 += a.width) {
+    const int w = min(a.width, cols - c0);
+    for (int e = tid; e < a.per * w; e += kTableThreads) {
+      const int i = e / w, c = e % w;
+      const bool held = c0 + c < blocks_of(s_len[i]);
+      s_tile[i * a.width + c] = held ? t.table[(int64_t)(base + i) * t.stride + c0 + c] : -1;
+    }
+    __syncthreads();
+    const int p0 = s_parent[0];
+    for (int e = tid; e < a.per * w; e += kTableThreads) {
+      const int i = e / w, c = e % w, p = s_parent[i];
+      const int was = s_tile[i * a.width + c], now = p < 0 ? -1 : s_tile[p * a.width + c];
+      if (now != was) {
+        t.table[(int64_t)(base + i) * t.stride + c0 + c] = now;
+        if ((uint32_t)was < (uint32_t)t.num_blocks)
+          atomicSub(t.refs + was, 1);
+        if ((uint32_t)now < (uint32_t)t.num_blocks)
+          atomicAdd(t.refs + now, 1);
+      }
+      if (now != (p0 < 0 ? -1 : s_tile[p0 * a.width + c]))
+        atomicMin(&s_first, c0 + c);
+    }
+    __syncthreads();
+  }
+  for (int i = tid; i < a.per; i += kTableThreads) {
+    const int len = s_parent[i] < 0 ? 0 : s_len[s_parent[i]];
+    t.lens[base + i] = len;
+    atomicMin(&s_min, len / kBlockTokens);
+  }
+  __syncthreads();
+  if (tid == 0 && a.shared)
+    a.shared[blockIdx.x] = min(s_min, s_first);
+}
+
+// ---- host side ------------------------------------------------------------------------
+
+static int tables_check(const gkv_tables &t) {
+  if (!t.table || !t.lens || !t.refs || t.table_stride <= 0 || t.n_seqs < 0 || t.num_blocks <= 0)
+    return GKV_ERR_ARG;
+  if (((uintptr_t)t.table | (uintptr_t)t.lens | (uintptr_t)t.refs) % 4 != 0)
+    return GKV_ERR_ARG;
+  if (t.table_stride > (1 << 27)) // (positions in 32 bits)
+    return GKV_ERR_UNSUPPORTED;
+  return GKV_OK;
+}
+
+static TablesArgs tables_args(const gkv_tables &t, uint32_t *dev_err) {
+  return TablesArgs{t.table, t.lens, t.refs, t.table_stride, t.n_seqs, t.num_blocks, dev_err};
+}
+
+struct TablesWorkspace {
+  size_t old, first, cu, ids, total; // (the flag comes first)
+};
+static TablesWorkspace tables_workspace(int32_t n_seqs, int32_t num_blocks) {
+  auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
+  TablesWorkspace w;
+  w.old = 256;
+  w.first = w.old + up((size_t)n_seqs * 4);
+  w.cu = w.first + up((size_t)n_seqs * 4);
+  w.ids = w.cu + up(((size_t)n_seqs + 1) * 4);
+  w.total = w.ids + (size_t)num_blocks * 4;
+  return w;
+}
+
+} // namespace gkv
+
+extern "C" int gkv_tables_init(void *stream, gkv_tables t) {
+  using namespace gkv;
+  const int st = tables_check(t);
+  if (st != GKV_OK)
+    return st;
+  const int64_t n = std::max<int64_t>((int64_t)t.n_seqs * t.table_stride, t.num_blocks);
+  const int64_t wgs = std::min<int64_t>((n + 255) / 256, 4096);
+  hipLaunchKernelGGL(tables_init_kernel, dim3((unsigned)wgs), dim3(256), 0, (hipStream_t)stream,
+                     tables_args(t, nullptr));
+  return launch_status("tables_init_kernel");
+}
+
+extern "C" size_t gkv_tables_workspace_bytes(int32_t n_seqs, int32_t num_blocks) {
+  if (n_seqs < 0 || num_blocks <= 0)
+    return 0;
+  return gkv::tables_workspace(n_seqs, num_blocks).total;
+}
+
+extern "C" int gkv_tables_resize(void *stream, gkv_tables t, const int32_t *new_lens,
+                                 int32_t *copy_src, int32_t *copy_dst, int32_t max_rows,
+                                 int32_t *cu_rows, int32_t *row_seq, int32_t *row_pos,
+                                 int64_t *row_slot, void *workspace, size_t workspace_bytes,
+                                 uint32_t *dev_err) {
+  using namespace gkv;
+  int st = tables_check(t);
+  if (st != GKV_OK)
+    return st;
+  const bool maps = row_seq || row_pos || row_slot;
+  if (!new_lens || (copy_src == nullptr) != (copy_dst == nullptr) || max_rows < 0)
+    return GKV_ERR_ARG;
+  if (((uintptr_t)new_lens | (uintptr_t)copy_src | (uintptr_t)copy_dst | (uintptr_t)cu_rows |
+       (uintptr_t)row_seq | (uintptr_t)row_pos) % 4 != 0 || (uintptr_t)row_slot % 8 != 0 ||
+      (uintptr_t)workspace % 16 != 0)
+    return GKV_ERR_ARG;
+  const TablesWorkspace w = tables_workspace(t.n_seqs, t.num_blocks);
+  if (!workspace || workspace_bytes < w.total)
+    return GKV_ERR_WORKSPACE;
+  char *ws = (char *)workspace;
+  ResizeArgs a{};
+  a.t = tables_args(t, dev_err);
+  a.new_lens = new_lens;
+  a.copy_src = copy_src;
+  a.copy_dst = copy_dst;
+  a.max_rows = maps ? max_rows : INT32_MAX;
+  a.cu_rows = cu_rows;
+  a.row_seq = row_seq;
+  a.row_pos = row_pos;
+  a.row_slot = row_slot;
+  a.ok = (int32_t *)ws;
+  a.old = (int32_t *)(ws + w.old);
+  a.first = (int32_t *)(ws + w.first);
+  a.cu = (int32_t *)(ws + w.cu);
+  a.ids = (int32_t *)(ws + w.ids);
+  const int seq_wgs = (int)(((int64_t)t.n_seqs + 3) / 4);
+  const int64_t wgs = seq_wgs + (maps ? ((int64_t)max_rows + 255) / 256 : 0);
+  if (!grid_fits(wgs, 256))
+    return GKV_ERR_UNSUPPORTED;
+  hipStream_t s = (hipStream_t)stream;
+  hipLaunchKernelGGL(tables_plan_kernel, dim3(1), dim3(kTableThreads), 0, s, a);
+  if ((st = launch_status("tables_plan_kernel")) || wgs == 0)
+    return st;
+  hipLaunchKernelGGL(tables_apply_kernel, dim3((unsigned)wgs), dim3(256), 0, s, a, seq_wgs);
+  return launch_status("tables_apply_kernel");
+}
+
+extern "C" int gkv_tables_reorder(void *stream, gkv_tables t, int32_t group_size,
+                                  const int32_t *parents, int32_t *shared_blocks,
+                                  uint32_t *dev_err) {
+  using namespace gkv;
+  const int st = tables_check(t);
+  if (st != GKV_OK)
+    return st;
+  if (!parents || group_size <= 0 || t.n_seqs % group_size != 0 ||
+      ((uintptr_t)parents | (uintptr_t)shared_blocks) % 4 != 0)
+    return GKV_ERR_ARG;
+  if (group_size > kTileEntries / 4)
+    return GKV_ERR_UNSUPPORTED;
+  if (t.n_seqs == 0)
+    return GKV_OK;
+  ReorderArgs a{tables_args(t, dev_err), parents, group_size, kTileEntries / group_size, shared_blocks};
+  a.width = std::min(a.width, t.table_stride);
+  const size_t lds = ((size_t)a.width * group_size + 2 * (size_t)group_size) * 4;
+  if (!grid_fits(t.n_seqs / group_size, kTableThreads))
+    return GKV_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL(tables_reorder_kernel, dim3((unsigned)(t.n_seqs / group_size)),
+                     dim3(kTableThreads), lds, (hipStream_t)stream, a);
+  return launch_status("tables_reorder_kernel");
+}

@@ -24,6 +24,7 @@ DEVERR_BLOCK_ID = 1
 DEVERR_LENGTH = 2
 DEVERR_ALIGN = 4
 DEVERR_RANGE = 8
+DEVERR_CAPACITY = 32
 F32 = 0
 BF16 = 1
 
@@ -39,6 +40,12 @@ class CacheView(ctypes.Structure):
     _fields_ = [("k", _vp), ("v", _vp), ("block_table", _vp), ("table_stride", _i32),
                 ("num_blocks", _i32), ("n_kv_heads", _i32), ("ring", _i32),
                 ("v_scale", _vp), ("v_format", _i32)]
+
+
+class BlockTables(ctypes.Structure):
+    """gkv_tables: made by block_tables() over torch tensors."""
+    _fields_ = [("table", _vp), ("lens", _vp), ("refs", _vp), ("table_stride", _i32),
+                ("n_seqs", _i32), ("num_blocks", _i32)]
 
 
 V_BF16, V_INT8, KV_FP8, KV_FP8_BLOCK = 0, 1, 2, 3
@@ -140,6 +147,18 @@ SIGNATURES = {
                                         _vp]),
     "gkv_copy_blocks": (ctypes.c_int, [_vp, ctypes.POINTER(CacheView), _i32, _i32, _vp, _vp,
                                        _vp]),
+    "gkv_shared_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32, _i32, _i32]),
+    "gkv_shared_decode": (ctypes.c_int, [_vp, _i32, _i32, _vp, _vp, _i32, _i32, _i32, _vp, _i64,
+                                         _vp, _vp, _vp, _i32, CacheView, _vp, _vp, _sz, _vp, _i64,
+                                         _i32, _vp]),
+    "gkv_beam_workspace_bytes": (_sz, [_i32, _i32, _i32, _i32]),
+    "gkv_beam_select": (ctypes.c_int, [_vp, _i32, _i32, _i32, _vp, _i64, _i32, _vp, _vp, _i32,
+                                       _i32, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "gkv_tables_init": (ctypes.c_int, [_vp, BlockTables]),
+    "gkv_tables_workspace_bytes": (_sz, [_i32, _i32]),
+    "gkv_tables_resize": (ctypes.c_int, [_vp, BlockTables, _vp, _vp, _vp, _i32, _vp, _vp, _vp,
+                                         _vp, _vp, _sz, _vp]),
+    "gkv_tables_reorder": (ctypes.c_int, [_vp, BlockTables, _i32, _vp, _vp, _vp]),
     "gkv_rope_exact": (ctypes.c_int, [_vp, _i32, _vp, _i64, _vp, _vp, _vp, _i32]),
     "gkv_kv_write_exact": (ctypes.c_int, [_vp, _i32, _vp, _i64, _i32, _i32, _vp, _vp, _i32, _i32,
                                           _i32, _vp, _i32, _vp]),
@@ -578,6 +597,141 @@ def copy_blocks(views, src, dst, dev_err=None, stream=None):
     st = L.gkv_copy_blocks(stream_handle(stream), views, len(views), src.numel(),
                            _ints(src, "src"), _ints(dst, "dst"), ptr(dev_err))
     check("gkv_copy_blocks", st)
+
+
+# Sequences that share blocks, beams, tables on the GPU. The same checks: ValueError for a
+# tensor whose address must not be handed over.
+
+
+def _of(n, t, what, dtype=None):
+    """Address of a contiguous device tensor of n int32 (or dtype) elements, which may be None."""
+    if t is None:
+        return None
+    if t.numel() != n:
+        _refuse(what, f"not {n} elements")
+    if dtype is None:
+        return _ints(t, what)
+    if t.dtype is not dtype or not t.is_contiguous():
+        _refuse(what, f"not contiguous {dtype}")
+    if not t.is_cuda and not t.is_pinned():
+        _refuse(what, "not in GPU memory")
+    return t.data_ptr()
+
+
+def _ws(t):
+    """Address and bytes of a workspace, which may be None."""
+    return (None, 0) if t is None else (t.data_ptr(), t.numel() * t.element_size())
+
+
+def shared_workspace_bytes(B, n_groups, n_q_heads, n_kv_heads, max_shared_blocks, max_own) -> int:
+    return lib().gkv_shared_workspace_bytes(B, n_groups, n_q_heads, n_kv_heads, max_shared_blocks,
+                                            max_own)
+
+
+def shared_decode(q, n_q_heads, cu_groups, shared_blocks, seq_lens, max_seq_len, view: CacheView,
+                  out, max_shared_blocks, max_own, sinks=None, cos_tab=None, sin_tab=None,
+                  workspace=None, dev_err=None, stream=None):
+    """gkv_shared_decode: kept_decode (window 0) for groups of sequences whose first
+    shared_blocks[g] blocks are the same, which are read once a group. max_shared_blocks and
+    max_own (tokens behind them) size the launches only. The types of kept_decode; ValueError
+    otherwise."""
+    L = lib()
+    B, n_groups = q.shape[0], shared_blocks.shape[0]
+    out_stride, out_dtype = _out_rows(out)
+    if out.shape[0] != B:
+        _refuse("out", f"not {B} rows")
+    ws, ws_bytes = _ws(workspace)
+    st = L.gkv_shared_decode(stream_handle(stream), B, n_groups,
+                             _of(n_groups + 1, cu_groups, "cu_groups"),
+                             _of(n_groups, shared_blocks, "shared_blocks"), max_shared_blocks,
+                             max_own, n_q_heads, q.data_ptr(), _row_stride(q, "q"),
+                             _floats(cos_tab, "cos_tab"), _floats(sin_tab, "sin_tab"),
+                             _of(B, seq_lens, "seq_lens"), max_seq_len, view,
+                             _floats(sinks, "sinks"), ws, ws_bytes, out.data_ptr(), out_stride,
+                             out_dtype, ptr(dev_err))
+    check("gkv_shared_decode", st)
+
+
+def beam_workspace_bytes(n_requests, n_beams, vocab, n_out) -> int:
+    return lib().gkv_beam_workspace_bytes(n_requests, n_beams, vocab, n_out)
+
+
+def beam_select(logits, cum_scores, n_beams, scores, parents, tokens, done=None, eos=-1,
+                done_out=None, workspace=None, dev_err=None, stream=None):
+    """gkv_beam_select: the best continuations of each request's n_beams rows of logits (fp32 or
+    bf16) into scores (fp32), parents and tokens (int32), all [requests, n_out]. ValueError for
+    other types, or sizes that do not fit together."""
+    L = lib()
+    rows, vocab = logits.shape
+    n_requests, n_out = scores.shape
+    row_stride, dtype = logits.stride(0), logits.dtype
+    if logits.stride(1) != 1 or dtype not in (_torch.float32, _torch.bfloat16):
+        _refuse("logits", "not rows of contiguous fp32 or bf16")
+    if rows != n_requests * n_beams:
+        _refuse("logits", f"not {n_requests} x {n_beams} rows")
+    ws, ws_bytes = _ws(workspace)
+    n = n_requests * n_out
+    st = L.gkv_beam_select(stream_handle(stream), n_requests, n_beams, vocab, logits.data_ptr(),
+                           max(row_stride, vocab) if rows == 1 else row_stride,
+                           F32 if dtype is _torch.float32 else BF16,
+                           _of(rows, cum_scores, "cum_scores", _torch.float32),
+                           _of(rows, done, "done"), eos, n_out,
+                           _of(n, scores, "scores", _torch.float32), _of(n, parents, "parents"),
+                           _of(n, tokens, "tokens"), _of(n, done_out, "done_out"), ws, ws_bytes,
+                           ptr(dev_err))
+    check("gkv_beam_select", st)
+
+
+def block_tables(table, lens, refs) -> BlockTables:
+    """The view that the tables_* calls take: table int32 [n_seqs, entries], lens int32 [n_seqs],
+    refs int32 [num_blocks], contiguous device tensors that the caller keeps (ValueError
+    otherwise)."""
+    lib()
+    n_seqs, stride = table.shape
+    return BlockTables(_of(n_seqs * stride, table, "table"), _of(n_seqs, lens, "lens"),
+                       _ints(refs, "refs"), stride, n_seqs, refs.numel())
+
+
+def tables_init(tables: BlockTables, stream=None):
+    """gkv_tables_init: empty rows, all blocks free."""
+    check("gkv_tables_init", lib().gkv_tables_init(stream_handle(stream), tables))
+
+
+def tables_workspace_bytes(n_seqs, num_blocks) -> int:
+    return lib().gkv_tables_workspace_bytes(n_seqs, num_blocks)
+
+
+def tables_resize(tables: BlockTables, new_lens, copy_src=None, copy_dst=None, cu_rows=None,
+                  row_seq=None, row_pos=None, row_slot=None, workspace=None, dev_err=None,
+                  stream=None):
+    """gkv_tables_resize: the lengths new_lens, blocks taken and given back, the copies that shared
+    last blocks need (pairs for copy_blocks) and the map of the new rows (row_seq and row_pos int32,
+    row_slot int64, of one size, which bounds the rows). int32 tensors; ValueError otherwise."""
+    L = lib()
+    n = tables.n_seqs
+    rows = next((t.numel() for t in (row_seq, row_pos, row_slot) if t is not None), 0)
+    ws, ws_bytes = _ws(workspace)
+    st = L.gkv_tables_resize(stream_handle(stream), tables, _of(n, new_lens, "new_lens"),
+                             _of(n, copy_src, "copy_src"), _of(n, copy_dst, "copy_dst"), rows,
+                             _of(n + 1, cu_rows, "cu_rows"), _of(rows, row_seq, "row_seq"),
+                             _of(rows, row_pos, "row_pos"),
+                             _of(rows, row_slot, "row_slot", _torch.int64), ws, ws_bytes,
+                             ptr(dev_err))
+    check("gkv_tables_resize", st)
+
+
+def tables_reorder(tables: BlockTables, parents, group_size, shared_blocks=None, dev_err=None,
+                   stream=None):
+    """gkv_tables_reorder: row s becomes what row parents[s] of its group was (-1: empty);
+    shared_blocks gets each group's common leading full blocks. int32 tensors; ValueError
+    otherwise."""
+    L = lib()
+    n = tables.n_seqs
+    groups = n // group_size if group_size > 0 else 0
+    st = L.gkv_tables_reorder(stream_handle(stream), tables, group_size,
+                              _of(n, parents, "parents"),
+                              _of(groups, shared_blocks, "shared_blocks"), ptr(dev_err))
+    check("gkv_tables_reorder", st)
 
 
 class Pool:
