@@ -586,8 +586,8 @@ size_t gkv_beam_workspace_bytes(int32_t n_requests, int32_t n_beams, int32_t voc
  *               one continuation is the token eos at the score that it has
  * and its continuation by token t scores cum_scores + logit[t] - log sum exp(logits). The n_out
  * largest logits of every beam (of equal ones the lower token) compete, best score
- * first, equal scores by the lower beam, then the lower token (scores of -inf too, where too few
- * others are there; formed and compared in 64 bits):
+ * first, of equal scores the lower beam's (scores of -inf too, where too few others are there;
+ * formed and compared in 64 bits):
  *   scores      fp32 [n_requests][n_out]
  *   parents     int32 [n_requests][n_out]: the row continued, r * n_beams + k
  *   tokens      int32 [n_requests][n_out]
@@ -609,6 +609,7 @@ int gkv_beam_select(void *stream, int32_t n_requests, int32_t n_beams, int32_t v
  * that are captured into a graph, and for beams, whose rows move with every token. All arrays are
  * the caller's, in device memory; the caches are too (num_blocks blocks, any format, any number of
  * layers under one table; window layers read it as the ring = 0 form of gkv_kept_*).
+ * table_stride <= 2^17 (2 million tokens; GKV_ERR_UNSUPPORTED).
  *   table  int32 [n_seqs][table_stride]: row s holds ceil(lens[s] / 16) blocks, -1 behind them
  *   lens   int32 [n_seqs]: tokens of each sequence (0: an idle place): the seq_lens of
  *          the appends and attention

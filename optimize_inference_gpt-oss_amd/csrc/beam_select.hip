@@ -44,30 +44,87 @@ __device__ __forceinline__ float plain_logit(float x) {
   return x != x ? -INFINITY : fminf(x, kFloatMax);
 }
 
-// The n best of what a wave has met, entry i in lane i, best first; equal ones in the order
-// in which they came.
-struct Best {
-  float x;
-  int token;      // -1: no entry
-  float low;      // the n-th (-inf while there are fewer)
-  bool full;
-};
+__device__ __forceinline__ float lane_of(float x, int lane) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
+}
 
-__device__ __forceinline__ void insert(Best &b, float x, int token, int n) {
-  const int lane = threadIdx.x & 63;
-  const uint64_t before = __ballot(b.token >= 0 && b.x >= x);
-  const int at = __popcll(before);
-  const float ux = __shfl_up(b.x, 1, 64);
-  const int ut = __shfl_up(b.token, 1, 64);
-  if (lane == at) {
-    b.x = x;
-    b.token = token;
-  } else if (lane > at) {
-    b.x = ux;
-    b.token = ut;
+// A logit and its token as one number that grows with the logit and, at equal ones, falls
+// with the token (-0 as 0). 0: none.
+__device__ __forceinline__ uint64_t key_of(float x, int token) {
+  return (uint64_t)order_of(x + 0.0f) << 32 | (uint32_t)~token;
+}
+__device__ __forceinline__ float logit_of(uint64_t key) {
+  const uint32_t u = (uint32_t)(key >> 32);
+  return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+}
+__device__ __forceinline__ int token_of(uint64_t key) { return (int)~(uint32_t)key; }
+
+// Between a wave's writes to LDS and its other lanes' reads: they keep their order by themselves,
+// the compiler has to as well.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
+// The key of lane (lane ^ X).
+template <int X>
+__device__ __forceinline__ uint64_t other(uint64_t key) {
+  uint32_t lo = (uint32_t)key, hi = (uint32_t)(key >> 32);
+  if (X < 32) { // (a pattern in the instruction, no address)
+    lo = __builtin_amdgcn_ds_swizzle(lo, X << 10 | 0x1f);
+    hi = __builtin_amdgcn_ds_swizzle(hi, X << 10 | 0x1f);
+  } else {
+    lo = __shfl_xor(lo, X);
+    hi = __shfl_xor(hi, X);
   }
-  b.low = __shfl(b.x, n - 1, 64);
-  b.full = __shfl(b.token, n - 1, 64) >= 0;
+  return (uint64_t)hi << 32 | lo;
+}
+
+// One step of a sort over the lanes: lane and lane ^ X, the larger key to the lower lane where
+// down, else to the upper.
+template <int X>
+__device__ __forceinline__ void sort_step(uint64_t &key, bool down) {
+  const uint64_t o = other<X>(key);
+  const bool lower = (threadIdx.x & X) == 0;
+  key = (key > o) == (lower == down) ? key : o;
+}
+
+// Largest first, of keys that rise and then fall (or the reverse).
+__device__ __forceinline__ void sort_bitonic(uint64_t &key) {
+  sort_step<32>(key, true);
+  sort_step<16>(key, true);
+  sort_step<8>(key, true);
+  sort_step<4>(key, true);
+  sort_step<2>(key, true);
+  sort_step<1>(key, true);
+}
+
+// The 64 lanes' keys, smallest first (so that the lanes of another, sorted the other way round, can
+// be compared one by one).
+__device__ __forceinline__ void sort_up(uint64_t &key) {
+  const int lane = threadIdx.x & 63;
+  auto down = [&](int size) { return (lane & size) != 0; };
+  sort_step<1>(key, down(2));
+  sort_step<2>(key, down(4));
+  sort_step<1>(key, down(4));
+  sort_step<4>(key, down(8));
+  sort_step<2>(key, down(8));
+  sort_step<1>(key, down(8));
+  sort_step<8>(key, down(16));
+  sort_step<4>(key, down(16));
+  sort_step<2>(key, down(16));
+  sort_step<1>(key, down(16));
+  sort_step<16>(key, down(32));
+  sort_step<8>(key, down(32));
+  sort_step<4>(key, down(32));
+  sort_step<2>(key, down(32));
+  sort_step<1>(key, down(32));
+  sort_step<32>(key, false);
+  sort_step<16>(key, false);
+  sort_step<8>(key, false);
+  sort_step<4>(key, false);
+  sort_step<2>(key, false);
+  sort_step<1>(key, false);
 }
 
 // The row's 16-byte granule i (aligned down from the row's start, off elements before it) as
@@ -99,33 +156,45 @@ __device__ __forceinline__ void load_granule(Granule<BF> &g, const char *base, i
   }
 }
 
-template <bool BF>
-__global__ __launch_bounds__(kBeamThreads) void beam_rows_kernel(BeamArgs a) {
+// One wave's tiles t0 .. t1 - 1 of a row: maximum and sum per lane, and the 64 best keys, best in
+// lane 0. What may be among the row's n best is put into the wave's list in LDS, 64 at a time are
+// sorted and joined with the best so far: a few hundred instructions for 64 candidates, where
+// putting them in one by one took some 80 each. Where it meets a NaN or +inf, l ends as NaN, and the
+// caller runs it again with PLAIN, which looks at every value.
+// low: the waves' n-th best so far, in LDS: what is below one of them is not among the row's n
+// best, whoever reads it when.
+template <bool BF, bool PLAIN>
+__device__ __forceinline__ void row_part(const BeamArgs &a, const char *base, int64_t off, int64_t t0,
+                                         int64_t t1, volatile float *low, uint64_t *list,
+                                         uint64_t &best, float &m, float &l) {
   constexpr int N = Granule<BF>::N, U = 16 / N; // granules a lane takes in one go
-  __shared__ float s_x[kBeamWaves][kBeamMost];
-  __shared__ int s_t[kBeamWaves][kBeamMost];
-  __shared__ float2 s_ml[kBeamWaves];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  const int row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
-  // (a row that is finished, or that no score can reach, is not read)
-  const float cum = a.cum[row];
-  if ((a.done && a.done[row] != 0) || !(cum > -INFINITY))
-    return;
-  const char *start = (const char *)a.x + (int64_t)row * a.stride * (BF ? 2 : 4);
-  const int64_t off = ((uintptr_t)start & 15) / (BF ? 2 : 4);
-  const char *base = (const char *)((uintptr_t)start & ~(uintptr_t)15);
-  // this wave's tiles of 64 U granules, in order
-  const int64_t granules = (off + a.V + N - 1) / N, tiles = (granules + 64 * U - 1) / (64 * U);
-  const int64_t w = (int64_t)part * kBeamWaves + wave, n_waves = (int64_t)a.parts * kBeamWaves;
-  const int64_t t0 = w * tiles / n_waves, t1 = (w + 1) * tiles / n_waves;
-
-  Best best{-INFINITY, -1, -INFINITY, false};
-  float m = -kFloatMax, l = 0.0f;
-  bool odd = false; // a NaN or +inf was met
+  best = 0;
+  m = -kFloatMax;
+  l = 0.0f;
+  uint64_t nth = 0; // the n-th best key (0: there are fewer)
+  int listed = 0;
+  auto join = [&]() { // the first 64 of the list with the best
+    wave_sync();
+    uint64_t key = lane < listed ? list[lane] : 0;
+    const uint64_t rest = lane + 64 < listed ? list[lane + 64] : 0;
+    sort_up(key);
+    best = best > key ? best : key;
+    sort_bitonic(best);
+    nth = (uint64_t)__builtin_amdgcn_readlane((uint32_t)(best >> 32), a.n - 1) << 32 |
+          (uint32_t)__builtin_amdgcn_readlane((uint32_t)best, a.n - 1);
+    listed = max(listed - 64, 0);
+    wave_sync();
+    list[lane] = rest;
+    wave_sync();
+    if (nth != 0 && lane == 0)
+      low[wave] = logit_of(nth);
+  };
   Granule<BF> g[U];
+  if (t0 < t1)
 #pragma unroll
-  for (int u = 0; u < U; u++)
-    load_granule<BF>(g[u], base, t0 < t1 ? t0 * 64 * U + u * 64 + lane : granules, off, a.V);
+    for (int u = 0; u < U; u++)
+      load_granule<BF>(g[u], base, t0 * 64 * U + u * 64 + lane, off, a.V);
   for (int64_t t = t0; t < t1; t++) {
     Granule<BF> c[U];
 #pragma unroll
@@ -140,8 +209,8 @@ __global__ __launch_bounds__(kBeamThreads) void beam_rows_kernel(BeamArgs a) {
     for (int u = 0; u < U; u++)
 #pragma unroll
       for (int j = 0; j < N; j++) {
-        odd |= !(c[u].v[j] <= kFloatMax);
-        c[u].v[j] = plain_logit(c[u].v[j]);
+        if (PLAIN)
+          c[u].v[j] = plain_logit(c[u].v[j]);
         mx = fmaxf(mx, c[u].v[j]);
       }
     const float mn = fmaxf(m, mx);
@@ -152,44 +221,72 @@ __global__ __launch_bounds__(kBeamThreads) void beam_rows_kernel(BeamArgs a) {
 #pragma unroll
       for (int j = 0; j < N; j++)
         l += __builtin_amdgcn_exp2f((c[u].v[j] - m) * kLog2e);
-    if (best.full && !__any(mx > best.low))
+    float least = fmaxf(fmaxf(low[0], low[1]), fmaxf(low[2], low[3]));
+    if (t == t0) {
+      // the n-th largest of the lanes' maxima: n values of this tile are no less
+      uint64_t top = key_of(mx, lane);
+      sort_up(top);
+      least = fmaxf(least, lane_of(logit_of(top), 64 - a.n));
+    }
+    // (a later token beats the n-th best only with a larger logit)
+    const bool full = nth != 0;
+    if (!__any(mx >= least && (!full || mx > logit_of(nth))))
       continue;
-    // in the order of the tokens: granule after granule, lane after lane
 #pragma unroll
     for (int u = 0; u < U; u++) {
       const int64_t e0 = (t * 64 * U + u * 64 + lane) * N - off;
-      uint32_t mask = 0;
 #pragma unroll
-      for (int j = 0; j < N; j++)
-        if (e0 + j >= 0 && e0 + j < a.V && (!best.full || c[u].v[j] > best.low))
-          mask |= 1u << j;
-      for (;;) {
-        const uint64_t who = __ballot(mask != 0);
+      for (int j = 0; j < N; j++) {
+        const float x = c[u].v[j];
+        const bool real = e0 + j >= 0 && e0 + j < a.V && x >= least;
+        const uint64_t key = key_of(x, (int)(e0 + j));
+        const uint64_t who = __ballot(real && key > nth);
         if (who == 0)
-          break;
-        const int from = __ffsll((unsigned long long)who) - 1;
-        const int j = __shfl(__ffs(mask) - 1, from, 64);
-        float x = c[u].v[0];
-#pragma unroll
-        for (int k = 1; k < N; k++)
-          x = j == k ? c[u].v[k] : x;
-        x = __shfl(x, from, 64);
-        const int64_t e = __shfl(e0, from, 64) + j;
-        if (lane == from)
-          mask &= mask - 1;
-        if (!best.full || x > best.low) {
-          insert(best, x, (int)e, a.n);
-          // (what no longer gets in is dropped at once)
-#pragma unroll
-          for (int k = 0; k < N; k++)
-            if (best.full && !(c[u].v[k] > best.low))
-              mask &= ~(1u << k);
-        }
+          continue;
+        if (real && key > nth)
+          list[listed + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32),
+                                                  __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] = key;
+        listed += __popcll(who);
+        if (listed >= 64)
+          join();
       }
     }
   }
-  if (__any(odd) && lane == 0 && a.dev_err)
-    atomicOr(a.dev_err, GKV_DEVERR_RANGE);
+  if (listed > 0)
+    join();
+}
+
+template <bool BF>
+__global__ __launch_bounds__(kBeamThreads) void beam_rows_kernel(BeamArgs a) {
+  constexpr int N = Granule<BF>::N, U = 16 / N;
+  __shared__ uint64_t s_list[kBeamWaves][2 * 64]; // candidates; then every wave's best
+  __shared__ float2 s_ml[kBeamWaves];
+  __shared__ float s_low[2][kBeamWaves];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
+  // (a row that is finished, or that no score can reach, is not read)
+  const float cum = a.cum[row];
+  if ((a.done && a.done[row] != 0) || !(cum > -INFINITY))
+    return;
+  if (threadIdx.x < 2 * kBeamWaves)
+    s_low[0][threadIdx.x] = -INFINITY;
+  __syncthreads();
+  const char *start = (const char *)a.x + (int64_t)row * a.stride * (BF ? 2 : 4);
+  const int64_t off = ((uintptr_t)start & 15) / (BF ? 2 : 4);
+  const char *base = (const char *)((uintptr_t)start & ~(uintptr_t)15);
+  // this wave's tiles of 64 U granules, in order
+  const int64_t granules = (off + a.V + N - 1) / N, tiles = (granules + 64 * U - 1) / (64 * U);
+  const int64_t w = (int64_t)part * kBeamWaves + wave, n_waves = (int64_t)a.parts * kBeamWaves;
+  const int64_t t0 = w * tiles / n_waves, t1 = (w + 1) * tiles / n_waves;
+  uint64_t best;
+  float m, l;
+  row_part<BF, false>(a, base, off, t0, t1, s_low[0], s_list[wave], best, m, l);
+  if (__syncthreads_or(l != l)) {
+    // (all waves again: what bounded them may have been taken from a NaN)
+    if (threadIdx.x == 0 && a.dev_err)
+      atomicOr(a.dev_err, GKV_DEVERR_RANGE);
+    row_part<BF, true>(a, base, off, t0, t1, s_low[1], s_list[wave], best, m, l);
+  }
   // the lanes' sums, then the waves'
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) {
@@ -199,8 +296,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_rows_kernel(BeamArgs a) {
   }
   if (lane == 0)
     s_ml[wave] = float2{m, l};
-  s_x[wave][lane] = best.x;
-  s_t[wave][lane] = lane < a.n ? best.token : -1;
+  s_list[wave][lane] = best;
   __syncthreads();
   const int64_t at = (int64_t)row * a.parts + part;
   if (threadIdx.x == 0) {
@@ -212,61 +308,83 @@ __global__ __launch_bounds__(kBeamThreads) void beam_rows_kernel(BeamArgs a) {
     }
     a.ml[at] = float2{m, l};
   }
-  // an entry's place among all the waves': those above it, and equal ones of lower tokens
-  const float x = s_x[wave][lane];
-  const int token = s_t[wave][lane];
-  int place = 0, entries = 0;
-  for (int k = 0; k < kBeamWaves; k++)
-    for (int i = 0; i < a.n; i++) {
-      const float y = s_x[k][i];
-      const int o = s_t[k][i];
-      entries += o >= 0;
-      place += o >= 0 && (y > x || (y == x && o < token));
-    }
-  if (token >= 0 && place < a.n) {
-    a.best[at * a.n + place] = x;
-    a.token[at * a.n + place] = token;
+  // the first wave: the waves' best to the n best of all
+  if (wave != 0)
+    return;
+#pragma unroll
+  for (int k = 1; k < kBeamWaves; k++) {
+    const uint64_t key = s_list[k][63 - lane];
+    best = best > key ? best : key;
+    sort_bitonic(best);
   }
-  for (int i = entries + threadIdx.x; i < a.n; i += kBeamThreads)
-    a.token[at * a.n + i] = -1;
-}
-
-// One candidate: its score and flat index beam * V + token (-1: none).
-struct Candidate {
-  double s;
-  int64_t at;
-};
-__device__ __forceinline__ bool beats(double s, int64_t at, double s2, int64_t at2) {
-  return at >= 0 && (at2 < 0 || s > s2 || (s == s2 && at < at2));
-}
-
-__device__ __forceinline__ void insert(Candidate &b, double s, int64_t at) {
-  const int lane = threadIdx.x & 63;
-  const int place = __popcll(__ballot(beats(b.s, b.at, s, at)));
-  const double us = __shfl_up(b.s, 1, 64);
-  const int64_t ua = __shfl_up(b.at, 1, 64);
-  if (lane == place) {
-    b.s = s;
-    b.at = at;
-  } else if (lane > place) {
-    b.s = us;
-    b.at = ua;
+  if (lane < a.n) {
+    a.best[at * a.n + lane] = logit_of(best);
+    a.token[at * a.n + lane] = best != 0 ? token_of(best) : -1;
   }
 }
 
-// A workgroup per request: the rows' sums, then the best of their best.
+// A workgroup per request. First one or more waves per row: the parts' sums to the row's, the
+// parts' best, sorted as they are, joined one by one to its n best, and their scores. Then
+// an entry's place among all: in each other row, which is sorted, those before it are found by
+// halving; as many threads an entry as there are, each for some of the rows.
 __global__ __launch_bounds__(64 * kMergeWaves) void beam_merge_kernel(BeamArgs a) {
-  __shared__ double s_lse[kBeamMost];
-  __shared__ double s_s[kMergeWaves][kBeamMost];
-  __shared__ int64_t s_at[kMergeWaves][kBeamMost];
-  const int r = blockIdx.x, lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  for (int k = wave; k < a.K; k += kMergeWaves) {
-    const int row = r * a.K + k;
+  extern __shared__ double s_score[];               // [K n] scores, then their tokens
+  int *s_token = (int *)(s_score + a.K * a.n);      // (-1: none)
+  __shared__ uint64_t s_best[kMergeWaves][64];
+  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  int shares = 1; // waves per row
+  while (2 * shares * a.K <= kMergeWaves && 2 * shares <= a.parts)
+    shares *= 2;
+  for (int k0 = 0; k0 < a.K; k0 += kMergeWaves / shares) {
+    const int k = k0 + wave / shares, share = wave % shares, row = r * a.K + min(k, a.K - 1);
     const float cum = a.cum[row];
+    const double c = cum != cum ? -INFINITY : (double)fminf(cum, kFloatMax);
+    const bool done = a.done && a.done[row] != 0;
+    const bool reads = k < a.K && !done && c > -INFINITY;
+    uint64_t best = 0;
+    if (reads) {
+      const float *xs = a.best + (int64_t)row * a.parts * a.n;
+      const int32_t *ts = a.token + (int64_t)row * a.parts * a.n;
+      const int e = min(63 - lane, a.n - 1); // (the other way round, so that a maximum joins them)
+      constexpr int A = 4; // loads under way
+      for (int p0 = share; p0 < a.parts; p0 += A * shares) {
+        float x[A];
+        int t[A];
+#pragma unroll
+        for (int i = 0; i < A; i++) {
+          const int p = min(p0 + i * shares, a.parts - 1);
+          x[i] = xs[p * a.n + e];
+          t[i] = ts[p * a.n + e];
+        }
+#pragma unroll
+        for (int i = 0; i < A; i++)
+          if (p0 + i * shares < a.parts) {
+            const uint64_t key = 63 - lane < a.n && t[i] >= 0 ? key_of(x[i], t[i]) : 0;
+            best = best > key ? best : key;
+            sort_bitonic(best);
+          }
+      }
+    }
+    if (shares > 1) { // (then all rows are taken at once)
+      s_best[wave][lane] = best;
+      __syncthreads();
+    }
+    if (k >= a.K || share != 0)
+      continue;
     if (!(cum <= kFloatMax) && lane == 0 && a.dev_err)
       atomicOr(a.dev_err, GKV_DEVERR_RANGE);
-    if ((a.done && a.done[row] != 0) || !(cum > -INFINITY))
+    if (!reads) { // its one continuation, and tokens that score -inf
+      if (lane < a.n) {
+        s_score[k * a.n + lane] = done && lane == 0 ? c : -INFINITY;
+        s_token[k * a.n + lane] = !done ? lane : lane == 0 ? a.eos : lane - 1 < a.eos ? lane - 1 : lane;
+      }
       continue;
+    }
+    for (int i = 1; i < shares; i++) {
+      const uint64_t key = s_best[wave + i][63 - lane];
+      best = best > key ? best : key;
+      sort_bitonic(best);
+    }
     float m = -kFloatMax;
     for (int p = lane; p < a.parts; p += 64)
       m = fmaxf(m, a.ml[(int64_t)row * a.parts + p].x);
@@ -281,79 +399,53 @@ __global__ __launch_bounds__(64 * kMergeWaves) void beam_merge_kernel(BeamArgs a
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1)
       l += __shfl_xor(l, o);
-    if (lane == 0) // (a row of -inf alone: every score is -inf)
-      s_lse[k] = l > 0 ? (double)m + log(l) : 0.0;
+    // (a row of -inf alone: every score is -inf)
+    const double lse = l > 0 ? (double)m + log(l) : 0.0;
+    if (lane < a.n) {
+      s_score[k * a.n + lane] = c + ((double)logit_of(best) - lse);
+      s_token[k * a.n + lane] = token_of(best);
+    }
   }
   __syncthreads();
-  Candidate b{0.0, -1};
-  const int per_row = a.parts * a.n;
-  double low = 0;
-  int64_t low_at = -1;
-  for (int i0 = wave * 64; i0 < a.K * per_row; i0 += 64 * kMergeWaves) {
-    const int i = i0 + lane, k = i / per_row, e = i % per_row, row = r * a.K + k;
-    double s = 0;
-    int64_t at = -1;
-    if (k < a.K) {
-      const float cum = a.cum[row];
-      const double c = cum != cum ? -INFINITY : (double)fminf(cum, kFloatMax);
-      if (a.done && a.done[row] != 0) {
-        // its one continuation, and tokens that score -inf
-        if (e < a.n) {
-          const int t = e == 0 ? a.eos : e - 1 < a.eos ? e - 1 : e;
-          s = e == 0 ? c : -INFINITY;
-          at = t < a.V ? (int64_t)k * a.V + t : -1;
-        }
-      } else if (!(c > -INFINITY)) {
-        if (e < a.n) {
-          s = -INFINITY;
-          at = (int64_t)k * a.V + e;
-        }
-      } else {
-        const int64_t p = (int64_t)row * per_row + e;
-        const int t = a.token[p];
-        if (t >= 0) {
-          s = c + ((double)a.best[p] - s_lse[k]);
-          at = (int64_t)k * a.V + t;
-        }
+  // every row has n: n <= V
+  const int all = a.K * a.n;
+  int each = 1; // threads an entry
+  while (each < 64 && 2 * each * all <= 64 * kMergeWaves)
+    each *= 2;
+  for (int e0 = 0; e0 < all; e0 += 64 * kMergeWaves / each) {
+    const int e = e0 + tid / each, k = min(e, all - 1) / a.n;
+    const double s = s_score[min(e, all - 1)];
+    const int t = s_token[min(e, all - 1)];
+    int place = 0;
+    for (int o = tid % each; o < a.K; o += each) {
+      int lo = 0, hi = o == k ? 0 : a.n; // of equal scores the lower row's come first
+      while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        const double x = s_score[o * a.n + mid];
+        if (x > s || (x == s && o < k))
+          lo = mid + 1;
+        else
+          hi = mid;
       }
+      place += o == k ? e - k * a.n : lo;
     }
-    bool in = beats(s, at, low, low_at);
-    for (;;) {
-      const uint64_t who = __ballot(in);
-      if (who == 0)
-        break;
-      const int from = __ffsll((unsigned long long)who) - 1;
-      const double fs = __shfl(s, from, 64);
-      const int64_t fa = __shfl(at, from, 64);
-      insert(b, fs, fa);
-      low = __shfl(b.s, a.n - 1, 64);
-      low_at = __shfl(b.at, a.n - 1, 64);
-      in = in && lane != from && beats(s, at, low, low_at);
+    for (int o = 1; o < each; o *= 2)
+      place += __shfl_xor(place, o);
+    if (e < all && tid % each == 0 && place < a.n) {
+      const int64_t o = (int64_t)r * a.n + place;
+      const int row = r * a.K + k;
+      a.scores[o] = (float)s;
+      a.parents[o] = row;
+      a.tokens[o] = t;
+      if (a.done_out)
+        a.done_out[o] = t == a.eos || (a.done && a.done[row] != 0);
     }
-  }
-  s_s[wave][lane] = b.s;
-  s_at[wave][lane] = lane < a.n ? b.at : -1;
-  __syncthreads();
-  if (b.at < 0 || lane >= a.n)
-    return;
-  int place = 0;
-  for (int k = 0; k < kMergeWaves; k++)
-    for (int i = 0; i < a.n; i++)
-      place += beats(s_s[k][i], s_at[k][i], b.s, b.at);
-  if (place < a.n) {
-    const int64_t o = (int64_t)r * a.n + place;
-    const int row = r * a.K + (int)(b.at / a.V), t = (int)(b.at % a.V);
-    a.scores[o] = (float)b.s;
-    a.parents[o] = row;
-    a.tokens[o] = t;
-    if (a.done_out)
-      a.done_out[o] = t == a.eos || (a.done && a.done[row] != 0);
   }
 }
 
 // Workgroups per row: as many as give every CU eight waves, as long as a wave keeps a tile of
 // 1024 logits.
-constexpr int kBeamWgs = 512;
+constexpr int kBeamWgs = 1024;
 static int beam_parts(int64_t rows, int32_t V) {
   const int64_t tiles = ((int64_t)V + 1023) / 1024;
   const int64_t most = std::max<int64_t>(1, tiles / kBeamWaves);
@@ -443,6 +535,7 @@ extern "C" int gkv_beam_select(void *stream, int32_t n_requests, int32_t n_beams
   const int st = launch_status("beam_rows_kernel");
   if (st)
     return st;
-  hipLaunchKernelGGL(beam_merge_kernel, dim3((unsigned)n_requests), dim3(64 * kMergeWaves), 0, s, a);
+  hipLaunchKernelGGL(beam_merge_kernel, dim3((unsigned)n_requests), dim3(64 * kMergeWaves),
+                     (size_t)n_beams * n_out * 12, s, a);
   return launch_status("beam_merge_kernel");
 }

@@ -69,12 +69,12 @@ struct ResizeArgs {
 };
 
 // Sum over the workgroup of the values before this thread's, and of all.
-__device__ __forceinline__ int64_t scan_before(int64_t x, int64_t *s_wave, int64_t &total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n_waves = blockDim.x >> 6;
-  int64_t incl = x;
+__device__ __forceinline__ uint64_t scan_before(uint64_t x, uint64_t *s_wave, uint64_t &total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint64_t incl = x;
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
-    const int64_t v = __shfl_up(incl, off, 64);
+    const uint64_t v = __shfl_up(incl, off, 64);
     if (lane >= off)
       incl += v;
   }
@@ -82,10 +82,11 @@ __device__ __forceinline__ int64_t scan_before(int64_t x, int64_t *s_wave, int64
   if (lane == 63)
     s_wave[wave] = incl;
   __syncthreads();
-  int64_t before = 0;
+  uint64_t before = 0;
   total = 0;
-  for (int w = 0; w < n_waves; w++) {
-    const int64_t v = s_wave[w];
+#pragma unroll
+  for (int w = 0; w < kTableThreads / 64; w++) {
+    const uint64_t v = s_wave[w];
     before += w < wave ? v : 0;
     total += v;
   }
@@ -94,20 +95,17 @@ __device__ __forceinline__ int64_t scan_before(int64_t x, int64_t *s_wave, int64
 
 // What a resize does to one row.
 struct RowPlan {
-  int old, now;
+  int old;     // -1: it is left as it is
   bool split;  // the block at its end is held by others too
   int take, rows;
 };
 
-__device__ __forceinline__ RowPlan row_plan(const ResizeArgs &a, int s) {
+__device__ __forceinline__ RowPlan row_plan(const ResizeArgs &a, int s, int len, int want) {
   const TablesArgs &t = a.t;
-  RowPlan p{};
-  const int len = t.lens[s], want = a.new_lens[s];
-  p.old = sane(len, t.stride);
-  p.now = want;
+  RowPlan p{sane(len, t.stride), false, 0, 0};
   if (p.old != len || want < 0 || blocks_of(want) > t.stride) {
     flag(t.dev_err, GKV_DEVERR_LENGTH);
-    p.old = -1; // left as it is
+    p.old = -1;
     return p;
   }
   if (want > p.old) {
@@ -122,61 +120,94 @@ __device__ __forceinline__ RowPlan row_plan(const ResizeArgs &a, int s) {
 }
 
 // One workgroup: what each row takes, where its rows begin, and the ids of the blocks; the
-// lengths, if there is room for all.
+// lengths, if there is room for all. A chain of dependent loads (lengths, the block at a row's
+// end, its holders), so the holders among which free ids are looked for are
+// loaded ahead of it, and of every next round ahead of the scan.
 constexpr int kRefsEach = 16; // holders a thread looks at in one go
-__global__ __launch_bounds__(kTableThreads) void tables_plan_kernel(ResizeArgs a) {
-  __shared__ int64_t s_wave[kTableThreads / 64];
-  const TablesArgs &t = a.t;
-  const int tid = threadIdx.x;
-  int64_t need = 0, rows = 0;
-  for (int s0 = 0; s0 < t.n_seqs; s0 += kTableThreads) {
-    const int s = s0 + tid;
-    RowPlan p{};
-    if (s < t.n_seqs)
-      p = row_plan(a, s);
-    int64_t all, all_rows;
-    const int64_t at = need + scan_before(p.take, s_wave, all);
-    const int64_t row = rows + scan_before(p.rows, s_wave, all_rows);
-    if (s < t.n_seqs) {
-      a.old[s] = p.old;
-      a.first[s] = (int)(at & 0x7fffffff) | (p.split ? (int)0x80000000u : 0);
-      a.cu[s] = (int)row;
-    }
-    need += all;
-    rows += all_rows;
-  }
-  bool ok = need <= t.num_blocks && rows <= a.max_rows;
-  // the lowest free ids, as many as are needed
-  int64_t found = 0;
-  const int n_tiles = (t.num_blocks + kTableThreads * kRefsEach - 1) / (kTableThreads * kRefsEach);
-  for (int k = 0; ok && k < n_tiles && found < need; k++) {
-    const int64_t base = ((int64_t)k * kTableThreads + tid) * kRefsEach;
-    uint32_t free = 0;
+__device__ __forceinline__ uint32_t free_mask(const TablesArgs &t, int64_t base) {
+  uint32_t free = 0;
+  if (base + kRefsEach <= t.num_blocks && ((uintptr_t)t.refs & 15) == 0) {
+    int4 x[kRefsEach / 4];
+#pragma unroll
+    for (int i = 0; i < kRefsEach / 4; i++)
+      x[i] = *((const int4 *)(t.refs + base) + i);
+#pragma unroll
+    for (int i = 0; i < kRefsEach / 4; i++)
+      free |= ((x[i].x == 0) | (x[i].y == 0) << 1 | (x[i].z == 0) << 2 | (x[i].w == 0) << 3) << (4 * i);
+  } else {
 #pragma unroll
     for (int i = 0; i < kRefsEach; i++)
       if (base + i < t.num_blocks && t.refs[base + i] == 0)
         free |= 1u << i;
-    int64_t all;
-    int64_t at = found + scan_before(__popc(free), s_wave, all);
+  }
+  return free;
+}
+
+__global__ __launch_bounds__(kTableThreads) void tables_plan_kernel(ResizeArgs a) {
+  __shared__ uint64_t s_wave[kTableThreads / 64];
+  const TablesArgs &t = a.t;
+  const int tid = threadIdx.x;
+  uint32_t free = free_mask(t, (int64_t)tid * kRefsEach);
+  int64_t need = 0, rows = 0;
+  int want = 0, row = 0;
+  RowPlan p{-1, false, 0, 0};
+  for (int s0 = 0; s0 < t.n_seqs; s0 += kTableThreads) {
+    const int s = s0 + tid;
+    p = RowPlan{-1, false, 0, 0};
+    if (s < t.n_seqs) {
+      want = a.new_lens[s];
+      p = row_plan(a, s, t.lens[s], want);
+    }
+    uint64_t all; // rows above, blocks below: a thousand rows' sums are under 2^32
+    const uint64_t at = scan_before((uint64_t)p.rows << 32 | (uint32_t)p.take, s_wave, all);
+    row = (int)(rows + (int64_t)(at >> 32));
+    if (s < t.n_seqs) {
+      a.old[s] = p.old;
+      a.first[s] = (int)((need + (int64_t)(uint32_t)at) & 0x7fffffff) | (p.split ? (int)0x80000000u : 0);
+      a.cu[s] = row;
+    }
+    need += (int64_t)(uint32_t)all;
+    rows += (int64_t)(all >> 32);
+  }
+  bool ok = need <= t.num_blocks && rows <= a.max_rows;
+  // the lowest free ids, as many as are needed
+  int64_t found = 0;
+  constexpr int64_t kRound = (int64_t)kTableThreads * kRefsEach;
+  for (int64_t r0 = 0; ok && found < need && r0 < t.num_blocks; r0 += kRound) {
+    const int64_t base = r0 + (int64_t)tid * kRefsEach;
+    const uint32_t next = free_mask(t, base + kRound);
+    uint64_t all;
+    int64_t at = found + (int64_t)scan_before(__popc(free), s_wave, all);
     for (; free != 0 && at < need; free &= free - 1)
       a.ids[at++] = (int)base + __ffs(free) - 1;
-    found += all;
+    found += (int64_t)all;
+    free = next;
   }
   ok = ok && found >= need;
   if (tid == 0) {
     *a.ok = ok;
     a.cu[t.n_seqs] = (int)rows;
+    if (a.cu_rows)
+      a.cu_rows[t.n_seqs] = ok ? (int)rows : 0;
     if (!ok)
       flag(t.dev_err, GKV_DEVERR_CAPACITY);
   }
+  if (t.n_seqs <= kTableThreads) { // (all is still at hand)
+    if (tid < t.n_seqs) {
+      if (ok && p.old >= 0)
+        t.lens[tid] = want;
+      if (a.cu_rows)
+        a.cu_rows[tid] = ok ? row : 0;
+    }
+    return;
+  }
   __syncthreads();
-  for (int s = tid; s <= t.n_seqs; s += kTableThreads)
+  for (int s = tid; s < t.n_seqs; s += kTableThreads) {
     if (a.cu_rows)
       a.cu_rows[s] = ok ? a.cu[s] : 0;
-  if (ok)
-    for (int s = tid; s < t.n_seqs; s += kTableThreads)
-      if (a.old[s] >= 0)
-        t.lens[s] = a.new_lens[s];
+    if (ok && a.old[s] >= 0)
+      t.lens[s] = a.new_lens[s];
+  }
 }
 
 // The sequence that new row r belongs to: the last s with cu[s] <= r, in 0 .. n - 1.
@@ -265,83 +296,188 @@ struct ReorderArgs {
   TablesArgs t;
   const int32_t *parents;
   int per;             // rows of a group
-  int width;           // columns of a tile
+  int width_log;       // columns of a tile: 2^width_log
+  int tiles;           // tiles per group that have a workgroup of their own (1: one takes all)
   int32_t *shared;     // NULL, or per group the leading blocks that all its rows hold
 };
 
-// One workgroup per group, tile of columns after tile: the rows' entries go to LDS, and each
-// row takes its parent's from there, so it works in place. Holders change only
-// where the entry does (rows of a beam search share most of their blocks).
-constexpr int kTileEntries = 1 << 13;
-__global__ __launch_bounds__(kTableThreads) void tables_reorder_kernel(ReorderArgs a) {
-  extern __shared__ int32_t s_mem[];
+// A group's parents (places in the group, -1: none) and lengths into LDS; the most
+// blocks that one of its rows holds.
+__device__ __forceinline__ int load_group(const ReorderArgs &a, int base, int32_t *s_parent,
+                                          int32_t *s_len, int *s_max, bool report) {
   const TablesArgs &t = a.t;
-  int32_t *s_tile = s_mem, *s_parent = s_mem + a.per * a.width, *s_len = s_parent + a.per;
-  __shared__ int s_max, s_min, s_first;
-  const int tid = threadIdx.x, base = blockIdx.x * a.per;
-  if (tid == 0) {
-    s_max = 0;
-    s_min = INT32_MAX;
-    s_first = INT32_MAX;
-  }
+  if (threadIdx.x == 0)
+    *s_max = 0;
   __syncthreads();
-  for (int i = tid; i < a.per; i += kTableThreads) {
+  for (int i = threadIdx.x; i < a.per; i += blockDim.x) {
     int p = a.parents[base + i];
+    const int len = t.lens[base + i];
     if (p != -1 && (p < base || p >= base + a.per)) {
-      flag(t.dev_err, GKV_DEVERR_BLOCK_ID);
+      if (report)
+        flag(t.dev_err, GKV_DEVERR_BLOCK_ID);
       p = base + i;
     }
     s_parent[i] = p < 0 ? -1 : p - base;
-    const int len = t.lens[base + i];
     s_len[i] = sane(len, t.stride);
-    if (s_len[i] != len)
+    if (s_len[i] != len && report)
       flag(t.dev_err, GKV_DEVERR_LENGTH);
-    atomicMax(&s_max, blocks_of(s_len[i]));
+    atomicMax(s_max, blocks_of(s_len[i]));
   }
   __syncthreads();
-  const int cols = s_max;
-  for (int c0 = 0; c0 < cols; c0 += a.width) {
-    const int w = min(a.width, cols - c0);
-    for (int e = tid; e < a.per * w; e += kTableThreads) {
-      const int i = e / w, c = e % w;
-      const bool held = c0 + c < blocks_of(s_len[i]);
-      s_tile[i * a.width + c] = held ? t.table[(int64_t)(base + i) * t.stride + c0 + c] : -1;
+  return *s_max;
+}
+
+// The lengths follow, and the blocks that all rows share are counted: fewer than first, where
+// rows are known to differ.
+__device__ __forceinline__ void finish_group(const ReorderArgs &a, int group, const int32_t *s_parent,
+                                             const int32_t *s_len, int *s_min, int first) {
+  const int base = group * a.per;
+  if (threadIdx.x == 0)
+    *s_min = first;
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.per; i += blockDim.x) {
+    const int len = s_parent[i] < 0 ? 0 : s_len[s_parent[i]];
+    a.t.lens[base + i] = len;
+    atomicMin(s_min, len / kBlockTokens);
+  }
+  __syncthreads();
+  if (threadIdx.x == 0 && a.shared)
+    a.shared[group] = *s_min;
+}
+
+// Tiles of columns: the rows' entries go to LDS, and each row takes its parent's from
+// there, so it works in place. A row's block gets as many more holders as the row has children,
+// less one; where all rows hold the same block that adds up to nothing (or what rows without a
+// parent take away), and beams share all but their last blocks: one atomic there, or none.
+// A thread's entries are loaded together. A workgroup takes a whole group and finishes it, or,
+// where groups are few and long, a tile, and another launch finishes.
+constexpr int kTileEntries = 1 << 13;
+constexpr int kTileParts = kTileEntries / kTableThreads;
+__global__ __launch_bounds__(kTableThreads) void tables_reorder_kernel(ReorderArgs a) {
+  extern __shared__ int32_t s_mem[];
+  const TablesArgs &t = a.t;
+  const int width = 1 << a.width_log;
+  int32_t *s_tile = s_mem, *s_parent = s_mem + a.per * width, *s_len = s_parent + a.per;
+  int32_t *s_more = s_len + a.per; // children of a row, less one
+  __shared__ uint8_t s_differ[kTileEntries]; // per column of the tile: not all rows hold the same
+  __shared__ int s_max, s_min, s_first, s_sum;
+  const int tid = threadIdx.x, group = blockIdx.x / a.tiles, tile = blockIdx.x % a.tiles;
+  const int base = group * a.per;
+  if (tid == 0) {
+    s_first = INT32_MAX;
+    s_sum = 0;
+  }
+  for (int i = tid; i < a.per; i += kTableThreads)
+    s_more[i] = -1;
+  const int cols = load_group(a, base, s_parent, s_len, &s_max, a.tiles == 1);
+  for (int i = tid; i < a.per; i += kTableThreads) {
+    if (s_parent[i] >= 0)
+      atomicAdd(&s_more[s_parent[i]], 1);
+    else
+      atomicSub(&s_sum, 1);
+  }
+  for (int c0 = tile * width; c0 < cols; c0 += a.tiles * width) {
+    int32_t was[kTileParts];
+#pragma unroll
+    for (int k = 0; k < kTileParts; k++) {
+      const int e = tid + k * kTableThreads, i = e >> a.width_log, c = c0 + (e & (width - 1));
+      was[k] = -1;
+      if (i < a.per && c < cols && c < blocks_of(s_len[i]))
+        was[k] = t.table[(int64_t)(base + i) * t.stride + c];
+    }
+    for (int c = tid; c < width; c += kTableThreads)
+      s_differ[c] = 0;
+#pragma unroll
+    for (int k = 0; k < kTileParts; k++) {
+      const int e = tid + k * kTableThreads;
+      if (e < a.per << a.width_log && c0 + (e & (width - 1)) < cols)
+        s_tile[e] = was[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kTileParts; k++) {
+      const int e = tid + k * kTableThreads, c = e & (width - 1);
+      if (e < a.per << a.width_log && c0 + c < cols && was[k] != s_tile[c])
+        s_differ[c] = 1;
     }
     __syncthreads();
     const int p0 = s_parent[0];
-    for (int e = tid; e < a.per * w; e += kTableThreads) {
-      const int i = e / w, c = e % w, p = s_parent[i];
-      const int was = s_tile[i * a.width + c], now = p < 0 ? -1 : s_tile[p * a.width + c];
-      if (now != was) {
+#pragma unroll
+    for (int k = 0; k < kTileParts; k++) {
+      const int e = tid + k * kTableThreads, i = e >> a.width_log, c = e & (width - 1);
+      if (i >= a.per || c0 + c >= cols)
+        continue;
+      const int p = s_parent[i], now = p < 0 ? -1 : s_tile[(p << a.width_log) + c];
+      if (now != was[k])
         t.table[(int64_t)(base + i) * t.stride + c0 + c] = now;
-        if ((uint32_t)was < (uint32_t)t.num_blocks)
-          atomicSub(t.refs + was, 1);
-        if ((uint32_t)now < (uint32_t)t.num_blocks)
-          atomicAdd(t.refs + now, 1);
-      }
-      if (now != (p0 < 0 ? -1 : s_tile[p0 * a.width + c]))
+      const int more = s_differ[c] ? s_more[i] : i == 0 ? s_sum : 0;
+      if (more != 0 && (uint32_t)was[k] < (uint32_t)t.num_blocks)
+        atomicAdd(t.refs + was[k], more);
+      // (one atomic a wave, whose lanes hold columns in order: thousands on one word of LDS
+      // would be served one after another)
+      const bool other = now != (p0 < 0 ? -1 : s_tile[(p0 << a.width_log) + c]);
+      const uint64_t others = __ballot(other);
+      if (other && (width < 64 || (tid & 63) == __ffsll((unsigned long long)others) - 1))
         atomicMin(&s_first, c0 + c);
     }
     __syncthreads();
   }
-  for (int i = tid; i < a.per; i += kTableThreads) {
-    const int len = s_parent[i] < 0 ? 0 : s_len[s_parent[i]];
-    t.lens[base + i] = len;
-    atomicMin(&s_min, len / kBlockTokens);
+  if (a.tiles == 1)
+    finish_group(a, group, s_parent, s_len, &s_min, s_first);
+}
+
+// The second launch where a group has several workgroups: its lengths, and the first column in
+// which the new rows differ, up to where the shortest ends.
+__global__ __launch_bounds__(kTableThreads) void tables_finish_kernel(ReorderArgs a) {
+  extern __shared__ int32_t s_mem[];
+  int32_t *s_parent = s_mem, *s_len = s_parent + a.per;
+  __shared__ int s_max, s_min, s_first;
+  const int base = blockIdx.x * a.per;
+  if (threadIdx.x == 0)
+    s_first = INT32_MAX;
+  load_group(a, base, s_parent, s_len, &s_max, true);
+  if (threadIdx.x == 0)
+    s_min = INT32_MAX;
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.per; i += kTableThreads)
+    atomicMin(&s_min, s_parent[i] < 0 ? 0 : s_len[s_parent[i]] / kBlockTokens);
+  __syncthreads();
+  const int full = s_min;
+  const int32_t *row = a.t.table + (int64_t)base * a.t.stride;
+  // (the columns of a round at once; the first round in which two differ is the last)
+  for (int c0 = 0; a.shared && c0 < full; c0 += kTableThreads) {
+    const int c = c0 + threadIdx.x;
+    if (c < full) {
+      const int32_t x = row[c];
+      bool same = true;
+#pragma unroll 8
+      for (int i = 1; i < a.per; i++)
+        same &= row[(int64_t)i * a.t.stride + c] == x;
+      const uint64_t others = __ballot(!same); // (one atomic a wave)
+      if (!same && (int)(threadIdx.x & 63) == __ffsll((unsigned long long)others) - 1)
+        atomicMin(&s_first, c);
+    }
+    __syncthreads();
+    const bool found = s_first != INT32_MAX;
+    __syncthreads(); // (nobody writes it again before all have looked)
+    if (found)
+      break;
   }
   __syncthreads();
-  if (tid == 0 && a.shared)
-    a.shared[blockIdx.x] = min(s_min, s_first);
+  finish_group(a, blockIdx.x, s_parent, s_len, &s_min, s_first);
 }
 
 // ---- host side ------------------------------------------------------------------------
+
+constexpr int kRowMost = 1 << 17; // blocks of a row: 2 million tokens
+constexpr int kReorderWgs = 512; // workgroups that a reorder of few long groups aims at
 
 static int tables_check(const gkv_tables &t) {
   if (!t.table || !t.lens || !t.refs || t.table_stride <= 0 || t.n_seqs < 0 || t.num_blocks <= 0)
     return GKV_ERR_ARG;
   if (((uintptr_t)t.table | (uintptr_t)t.lens | (uintptr_t)t.refs) % 4 != 0)
     return GKV_ERR_ARG;
-  if (t.table_stride > (1 << 27)) // (positions in 32 bits)
+  if (t.table_stride > kRowMost) // (a thousand rows' sums in 32 bits)
     return GKV_ERR_UNSUPPORTED;
   return GKV_OK;
 }
@@ -435,7 +571,7 @@ extern "C" int gkv_tables_reorder(void *stream, gkv_tables t, int32_t group_size
                                   const int32_t *parents, int32_t *shared_blocks,
                                   uint32_t *dev_err) {
   using namespace gkv;
-  const int st = tables_check(t);
+  int st = tables_check(t);
   if (st != GKV_OK)
     return st;
   if (!parents || group_size <= 0 || t.n_seqs % group_size != 0 ||
@@ -445,12 +581,30 @@ extern "C" int gkv_tables_reorder(void *stream, gkv_tables t, int32_t group_size
     return GKV_ERR_UNSUPPORTED;
   if (t.n_seqs == 0)
     return GKV_OK;
-  ReorderArgs a{tables_args(t, dev_err), parents, group_size, kTileEntries / group_size, shared_blocks};
-  a.width = std::min(a.width, t.table_stride);
-  const size_t lds = ((size_t)a.width * group_size + 2 * (size_t)group_size) * 4;
-  if (!grid_fits(t.n_seqs / group_size, kTableThreads))
+  const int groups = t.n_seqs / group_size;
+  ReorderArgs a{};
+  a.t = tables_args(t, dev_err);
+  a.parents = parents;
+  a.per = group_size;
+  a.shared = shared_blocks;
+  while ((group_size << (a.width_log + 1)) <= kTileEntries && 1 << a.width_log < t.table_stride)
+    a.width_log++;
+  const int width = 1 << a.width_log;
+  a.tiles = 1;
+  const int64_t all = ((int64_t)t.table_stride + width - 1) / width;
+  if (all > 2 && groups < kReorderWgs)
+    a.tiles = (int)std::min<int64_t>(all, (kReorderWgs + groups - 1) / groups);
+  const int64_t wgs = (int64_t)groups * a.tiles;
+  if (!grid_fits(wgs, kTableThreads))
     return GKV_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL(tables_reorder_kernel, dim3((unsigned)(t.n_seqs / group_size)),
-                     dim3(kTableThreads), lds, (hipStream_t)stream, a);
-  return launch_status("tables_reorder_kernel");
+  const size_t rows = 3 * (size_t)group_size * 4;
+  hipStream_t s = (hipStream_t)stream;
+  hipLaunchKernelGGL(tables_reorder_kernel, dim3((unsigned)wgs), dim3(kTableThreads),
+                     (size_t)width * group_size * 4 + rows, s, a);
+  if (a.tiles == 1)
+    return launch_status("tables_reorder_kernel");
+  if ((st = launch_status("tables_reorder_kernel")))
+    return st;
+  hipLaunchKernelGGL(tables_finish_kernel, dim3((unsigned)groups), dim3(kTableThreads), rows, s, a);
+  return launch_status("tables_finish_kernel");
 }

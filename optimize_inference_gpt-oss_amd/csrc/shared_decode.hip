@@ -16,6 +16,7 @@
 // A sequence shorter than the shared blocks is read on its own, so the prefix
 // needs no mask.
 #include "kept_attend.hpp"
+#include "lds_dma.hpp"
 
 #include <algorithm>
 
@@ -27,22 +28,31 @@ struct SharedArgs {
   KeptDecodeArgs a;
   const int32_t *cu_groups, *shared;
   int n_groups;
-  int seqs_per_wave, wq; // sequences of a wave's tiles; waves of a workgroup side by side on them
-  int splits, min_steps; // parts of a group's shared blocks; steps of a part, at least
+  int per, tiles_each;   // sequences of a prefix workgroup; tiles that a group has room for
+  int splits, part_steps; // parts of a group's shared blocks, at most; steps of a part, at least
   int own_pieces, own_steps; // pieces before the last of a sequence's own blocks, at most; steps of one
   float *ws_ml, *ws_o;   // [splits + own_pieces][B][Hq]: (m, l), o[64]
 };
 
-// The last i in 0 .. n - 1 with key(i) <= x (key does not fall), -1 if there is none: by 64
-// probes at a time.
+// The last i in 0 .. n - 1 with key(i) <= x (key does not fall), -1 if there is none: by 256
+// probes at a time, so that up to 256 groups take one round trip.
 template <typename Key>
 __device__ __forceinline__ int last_at_most(int n, int64_t x, Key key) {
+  constexpr int P = 4;
   const int lane = threadIdx.x & 63;
   int64_t lo = 0, len = n;
   while (len > 0) {
-    const int64_t step = (len + 63) / 64, i = lo + lane * step;
-    const bool ok = lane * step < len && key((int)i) <= x;
-    const int c = __popcll(__ballot(ok));
+    const int64_t step = (len + 64 * P - 1) / (64 * P);
+    bool ok[P];
+#pragma unroll
+    for (int k = 0; k < P; k++) {
+      const int64_t i = (lane + 64 * k) * step;
+      ok[k] = i < len && key((int)(lo + i)) <= x;
+    }
+    int c = 0;
+#pragma unroll
+    for (int k = 0; k < P; k++)
+      c += __popcll(__ballot(ok[k]));
     if (c == 0)
       return -1; // (only in the first round)
     lo += (c - 1) * step;
@@ -67,7 +77,7 @@ __device__ __forceinline__ int shared_of(const SharedArgs &s, int grp) {
 
 // Steps of a part of n, and how many parts that makes.
 __device__ __forceinline__ int part_steps(const SharedArgs &s, int n) {
-  return max((n + s.splits - 1) / s.splits, s.min_steps);
+  return max((n + s.splits - 1) / s.splits, s.part_steps);
 }
 
 __device__ __forceinline__ int64_t piece_at(const SharedArgs &s, int i, int b) {
@@ -76,25 +86,41 @@ __device__ __forceinline__ int64_t piece_at(const SharedArgs &s, int i, int b) {
 
 // ---- prefix ----------------------------------------------------------------------------
 
+// A workgroup's four waves hold 16 NT WQ query heads, WQ waves side by side; with WQ = 2 two pairs
+// take a half of the tokens each and are joined at the end. The blocks come into
+// LDS by loads of their own, in a ring of DP steps that the WQ waves share: a step is read from
+// memory once for all of them, DP - 1 are under way while one is computed, and none of
+// it takes registers. One barrier a step. A block's scales come the same way, and the block ids
+// 64 at a time into a register's lanes: a scalar load in the loop would be waited for with
+// the step's LDS reads, which share its counter (8 beams of 64 requests, codes: 65 us so).
 // NT: tiles of 16 query heads per wave. Pieces of q: bf16 K two in bf16 (FINE three), codes one
 // in fp16 (FINE two); p: one in bf16 (FINE three). A bf16 output's own rounding is off by at most
 // 2^-8 of it; so is a weight here, each at random, and q's 11 (16) bits leave far less.
-template <bool BLK, int NT, bool FINE>
-__global__ __launch_bounds__(64 * kSharedWaves) __attribute__((amdgpu_waves_per_eu(FINE ? 1 : 2)))
+template <bool BLK, int NT, int WQ, bool FINE>
+__global__ __launch_bounds__(64 * kSharedWaves)
+__attribute__((amdgpu_waves_per_eu(NT == 1 ? (FINE ? 3 : 4) : 2)))
 void shared_prefix_kernel(SharedArgs s) {
-  constexpr int D = kHeadDim;
+  constexpr int D = kHeadDim, WT = kSharedWaves / WQ;
   constexpr int kHeadBytes = kBlockTokens * D * (BLK ? 1 : 2);
   constexpr int QP = BLK ? (FINE ? 2 : 1) : (FINE ? 3 : 2);
+  constexpr int kData = 4 * kHeadBytes;          // K and V of two blocks
+  constexpr int kStage = kData + (BLK ? 256 : 0); // and their scales: K0, V0, K1, V1, in the first lanes
+  constexpr int DP = BLK && WQ == 2 ? 6 : 4;
+  constexpr int UPW = kData / 1024 / WQ; // loads of a wave per step, 1 KB each
+  constexpr int kRing = WT * DP * kStage, kJoin = (kSharedWaves / 2) * NT * 5 * 1024;
+  __shared__ __attribute__((aligned(1024))) char s_mem[kRing > kJoin || WT == 1 ? kRing : kJoin];
   const KeptDecodeArgs &a = s.a;
-  extern __shared__ f32x4 s_part[]; // per wave of a tile's upper half [NT][5][64]: o, (m, l)
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15, kg = lane >> 4;
   int item = blockIdx.x;
   const int g = item % a.n_kv_heads;
   item /= a.n_kv_heads;
-  const int split = item % s.splits, tile = item / s.splits;
-  const int per = s.seqs_per_wave * s.wq;
   // Groups' tiles lie end to end, group i's from cu[i] / per + i on: room for all of them,
-  // as every group wastes less than one.
+  // as every group wastes less than one. Workgroups take the groups' first tiles, part after part,
+  // then the second ones and so on: the tiles that are not there come last. (In the order of the
+  // tiles those that groups of one size leave empty, every second one, would leave every second CU
+  // without work: 8 beams of 64 requests 64 us, 2 x 16 sequences 99.)
+  const int order = item / s.n_groups, per = s.per, split = order % s.splits;
+  const int tile = item % s.n_groups * s.tiles_each + order / s.splits;
   const int grp = last_at_most(s.n_groups, tile, [&](int i) {
     return (int64_t)(max(s.cu_groups[i], 0) / per) + i;
   });
@@ -108,20 +134,59 @@ void shared_prefix_kernel(SharedArgs s) {
   const int64_t at0 = b0 + (int64_t)(tile - (b0 / per + grp)) * per;
   if (p0 >= p1 || at0 < b0 || at0 >= b1)
     return;
-  const int t0 = (int)at0;
-  const int wt = kSharedWaves / s.wq, part = wave / s.wq;
-  const int seq0 = t0 + (wave % s.wq) * s.seqs_per_wave;
-  const int n_cols = min(max(b1 - seq0, 0), s.seqs_per_wave) * a.G;
-  const int s0 = p0 + part * (p1 - p0) / wt, s1 = p0 + (part + 1) * (p1 - p0) / wt;
+  const int t0 = (int)at0, n_cols = min(b1 - t0, per) * a.G;
+  const int part = wave / WQ, wq = wave % WQ;
+  const int n_it = (p1 - p0 + WT - 1) / WT;
+  const int s0 = min(p0 + part * n_it, p1), count = min(s0 + n_it, p1) - s0;
+
+  // The block ids of this wave's steps, 32 steps in the lanes of a register, two registers in turn.
+  const int32_t *trow = a.table + (int64_t)b0 * a.table_stride;
+  auto ids_from = [&](int i) -> int { // ids of steps i .. i + 31
+    const int at = 2 * (s0 + i) + lane;
+    return at < 2 * (s0 + count) && at < first ? trow[at] : kNoBlock;
+  };
+  int ids_even = ids_from(0), ids_odd = kNoBlock;
+  auto ids_of = [&](int i) -> int2 {
+    const int v = i & 32 ? ids_odd : ids_even, at = 2 * (i & 31);
+    return int2{__builtin_amdgcn_readlane(v, at), __builtin_amdgcn_readlane(v, at + 1)};
+  };
+  const char *k_head = a.kc + g * kHeadBytes, *v_head = a.vc + g * kHeadBytes;
+  const uint32_t stride = (uint32_t)a.n_kv_heads * kHeadBytes;
+  const uint32_t ring = lds_addr(s_mem) + part * DP * kStage;
+  auto in_pool = [&](int id) { return (uint32_t)id < (uint32_t)a.num_blocks; };
+  // A wave's loads of a step: units wq, wq + WQ, .. of its K0, K1, V0, V1 (KBs). A block that
+  // is not there is read as block 0, whose values are dropped later.
+  auto issue = [&](int i) {
+    const int2 ids = ids_of(i);
+#pragma unroll
+    for (int x = 0; x < UPW; x++) {
+      const int u = wq + x * WQ, v = u / (2 * kHeadBytes / 1024), j = u / (kHeadBytes / 1024) % 2;
+      const int id = j ? ids.y : ids.x;
+      const uint64_t off = (uint64_t)(in_pool(id) ? (uint32_t)id : 0u) * stride +
+                           (BLK ? 0 : (uint32_t)(u % 2) * 1024u);
+      // (codes of V: each lane's operand, in lane order)
+      const uint32_t lane_off = BLK && v ? (uint32_t)(col * 4 + kg) * 16 : (uint32_t)lane * 16;
+      dma16_at<false>((v ? v_head : k_head) + off, lane_off, ring + (i % DP) * kStage + u * 1024);
+    }
+    if (BLK && wq == 0) {
+      const int id = lane & 2 ? ids.y : ids.x;
+      dma4(a.scales + ((int64_t)(in_pool(id) ? id : 0) * a.n_kv_heads + g) * 2 + (lane & 1),
+           s_mem + (part * DP + i % DP) * kStage + kData);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < DP - 1; i++)
+    if (i < count)
+      issue(i);
 
   // The columns' sequences and queries
   int seq[NT], head[NT], len[NT];
   bool on[NT], any = false;
 #pragma unroll
   for (int j = 0; j < NT; j++) {
-    const int c = 16 * j + col;
+    const int c = 16 * (wq * NT + j) + col;
     on[j] = c < n_cols;
-    seq[j] = on[j] ? seq0 + c / a.G : seq0;
+    seq[j] = on[j] ? t0 + c / a.G : t0;
     head[j] = on[j] ? g * a.G + c % a.G : 0;
     len[j] = 0;
     if (on[j]) {
@@ -130,7 +195,7 @@ void shared_prefix_kernel(SharedArgs s) {
     }
     any |= on[j];
   }
-  const bool works = __any(any) && s0 < s1;
+  const bool works = __any(any);
   u32x4 q[NT][QP][2];
   float qf[NT];
 #pragma unroll
@@ -207,113 +272,100 @@ void shared_prefix_kernel(SharedArgs s) {
       st[j].o[nn] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
-  if (works) {
-    const uint32_t k_off = lane * 16, v_off = BLK ? (col * 4 + kg) * 16 : lane * 16;
-    const ScalarI32 trow = (ScalarI32)a.table + (int64_t)b0 * a.table_stride;
-    bool bad = false;
-    auto ids_of = [&](int i) -> int2 {
-      int2 r{kNoBlock, kNoBlock};
-      if (i < s1) {
-        r.x = trow[2 * i];
-        if (2 * i + 1 < first)
-          r.y = trow[2 * i + 1];
+  // What the scores' sums begin with: 0, or -inf for a block that is not there.
+  f32x4 begin[2] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
+  int begun = 0; // bit j: so it is of block j
+  auto compute = [&](int slot, int miss) {
+      f32x2 sc[2] = {f32x2{0.0f, 0.0f}, f32x2{0.0f, 0.0f}};
+      if (BLK) {
+        const f32x2 *in_sc = (const f32x2 *)(s_mem + (part * DP + slot) * kStage + kData);
+        sc[0] = in_sc[0];
+        sc[1] = in_sc[1];
       }
-      return r;
-    };
-    const char *k_head = a.kc + g * kHeadBytes, *v_head = a.vc + g * kHeadBytes;
-    const char *s_head = (const char *)a.scales + g * 8;
-    const uint32_t stride = (uint32_t)a.n_kv_heads * kHeadBytes;
-    auto load = [&](StepData<BLK> &x, int2 ids, int i) {
-      x.miss = 0;
-      const bool one = i < s1, two = one && 2 * i + 1 < first;
+      const u32x4 *in = (const u32x4 *)(s_mem + (part * DP + slot) * kStage) + lane;
+      u32x4 x[BLK ? 2 : 4], y[BLK ? 2 : 4]; // K and V as they are stored
 #pragma unroll
-      for (int j = 0; j < 2; j++) {
-        const int id = uniform(j ? ids.y : ids.x);
-        const bool ok = (uint32_t)id < (uint32_t)a.num_blocks;
-        bad |= !ok && (j ? two : one);
-        x.miss |= ok ? 0u : 1u << j;
-        const uint64_t off = (uint64_t)(ok ? (uint32_t)id : 0u) * stride;
-        const __amdgpu_buffer_rsrc_t kr = head_rsrc(k_head + off, ok ? kHeadBytes : 0);
-        const __amdgpu_buffer_rsrc_t vr = head_rsrc(v_head + off, ok ? kHeadBytes : 0);
-        if (BLK) {
-          x.sc[j] = *(ScalarF2)(s_head + off / 128);
-          x.k[j] = __builtin_amdgcn_raw_buffer_load_b128(kr, k_off, 0, 0);
-          x.v[j] = __builtin_amdgcn_raw_buffer_load_b128(vr, v_off, 0, 0);
-        } else {
+      for (int j = 0; j < (BLK ? 2 : 4); j++) {
+        x[j] = in[j * 64];
+        y[j] = in[(BLK ? 128 : 256) + j * 64];
+      }
+      if (miss != begun) {
 #pragma unroll
-          for (int h = 0; h < 2; h++) {
-            x.k[2 * j + h] = __builtin_amdgcn_raw_buffer_load_b128(kr, k_off + h * 1024, 0, 0);
-            x.v[2 * j + h] = __builtin_amdgcn_raw_buffer_load_b128(vr, v_off + h * 1024, 0, 0);
-          }
+        for (int j = 0; j < 2; j++) {
+          const float f = (miss >> j) & 1 ? -INFINITY : 0.0f;
+          begin[j] = f32x4{f, f, f, f};
         }
+        begun = miss;
       }
-    };
-    auto compute = [&](StepData<BLK> &x) {
+      if (miss != 0) { // (another block's values and scales)
+#pragma unroll
+        for (int j = 0; j < (BLK ? 2 : 4); j++)
+          if ((miss >> (BLK ? j : j / 2)) & 1) {
+            x[j] = y[j] = u32x4{0, 0, 0, 0};
+            sc[j / (BLK ? 1 : 2)] = f32x2{0.0f, 0.0f};
+          }
+      }
       u32x4 k[2][2]; // [block][dims 0..31, 32..63]
 #pragma unroll
       for (int j = 0; j < 2; j++)
         if (BLK) {
-          const u32x2 c0 = codes_to_f16(x.k[j][0]), c1 = codes_to_f16(x.k[j][1]);
-          const u32x2 c2 = codes_to_f16(x.k[j][2]), c3 = codes_to_f16(x.k[j][3]);
+          const u32x2 c0 = codes_to_f16(x[j][0]), c1 = codes_to_f16(x[j][1]);
+          const u32x2 c2 = codes_to_f16(x[j][2]), c3 = codes_to_f16(x[j][3]);
           k[j][0] = u32x4{c0[0], c0[1], c1[0], c1[1]};
           k[j][1] = u32x4{c2[0], c2[1], c3[0], c3[1]};
         } else {
-          k[j][0] = x.k[2 * j];
-          k[j][1] = x.k[2 * j + 1];
+          k[j][0] = x[2 * j];
+          k[j][1] = x[2 * j + 1];
         }
-      if (x.miss != 0) { // a block that is not there: its values become 0, its weights too
-#pragma unroll
-        for (int j = 0; j < 2; j++)
-          if ((x.miss >> j) & 1) {
-            x.sc[j] = f32x2{0.0f, 0.0f};
-            if (BLK)
-              x.v[j] = u32x4{0, 0, 0, 0};
-            else
-              x.v[2 * j] = x.v[2 * j + 1] = u32x4{0, 0, 0, 0};
-          }
-      }
       u32x4 v[4];
 #pragma unroll
       for (int nn = 0; nn < 4; nn++) {
         if (BLK) {
-          const u32x2 y0 = fp8x4_to_bf16x4(x.v[0][nn]), y1 = fp8x4_to_bf16x4(x.v[1][nn]);
+          const u32x2 y0 = fp8x4_to_bf16x4(y[0][nn]), y1 = fp8x4_to_bf16x4(y[1][nn]);
           v[nn] = u32x4{y0[0], y0[1], y1[0], y1[1]};
         } else {
-          const u32x4 y0 = x.v[nn / 2], y1 = x.v[2 + nn / 2];
           const int k0 = 2 * (nn & 1);
-          v[nn] = u32x4{y0[k0], y0[k0 + 1], y1[k0], y1[k0 + 1]};
+          v[nn] = u32x4{y[nn / 2][k0], y[nn / 2][k0 + 1], y[2 + nn / 2][k0], y[2 + nn / 2][k0 + 1]};
         }
       }
+      // All tiles' scores, then one test of their maxima, then weights and outputs tile by tile:
+      // one tile's matrix ops under the next one's vector instructions.
+      f32x4 acc[NT][2];
+      float c[NT][2], mx[NT];
+      bool moves = false;
 #pragma unroll
       for (int j = 0; j < NT; j++) {
-        f32x4 acc[2];
-        float c[2];
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-          acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+          acc[j][i] = begin[i];
 #pragma unroll
           for (int p = 0; p < QP; p++)
 #pragma unroll
             for (int h = 0; h < 2; h++)
-              acc[i] = BLK ? __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                 __builtin_bit_cast(f16x8, k[i][h]),
-                                 __builtin_bit_cast(f16x8, q[j][p][h]), acc[i], 0, 0, 0)
-                           : __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                                 __builtin_bit_cast(bf16x8, k[i][h]),
-                                 __builtin_bit_cast(bf16x8, q[j][p][h]), acc[i], 0, 0, 0);
-          if ((x.miss >> i) & 1)
-            acc[i] = f32x4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+              acc[j][i] = BLK ? __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                    __builtin_bit_cast(f16x8, k[i][h]),
+                                    __builtin_bit_cast(f16x8, q[j][p][h]), acc[j][i], 0, 0, 0)
+                              : __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                                    __builtin_bit_cast(bf16x8, k[i][h]),
+                                    __builtin_bit_cast(bf16x8, q[j][p][h]), acc[j][i], 0, 0, 0);
           // (never 0: a masked score of -inf stays one; a NaN stays a NaN)
-          c[i] = BLK ? __builtin_elementwise_maximum(qf[j] * x.sc[i][0], 1e-37f) : 1.0f;
+          c[j][i] = BLK ? __builtin_elementwise_maximum(qf[j] * sc[i][0], 1e-37f) : 1.0f;
         }
-        State &t = st[j];
-        float mx = fmaxf(fmaxf(fmaxf(acc[0][0], acc[0][1]), fmaxf(acc[0][2], acc[0][3])) * c[0],
-                         fmaxf(fmaxf(acc[1][0], acc[1][1]), fmaxf(acc[1][2], acc[1][3])) * c[1]);
-        // (the running maximum moves only when a score passes it by more than 8)
-        if (__any(mx > t.m + 8.0f)) {
-          mx = fmaxf(mx, __shfl_xor(mx, 16));
-          mx = fmaxf(mx, __shfl_xor(mx, 32));
-          const float m = fmaxf(t.m, mx);
+        // (a NaN stays one, and the output becomes one)
+        auto top = [](float x, float y) { return __builtin_elementwise_maximum(x, y); };
+        const f32x4 &x0 = acc[j][0], &x1 = acc[j][1];
+        mx[j] = top(top(top(x0[0], x0[1]), top(x0[2], x0[3])) * c[j][0],
+                    top(top(x1[0], x1[1]), top(x1[2], x1[3])) * c[j][1]);
+        moves |= mx[j] > st[j].m + 8.0f;
+      }
+      // (the running maximum moves only when a score passes it by more than 8)
+      if (__any(moves)) {
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+          State &t = st[j];
+          float y = fmaxf(mx[j], __shfl_xor(mx[j], 16));
+          y = fmaxf(y, __shfl_xor(y, 32));
+          const float m = y > t.m + 8.0f ? y : t.m;
           const float f = __builtin_amdgcn_exp2f(t.m - m);
           t.m = m;
           t.l *= f;
@@ -321,15 +373,19 @@ void shared_prefix_kernel(SharedArgs s) {
           for (int nn = 0; nn < 4; nn++)
             t.o[nn] *= f;
         }
+      }
+#pragma unroll
+      for (int j = 0; j < NT; j++) {
+        State &t = st[j];
         float p[2][4];
 #pragma unroll
         for (int i = 0; i < 2; i++)
 #pragma unroll
           for (int r = 0; r < 4; r++) {
-            p[i][r] = __builtin_amdgcn_exp2f(fmaf(acc[i][r], c[i], -t.m));
+            p[i][r] = __builtin_amdgcn_exp2f(fmaf(acc[j][i][r], c[j][i], -t.m));
             t.l += p[i][r];
             if (BLK)
-              p[i][r] *= x.sc[i][1];
+              p[i][r] *= sc[i][1];
           }
 #pragma unroll
         for (int piece = 0; piece < (FINE ? 3 : 1); piece++) {
@@ -352,48 +408,56 @@ void shared_prefix_kernel(SharedArgs s) {
         }
       }
     };
-    StepData<BLK> buf[2];
-    int2 ids = ids_of(s0);
-    load(buf[0], ids, s0);
-    ids = ids_of(s0 + 1);
-    for (int i = s0; i < s1; i += 2) {
-#pragma unroll
-      for (int r = 0; r < 2; r++) {
-        if (i + r >= s1)
-          break;
-        const int2 next = ids_of(i + r + 2);
-        load(buf[r ^ 1], ids, i + r + 1);
-        ids = next;
-        compute(buf[r]);
-      }
+  bool bad = false;
+  for (int i = 0; i < n_it; i++) {
+    // this wave's loads of step i are done: the steps behind it may be under way
+    if (i + DP - 1 > count)
+      wait_vmcnt<0>();
+    else if (BLK && wq == 0)
+      wait_vmcnt<(DP - 2) * (UPW + 1)>();
+    else
+      wait_vmcnt<(DP - 2) * UPW>();
+    lds_barrier(); // the others' too; and all are done with step i - 1, whose place is taken now
+    if ((i & 31) == 0) { // the register that step i - 1 was the last to need
+      const int next = i + 32 < count ? ids_from(i + 32) : kNoBlock;
+      ids_even = i & 32 ? next : ids_even;
+      ids_odd = i & 32 ? ids_odd : next;
     }
-    if (bad && lane == 0 && a.dev_err)
-      atomicOr(a.dev_err, GKV_DEVERR_BLOCK_ID);
-#pragma unroll
-    for (int j = 0; j < NT; j++) {
-      st[j].l += __shfl_xor(st[j].l, 16);
-      st[j].l += __shfl_xor(st[j].l, 32);
+    if (i + DP - 1 < count)
+      issue(i + DP - 1);
+    if (i < count) {
+      const int2 ids = ids_of(i);
+      const int miss = uniform((in_pool(ids.x) ? 0 : 1) | (in_pool(ids.y) ? 0 : 2));
+      bad |= miss & 1 || (miss && 2 * (s0 + i) + 1 < first);
+      if (works)
+        compute(i % DP, miss);
     }
   }
+  if (bad && wq == 0 && lane == 0 && a.dev_err)
+    atomicOr(a.dev_err, GKV_DEVERR_BLOCK_ID);
+#pragma unroll
+  for (int j = 0; j < NT; j++) {
+    st[j].l += __shfl_xor(st[j].l, 16);
+    st[j].l += __shfl_xor(st[j].l, 32);
+  }
 
-  // the waves of a tile that split its tokens: the upper half of them hands over to the lower,
-  // until one is left
-  for (int half = wt / 2; half >= 1; half /= 2) {
-    const int place = (part - half) * s.wq + wave % s.wq;
-    if (part >= half && part < 2 * half) {
+  if (WT == 2) { // the pair of the second half hands over to that of the first
+    f32x4 *s_part = (f32x4 *)s_mem; // per wave [NT][5][64]: o, (m, l)
+    lds_barrier(); // (the ring is free)
+    if (part == 1) {
 #pragma unroll
       for (int j = 0; j < NT; j++) {
 #pragma unroll
         for (int nn = 0; nn < 4; nn++)
-          s_part[((place * NT + j) * 5 + nn) * 64 + lane] = st[j].o[nn];
-        s_part[((place * NT + j) * 5 + 4) * 64 + lane] = f32x4{st[j].m, st[j].l, 0.0f, 0.0f};
+          s_part[((wq * NT + j) * 5 + nn) * 64 + lane] = st[j].o[nn];
+        s_part[((wq * NT + j) * 5 + 4) * 64 + lane] = f32x4{st[j].m, st[j].l, 0.0f, 0.0f};
       }
     }
-    __syncthreads();
-    if (part < half) {
+    lds_barrier();
+    if (part == 0) {
 #pragma unroll
       for (int j = 0; j < NT; j++) {
-        const f32x4 *from = s_part + (wave * NT + j) * 5 * 64 + lane; // (place of wave + half wq)
+        const f32x4 *from = s_part + (wq * NT + j) * 5 * 64 + lane;
         const f32x4 ml = from[4 * 64];
         const float m = fmaxf(st[j].m, ml[0]);
         const float f0 = __builtin_amdgcn_exp2f(st[j].m - m), f1 = __builtin_amdgcn_exp2f(ml[0] - m);
@@ -404,7 +468,6 @@ void shared_prefix_kernel(SharedArgs s) {
           st[j].o[nn] = st[j].o[nn] * f0 + from[nn * 64] * f1;
       }
     }
-    __syncthreads();
   }
   if (part != 0)
     return;
@@ -550,37 +613,38 @@ void shared_own_kernel(SharedArgs s) {
 
 // ---- host side ------------------------------------------------------------------------
 
-constexpr int kSharedWgs = 512;    // workgroups that a prefix launch aims at: two per CU
 constexpr int kSharedPieces = 2048; // pieces (times sequences) per kind, at most, or one per sequence
 constexpr int kOwnSteps = 72;      // steps of own blocks that one workgroup takes in the last launch
 
 struct SharedPlan {
-  int nt, wq, seqs_per_wave;
+  int nt, wq, per, tiles_each;
   int64_t tiles;
-  int splits, min_steps, own_pieces;
+  int splits, part_steps, own_pieces;
   size_t o, total; // workspace
 };
 
 static SharedPlan shared_plan(int32_t B, int32_t n_groups, int32_t n_q_heads, int32_t n_kv_heads,
-                              int32_t max_shared, int32_t max_own, bool blk, bool fine) {
+                              int32_t max_shared, int32_t max_own, bool fine) {
   SharedPlan p{};
   const int G = n_q_heads / n_kv_heads;
   const int64_t avg = n_groups > 0 ? std::max<int64_t>(1, ((int64_t)B + n_groups - 1) / n_groups) : 1;
   const int64_t cols = avg * G;
-  p.nt = cols <= 16 ? 1 : cols <= 32 || fine || !blk ? 2 : 4;
-  p.seqs_per_wave = 16 * p.nt / G;
-  const int64_t wave_tiles = (avg + p.seqs_per_wave - 1) / p.seqs_per_wave;
-  p.wq = wave_tiles >= 3 ? 4 : (int)wave_tiles;
-  const int64_t per = (int64_t)p.seqs_per_wave * p.wq;
-  p.tiles = B / per + n_groups;
-  const int64_t busy = n_groups * ((avg + per - 1) / per) * n_kv_heads;
-  const int64_t steps = ((int64_t)max_shared + 1) / 2;
-  const int wt = kSharedWaves / p.wq;
-  p.min_steps = 4 * wt;
+  p.wq = cols <= 32 ? 2 : 4;
+  p.nt = cols <= 64 ? 1 : cols <= 128 || fine ? 2 : 4;
+  p.per = 16 * p.nt * p.wq / G;
+  // (as many tiles a group has room for as all of the even size need, and one)
+  const int64_t each = (avg + p.per - 1) / p.per;
+  p.tiles_each = (int)each + 1;
+  p.tiles = p.tiles_each * (int64_t)n_groups;
+  // Parts of equal steps, so that long groups have more of them and no workgroup is
+  // longer than the rest; as many as the GPU holds at once.
+  const int64_t busy = std::max<int64_t>(n_groups * each * n_kv_heads, 1);
+  const int64_t steps = ((int64_t)max_shared + 1) / 2, wgs = p.nt == 1 ? 1024 : 512;
   const int64_t room = std::max<int64_t>(1, kSharedPieces / std::max(B, 1));
-  int64_t splits = std::min(kSharedWgs / std::max<int64_t>(busy, 1), room);
-  splits = std::min(splits, (steps + p.min_steps - 1) / p.min_steps);
+  const int least = 4 * (kSharedWaves / p.wq);
+  const int64_t splits = std::min({wgs / busy, room, (steps + least - 1) / least});
   p.splits = n_groups > 0 ? (int)std::max<int64_t>(1, splits) : 0;
+  p.part_steps = p.splits > 0 ? (int)std::max<int64_t>(least, (steps + p.splits - 1) / p.splits) : 1;
   const int64_t own_steps = (((int64_t)max_own + kBlockTokens - 1) / kBlockTokens + 1) / 2;
   p.own_pieces = (int)std::min((own_steps + kOwnSteps - 1) / kOwnSteps - 1, room);
   p.own_pieces = std::max(p.own_pieces, 0);
@@ -600,19 +664,17 @@ static bool shared_sizes_ok(int32_t B, int32_t n_groups, int32_t n_q_heads, int3
          max_own >= 0;
 }
 
-template <bool BLK>
-static void launch_prefix(int nt, bool fine, dim3 grid, dim3 block, size_t lds, hipStream_t hs,
-                          const SharedArgs &s) {
-  if (fine && nt == 1)
-    hipLaunchKernelGGL((shared_prefix_kernel<BLK, 1, true>), grid, block, lds, hs, s);
-  else if (fine)
-    hipLaunchKernelGGL((shared_prefix_kernel<BLK, 2, true>), grid, block, lds, hs, s);
-  else if (nt == 1)
-    hipLaunchKernelGGL((shared_prefix_kernel<BLK, 1, false>), grid, block, lds, hs, s);
-  else if (nt == 2)
-    hipLaunchKernelGGL((shared_prefix_kernel<BLK, 2, false>), grid, block, lds, hs, s);
-  else if constexpr (BLK)
-    hipLaunchKernelGGL((shared_prefix_kernel<BLK, 4, false>), grid, block, lds, hs, s);
+template <bool BLK, bool FINE>
+static void launch_prefix(const SharedPlan &p, dim3 grid, hipStream_t hs, const SharedArgs &s) {
+  const dim3 block(64 * kSharedWaves);
+  if (p.wq == 2)
+    hipLaunchKernelGGL((shared_prefix_kernel<BLK, 1, 2, FINE>), grid, block, 0, hs, s);
+  else if (p.nt == 1)
+    hipLaunchKernelGGL((shared_prefix_kernel<BLK, 1, 4, FINE>), grid, block, 0, hs, s);
+  else if (p.nt == 2)
+    hipLaunchKernelGGL((shared_prefix_kernel<BLK, 2, 4, FINE>), grid, block, 0, hs, s);
+  else if constexpr (!FINE)
+    hipLaunchKernelGGL((shared_prefix_kernel<BLK, 4, 4, false>), grid, block, 0, hs, s);
 }
 
 template <bool LAST>
@@ -636,11 +698,8 @@ extern "C" size_t gkv_shared_workspace_bytes(int32_t B, int32_t n_groups, int32_
   using namespace gkv;
   if (!shared_sizes_ok(B, n_groups, n_q_heads, n_kv_heads, max_shared_blocks, max_own))
     return 0;
-  size_t most = 0; // (whatever the formats)
-  for (int k = 0; k < 4; k++)
-    most = std::max(most, shared_plan(B, n_groups, n_q_heads, n_kv_heads, max_shared_blocks, max_own,
-                                      k & 1, k & 2).total);
-  return most;
+  return std::max(shared_plan(B, n_groups, n_q_heads, n_kv_heads, max_shared_blocks, max_own, false).total,
+                  shared_plan(B, n_groups, n_q_heads, n_kv_heads, max_shared_blocks, max_own, true).total);
 }
 
 extern "C" int gkv_shared_decode(void *stream, int32_t B, int32_t n_groups, const int32_t *cu_groups,
@@ -673,7 +732,7 @@ extern "C" int gkv_shared_decode(void *stream, int32_t B, int32_t n_groups, cons
       ((uintptr_t)cu_groups | (uintptr_t)shared_blocks) % 4 != 0 || (uintptr_t)workspace % 16 != 0)
     return GKV_ERR_ARG;
   const bool blk = cache.v_format == GKV_KV_FP8_BLOCK, fine = out_dtype == GKV_F32;
-  const SharedPlan p = shared_plan(B, n_groups, n_q_heads, Hkv, max_shared_blocks, max_own, blk, fine);
+  const SharedPlan p = shared_plan(B, n_groups, n_q_heads, Hkv, max_shared_blocks, max_own, fine);
   SharedArgs s{};
   KeptDecodeArgs &a = s.a;
   a.q = q;
@@ -699,10 +758,10 @@ extern "C" int gkv_shared_decode(void *stream, int32_t B, int32_t n_groups, cons
   s.cu_groups = cu_groups;
   s.shared = shared_blocks;
   s.n_groups = n_groups;
-  s.seqs_per_wave = p.seqs_per_wave;
-  s.wq = p.wq;
+  s.per = p.per;
+  s.tiles_each = p.tiles_each;
   s.splits = p.splits;
-  s.min_steps = p.min_steps;
+  s.part_steps = p.part_steps;
   s.own_pieces = p.own_pieces;
   s.own_steps = kOwnSteps;
   if (B == 0)
@@ -724,12 +783,15 @@ extern "C" int gkv_shared_decode(void *stream, int32_t B, int32_t n_groups, cons
   s.ws_o = (float *)((char *)workspace + p.o);
   hipStream_t hs = (hipStream_t)stream;
   if (p.splits > 0) {
-    const size_t lds = p.wq == kSharedWaves ? 0 : (size_t)kSharedWaves / 2 * p.nt * 5 * 64 * 16;
-    const dim3 grid((unsigned)prefix_wgs), block(64 * kSharedWaves);
-    if (blk)
-      launch_prefix<true>(p.nt, fine, grid, block, lds, hs, s);
+    const dim3 grid((unsigned)prefix_wgs);
+    if (blk && fine)
+      launch_prefix<true, true>(p, grid, hs, s);
+    else if (blk)
+      launch_prefix<true, false>(p, grid, hs, s);
+    else if (fine)
+      launch_prefix<false, true>(p, grid, hs, s);
     else
-      launch_prefix<false>(p.nt, fine, grid, block, lds, hs, s);
+      launch_prefix<false, false>(p, grid, hs, s);
     if ((st = launch_status("shared_prefix_kernel")))
       return st;
   }

@@ -97,7 +97,7 @@ def reorder(gkv, t=None, per=4, parents=FAKE, sh=None):
 @pytest.mark.parametrize("bad,why", [
     (dict(table=None), "ARG"), (dict(lens=None), "ARG"), (dict(refs=None), "ARG"), (dict(table=FAKE + 2), "ARG"),
     (dict(refs=FAKE + 1), "ARG"), (dict(table_stride=0), "ARG"), (dict(n_seqs=-4), "ARG"), (dict(num_blocks=0), "ARG"),
-    (dict(table_stride=(1 << 27) + 1), "UNSUPPORTED")])
+    (dict(table_stride=(1 << 17) + 1), "UNSUPPORTED")])
 def test_tables_that_are_none(gkv, bad, why):
     t = tables(gkv, **bad)
     want = getattr(gkv, "GKV_ERR_" + why)
