@@ -594,7 +594,8 @@ size_t gkv_beam_workspace_bytes(int32_t n_requests, int32_t n_beams, int32_t voc
  *   done_out    NULL, or int32 [n_requests][n_out]: 1 where the token is eos or the beam had ended
  * With n_out = n_beams, scores, done_out and parents are the next step's cum_scores and done and
  * gkv_tables_reorder's parents (of groups of n_beams). eos < 0: no token ends a beam (done NULL).
- * n_out <= 64 and vocab, n_beams <= 64, fewer than 2^23 rows (GKV_ERR_UNSUPPORTED). A logit
+ * n_out <= 64 and vocab, n_beams <= 64, vocab <= 2^30, fewer than 2^23 rows
+ * (GKV_ERR_UNSUPPORTED). A logit
  * that is NaN counts as -inf, one of +inf as the largest fp32 number, cum_scores the same:
  * GKV_DEVERR_RANGE. Inputs and outputs do not overlap. No counterpart in the reference. */
 int gkv_beam_select(void *stream, int32_t n_requests, int32_t n_beams, int32_t vocab,

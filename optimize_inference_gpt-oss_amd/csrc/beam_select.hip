@@ -127,34 +127,46 @@ __device__ __forceinline__ void sort_up(uint64_t &key) {
   sort_step<1>(key, false);
 }
 
-// The row's 16-byte granule i (aligned down from the row's start, off elements before it) as
-// fp32; elements outside the row are -inf and not read.
+// A lane's 16 logits of tile t of a row as fp32: 16-byte granules, 64 lanes side by side, counted
+// from the 16-byte line that the row begins in, off elements before it. Elements outside the row
+// are -inf and not read.
 template <bool BF>
-struct Granule {
-  static constexpr int N = BF ? 8 : 4;
-  float v[N];
-};
-template <bool BF>
-__device__ __forceinline__ void load_granule(Granule<BF> &g, const char *base, int64_t i, int64_t off,
-                                             int64_t V) {
-  constexpr int N = Granule<BF>::N;
-  const int64_t e = i * N - off;
-  if (e >= 0 && e + N <= V) {
-    const u32x4 w = __builtin_nontemporal_load((const u32x4 *)base + i);
+struct Tile {
+  static constexpr int N = BF ? 8 : 4, U = 16 / N; // of a granule; granules
+  u32x4 raw[U];
+  // The element (token) that the lane's granule u begins with.
+  __device__ __forceinline__ static int first(int t, int u, int off) {
+    return (t * 64 * U + u * 64 + (int)(threadIdx.x & 63)) * N - off;
+  }
+  __device__ __forceinline__ void load(const char *base, int t, int off, int V) {
 #pragma unroll
-    for (int j = 0; j < N; j++)
-      g.v[j] = BF ? __uint_as_float(j & 1 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16)
-                  : __uint_as_float(w[j % 4]);
-  } else {
+    for (int u = 0; u < U; u++) {
+      const int e = first(t, u, off);
+      const int64_t i = (int64_t)t * 64 * U + u * 64 + (threadIdx.x & 63);
+      if (e >= 0 && e <= V - N) {
+        raw[u] = __builtin_nontemporal_load((const u32x4 *)base + i);
+      } else {
+        float v[N];
 #pragma unroll
-    for (int j = 0; j < N; j++) {
-      g.v[j] = -INFINITY;
-      if (e + j >= 0 && e + j < V)
-        g.v[j] = BF ? bf16_to_f32(((const uint16_t *)base)[i * N + j])
-                    : ((const float *)base)[i * N + j];
+        for (int j = 0; j < N; j++) {
+          v[j] = -INFINITY;
+          if (e + j >= 0 && e + j < V)
+            v[j] = BF ? bf16_to_f32(((const uint16_t *)base)[i * N + j])
+                      : ((const float *)base)[i * N + j];
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+          raw[u][j] = BF ? __float_as_uint(v[2 * j % N]) >> 16 | __float_as_uint(v[(2 * j + 1) % N])
+                         : __float_as_uint(v[j % N]);
+      }
     }
   }
-}
+  __device__ __forceinline__ float at(int k) const { // element k of the lane's 16
+    if (BF)
+      return __uint_as_float(k & 1 ? raw[k / 8][k % 8 / 2] & 0xffff0000u : raw[k / 8][k % 8 / 2] << 16);
+    return __uint_as_float(raw[k / 4 % U][k % 4]);
+  }
+};
 
 // One wave's tiles t0 .. t1 - 1 of a row: maximum and sum per lane, and the 64 best keys, best in
 // lane 0. What may be among the row's n best is put into the wave's list in LDS, 64 at a time are
@@ -162,12 +174,13 @@ __device__ __forceinline__ void load_granule(Granule<BF> &g, const char *base, i
 // putting them in one by one took some 80 each. Where it meets a NaN or +inf, l ends as NaN, and the
 // caller runs it again with PLAIN, which looks at every value.
 // low: the waves' n-th best so far, in LDS: what is below one of them is not among the row's n
-// best, whoever reads it when.
+// best, whoever reads it when. The waves begin with what their first tiles say: the n-th largest
+// of one wave's lanes' maxima, or the least of the four waves' n / 4-th.
 template <bool BF, bool PLAIN>
-__device__ __forceinline__ void row_part(const BeamArgs &a, const char *base, int64_t off, int64_t t0,
-                                         int64_t t1, volatile float *low, uint64_t *list,
-                                         uint64_t &best, float &m, float &l) {
-  constexpr int N = Granule<BF>::N, U = 16 / N; // granules a lane takes in one go
+__device__ __forceinline__ void row_part(const BeamArgs &a, const char *base, int off, int t0, int t1,
+                                         volatile float *low, uint64_t *list, uint64_t &best,
+                                         float &m, float &l) {
+  constexpr int N = Tile<BF>::N;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   best = 0;
   m = -kFloatMax;
@@ -187,63 +200,67 @@ __device__ __forceinline__ void row_part(const BeamArgs &a, const char *base, in
     wave_sync();
     list[lane] = rest;
     wave_sync();
-    if (nth != 0 && lane == 0)
+    if (nth != 0 && lane == 0 && logit_of(nth) > low[wave])
       low[wave] = logit_of(nth);
   };
-  Granule<BF> g[U];
+  Tile<BF> next, then; // two tiles under way
   if (t0 < t1)
-#pragma unroll
-    for (int u = 0; u < U; u++)
-      load_granule<BF>(g[u], base, t0 * 64 * U + u * 64 + lane, off, a.V);
-  for (int64_t t = t0; t < t1; t++) {
-    Granule<BF> c[U];
-#pragma unroll
-    for (int u = 0; u < U; u++)
-      c[u] = g[u];
-    if (t + 1 < t1)
-#pragma unroll
-      for (int u = 0; u < U; u++)
-        load_granule<BF>(g[u], base, (t + 1) * 64 * U + u * 64 + lane, off, a.V);
+    next.load(base, t0, off, a.V);
+  if (t0 + 1 < t1)
+    then.load(base, t0 + 1, off, a.V);
+  {
     float mx = -INFINITY;
+    if (t0 < t1)
 #pragma unroll
-    for (int u = 0; u < U; u++)
+      for (int k = 0; k < 16; k++)
+        mx = fmaxf(mx, PLAIN ? plain_logit(next.at(k)) : next.at(k));
+    uint64_t top = key_of(mx, lane);
+    sort_up(top);
+    mx = logit_of(top);
+    if (lane == 64 - a.n)
+      low[wave] = mx;
+    if (lane == 64 - (a.n + kBeamWaves - 1) / kBeamWaves)
+      low[kBeamWaves + wave] = mx;
+    __syncthreads();
+  }
+  const float fourth = fminf(fminf(low[4], low[5]), fminf(low[6], low[7]));
+  for (int t = t0; t < t1; t++) {
+    float x[16], top[4], mx; // the largest of four, of all
 #pragma unroll
-      for (int j = 0; j < N; j++) {
-        if (PLAIN)
-          c[u].v[j] = plain_logit(c[u].v[j]);
-        mx = fmaxf(mx, c[u].v[j]);
-      }
+    for (int k = 0; k < 16; k++)
+      x[k] = PLAIN ? plain_logit(next.at(k)) : next.at(k);
+    next = then;
+    if (t + 2 < t1)
+      then.load(base, t + 2, off, a.V);
+#pragma unroll
+    for (int q = 0; q < 4; q++)
+      top[q] = fmaxf(fmaxf(x[4 * q], x[4 * q + 1]), fmaxf(x[4 * q + 2], x[4 * q + 3]));
+    mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
     const float mn = fmaxf(m, mx);
     l *= __builtin_amdgcn_exp2f((m - mn) * kLog2e);
     m = mn;
 #pragma unroll
-    for (int u = 0; u < U; u++)
-#pragma unroll
-      for (int j = 0; j < N; j++)
-        l += __builtin_amdgcn_exp2f((c[u].v[j] - m) * kLog2e);
-    float least = fmaxf(fmaxf(low[0], low[1]), fmaxf(low[2], low[3]));
-    if (t == t0) {
-      // the n-th largest of the lanes' maxima: n values of this tile are no less
-      uint64_t top = key_of(mx, lane);
-      sort_up(top);
-      least = fmaxf(least, lane_of(logit_of(top), 64 - a.n));
-    }
+    for (int k = 0; k < 16; k++)
+      l += __builtin_amdgcn_exp2f((x[k] - m) * kLog2e);
+    const float least = fmaxf(fmaxf(fmaxf(low[0], low[1]), fmaxf(low[2], low[3])), fourth);
     // (a later token beats the n-th best only with a larger logit)
+    const float over = nth != 0 ? logit_of(nth) : -INFINITY;
     const bool full = nth != 0;
-    if (!__any(mx >= least && (!full || mx > logit_of(nth))))
+    if (!__any(mx >= least && (!full || mx > over)))
       continue;
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      const int64_t e0 = (t * 64 * U + u * 64 + lane) * N - off;
+    for (int q = 0; q < 4; q++) {
+      if (!__any(top[q] >= least && (!full || top[q] > over)))
+        continue;
 #pragma unroll
-      for (int j = 0; j < N; j++) {
-        const float x = c[u].v[j];
-        const bool real = e0 + j >= 0 && e0 + j < a.V && x >= least;
-        const uint64_t key = key_of(x, (int)(e0 + j));
-        const uint64_t who = __ballot(real && key > nth);
+      for (int k = 4 * q; k < 4 * q + 4; k++) {
+        const int e = Tile<BF>::first(t, k / N, off) + k % N;
+        const uint64_t key = key_of(x[k], e);
+        const bool in = (uint32_t)e < (uint32_t)a.V && x[k] >= least && key > nth;
+        const uint64_t who = __ballot(in);
         if (who == 0)
           continue;
-        if (real && key > nth)
+        if (in)
           list[listed + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32),
                                                   __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] = key;
         listed += __popcll(who);
@@ -258,26 +275,22 @@ __device__ __forceinline__ void row_part(const BeamArgs &a, const char *base, in
 
 template <bool BF>
 __global__ __launch_bounds__(kBeamThreads) void beam_rows_kernel(BeamArgs a) {
-  constexpr int N = Granule<BF>::N, U = 16 / N;
   __shared__ uint64_t s_list[kBeamWaves][2 * 64]; // candidates; then every wave's best
   __shared__ float2 s_ml[kBeamWaves];
-  __shared__ float s_low[2][kBeamWaves];
+  __shared__ float s_low[2][2 * kBeamWaves];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
   // (a row that is finished, or that no score can reach, is not read)
   const float cum = a.cum[row];
   if ((a.done && a.done[row] != 0) || !(cum > -INFINITY))
     return;
-  if (threadIdx.x < 2 * kBeamWaves)
-    s_low[0][threadIdx.x] = -INFINITY;
-  __syncthreads();
   const char *start = (const char *)a.x + (int64_t)row * a.stride * (BF ? 2 : 4);
-  const int64_t off = ((uintptr_t)start & 15) / (BF ? 2 : 4);
+  const int off = (int)((uintptr_t)start & 15) / (BF ? 2 : 4);
   const char *base = (const char *)((uintptr_t)start & ~(uintptr_t)15);
-  // this wave's tiles of 64 U granules, in order
-  const int64_t granules = (off + a.V + N - 1) / N, tiles = (granules + 64 * U - 1) / (64 * U);
+  // this wave's tiles, in order
+  const int tiles = (int)(((int64_t)off + a.V + 1023) / 1024);
   const int64_t w = (int64_t)part * kBeamWaves + wave, n_waves = (int64_t)a.parts * kBeamWaves;
-  const int64_t t0 = w * tiles / n_waves, t1 = (w + 1) * tiles / n_waves;
+  const int t0 = (int)(w * tiles / n_waves), t1 = (int)((w + 1) * tiles / n_waves);
   uint64_t best;
   float m, l;
   row_part<BF, false>(a, base, off, t0, t1, s_low[0], s_list[wave], best, m, l);
@@ -466,7 +479,7 @@ static BeamWorkspace beam_workspace(int64_t rows, int n) {
 }
 
 static bool beam_sizes_ok(int32_t R, int32_t K, int32_t V, int32_t n) {
-  return R >= 0 && K > 0 && V > 0 && n > 0 && n <= V && n <= kBeamMost && K <= kBeamMost &&
+  return R >= 0 && K > 0 && V > 0 && V <= 1 << 30 && n > 0 && n <= V && n <= kBeamMost && K <= kBeamMost &&
          (int64_t)R * K < (1 << 23);
 }
 

@@ -32,6 +32,8 @@ struct SharedArgs {
   int splits, part_steps; // parts of a group's shared blocks, at most; steps of a part, at least
   int own_pieces, own_steps; // pieces before the last of a sequence's own blocks, at most; steps of one
   float *ws_ml, *ws_o;   // [splits + own_pieces][B][Hq]: (m, l), o[64]
+  int32_t *first;        // [B] shared blocks of a sequence that it does not read itself
+  int prefix_wgs;        // of the first launch; behind them, those that fill first
 };
 
 // The last i in 0 .. n - 1 with key(i) <= x (key does not fall), -1 if there is none: by 256
@@ -111,6 +113,18 @@ void shared_prefix_kernel(SharedArgs s) {
   __shared__ __attribute__((aligned(1024))) char s_mem[kRing > kJoin || WT == 1 ? kRing : kJoin];
   const KeptDecodeArgs &a = s.a;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15, kg = lane >> 4;
+  if ((int)blockIdx.x >= s.prefix_wgs) { // what the second launch asks of every sequence's group
+    const int b = ((int)blockIdx.x - s.prefix_wgs) * kSharedWaves + wave;
+    if (b >= a.B)
+      return;
+    const int grp = group_of(s, b), n = grp < 0 ? 0 : shared_of(s, grp);
+    if (lane == 0) {
+      s.first[b] = span_len(a, b) < n * kBlockTokens ? 0 : n;
+      if (grp >= 0 && n != s.shared[grp] && a.dev_err)
+        atomicOr(a.dev_err, GKV_DEVERR_LENGTH);
+    }
+    return;
+  }
   int item = blockIdx.x;
   const int g = item % a.n_kv_heads;
   item /= a.n_kv_heads;
@@ -153,7 +167,10 @@ void shared_prefix_kernel(SharedArgs s) {
   const char *k_head = a.kc + g * kHeadBytes, *v_head = a.vc + g * kHeadBytes;
   const uint32_t stride = (uint32_t)a.n_kv_heads * kHeadBytes;
   const uint32_t ring = lds_addr(s_mem) + part * DP * kStage;
-  auto in_pool = [&](int id) { return (uint32_t)id < (uint32_t)a.num_blocks; };
+  // 1: an id outside the pool (by its signs: scalar arithmetic, where a comparison becomes a mask)
+  auto outside = [&](int id) -> uint32_t {
+    return ((uint32_t)id | ((uint32_t)a.num_blocks - 1u - (uint32_t)id)) >> 31;
+  };
   // A wave's loads of a step: units wq, wq + WQ, .. of its K0, K1, V0, V1 (KBs). A block that
   // is not there is read as block 0, whose values are dropped later.
   auto issue = [&](int i) {
@@ -162,7 +179,7 @@ void shared_prefix_kernel(SharedArgs s) {
     for (int x = 0; x < UPW; x++) {
       const int u = wq + x * WQ, v = u / (2 * kHeadBytes / 1024), j = u / (kHeadBytes / 1024) % 2;
       const int id = j ? ids.y : ids.x;
-      const uint64_t off = (uint64_t)(in_pool(id) ? (uint32_t)id : 0u) * stride +
+      const uint64_t off = (uint64_t)((uint32_t)id & (outside(id) - 1u)) * stride +
                            (BLK ? 0 : (uint32_t)(u % 2) * 1024u);
       // (codes of V: each lane's operand, in lane order)
       const uint32_t lane_off = BLK && v ? (uint32_t)(col * 4 + kg) * 16 : (uint32_t)lane * 16;
@@ -170,29 +187,36 @@ void shared_prefix_kernel(SharedArgs s) {
     }
     if (BLK && wq == 0) {
       const int id = lane & 2 ? ids.y : ids.x;
-      dma4(a.scales + ((int64_t)(in_pool(id) ? id : 0) * a.n_kv_heads + g) * 2 + (lane & 1),
+      dma4(a.scales + ((int64_t)((uint32_t)id & (outside(id) - 1u)) * a.n_kv_heads + g) * 2 + (lane & 1),
            s_mem + (part * DP + i % DP) * kStage + kData);
     }
   };
-#pragma unroll
-  for (int i = 0; i < DP - 1; i++)
-    if (i < count)
-      issue(i);
-
   // The columns' sequences and queries
   int seq[NT], head[NT], len[NT];
   bool on[NT], any = false;
+  f32x4 qr[NT][4]; // dims 8 kg .. + 7 and 32 + 8 kg .. + 7
 #pragma unroll
   for (int j = 0; j < NT; j++) {
     const int c = 16 * (wq * NT + j) + col;
     on[j] = c < n_cols;
     seq[j] = on[j] ? t0 + c / a.G : t0;
     head[j] = on[j] ? g * a.G + c % a.G : 0;
-    len[j] = 0;
-    if (on[j]) {
-      len[j] = span_len(a, seq[j]);
-      on[j] = len[j] >= first * kBlockTokens;
-    }
+    len[j] = on[j] ? a.seq_lens[seq[j]] : 0;
+    const f32x4 *qp = (const f32x4 *)(a.q + (int64_t)seq[j] * a.q_stride + head[j] * D + 8 * kg);
+    qr[j][0] = qp[0];
+    qr[j][1] = qp[1];
+    qr[j][2] = qp[8];
+    qr[j][3] = qp[9];
+  }
+#pragma unroll
+  for (int i = 0; i < DP - 1; i++)
+    if (i < count)
+      issue(i);
+
+#pragma unroll
+  for (int j = 0; j < NT; j++) {
+    len[j] = max(min(len[j], a.max_len), 0);
+    on[j] &= len[j] >= first * kBlockTokens;
     any |= on[j];
   }
   const bool works = __any(any);
@@ -202,26 +226,19 @@ void shared_prefix_kernel(SharedArgs s) {
   for (int j = 0; j < NT; j++) {
     float x[2][8];
 #pragma unroll
-    for (int i = 0; i < 8; i++)
-      x[0][i] = x[1][i] = 0.0f;
-    if (on[j]) {
-      const f32x4 *qp = (const f32x4 *)(a.q + (int64_t)seq[j] * a.q_stride + head[j] * D + 8 * kg);
-      const f32x4 qr[4] = {qp[0], qp[1], qp[8], qp[9]};
+    for (int i = 0; i < 8; i++) {
+      x[0][i] = on[j] ? qr[j][i / 4][i % 4] : 0.0f;
+      x[1][i] = on[j] ? qr[j][2 + i / 4][i % 4] : 0.0f;
+    }
+    if (a.cos_tab && on[j]) {
+      const f32x4 *cp = (const f32x4 *)(a.cos_tab + (int64_t)(len[j] - 1) * (D / 2) + 8 * kg);
+      const f32x4 *np = (const f32x4 *)(a.sin_tab + (int64_t)(len[j] - 1) * (D / 2) + 8 * kg);
+      const f32x4 an[4] = {cp[0], cp[1], np[0], np[1]};
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        x[0][i] = qr[i / 4][i % 4];
-        x[1][i] = qr[2 + i / 4][i % 4];
-      }
-      if (a.cos_tab) {
-        const f32x4 *cp = (const f32x4 *)(a.cos_tab + (int64_t)(len[j] - 1) * (D / 2) + 8 * kg);
-        const f32x4 *np = (const f32x4 *)(a.sin_tab + (int64_t)(len[j] - 1) * (D / 2) + 8 * kg);
-        const f32x4 an[4] = {cp[0], cp[1], np[0], np[1]};
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const float y1 = x[0][i], y2 = x[1][i];
-          x[0][i] = rope_first(y1, y2, an[i / 4][i % 4], an[2 + i / 4][i % 4]);
-          x[1][i] = rope_second(y1, y2, an[i / 4][i % 4], an[2 + i / 4][i % 4]);
-        }
+        const float y1 = x[0][i], y2 = x[1][i];
+        x[0][i] = rope_first(y1, y2, an[i / 4][i % 4], an[2 + i / 4][i % 4]);
+        x[1][i] = rope_second(y1, y2, an[i / 4][i % 4], an[2 + i / 4][i % 4]);
       }
     }
     qf[j] = 0.125f * kLog2e; // 1 / sqrt(64); exp -> exp2
@@ -274,8 +291,8 @@ void shared_prefix_kernel(SharedArgs s) {
 
   // What the scores' sums begin with: 0, or -inf for a block that is not there.
   f32x4 begin[2] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
-  int begun = 0; // bit j: so it is of block j
-  auto compute = [&](int slot, int miss) {
+  uint32_t begun = 0; // bit j: so it is of block j
+  auto compute = [&](int slot, uint32_t miss) {
       f32x2 sc[2] = {f32x2{0.0f, 0.0f}, f32x2{0.0f, 0.0f}};
       if (BLK) {
         const f32x2 *in_sc = (const f32x2 *)(s_mem + (part * DP + slot) * kStage + kData);
@@ -408,7 +425,7 @@ void shared_prefix_kernel(SharedArgs s) {
         }
       }
     };
-  bool bad = false;
+  uint32_t bad = 0;
   for (int i = 0; i < n_it; i++) {
     // this wave's loads of step i are done: the steps behind it may be under way
     if (i + DP - 1 > count)
@@ -427,13 +444,13 @@ void shared_prefix_kernel(SharedArgs s) {
       issue(i + DP - 1);
     if (i < count) {
       const int2 ids = ids_of(i);
-      const int miss = uniform((in_pool(ids.x) ? 0 : 1) | (in_pool(ids.y) ? 0 : 2));
-      bad |= miss & 1 || (miss && 2 * (s0 + i) + 1 < first);
+      const uint32_t miss = outside(ids.x) | outside(ids.y) << 1;
+      bad |= miss & (2 * (s0 + i) + 1 < first ? 3u : 1u);
       if (works)
         compute(i % DP, miss);
     }
   }
-  if (bad && wq == 0 && lane == 0 && a.dev_err)
+  if (bad != 0 && wq == 0 && lane == 0 && a.dev_err)
     atomicOr(a.dev_err, GKV_DEVERR_BLOCK_ID);
 #pragma unroll
   for (int j = 0; j < NT; j++) {
@@ -491,7 +508,7 @@ void shared_prefix_kernel(SharedArgs s) {
 template <bool BLK, bool FINE, bool LAST>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4)))
 void shared_own_kernel(SharedArgs s) {
-  __shared__ float s_o[8][kPieceFloats];
+  __shared__ __attribute__((aligned(1024))) float s_o[8][kPieceFloats];
   __shared__ float2 s_ml[8][kHeads];
   const KeptDecodeArgs &a = s.a;
   const int n_wg = (a.n_kv_heads + a.heads_per_wg - 1) / a.heads_per_wg;
@@ -510,12 +527,7 @@ void shared_own_kernel(SharedArgs s) {
                 part * 64 + lane, a.parts * 64);
     return;
   }
-  const int grp = group_of(s, b);
-  int first = grp < 0 ? 0 : uniform(shared_of(s, grp));
-  if (LAST && grp >= 0 && threadIdx.x == 0 && first != s.shared[grp] && a.dev_err)
-    atomicOr(a.dev_err, GKV_DEVERR_LENGTH);
-  if (L < first * kBlockTokens)
-    first = 0;
+  const int first = s.n_groups > 0 ? uniform(s.first[b]) : 0;
   Span sp;
   sp.L = L;
   sp.first_blocks = sp.ring0 = 0;
@@ -536,50 +548,64 @@ void shared_own_kernel(SharedArgs s) {
   for (int nn = 0; nn < 4; nn++)
     st.o[nn] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   if (ok) {
-    if (LAST) { // the pieces first, into LDS: head lane / 8, dims 8 (lane % 8) ..
-      float pm = kLowest, pl = 0.0f;
-      f32x4 po[2] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
-      const int h = lane >> 3, d0 = 8 * (lane & 7);
-      const int steps = (first + 1) / 2;
-      const int n_prefix = first > 0 ? (steps + part_steps(s, steps) - 1) / part_steps(s, steps) : 0;
-      const int hc = g * a.G + min(h, a.G - 1);
-      for (int i = part; i < n_prefix + before; i += a.parts) {
-        const int64_t at = piece_at(s, i < n_prefix ? i : s.splits + i - n_prefix, b) + hc;
-        const float2 ml = *(const float2 *)(s.ws_ml + 2 * at);
-        const f32x4 *o = (const f32x4 *)(s.ws_o + at * kHeadDim + d0);
-        const f32x4 x0 = o[0], x1 = o[1];
-        const float m = fmaxf(pm, ml.x);
-        const float f0 = __builtin_amdgcn_exp2f(pm - m), f1 = __builtin_amdgcn_exp2f(ml.x - m);
-        pm = m;
-        pl = pl * f0 + ml.y * f1;
-        po[0] = po[0] * f0 + x0 * f1;
-        po[1] = po[1] * f0 + x1 * f1;
-      }
-      f32x4 *o = (f32x4 *)&s_o[wave][h * kHeadDim + d0];
-      o[0] = po[0];
-      o[1] = po[1];
-      if ((lane & 7) == 0)
-        s_ml[wave][h] = float2{pm, pl};
+    // This wave's pieces: the first comes into LDS while its blocks are read, the others behind.
+    const int steps = (first + 1) / 2;
+    const int n_prefix = first > 0 ? (steps + part_steps(s, steps) - 1) / part_steps(s, steps) : 0;
+    const int n_pieces = LAST ? n_prefix + before : 0;
+    auto piece = [&](int i) {
+      return piece_at(s, i < n_prefix ? i : s.splits + i - n_prefix, b) + g * a.G;
+    };
+    const int hc = min(col, a.G - 1);
+    float2 ml{kLowest, 0.0f};
+    if (part < n_pieces) {
+      const char *o = (const char *)(s.ws_o + piece(part) * kHeadDim);
+#pragma unroll
+      for (int x = 0; x < 2; x++)
+        dma16(o + min(x * 1024 + lane * 16, a.G * kHeadDim * 4 - 16), (char *)s_o[wave] + x * 1024);
+      ml = *(const float2 *)(s.ws_ml + 2 * (piece(part) + hc));
     }
     const int s0 = b0 + part * (b1 - b0) / a.parts, s1 = b0 + (part + 1) * (b1 - b0) / a.parts;
     if (s0 < s1)
       st = attend<BLK, 2, FINE>(a, b, g, sp, s0, s1);
-    __builtin_amdgcn_wave_barrier(); // (a wave's LDS accesses keep their order)
-    if (col < kHeads) {
-      if (LAST) { // the pieces onto what the blocks gave
-        const float2 ml = s_ml[wave][col];
-        const float m = fmaxf(st.m, ml.x);
-        const float f0 = __builtin_amdgcn_exp2f(st.m - m), f1 = __builtin_amdgcn_exp2f(ml.x - m);
-        st.m = m;
-        st.l = st.l * f0 + ml.y * f1;
-#pragma unroll
-        for (int nn = 0; nn < 4; nn++)
-          st.o[nn] = st.o[nn] * f0 + *(const f32x4 *)&s_o[wave][col * kHeadDim + 16 * nn + 4 * kg] * f1;
-        __builtin_amdgcn_wave_barrier();
-      }
+    // a piece onto what there is: 4 dims of each 16 of the column's head
+    auto join = [&](float2 with, const f32x4 (&o)[4]) {
+      const float m = fmaxf(st.m, with.x);
+      const float f0 = __builtin_amdgcn_exp2f(st.m - m), f1 = __builtin_amdgcn_exp2f(with.x - m);
+      st.m = m;
+      st.l = st.l * f0 + with.y * f1;
 #pragma unroll
       for (int nn = 0; nn < 4; nn++)
-        *(f32x4 *)&s_o[wave][col * kHeadDim + 16 * nn + 4 * kg] = st.o[nn];
+        st.o[nn] = st.o[nn] * f0 + o[nn] * f1;
+    };
+    f32x4 *mine = (f32x4 *)&s_o[wave][(col & 7) * kHeadDim + 4 * kg];
+    if (part < n_pieces) {
+      wait_vmcnt<0>();
+      asm volatile("" ::: "memory"); // (its LDS reads stay behind the wait)
+      const f32x4 o[4] = {mine[0], mine[4], mine[8], mine[12]};
+      join(ml, o);
+    }
+    constexpr int A = 4; // pieces under way
+    for (int i = part + a.parts; i < n_pieces; i += A * a.parts) {
+      float2 m[A];
+      f32x4 o[A][4];
+#pragma unroll
+      for (int x = 0; x < A; x++) {
+        const int64_t at = piece(min(i + x * a.parts, n_pieces - 1)) + hc;
+        m[x] = *(const float2 *)(s.ws_ml + 2 * at);
+#pragma unroll
+        for (int nn = 0; nn < 4; nn++)
+          o[x][nn] = *(const f32x4 *)(s.ws_o + at * kHeadDim + 16 * nn + 4 * kg);
+      }
+#pragma unroll
+      for (int x = 0; x < A; x++)
+        if (i + x * a.parts < n_pieces)
+          join(m[x], o[x]);
+    }
+    __builtin_amdgcn_wave_barrier(); // (a wave's LDS accesses keep their order)
+    if (col < kHeads) {
+#pragma unroll
+      for (int nn = 0; nn < 4; nn++)
+        mine[4 * nn] = st.o[nn];
       if (kg == 0)
         s_ml[wave][col] = float2{st.m, st.l};
     }
@@ -620,7 +646,7 @@ struct SharedPlan {
   int nt, wq, per, tiles_each;
   int64_t tiles;
   int splits, part_steps, own_pieces;
-  size_t o, total; // workspace
+  size_t ml, o, total; // workspace (the sequences' first blocks come first)
 };
 
 static SharedPlan shared_plan(int32_t B, int32_t n_groups, int32_t n_q_heads, int32_t n_kv_heads,
@@ -639,7 +665,7 @@ static SharedPlan shared_plan(int32_t B, int32_t n_groups, int32_t n_q_heads, in
   // Parts of equal steps, so that long groups have more of them and no workgroup is
   // longer than the rest; as many as the GPU holds at once.
   const int64_t busy = std::max<int64_t>(n_groups * each * n_kv_heads, 1);
-  const int64_t steps = ((int64_t)max_shared + 1) / 2, wgs = p.nt == 1 ? 1024 : 512;
+  const int64_t steps = ((int64_t)max_shared + 1) / 2, wgs = p.nt == 1 ? 2048 : 512;
   const int64_t room = std::max<int64_t>(1, kSharedPieces / std::max(B, 1));
   const int least = 4 * (kSharedWaves / p.wq);
   const int64_t splits = std::min({wgs / busy, room, (steps + least - 1) / least});
@@ -652,7 +678,8 @@ static SharedPlan shared_plan(int32_t B, int32_t n_groups, int32_t n_q_heads, in
     p.own_pieces = 0;
   auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
   const size_t rows = (size_t)(p.splits + p.own_pieces) * B * n_q_heads;
-  p.o = up(rows * 8);
+  p.ml = n_groups > 0 ? up((size_t)B * 4) : 0;
+  p.o = p.ml + up(rows * 8);
   p.total = p.o + rows * kHeadDim * 4;
   return p;
 }
@@ -775,15 +802,17 @@ extern "C" int gkv_shared_decode(void *stream, int32_t B, int32_t n_groups, cons
   const int64_t own_wgs = (int64_t)B * ((Hkv + a.heads_per_wg - 1) / a.heads_per_wg);
   const int own_threads = 64 * a.parts * a.heads_per_wg;
   const int64_t prefix_wgs = p.tiles * p.splits * Hkv;
-  if (!grid_fits(own_wgs, own_threads) || !grid_fits(prefix_wgs, 64 * kSharedWaves))
+  if (!grid_fits(own_wgs, own_threads) || !grid_fits(prefix_wgs + B / kSharedWaves + 1, 64 * kSharedWaves))
     return GKV_ERR_UNSUPPORTED;
   if (p.total > 0 && (!workspace || workspace_bytes < p.total))
     return GKV_ERR_WORKSPACE;
-  s.ws_ml = (float *)workspace;
+  s.first = (int32_t *)workspace;
+  s.ws_ml = (float *)((char *)workspace + p.ml);
   s.ws_o = (float *)((char *)workspace + p.o);
+  s.prefix_wgs = (int)prefix_wgs;
   hipStream_t hs = (hipStream_t)stream;
   if (p.splits > 0) {
-    const dim3 grid((unsigned)prefix_wgs);
+    const dim3 grid((unsigned)(prefix_wgs + (B + kSharedWaves - 1) / kSharedWaves));
     if (blk && fine)
       launch_prefix<true, true>(p, grid, hs, s);
     else if (blk)

@@ -59,7 +59,7 @@ def beam(gkv, **o):
 
 @pytest.mark.parametrize("bad,why", [
     (dict(R=-1), "ARG"), (dict(K=0), "ARG"), (dict(V=0), "ARG"), (dict(n=0), "ARG"), (dict(n=1001), "ARG"),
-    (dict(V=5, n=6), "ARG"), (dict(n=65), "UNSUPPORTED"), (dict(K=65), "UNSUPPORTED"), (dict(R=1 << 23), "UNSUPPORTED"),
+    (dict(V=5, n=6), "ARG"), (dict(n=65), "UNSUPPORTED"), (dict(K=65), "UNSUPPORTED"), (dict(R=1 << 23), "UNSUPPORTED"), (dict(V=(1 << 30) + 1, stride=1 << 31), "UNSUPPORTED"),
     (dict(x=None), "ARG"), (dict(x=FAKE + 2), "ARG"), (dict(x=FAKE + 1, dtype=1), "ARG"), (dict(stride=999), "ARG"),
     (dict(dtype=2), "ARG"), (dict(cum=None), "ARG"), (dict(cum=FAKE + 2), "ARG"), (dict(done=FAKE, eos=-1), "ARG"),
     (dict(done=FAKE + 2), "ARG"), (dict(eos=1000), "ARG"), (dict(s=None), "ARG"), (dict(p=None), "ARG"),
