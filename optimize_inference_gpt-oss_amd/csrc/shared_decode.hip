@@ -107,7 +107,7 @@ void shared_prefix_kernel(SharedArgs s) {
   constexpr int QP = BLK ? (FINE ? 2 : 1) : (FINE ? 3 : 2);
   constexpr int kData = 4 * kHeadBytes;          // K and V of two blocks
   constexpr int kStage = kData + (BLK ? 256 : 0); // and their scales: K0, V0, K1, V1, in the first lanes
-  constexpr int DP = BLK && WQ == 2 ? 6 : 4;
+  constexpr int DP = WQ == 4 || BLK ? 3 : 2; // (deeper rings cost workgroups, and ran level)
   constexpr int UPW = kData / 1024 / WQ; // loads of a wave per step, 1 KB each
   constexpr int kRing = WT * DP * kStage, kJoin = (kSharedWaves / 2) * NT * 5 * 1024;
   __shared__ __attribute__((aligned(1024))) char s_mem[kRing > kJoin || WT == 1 ? kRing : kJoin];
@@ -650,13 +650,18 @@ struct SharedPlan {
 };
 
 static SharedPlan shared_plan(int32_t B, int32_t n_groups, int32_t n_q_heads, int32_t n_kv_heads,
-                              int32_t max_shared, int32_t max_own, bool fine) {
+                              int32_t max_shared, int32_t max_own, bool blk, bool fine) {
   SharedPlan p{};
   const int G = n_q_heads / n_kv_heads;
   const int64_t avg = n_groups > 0 ? std::max<int64_t>(1, ((int64_t)B + n_groups - 1) / n_groups) : 1;
   const int64_t cols = avg * G;
-  p.wq = cols <= 32 ? 2 : 4;
-  p.nt = cols <= 64 ? 1 : cols <= 128 || fine ? 2 : 4;
+  // Shapes by the even group's query heads, us of the first launch (64 groups of 256 .. 2048 shared
+  // tokens, 8 kv heads): 32 heads, two waves of a tile 35 (codes 29), four 40 (42); 64 heads,
+  // four waves of one tile 45 (44, fp32 outputs 55), two of two 50 (41, 58); 128 heads, four waves of
+  // two 43 (42), two of four 39 (43). 512 sequences behind one prompt of 2048 tokens:
+  // four waves of four tiles 45, of two 49.
+  p.wq = cols <= 32 || (cols <= 64 && blk && !fine) ? 2 : 4;
+  p.nt = cols <= 32 ? 1 : cols <= 64 ? 4 / p.wq : cols <= 128 || fine ? 2 : 4;
   p.per = 16 * p.nt * p.wq / G;
   // (as many tiles a group has room for as all of the even size need, and one)
   const int64_t each = (avg + p.per - 1) / p.per;
@@ -665,7 +670,7 @@ static SharedPlan shared_plan(int32_t B, int32_t n_groups, int32_t n_q_heads, in
   // Parts of equal steps, so that long groups have more of them and no workgroup is
   // longer than the rest; as many as the GPU holds at once.
   const int64_t busy = std::max<int64_t>(n_groups * each * n_kv_heads, 1);
-  const int64_t steps = ((int64_t)max_shared + 1) / 2, wgs = p.nt == 1 ? 2048 : 512;
+  const int64_t steps = ((int64_t)max_shared + 1) / 2, wgs = p.nt == 4 ? 512 : p.nt == 1 && p.wq == 4 ? 2048 : 1024;
   const int64_t room = std::max<int64_t>(1, kSharedPieces / std::max(B, 1));
   const int least = 4 * (kSharedWaves / p.wq);
   const int64_t splits = std::min({wgs / busy, room, (steps + least - 1) / least});
@@ -694,9 +699,12 @@ static bool shared_sizes_ok(int32_t B, int32_t n_groups, int32_t n_q_heads, int3
 template <bool BLK, bool FINE>
 static void launch_prefix(const SharedPlan &p, dim3 grid, hipStream_t hs, const SharedArgs &s) {
   const dim3 block(64 * kSharedWaves);
-  if (p.wq == 2)
+  if (p.wq == 2 && p.nt == 1)
     hipLaunchKernelGGL((shared_prefix_kernel<BLK, 1, 2, FINE>), grid, block, 0, hs, s);
-  else if (p.nt == 1)
+  else if (p.wq == 2) {
+    if constexpr (BLK && !FINE)
+      hipLaunchKernelGGL((shared_prefix_kernel<BLK, 2, 2, FINE>), grid, block, 0, hs, s);
+  } else if (p.nt == 1)
     hipLaunchKernelGGL((shared_prefix_kernel<BLK, 1, 4, FINE>), grid, block, 0, hs, s);
   else if (p.nt == 2)
     hipLaunchKernelGGL((shared_prefix_kernel<BLK, 2, 4, FINE>), grid, block, 0, hs, s);
@@ -725,8 +733,11 @@ extern "C" size_t gkv_shared_workspace_bytes(int32_t B, int32_t n_groups, int32_
   using namespace gkv;
   if (!shared_sizes_ok(B, n_groups, n_q_heads, n_kv_heads, max_shared_blocks, max_own))
     return 0;
-  return std::max(shared_plan(B, n_groups, n_q_heads, n_kv_heads, max_shared_blocks, max_own, false).total,
-                  shared_plan(B, n_groups, n_q_heads, n_kv_heads, max_shared_blocks, max_own, true).total);
+  size_t most = 0; // (whatever the formats)
+  for (int k = 0; k < 4; k++)
+    most = std::max(most, shared_plan(B, n_groups, n_q_heads, n_kv_heads, max_shared_blocks, max_own,
+                                      k & 1, k & 2).total);
+  return most;
 }
 
 extern "C" int gkv_shared_decode(void *stream, int32_t B, int32_t n_groups, const int32_t *cu_groups,
@@ -759,7 +770,7 @@ extern "C" int gkv_shared_decode(void *stream, int32_t B, int32_t n_groups, cons
       ((uintptr_t)cu_groups | (uintptr_t)shared_blocks) % 4 != 0 || (uintptr_t)workspace % 16 != 0)
     return GKV_ERR_ARG;
   const bool blk = cache.v_format == GKV_KV_FP8_BLOCK, fine = out_dtype == GKV_F32;
-  const SharedPlan p = shared_plan(B, n_groups, n_q_heads, Hkv, max_shared_blocks, max_own, fine);
+  const SharedPlan p = shared_plan(B, n_groups, n_q_heads, Hkv, max_shared_blocks, max_own, blk, fine);
   SharedArgs s{};
   KeptDecodeArgs &a = s.a;
   a.q = q;
