@@ -612,11 +612,16 @@ extern "C" int gkv_tables_reorder(void *stream, gkv_tables t, int32_t group_size
   a.shared = shared_blocks;
   while ((group_size << (a.width_log + 1)) <= kTileEntries && 1 << a.width_log < t.table_stride)
     a.width_log++;
-  const int width = 1 << a.width_log;
   a.tiles = 1;
-  const int64_t all = ((int64_t)t.table_stride + width - 1) / width;
-  if (all > 2 && groups < kReorderWgs)
-    a.tiles = (int)std::min<int64_t>(all, (kReorderWgs + groups - 1) / groups);
+  auto tiles = [&]() { return (((int64_t)t.table_stride - 1) >> a.width_log) + 1; };
+  if (tiles() > 2 && groups < kReorderWgs) {
+    // (narrower tiles where they would be fewer than the CUs: 16 rows of 6258 blocks, 13 of 512
+    // columns 17 us, 98 of 64 7.6)
+    while (a.width_log > 6 && groups * tiles() < kReorderWgs / 2)
+      a.width_log--;
+    a.tiles = (int)std::min<int64_t>(tiles(), (kReorderWgs + groups - 1) / groups);
+  }
+  const int width = 1 << a.width_log;
   const int64_t wgs = (int64_t)groups * a.tiles;
   if (!grid_fits(wgs, kTableThreads))
     return GKV_ERR_UNSUPPORTED;

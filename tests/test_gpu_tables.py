@@ -234,3 +234,33 @@ def test_captured_steps_on_a_stream(gkv, cuda):
         t.same_state()
         assert t.slot[:len(slot)].tolist() == slot and t.dst.tolist() == dst.tolist()
     assert int(t.err.item()) == 0
+
+
+def test_on_another_stream(gkv, cuda):
+    t = Tables(gkv, 70, 8, 600)
+    side = torch.cuda.Stream()
+    new, parents = torch.zeros(70, dtype=torch.int32, device="cuda"), torch.zeros(70, dtype=torch.int32, device="cuda")
+    a, b = np.arange(70, dtype=np.int32) + 5, np.arange(70, dtype=np.int32) // 10 * 10
+    da, db = dev(a), dev(b)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(2000000)
+        new.copy_(da)
+        parents.copy_(db)
+    t.resize(new, stream=side)
+    gkv.tables_reorder(t.t, parents, 10, dev_err=t.err, stream=side)
+    side.synchronize()
+    t.m.resize(a)
+    t.m.reorder(b, 10)
+    t.same_state()
+
+
+@pytest.mark.parametrize("S,rows", [(64, 4096), (64, 4097), (65, 4096), (1024, 30000), (1025, 30000)])
+def test_both_sides_of_the_forms(gkv, cuda, S, rows):
+    """One launch, two, and more sequences than threads."""
+    rng = np.random.default_rng(S + rows)
+    t = Tables(gkv, S, 12, S * 14, rows=rows)
+    t.check_resize(rng.integers(0, 26, S))
+    t.check_reorder(rng.integers(0, S, S), S)
+    t.check_resize(np.minimum(t.m.lens + rng.integers(0, 4, S), 190))
+    t.check_resize(rng.integers(0, 26, S))
