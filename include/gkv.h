@@ -90,7 +90,7 @@ typedef enum { GKV_F32 = 0, GKV_BF16 = 1 } gkv_dtype;
  * GKV_KV_FP8_BLOCK stores the same codes in the same places with one fp32
  * scale of K and one of V per BLOCK of 16 tokens and head (129 bytes a token and
  * head for K and V together, against 136): for the gkv_kept_* entry points,
- * gkv_copy_blocks and the pool; the other kernels refuse it. Readers take any
+ * gkv_shared_decode, gkv_copy_blocks and the pool; the other kernels refuse it. Readers take any
  * finite scale >= 0 (what sees a block with a NaN for a scale gives NaN);
  * gkv_kept_append writes powers of two (see there). */
 typedef enum {
@@ -527,7 +527,7 @@ int gkv_kept_prefill(void *stream, int32_t B, const int32_t *cu_seqlens, const i
 /* Copies block src[i] to block dst[i] (device int32 [n_pairs]) in every one of
  * n_views caches (host array; any format, K, V and scales; the block tables are
  * not used), all in one launch per 32 views (fewer from 2^18 pairs on). The targets are distinct and no
- * target is a source. An id outside a cache sets GKV_DEVERR_BLOCK_ID and is not
+ * target is a source (a pair of a block with itself is no pair: gkv_tables_resize fills up with those). An id outside a cache sets GKV_DEVERR_BLOCK_ID and is not
  * copied there. No counterpart in the reference. */
 int gkv_copy_blocks(void *stream, const gkv_cache_view *views, int32_t n_views, int32_t n_pairs,
                     const int32_t *src, const int32_t *dst, uint32_t *dev_err);
@@ -615,6 +615,7 @@ int gkv_beam_select(void *stream, int32_t n_requests, int32_t n_beams, int32_t v
  *   lens   int32 [n_seqs]: tokens of each sequence (0: an idle place): the seq_lens of
  *          the appends and attention
  *   refs   int32 [num_blocks]: how many table entries hold the block (0: free)
+ * Calls on the same tables, and what reads them, follow one another on a stream.
  * No counterpart in the reference. */
 typedef struct {
   int32_t *table;

@@ -119,7 +119,7 @@ void shared_prefix_kernel(SharedArgs s) {
       return;
     const int grp = group_of(s, b), n = grp < 0 ? 0 : shared_of(s, grp);
     if (lane == 0) {
-      s.first[b] = span_len(a, b) < n * kBlockTokens ? 0 : n;
+      s.first[b] = span_len(a, b) / kBlockTokens < n ? 0 : n;
       if (grp >= 0 && n != s.shared[grp] && a.dev_err)
         atomicOr(a.dev_err, GKV_DEVERR_LENGTH);
     }
@@ -143,6 +143,8 @@ void shared_prefix_kernel(SharedArgs s) {
   const int b0 = min(max(uniform(s.cu_groups[grp]), 0), a.B);
   const int b1 = min(max(uniform(s.cu_groups[grp + 1]), b0), a.B);
   const int first = uniform(shared_of(s, grp));
+  if (first > a.max_len / kBlockTokens) // (no sequence is that long)
+    return;
   const int n = (first + 1) / 2, each = part_steps(s, n);
   const int p0 = min(split * each, n), p1 = min(p0 + each, n);
   const int64_t at0 = b0 + (int64_t)(tile - (b0 / per + grp)) * per;

@@ -4,7 +4,8 @@ import numpy as np
 import pytest
 import torch
 
-from keptcase import BF16, BLOCK, BT, Layout
+from keptcase import BF16, BLOCK, BT
+from oracle import kv_oracle as O
 from sharedcase import Shared, dev, shared_bound, within
 
 pytestmark = pytest.mark.gpu
@@ -232,3 +233,40 @@ def test_captured_calls_share_a_workspace_in_order(gkv, cuda, fmt, bf16):
             gkv.shared_decode(q, 64, cu, sh, lens, 400, view, eager, 18, 200, workspace=ws, dev_err=s.c.err)
             assert torch.equal(eager, out)
             assert int(s.c.err.item()) == 0
+
+
+def test_on_another_stream(gkv, cuda):
+    """Inputs made on a stream of its own, the call on that stream, by name or as the current one."""
+    s = Shared([300, 310, 290], [3], [18], 8, BLOCK, seed=4)
+    whole = s.run(gkv, 64, None, True)
+    x, out = whole[2], whole[3]
+    view = s.c.device(gkv)
+    cu, sh, lens, ws = dev(s.cu), dev(s.shared), dev(s.c.lens), s.ws
+    cos, sin = (dev(t) for t in O.rope_table(310))
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for named in (True, False):
+        q, got = torch.zeros_like(x), torch.zeros_like(out)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(2000000)
+            q.copy_(x)
+            call = dict(sinks=None, cos_tab=cos, sin_tab=sin, workspace=ws, dev_err=s.c.err)
+            if not named:
+                gkv.shared_decode(q, 64, cu, sh, lens, 310, view, got, 18, 20, **call)
+        if named:
+            gkv.shared_decode(q, 64, cu, sh, lens, 310, view, got, 18, 20, stream=side, **call)
+        side.synchronize()
+        assert torch.equal(got, out)
+
+
+@pytest.mark.parametrize("shared", [2**27, 2**27 + 1, 2**31 - 1, 9])
+def test_more_shared_blocks_than_a_sequence_has(gkv, cuda, shared):
+    """(A row of 40 entries.) Nobody is that long: each on its own."""
+    s = Shared([100, 90], [2], [5], 1, BF16)
+    whole = s.run(gkv, 8, None, False)[0]
+    s.c.table[1, :5] = s.c.table[0, :5]
+    s.shared[:] = shared
+    got = s.run(gkv, 8, None, False, hints=(min(shared, 2**20), 100))[0]
+    assert int(s.c.err.item()) == (2 if shared > s.c.table.shape[1] else 0)
+    assert np.allclose(got, whole, atol=1e-5)
