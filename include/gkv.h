@@ -90,9 +90,9 @@ typedef enum { GKV_F32 = 0, GKV_BF16 = 1 } gkv_dtype;
  * GKV_KV_FP8_BLOCK stores the same codes in the same places with one fp32
  * scale of K and one of V per BLOCK of 16 tokens and head (129 bytes a token and
  * head for K and V together, against 136): for the gkv_kept_* entry points,
- * gkv_shared_decode, gkv_copy_blocks and the pool; the other kernels refuse it. Readers take any
- * finite scale >= 0 (what sees a block with a NaN for a scale gives NaN);
- * gkv_kept_append writes powers of two (see there). */
+ * gkv_shared_decode, gkv_copy_blocks and the pool; the other kernels refuse it.
+ * Readers take any finite scale >= 0 (what sees a block with a NaN for a scale
+ * gives NaN); gkv_kept_append writes powers of two (see there). */
 typedef enum {
   GKV_V_BF16 = 0,
   GKV_V_INT8 = 1,
@@ -527,7 +527,8 @@ int gkv_kept_prefill(void *stream, int32_t B, const int32_t *cu_seqlens, const i
 /* Copies block src[i] to block dst[i] (device int32 [n_pairs]) in every one of
  * n_views caches (host array; any format, K, V and scales; the block tables are
  * not used), all in one launch per 32 views (fewer from 2^18 pairs on). The targets are distinct and no
- * target is a source (a pair of a block with itself is no pair: gkv_tables_resize fills up with those). An id outside a cache sets GKV_DEVERR_BLOCK_ID and is not
+ * target is a source (a pair of a block with itself is no pair: gkv_tables_resize
+ * fills up with those). An id outside a cache sets GKV_DEVERR_BLOCK_ID and is not
  * copied there. No counterpart in the reference. */
 int gkv_copy_blocks(void *stream, const gkv_cache_view *views, int32_t n_views, int32_t n_pairs,
                     const int32_t *src, const int32_t *dst, uint32_t *dev_err);
@@ -535,7 +536,8 @@ int gkv_copy_blocks(void *stream, const gkv_cache_view *views, int32_t n_views, 
 /* ---- Sequences that share their first blocks ------------------------------ */
 
 /* Bytes of workspace that gkv_shared_decode needs for these sizes (0: none; workspace may be
- * NULL then). */
+ * NULL then). Fewer sequences may need more: calls of several sizes that share one take the
+ * most of theirs. */
 size_t gkv_shared_workspace_bytes(int32_t B, int32_t n_groups, int32_t n_q_heads,
                                   int32_t n_kv_heads, int32_t max_shared_blocks, int32_t max_own);
 

@@ -599,8 +599,14 @@ def copy_blocks(views, src, dst, dev_err=None, stream=None):
     check("gkv_copy_blocks", st)
 
 
-# Sequences that share blocks, beams, tables on the GPU. The same checks: ValueError for a
-# tensor whose address must not be handed over.
+# Sequences that share blocks, beams, tables on the GPU. ValueError for a tensor whose address
+# must not be handed over: the checks above, and that all of them are where the GPU reads.
+
+
+def _there(t, what):
+    if not t.is_cuda and not t.is_pinned():
+        _refuse(what, "not in GPU memory")
+    return t.data_ptr()
 
 
 def _of(n, t, what, dtype=None):
@@ -613,14 +619,21 @@ def _of(n, t, what, dtype=None):
         return _ints(t, what)
     if t.dtype is not dtype or not t.is_contiguous():
         _refuse(what, f"not contiguous {dtype}")
-    if not t.is_cuda and not t.is_pinned():
-        _refuse(what, "not in GPU memory")
-    return t.data_ptr()
+    return _there(t, what)
+
+
+def _table(t, what):
+    """Address of contiguous fp32, which may be None."""
+    return None if t is None else _of(t.numel(), t, what, _torch.float32)
 
 
 def _ws(t):
     """Address and bytes of a workspace, which may be None."""
-    return (None, 0) if t is None else (t.data_ptr(), t.numel() * t.element_size())
+    if t is None:
+        return None, 0
+    if not t.is_contiguous():
+        _refuse("workspace", "not contiguous")
+    return _there(t, "workspace"), t.numel() * t.element_size()
 
 
 def shared_workspace_bytes(B, n_groups, n_q_heads, n_kv_heads, max_shared_blocks, max_own) -> int:
@@ -638,17 +651,19 @@ def shared_decode(q, n_q_heads, cu_groups, shared_blocks, seq_lens, max_seq_len,
     L = lib()
     B, n_groups = q.shape[0], shared_blocks.shape[0]
     out_stride, out_dtype = _out_rows(out)
-    if out.shape[0] != B:
-        _refuse("out", f"not {B} rows")
+    if q.shape[1] < n_q_heads * 64:
+        _refuse("q", f"not {n_q_heads} heads of 64")
+    if out.shape[0] != B or out.shape[1] < n_q_heads * 64:
+        _refuse("out", f"not {B} rows of {n_q_heads} heads of 64")
     ws, ws_bytes = _ws(workspace)
     st = L.gkv_shared_decode(stream_handle(stream), B, n_groups,
                              _of(n_groups + 1, cu_groups, "cu_groups"),
                              _of(n_groups, shared_blocks, "shared_blocks"), max_shared_blocks,
-                             max_own, n_q_heads, q.data_ptr(), _row_stride(q, "q"),
-                             _floats(cos_tab, "cos_tab"), _floats(sin_tab, "sin_tab"),
+                             max_own, n_q_heads, _there(q, "q"), _row_stride(q, "q"),
+                             _table(cos_tab, "cos_tab"), _table(sin_tab, "sin_tab"),
                              _of(B, seq_lens, "seq_lens"), max_seq_len, view,
-                             _floats(sinks, "sinks"), ws, ws_bytes, out.data_ptr(), out_stride,
-                             out_dtype, ptr(dev_err))
+                             _of(n_q_heads, sinks, "sinks", _torch.float32), ws, ws_bytes,
+                             _there(out, "out"), out_stride, out_dtype, ptr(dev_err))
     check("gkv_shared_decode", st)
 
 
@@ -671,7 +686,8 @@ def beam_select(logits, cum_scores, n_beams, scores, parents, tokens, done=None,
         _refuse("logits", f"not {n_requests} x {n_beams} rows")
     ws, ws_bytes = _ws(workspace)
     n = n_requests * n_out
-    st = L.gkv_beam_select(stream_handle(stream), n_requests, n_beams, vocab, logits.data_ptr(),
+    st = L.gkv_beam_select(stream_handle(stream), n_requests, n_beams, vocab,
+                           _there(logits, "logits"),
                            max(row_stride, vocab) if rows == 1 else row_stride,
                            F32 if dtype is _torch.float32 else BF16,
                            _of(rows, cum_scores, "cum_scores", _torch.float32),

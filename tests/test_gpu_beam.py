@@ -59,7 +59,7 @@ def run(gkv, x, cum, K, n, done=None, eos=-1, stream=None, ws=None):
 def compare(got, want, V):
     """Scores: the row's sum is off by at most its terms' roundings (2^-24 each in the difference, the
     factor and the exponential, which moves by |d| log2 e of it, |d| < 128: 2^-16; sums of at most 2^11
-    terms a lane 2^-13: never all one way, 2^-12 covers them), the output by half a step."""
+    terms a lane 2^-13: together under 2^-12), the output by half a step."""
     scores, parents, tokens, ended, err = got
     s, p, t, d = want
     assert np.array_equal(parents, p) and np.array_equal(tokens, t) and np.array_equal(ended, d)
@@ -225,3 +225,12 @@ def test_captured_selections_share_a_workspace(gkv, cuda):
             s, p, tok, _ = expect(t.float().cpu().numpy(), c.cpu().numpy(), K, n)
             assert np.array_equal(o[1].cpu().numpy(), p) and np.array_equal(o[2].cpu().numpy(), tok)
             assert np.abs(o[0].cpu().numpy() - s).max() <= 2.0 ** -12
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_past_32_bit_offsets(gkv, cuda, dtype):
+    V, stride = 4001, 2**31 + 7
+    x = torch.empty(stride + V, dtype=dtype, device="cuda").as_strided((2, V), (stride, 1))
+    x.copy_(torch.from_numpy(logits(np.random.default_rng(5), 2, V)))
+    cum = np.array([-1.5, -1.25], np.float32)
+    compare(run(gkv, x, cum, 2, 6), expect(x.float().cpu().numpy(), cum, 2, 6), V)

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from keptcase import BF16, BLOCK, BT
+from keptcase import BF16, BLOCK, BT, D
 from oracle import kv_oracle as O
 from sharedcase import Shared, dev, shared_bound, within
 
@@ -270,3 +270,37 @@ def test_more_shared_blocks_than_a_sequence_has(gkv, cuda, shared):
     got = s.run(gkv, 8, None, False, hints=(min(shared, 2**20), 100))[0]
     assert int(s.c.err.item()) == (2 if shared > s.c.table.shape[1] else 0)
     assert np.allclose(got, whole, atol=1e-5)
+
+
+@pytest.mark.parametrize("fmt,bf16", FORMS)
+@pytest.mark.parametrize("size", [3, 7, 14, 40])
+def test_many_steps_of_a_wave(gkv, cuda, fmt, bf16, size):
+    """75 or 150 steps of two blocks, ids outside the pool among them: 24, 56, 112 and 320 query heads to
+    a kv head, all blocks in one part (told of no shared ones)."""
+    blocks, which = 299, [0, 63, 64, 127, 128, 131, 192, 298]
+    lens = blocks * BT + np.arange(size) % 18
+    seen = [np.array([t for t in range(L) if t // BT not in which]) for L in lens]
+
+    def spoil(s):
+        s.c.table[0, which] = [-1, s.c.nb, 2**31 - 1, -2**31, -7, -5, s.c.nb + 1, -1]
+
+    check(gkv, lens, [size], [blocks], 8, 1, fmt, bf16, hints=(0, 0), prepare=spoil, seen=seen, err=1, seed=size)
+
+
+@pytest.mark.parametrize("fmt", [BF16, BLOCK])
+def test_blocks_past_4_gib(gkv, cuda, fmt):
+    """The same blocks behind 4 GiB of others: the same bits."""
+    s = Shared([300, 310, 290], [3], [17], 8, fmt, seed=4)
+    got, q, x, out, _ = s.run(gkv, 64, None, True, rotate=False)
+    ahead = 2**32 // (8 * BT * D * (2 if fmt == BF16 else 1)) + 5
+    far = [None if t is None else torch.zeros((ahead + s.c.nb,) + t.shape[1:], dtype=t.dtype, device="cuda")
+           for t in (s.c.dk, s.c.dv, s.c.ds)]
+    for t, f in zip((s.c.dk, s.c.dv, s.c.ds), far):
+        if t is not None:
+            f[ahead:] = t
+    table = dev(np.where(s.c.table >= 0, s.c.table + ahead, s.c.table).astype(np.int32))
+    view = gkv.cache_view(far[0], far[1], table, 8, v_scale=far[2], v_format=fmt)
+    again = torch.zeros_like(out)
+    gkv.shared_decode(x, 64, dev(s.cu), dev(s.shared), dev(s.c.lens), 310, view, again, 17, 38, workspace=s.ws,
+                      dev_err=s.c.err)
+    assert torch.equal(again, out) and int(s.c.err.item()) == 0

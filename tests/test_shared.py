@@ -166,6 +166,9 @@ CASES = [(py_shared, dict(q=torch.zeros(2, 128, dtype=HALF))), (py_shared, dict(
          (py_shared, dict(cu_groups=L4[:3])), (py_shared, dict(shared_blocks=L4[:2])), (py_shared, dict(seq_lens=ints(3))),
          (py_shared, dict(out=torch.zeros(1, 128))), (py_shared, dict(out=torch.zeros(2, 128, dtype=HALF))),
          (py_shared, dict(sinks=torch.zeros(2, dtype=HALF))), (py_shared, dict(cos_tab=torch.zeros(8, 32, dtype=HALF))),
+         (py_shared, dict(sinks=torch.zeros(1))), (py_shared, dict(sin_tab=torch.zeros(32, 8).t())),
+         (py_shared, dict(q=torch.zeros(2, 64))), (py_shared, dict(out=torch.zeros(2, 64))),
+         (py_shared, dict(workspace=torch.zeros(8, 2)[:, 0])),
          (py_beam, dict(logits=torch.zeros(4, 10, dtype=HALF))), (py_beam, dict(logits=torch.zeros(10, 4).t())),
          (py_beam, dict(logits=torch.zeros(3, 10))), (py_beam, dict(cum_scores=torch.zeros(3))),
          (py_beam, dict(cum_scores=torch.zeros(4, dtype=torch.float64))), (py_beam, dict(parents=ints(2, 2))),
@@ -189,3 +192,16 @@ def test_refused_tensors(gkv, monkeypatch, call, bad):
 def test_host_memory_is_refused(gkv, call):
     with pytest.raises(ValueError, match="not in GPU memory"):
         call(gkv)
+
+
+@pytest.mark.parametrize("call,what", [
+    (py_shared, "q"), (py_shared, "out"), (py_shared, "cos_tab"), (py_shared, "sin_tab"), (py_shared, "sinks"),
+    (py_beam, "logits"), (py_beam, "scores"), (py_resize, "row_slot"), (py_shared, "workspace"), (py_beam, "workspace"),
+    (py_resize, "workspace")])
+def test_any_tensor_in_host_memory_is_refused(gkv, monkeypatch, call, what):
+    """All others are where the GPU reads."""
+    far = {"sinks": torch.zeros(2), "logits": torch.zeros(4, 10), "scores": torch.zeros(2, 3),
+           "row_slot": torch.zeros(5, dtype=torch.int64)}.get(what, torch.zeros(2, 128))
+    monkeypatch.setattr(torch.Tensor, "is_pinned", lambda self: self is not far)
+    with pytest.raises(ValueError, match=what + ": not in GPU memory"):
+        call(gkv, **{what: far})
