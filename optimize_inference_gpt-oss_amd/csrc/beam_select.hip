@@ -53,10 +53,10 @@ __device__ __forceinline__ float lane_of(float x, int lane) {
 __device__ __forceinline__ uint64_t key_of(float x, int token) {
   return (uint64_t)order_of(x + 0.0f) << 32 | (uint32_t)~token;
 }
-__device__ __forceinline__ float logit_of(uint64_t key) {
-  const uint32_t u = (uint32_t)(key >> 32);
+__device__ __forceinline__ float value_of(uint32_t u) { // of order_of's number
   return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
+__device__ __forceinline__ float logit_of(uint64_t key) { return value_of((uint32_t)(key >> 32)); }
 __device__ __forceinline__ int token_of(uint64_t key) { return (int)~(uint32_t)key; }
 
 // Between a wave's writes to LDS and its other lanes' reads: they keep their order by themselves,
@@ -66,27 +66,36 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_wave_barrier();
 }
 
-// The key of lane (lane ^ X).
+// The words of lane and of lane ^ X, in either order, by vector moves (an LDS swizzle's latency would
+// be most of a step's).
 template <int X>
-__device__ __forceinline__ uint64_t other(uint64_t key) {
-  uint32_t lo = (uint32_t)key, hi = (uint32_t)(key >> 32);
-  if (X < 32) { // (a pattern in the instruction, no address)
-    lo = __builtin_amdgcn_ds_swizzle(lo, X << 10 | 0x1f);
-    hi = __builtin_amdgcn_ds_swizzle(hi, X << 10 | 0x1f);
-  } else {
-    lo = __shfl_xor(lo, X);
-    hi = __shfl_xor(hi, X);
+__device__ __forceinline__ void pair_of(uint32_t x, uint32_t &a, uint32_t &b) {
+  if (X >= 16) { // (swaps odd rows of one register with even rows of the other, or halves)
+    const auto r = X == 16 ? __builtin_amdgcn_permlane16_swap(x, x, false, false)
+                           : __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    a = r[0];
+    b = r[1];
+    return;
   }
-  return (uint64_t)hi << 32 | lo;
+  constexpr int kSwap1 = 0xb1, kSwap2 = 0x4e, kSwap3 = 0x1b, kHalfMirror = 0x141, kTurn8 = 0x128;
+  constexpr int ctrl = X == 1 ? kSwap1 : X == 2 ? kSwap2 : X == 4 ? kHalfMirror : kTurn8;
+  uint32_t o = __builtin_amdgcn_mov_dpp(x, ctrl, 0xf, 0xf, true);
+  if (X == 4) // (lane ^ 7, then ^ 3)
+    o = __builtin_amdgcn_mov_dpp(o, kSwap3, 0xf, 0xf, true);
+  a = x;
+  b = o;
 }
 
 // One step of a sort over the lanes: lane and lane ^ X, the larger key to the lower lane where
 // down, else to the upper.
 template <int X>
 __device__ __forceinline__ void sort_step(uint64_t &key, bool down) {
-  const uint64_t o = other<X>(key);
+  uint32_t a[2], b[2];
+  pair_of<X>((uint32_t)key, a[0], b[0]);
+  pair_of<X>((uint32_t)(key >> 32), a[1], b[1]);
+  const uint64_t x = (uint64_t)a[1] << 32 | a[0], y = (uint64_t)b[1] << 32 | b[0];
   const bool lower = (threadIdx.x & X) == 0;
-  key = (key > o) == (lower == down) ? key : o;
+  key = (x > y) == (lower == down) ? x : y;
 }
 
 // Largest first, of keys that rise and then fall (or the reverse).
@@ -185,7 +194,7 @@ __device__ __forceinline__ void row_part(const BeamArgs &a, const char *base, in
   best = 0;
   m = -kFloatMax;
   l = 0.0f;
-  uint64_t nth = 0; // the n-th best key (0: there are fewer)
+  float over = -INFINITY; // the least logit that may join: above the n-th best, whose token is lower
   int listed = 0;
   auto join = [&]() { // the first 64 of the list with the best
     wave_sync();
@@ -194,14 +203,16 @@ __device__ __forceinline__ void row_part(const BeamArgs &a, const char *base, in
     sort_up(key);
     best = best > key ? best : key;
     sort_bitonic(best);
-    nth = (uint64_t)__builtin_amdgcn_readlane((uint32_t)(best >> 32), a.n - 1) << 32 |
-          (uint32_t)__builtin_amdgcn_readlane((uint32_t)best, a.n - 1);
+    const uint32_t nth = __builtin_amdgcn_readlane((uint32_t)(best >> 32), a.n - 1); // (0: there are fewer)
     listed = max(listed - 64, 0);
     wave_sync();
     list[lane] = rest;
     wave_sync();
-    if (nth != 0 && lane == 0 && logit_of(nth) > low[wave])
-      low[wave] = logit_of(nth);
+    if (nth != 0) {
+      over = value_of(nth + 1);
+      if (lane == 0 && value_of(nth) > low[wave])
+        low[wave] = value_of(nth);
+    }
   };
   Tile<BF> next, then; // two tiles under way
   if (t0 < t1)
@@ -214,6 +225,10 @@ __device__ __forceinline__ void row_part(const BeamArgs &a, const char *base, in
 #pragma unroll
       for (int k = 0; k < 16; k++)
         mx = fmaxf(mx, PLAIN ? plain_logit(next.at(k)) : next.at(k));
+    if (t0 + 1 < t1)
+#pragma unroll
+      for (int k = 0; k < 16; k++)
+        mx = fmaxf(mx, PLAIN ? plain_logit(then.at(k)) : then.at(k));
     uint64_t top = key_of(mx, lane);
     sort_up(top);
     mx = logit_of(top);
@@ -226,6 +241,7 @@ __device__ __forceinline__ void row_part(const BeamArgs &a, const char *base, in
   const float fourth = fminf(fminf(low[4], low[5]), fminf(low[6], low[7]));
   for (int t = t0; t < t1; t++) {
     float x[16], top[4], mx; // the largest of four, of all
+    const float l0 = low[0], l1 = low[1], l2 = low[2], l3 = low[3]; // (here: nothing waits for them)
 #pragma unroll
     for (int k = 0; k < 16; k++)
       x[k] = PLAIN ? plain_logit(next.at(k)) : next.at(k);
@@ -242,27 +258,24 @@ __device__ __forceinline__ void row_part(const BeamArgs &a, const char *base, in
 #pragma unroll
     for (int k = 0; k < 16; k++)
       l += __builtin_amdgcn_exp2f((x[k] - m) * kLog2e);
-    const float least = fmaxf(fmaxf(fmaxf(low[0], low[1]), fmaxf(low[2], low[3])), fourth);
-    // (a later token beats the n-th best only with a larger logit)
-    const float over = nth != 0 ? logit_of(nth) : -INFINITY;
-    const bool full = nth != 0;
-    if (!__any(mx >= least && (!full || mx > over)))
+    const float least = fmaxf(fmaxf(fmaxf(l0, l1), fmaxf(l2, l3)), fmaxf(fourth, over));
+    if (!__any(mx >= least))
       continue;
 #pragma unroll
     for (int q = 0; q < 4; q++) {
-      if (!__any(top[q] >= least && (!full || top[q] > over)))
+      if (!__any(top[q] >= least))
         continue;
 #pragma unroll
       for (int k = 4 * q; k < 4 * q + 4; k++) {
-        const int e = Tile<BF>::first(t, k / N, off) + k % N;
-        const uint64_t key = key_of(x[k], e);
-        const bool in = (uint32_t)e < (uint32_t)a.V && x[k] >= least && key > nth;
-        const uint64_t who = __ballot(in);
-        if (who == 0)
+        if (!__any(x[k] >= least))
           continue;
+        const int e = Tile<BF>::first(t, k / N, off) + k % N;
+        const bool in = (uint32_t)e < (uint32_t)a.V && x[k] >= least;
+        const uint64_t who = __ballot(in);
         if (in)
           list[listed + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32),
-                                                  __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] = key;
+                                                  __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] =
+              key_of(x[k], e);
         listed += __popcll(who);
         if (listed >= 64)
           join();
