@@ -30,10 +30,11 @@ struct SharedArgs {
   int n_groups;
   int per, tiles_each;   // sequences of a prefix workgroup; tiles that a group has room for
   int splits, part_steps; // parts of a group's shared blocks, at most; steps of a part, at least
-  int own_pieces, own_steps; // pieces before the last of a sequence's own blocks, at most; steps of one
+  int own_pieces, own_steps; // parts of a sequence's own blocks, at most; steps of one, at least
   float *ws_ml, *ws_o;   // [splits + own_pieces][B][Hq]: (m, l), o[64]
   int32_t *first;        // [B] shared blocks of a sequence that it does not read itself
-  int prefix_wgs;        // of the first launch; behind them, those that fill first
+  int prefix_wgs, own_wgs; // of the first launch
+  int join_parts;        // waves per (sequence, kv head) of the second
 };
 
 // The last i in 0 .. n - 1 with key(i) <= x (key does not fall), -1 if there is none: by 256
@@ -82,8 +83,96 @@ __device__ __forceinline__ int part_steps(const SharedArgs &s, int n) {
   return max((n + s.splits - 1) / s.splits, s.part_steps);
 }
 
+// The same of a sequence's own blocks.
+__device__ __forceinline__ int own_part_steps(const SharedArgs &s, int n) {
+  return max((n + s.own_pieces - 1) / s.own_pieces, s.own_steps);
+}
+
 __device__ __forceinline__ int64_t piece_at(const SharedArgs &s, int i, int b) {
   return ((int64_t)i * s.a.B + b) * (s.a.n_kv_heads * s.a.G);
+}
+
+// ---- own ---------------------------------------------------------------------------------
+
+// A workgroup's four waves take parts waves each of (sequence, kv head)s: the steps of a piece of its
+// own blocks cut among them, joined in LDS.
+constexpr int kOwnBytes = kSharedWaves * (kPieceFloats + 2 * kHeads) * 4; // of LDS
+template <bool BLK, bool FINE>
+__device__ __forceinline__ void own_piece(const SharedArgs &s, int item, float *s_own) {
+  const KeptDecodeArgs &a = s.a;
+  float *s_o = s_own; // [4][kPieceFloats]
+  float2 *s_ml = (float2 *)(s_own + kSharedWaves * kPieceFloats); // [4][kHeads]
+  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, kg = lane >> 4;
+  const int pairs = a.B * a.n_kv_heads, each_wg = kSharedWaves / a.parts;
+  const int wgs = (pairs + each_wg - 1) / each_wg; // of a piece
+  const int slot = wave / a.parts, part = wave % a.parts;
+  const int e = item / wgs, pair = item % wgs * each_wg + slot;
+  const int b = min(pair, pairs - 1) / a.n_kv_heads, g = min(pair, pairs - 1) % a.n_kv_heads;
+  const int len = uniform(a.seq_lens[b]), L = max(min(len, a.max_len), 0);
+  const int grp = group_of(s, b), shared = grp < 0 ? 0 : uniform(shared_of(s, grp));
+  const int first = L / kBlockTokens < shared ? 0 : shared;
+  if (e == 0 && g == 0 && part == 0 && lane == 0 && pair < pairs) {
+    s.first[b] = first;
+    if (a.dev_err && (len > a.max_len || (grp >= 0 && shared != s.shared[grp])))
+      atomicOr(a.dev_err, GKV_DEVERR_LENGTH);
+  }
+  Span sp;
+  sp.L = L;
+  sp.first_blocks = sp.ring0 = 0;
+  sp.win0 = first;
+  sp.n_blocks = (L + kBlockTokens - 1) / kBlockTokens - first;
+  const int n = span_steps(sp), each = own_part_steps(s, n);
+  const int b0 = min(e * each, n), b1 = min(b0 + each, n);
+  const bool ok = pair < pairs && b0 < b1;
+  State st;
+  st.m = kLowest;
+  st.l = 0.0f;
+#pragma unroll
+  for (int nn = 0; nn < 4; nn++)
+    st.o[nn] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  const int s0 = b0 + part * (b1 - b0) / a.parts, s1 = b0 + (part + 1) * (b1 - b0) / a.parts;
+  if (ok && s0 < s1)
+    st = attend<BLK, 2, FINE>(a, b, g, sp, s0, s1);
+  if (a.parts > 1) {
+    if (ok && col < kHeads) {
+#pragma unroll
+      for (int nn = 0; nn < 4; nn++)
+        *(f32x4 *)&s_o[wave * kPieceFloats + col * kHeadDim + 16 * nn + 4 * kg] = st.o[nn];
+      if (kg == 0)
+        s_ml[wave * kHeads + col] = float2{st.m, st.l};
+    }
+    __syncthreads();
+  }
+  if (!ok)
+    return;
+  const int64_t at = piece_at(s, s.splits + e, b) + g * a.G;
+  if (a.parts == 1) {
+    if (col < a.G) {
+#pragma unroll
+      for (int nn = 0; nn < 4; nn++)
+        *(f32x4 *)(s.ws_o + (at + col) * kHeadDim + 16 * nn + 4 * kg) = st.o[nn];
+      if (kg == 0)
+        *(float2 *)(s.ws_ml + 2 * (at + col)) = float2{st.m, st.l};
+    }
+    return;
+  }
+  const int w0 = slot * a.parts;
+  for (int i = part * 64 + lane; i < a.G * (kHeadDim / 4); i += a.parts * 64) {
+    const int hh = i / (kHeadDim / 4);
+    float m = kLowest, l = 0.0f;
+    for (int p = 0; p < a.parts; p++)
+      m = fmaxf(m, s_ml[(w0 + p) * kHeads + hh].x);
+    f32x4 o{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int p = 0; p < a.parts; p++) {
+      const float2 ml = s_ml[(w0 + p) * kHeads + hh];
+      const float f = __builtin_amdgcn_exp2f(ml.x - m);
+      l = fmaf(ml.y, f, l);
+      o += *(const f32x4 *)&s_o[(w0 + p) * kPieceFloats + 4 * i] * f;
+    }
+    *(f32x4 *)(s.ws_o + at * kHeadDim + 4 * i) = o;
+    if (i % (kHeadDim / 4) == 0)
+      *(float2 *)(s.ws_ml + 2 * (at + hh)) = float2{m, l};
+  }
 }
 
 // ---- prefix ----------------------------------------------------------------------------
@@ -100,8 +189,8 @@ __device__ __forceinline__ int64_t piece_at(const SharedArgs &s, int i, int b) {
 // 2^-8 of it; so is a weight here, each at random, and q's 11 (16) bits leave far less.
 template <bool BLK, int NT, int WQ, bool FINE>
 __global__ __launch_bounds__(64 * kSharedWaves)
-__attribute__((amdgpu_waves_per_eu(NT == 1 ? (FINE ? 3 : 4) : 2)))
-void shared_prefix_kernel(SharedArgs s) {
+__attribute__((amdgpu_waves_per_eu(NT == 1 ? (FINE ? 3 : 4) : NT == 2 && BLK && !FINE ? 4 : 2)))
+void shared_read_kernel(SharedArgs s) {
   constexpr int D = kHeadDim, WT = kSharedWaves / WQ;
   constexpr int kHeadBytes = kBlockTokens * D * (BLK ? 1 : 2);
   constexpr int QP = BLK ? (FINE ? 2 : 1) : (FINE ? 3 : 2);
@@ -111,21 +200,25 @@ void shared_prefix_kernel(SharedArgs s) {
   constexpr int UPW = kData / 1024 / WQ; // loads of a wave per step, 1 KB each
   constexpr int kRing = WT * DP * kStage, kJoin = (kSharedWaves / 2) * NT * 5 * 1024;
   __shared__ __attribute__((aligned(1024))) char s_mem[kRing > kJoin || WT == 1 ? kRing : kJoin];
+  static_assert(sizeof(s_mem) >= kOwnBytes, "room for either kind");
   const KeptDecodeArgs &a = s.a;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15, kg = lane >> 4;
-  if ((int)blockIdx.x >= s.prefix_wgs) { // what the second launch asks of every sequence's group
-    const int b = ((int)blockIdx.x - s.prefix_wgs) * kSharedWaves + wave;
-    if (b >= a.B)
-      return;
-    const int grp = group_of(s, b), n = grp < 0 ? 0 : shared_of(s, grp);
-    if (lane == 0) {
-      s.first[b] = span_len(a, b) / kBlockTokens < n ? 0 : n;
-      if (grp >= 0 && n != s.shared[grp] && a.dev_err)
-        atomicOr(a.dev_err, GKV_DEVERR_LENGTH);
-    }
+  // Both kinds of workgroups in turn, 256 at a time (one a CU), then what is left of either.
+  const int turns = min(s.prefix_wgs, s.own_wgs) >> 8;
+  int item = blockIdx.x;
+  bool own;
+  if (item < 2 * turns << 8) {
+    own = item >> 8 & 1;
+    item = (item >> 9 << 8) + (item & 255);
+  } else {
+    item -= turns << 8;
+    own = item >= s.prefix_wgs;
+    item -= own ? s.prefix_wgs - (turns << 8) : 0;
+  }
+  if (own) {
+    own_piece<BLK, FINE>(s, item, (float *)s_mem);
     return;
   }
-  int item = blockIdx.x;
   const int g = item % a.n_kv_heads;
   item /= a.n_kv_heads;
   // Groups' tiles lie end to end, group i's from cu[i] / per + i on: room for all of them,
@@ -502,147 +595,71 @@ void shared_prefix_kernel(SharedArgs s) {
     }
 }
 
-// ---- own ---------------------------------------------------------------------------------
+// ---- join --------------------------------------------------------------------------------
 
-// parts waves of a workgroup per (sequence, kv head): the steps of its own blocks cut among
-// them, the pieces of the prefix (and of earlier own blocks) too; joined in LDS. LAST: the
-// last part, which joins and writes; else part blockIdx.y, which leaves a piece.
-template <bool BLK, bool FINE, bool LAST>
-__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(4)))
-void shared_own_kernel(SharedArgs s) {
-  __shared__ __attribute__((aligned(1024))) float s_o[8][kPieceFloats];
-  __shared__ float2 s_ml[8][kHeads];
+// join_parts waves (1 or 4) per (sequence, kv head) go through its pieces, the prefix's and its own,
+// 8 dims of a head a lane, and the first of them writes.
+__global__ __launch_bounds__(64 * kSharedWaves) void shared_join_kernel(SharedArgs s) {
+  __shared__ f32x4 s_o[kSharedWaves][2][64];
+  __shared__ float2 s_ml[kSharedWaves][64];
   const KeptDecodeArgs &a = s.a;
-  const int n_wg = (a.n_kv_heads + a.heads_per_wg - 1) / a.heads_per_wg;
-  const int b = blockIdx.x / n_wg;
-  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 15, kg = lane >> 4;
-  const int slot = wave / a.parts, part = wave % a.parts;
-  const int g = (int)(blockIdx.x % n_wg) * a.heads_per_wg + slot;
-  const bool ok = g < a.n_kv_heads;
-  const int len = uniform(a.seq_lens[b]), L = max(min(len, a.max_len), 0);
-  if (LAST && len > a.max_len && threadIdx.x == 0 && a.dev_err)
-    atomicOr(a.dev_err, GKV_DEVERR_LENGTH);
-  const int Hq = a.n_kv_heads * a.G;
-  if (L == 0) {
-    if (LAST && ok)
-      put_zeros(a, (int64_t)b * a.out_stride + (int64_t)g * a.G * kHeadDim, a.G * kHeadDim,
-                part * 64 + lane, a.parts * 64);
-    return;
+  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int each_wg = kSharedWaves / s.join_parts, part = wave % s.join_parts;
+  const int pairs = a.B * a.n_kv_heads, pair = blockIdx.x * each_wg + wave / s.join_parts;
+  const int b = min(pair, pairs - 1) / a.n_kv_heads, g = min(pair, pairs - 1) % a.n_kv_heads;
+  const int L = uniform(span_len(a, b)), first = uniform(s.first[b]);
+  const int head = min(lane >> 3, a.G - 1), dim = 8 * (lane & 7);
+  const int steps = (first + 1) / 2, own = ((L + kBlockTokens - 1) / kBlockTokens - first + 1) / 2;
+  const int n_prefix = (steps + part_steps(s, steps) - 1) / part_steps(s, steps);
+  const int n = n_prefix + (own + own_part_steps(s, own) - 1) / own_part_steps(s, own);
+  float m = kLowest, l = 0.0f;
+  f32x4 o[2] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}, f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
+  auto join = [&](float2 with, f32x4 o0, f32x4 o1) {
+    const float mn = fmaxf(m, with.x);
+    const float f0 = __builtin_amdgcn_exp2f(m - mn), f1 = __builtin_amdgcn_exp2f(with.x - mn);
+    m = mn;
+    l = l * f0 + with.y * f1;
+    o[0] = o[0] * f0 + o0 * f1;
+    o[1] = o[1] * f0 + o1 * f1;
+  };
+  constexpr int A = 4; // pieces under way
+  for (int i = part; i < n; i += A * s.join_parts) {
+    float2 ml[A];
+    f32x4 x[A][2];
+#pragma unroll
+    for (int k = 0; k < A; k++) {
+      const int p = min(i + k * s.join_parts, n - 1);
+      const int64_t at = piece_at(s, p < n_prefix ? p : s.splits + p - n_prefix, b) + g * a.G + head;
+      ml[k] = *(const float2 *)(s.ws_ml + 2 * at);
+      x[k][0] = *(const f32x4 *)(s.ws_o + at * kHeadDim + dim);
+      x[k][1] = *(const f32x4 *)(s.ws_o + at * kHeadDim + dim + 4);
+    }
+#pragma unroll
+    for (int k = 0; k < A; k++)
+      if (i + k * s.join_parts < n)
+        join(ml[k], x[k][0], x[k][1]);
   }
-  const int first = s.n_groups > 0 ? uniform(s.first[b]) : 0;
-  Span sp;
-  sp.L = L;
-  sp.first_blocks = sp.ring0 = 0;
-  sp.win0 = first;
-  sp.n_blocks = (L + kBlockTokens - 1) / kBlockTokens - first;
-  // this workgroup's steps: part e of own_pieces + 1
-  const int n = span_steps(sp);
-  const int each = max((n + s.own_pieces) / (s.own_pieces + 1), s.own_steps);
-  const int before = n > 0 ? (n - 1) / each : 0; // pieces before the last
-  const int e = LAST ? before : (int)blockIdx.y;
-  if (!LAST && e >= before)
-    return;
-  const int b0 = e * each, b1 = min(b0 + each, n);
-  State st;
-  st.m = kLowest;
-  st.l = 0.0f;
-#pragma unroll
-  for (int nn = 0; nn < 4; nn++)
-    st.o[nn] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  if (ok) {
-    // This wave's pieces: the first comes into LDS while its blocks are read, the others behind.
-    const int steps = (first + 1) / 2;
-    const int n_prefix = first > 0 ? (steps + part_steps(s, steps) - 1) / part_steps(s, steps) : 0;
-    const int n_pieces = LAST ? n_prefix + before : 0;
-    auto piece = [&](int i) {
-      return piece_at(s, i < n_prefix ? i : s.splits + i - n_prefix, b) + g * a.G;
-    };
-    const int hc = min(col, a.G - 1);
-    float2 ml{kLowest, 0.0f};
-    if (part < n_pieces) {
-      const char *o = (const char *)(s.ws_o + piece(part) * kHeadDim);
-#pragma unroll
-      for (int x = 0; x < 2; x++)
-        dma16(o + min(x * 1024 + lane * 16, a.G * kHeadDim * 4 - 16), (char *)s_o[wave] + x * 1024);
-      ml = *(const float2 *)(s.ws_ml + 2 * (piece(part) + hc));
-    }
-    const int s0 = b0 + part * (b1 - b0) / a.parts, s1 = b0 + (part + 1) * (b1 - b0) / a.parts;
-    if (s0 < s1)
-      st = attend<BLK, 2, FINE>(a, b, g, sp, s0, s1);
-    // a piece onto what there is: 4 dims of each 16 of the column's head
-    auto join = [&](float2 with, const f32x4 (&o)[4]) {
-      const float m = fmaxf(st.m, with.x);
-      const float f0 = __builtin_amdgcn_exp2f(st.m - m), f1 = __builtin_amdgcn_exp2f(with.x - m);
-      st.m = m;
-      st.l = st.l * f0 + with.y * f1;
-#pragma unroll
-      for (int nn = 0; nn < 4; nn++)
-        st.o[nn] = st.o[nn] * f0 + o[nn] * f1;
-    };
-    f32x4 *mine = (f32x4 *)&s_o[wave][(col & 7) * kHeadDim + 4 * kg];
-    if (part < n_pieces) {
-      wait_vmcnt<0>();
-      asm volatile("" ::: "memory"); // (its LDS reads stay behind the wait)
-      const f32x4 o[4] = {mine[0], mine[4], mine[8], mine[12]};
-      join(ml, o);
-    }
-    constexpr int A = 4; // pieces under way
-    for (int i = part + a.parts; i < n_pieces; i += A * a.parts) {
-      float2 m[A];
-      f32x4 o[A][4];
-#pragma unroll
-      for (int x = 0; x < A; x++) {
-        const int64_t at = piece(min(i + x * a.parts, n_pieces - 1)) + hc;
-        m[x] = *(const float2 *)(s.ws_ml + 2 * at);
-#pragma unroll
-        for (int nn = 0; nn < 4; nn++)
-          o[x][nn] = *(const f32x4 *)(s.ws_o + at * kHeadDim + 16 * nn + 4 * kg);
-      }
-#pragma unroll
-      for (int x = 0; x < A; x++)
-        if (i + x * a.parts < n_pieces)
-          join(m[x], o[x]);
-    }
-    __builtin_amdgcn_wave_barrier(); // (a wave's LDS accesses keep their order)
-    if (col < kHeads) {
-#pragma unroll
-      for (int nn = 0; nn < 4; nn++)
-        mine[4 * nn] = st.o[nn];
-      if (kg == 0)
-        s_ml[wave][col] = float2{st.m, st.l};
-    }
+  if (s.join_parts > 1) {
+    s_ml[wave][lane] = float2{m, l};
+    s_o[wave][0][lane] = o[0];
+    s_o[wave][1][lane] = o[1];
+    __syncthreads();
+    if (part == 0)
+      for (int k = 1; k < s.join_parts; k++)
+        join(s_ml[wave + k][lane], s_o[wave + k][0][lane], s_o[wave + k][1][lane]);
   }
-  __syncthreads();
-  if (!ok)
+  if (part != 0 || pair >= pairs || lane >= 8 * a.G)
     return;
-  const int w0 = slot * a.parts;
-  for (int i = part * 64 + lane; i < a.G * (kHeadDim / 4); i += a.parts * 64) {
-    const int hh = i / (kHeadDim / 4);
-    float m = kLowest, l = 0.0f;
-    for (int p = 0; p < a.parts; p++)
-      m = fmaxf(m, s_ml[w0 + p][hh].x);
-    f32x4 o{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int p = 0; p < a.parts; p++) {
-      const float f = __builtin_amdgcn_exp2f(s_ml[w0 + p][hh].x - m);
-      l = fmaf(s_ml[w0 + p][hh].y, f, l);
-      o += *(const f32x4 *)&s_o[w0 + p][4 * i] * f;
-    }
-    if (LAST) {
-      put(a.out, (int64_t)b * a.out_stride + (int64_t)g * a.G * kHeadDim + 4 * i,
-          o * out_factor(m, l, sink_of(a, g, hh)), a.out_bf16);
-    } else {
-      const int64_t at = piece_at(s, s.splits + e, b) + g * a.G + hh;
-      *(f32x4 *)(s.ws_o + at * kHeadDim + 4 * (i % (kHeadDim / 4))) = o;
-      if (i % (kHeadDim / 4) == 0)
-        *(float2 *)(s.ws_ml + 2 * at) = float2{m, l};
-    }
-  }
+  const float f = L > 0 ? out_factor(m, l, sink_of(a, g, head)) : 0.0f;
+  const int64_t at = (int64_t)b * a.out_stride + (int64_t)(g * a.G + head) * kHeadDim + dim;
+  put(a.out, at, o[0] * f, a.out_bf16);
+  put(a.out, at + 4, o[1] * f, a.out_bf16);
 }
 
 // ---- host side ------------------------------------------------------------------------
 
 constexpr int kSharedPieces = 2048; // pieces (times sequences) per kind, at most, or one per sequence
-constexpr int kOwnSteps = 72;      // steps of own blocks that one workgroup takes in the last launch
+constexpr int kOwnSteps = 72;      // steps of own blocks of a piece, at least
 
 struct SharedPlan {
   int nt, wq, per, tiles_each;
@@ -678,16 +695,13 @@ static SharedPlan shared_plan(int32_t B, int32_t n_groups, int32_t n_q_heads, in
   const int64_t room = std::max<int64_t>(1, kSharedPieces / std::max(B, 1));
   const int least = 4 * (kSharedWaves / p.wq);
   const int64_t splits = std::min({wgs / busy, room, (steps + least - 1) / least});
-  p.splits = n_groups > 0 ? (int)std::max<int64_t>(1, splits) : 0;
-  p.part_steps = p.splits > 0 ? (int)std::max<int64_t>(least, (steps + p.splits - 1) / p.splits) : 1;
+  p.splits = (int)std::max<int64_t>(1, splits);
+  p.part_steps = (int)std::max<int64_t>(least, (steps + p.splits - 1) / p.splits);
   const int64_t own_steps = (((int64_t)max_own + kBlockTokens - 1) / kBlockTokens + 1) / 2;
-  p.own_pieces = (int)std::min((own_steps + kOwnSteps - 1) / kOwnSteps - 1, room);
-  p.own_pieces = std::max(p.own_pieces, 0);
-  if (B > kSharedPieces)
-    p.own_pieces = 0;
+  p.own_pieces = (int)std::max<int64_t>(1, std::min((own_steps + kOwnSteps - 1) / kOwnSteps, room));
   auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
   const size_t rows = (size_t)(p.splits + p.own_pieces) * B * n_q_heads;
-  p.ml = n_groups > 0 ? up((size_t)B * 4) : 0;
+  p.ml = up((size_t)B * 4);
   p.o = p.ml + up(rows * 8);
   p.total = p.o + rows * kHeadDim * 4;
   return p;
@@ -701,32 +715,19 @@ static bool shared_sizes_ok(int32_t B, int32_t n_groups, int32_t n_q_heads, int3
 }
 
 template <bool BLK, bool FINE>
-static void launch_prefix(const SharedPlan &p, dim3 grid, hipStream_t hs, const SharedArgs &s) {
+static void launch_read(const SharedPlan &p, dim3 grid, hipStream_t hs, const SharedArgs &s) {
   const dim3 block(64 * kSharedWaves);
   if (p.wq == 2 && p.nt == 1)
-    hipLaunchKernelGGL((shared_prefix_kernel<BLK, 1, 2, FINE>), grid, block, 0, hs, s);
+    hipLaunchKernelGGL((shared_read_kernel<BLK, 1, 2, FINE>), grid, block, 0, hs, s);
   else if (p.wq == 2) {
     if constexpr (BLK && !FINE)
-      hipLaunchKernelGGL((shared_prefix_kernel<BLK, 2, 2, FINE>), grid, block, 0, hs, s);
+      hipLaunchKernelGGL((shared_read_kernel<BLK, 2, 2, FINE>), grid, block, 0, hs, s);
   } else if (p.nt == 1)
-    hipLaunchKernelGGL((shared_prefix_kernel<BLK, 1, 4, FINE>), grid, block, 0, hs, s);
+    hipLaunchKernelGGL((shared_read_kernel<BLK, 1, 4, FINE>), grid, block, 0, hs, s);
   else if (p.nt == 2)
-    hipLaunchKernelGGL((shared_prefix_kernel<BLK, 2, 4, FINE>), grid, block, 0, hs, s);
+    hipLaunchKernelGGL((shared_read_kernel<BLK, 2, 4, FINE>), grid, block, 0, hs, s);
   else if constexpr (!FINE)
-    hipLaunchKernelGGL((shared_prefix_kernel<BLK, 4, 4, false>), grid, block, 0, hs, s);
-}
-
-template <bool LAST>
-static void launch_own(bool blk, bool fine, dim3 grid, dim3 block, hipStream_t hs,
-                       const SharedArgs &s) {
-  if (blk && fine)
-    hipLaunchKernelGGL((shared_own_kernel<true, true, LAST>), grid, block, 0, hs, s);
-  else if (blk)
-    hipLaunchKernelGGL((shared_own_kernel<true, false, LAST>), grid, block, 0, hs, s);
-  else if (fine)
-    hipLaunchKernelGGL((shared_own_kernel<false, true, LAST>), grid, block, 0, hs, s);
-  else
-    hipLaunchKernelGGL((shared_own_kernel<false, false, LAST>), grid, block, 0, hs, s);
+    hipLaunchKernelGGL((shared_read_kernel<BLK, 4, 4, false>), grid, block, 0, hs, s);
 }
 
 } // namespace gkv
@@ -810,41 +811,35 @@ extern "C" int gkv_shared_decode(void *stream, int32_t B, int32_t n_groups, cons
     return GKV_OK;
   // waves per (sequence, head): a few steps each, more where few sequences are there
   const int64_t own = std::min<int64_t>((((int64_t)max_own + 15) / 16 + 1) / 2, kOwnSteps);
+  const int64_t pairs = (int64_t)B * Hkv;
   a.parts = 1;
-  while (a.parts < 8 && ((int64_t)2 * a.parts * B * Hkv <= 2048 || own > 16 * a.parts))
+  while (a.parts < kSharedWaves && (2 * a.parts * pairs <= 2048 || own > 16 * a.parts))
     a.parts *= 2;
-  a.heads_per_wg = std::min(8 / a.parts, Hkv);
-  const int64_t own_wgs = (int64_t)B * ((Hkv + a.heads_per_wg - 1) / a.heads_per_wg);
-  const int own_threads = 64 * a.parts * a.heads_per_wg;
+  s.join_parts = p.splits + p.own_pieces > 4 && pairs <= 1024 ? kSharedWaves : 1;
+  const int64_t own_wgs = p.own_pieces * ((pairs * a.parts + kSharedWaves - 1) / kSharedWaves);
+  const int64_t join_wgs = (pairs * s.join_parts + kSharedWaves - 1) / kSharedWaves;
   const int64_t prefix_wgs = p.tiles * p.splits * Hkv;
-  if (!grid_fits(own_wgs, own_threads) || !grid_fits(prefix_wgs + B / kSharedWaves + 1, 64 * kSharedWaves))
+  if (pairs > INT32_MAX || !grid_fits(prefix_wgs + own_wgs, 64 * kSharedWaves))
     return GKV_ERR_UNSUPPORTED;
-  if (p.total > 0 && (!workspace || workspace_bytes < p.total))
+  if (!workspace || workspace_bytes < p.total)
     return GKV_ERR_WORKSPACE;
   s.first = (int32_t *)workspace;
   s.ws_ml = (float *)((char *)workspace + p.ml);
   s.ws_o = (float *)((char *)workspace + p.o);
   s.prefix_wgs = (int)prefix_wgs;
+  s.own_wgs = (int)own_wgs;
   hipStream_t hs = (hipStream_t)stream;
-  if (p.splits > 0) {
-    const dim3 grid((unsigned)(prefix_wgs + (B + kSharedWaves - 1) / kSharedWaves));
-    if (blk && fine)
-      launch_prefix<true, true>(p, grid, hs, s);
-    else if (blk)
-      launch_prefix<true, false>(p, grid, hs, s);
-    else if (fine)
-      launch_prefix<false, true>(p, grid, hs, s);
-    else
-      launch_prefix<false, false>(p, grid, hs, s);
-    if ((st = launch_status("shared_prefix_kernel")))
-      return st;
-  }
-  const dim3 block(own_threads);
-  if (p.own_pieces > 0) {
-    launch_own<false>(blk, fine, dim3((unsigned)own_wgs, (unsigned)p.own_pieces), block, hs, s);
-    if ((st = launch_status("shared_own_kernel")))
-      return st;
-  }
-  launch_own<true>(blk, fine, dim3((unsigned)own_wgs), block, hs, s);
-  return launch_status("shared_own_kernel");
+  const dim3 grid((unsigned)(prefix_wgs + own_wgs));
+  if (blk && fine)
+    launch_read<true, true>(p, grid, hs, s);
+  else if (blk)
+    launch_read<true, false>(p, grid, hs, s);
+  else if (fine)
+    launch_read<false, true>(p, grid, hs, s);
+  else
+    launch_read<false, false>(p, grid, hs, s);
+  if ((st = launch_status("shared_read_kernel")))
+    return st;
+  hipLaunchKernelGGL(shared_join_kernel, dim3((unsigned)join_wgs), dim3(64 * kSharedWaves), 0, hs, s);
+  return launch_status("shared_join_kernel");
 }

@@ -7,7 +7,7 @@ from test_isa import device_asm, kernels, no_spills
 
 @pytest.mark.timeout(600)
 @pytest.mark.parametrize("src,prefix,streams", [
-    ("shared_decode", "shared_prefix_kernel", True), ("shared_decode", "shared_own_kernel", True),
+    ("shared_decode", "shared_read_kernel", True), ("shared_decode", "shared_join_kernel", False),
     ("beam_select", "beam_rows_kernel", False), ("beam_select", "beam_merge_kernel", False),
     ("block_tables", "tables_plan_kernel", False), ("block_tables", "tables_apply_kernel", False),
     ("block_tables", "tables_reorder_kernel", False), ("block_tables", "tables_init_kernel", False)])
