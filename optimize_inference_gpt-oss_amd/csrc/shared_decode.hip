@@ -9,12 +9,19 @@
 // them are a sequence's own and stream as in kept_decode.hip.
 //
 // Two launches:
-//   prefix   a workgroup of four waves takes tiles of a group's query heads and a part of its
-//            shared blocks, and leaves (m, l, o) per query head
-//   own      a workgroup takes a sequence's own blocks (or, with long ones, its last part:
-//            the others leave pieces in a launch before it), joins the pieces and writes
+//   read     a workgroup of four waves takes tiles of a group's query heads and a part of its
+//            shared blocks, or parts of some sequences' own blocks, and leaves (m, l, o) per
+//            query head. Shared blocks are bound by the instructions that go with the matrix
+//            ops, own blocks by HBM: both kinds of workgroups run side by side
+//   join     the pieces of a sequence's query heads, in their order, the sink, the output
 // A sequence shorter than the shared blocks is read on its own, so the prefix
 // needs no mask.
+//
+// 8 kv heads of 8 query heads, bf16 outputs, both launches: 512 sequences of 129 .. 1025 own
+// tokens behind a prompt of 2048, bf16, 148 us (4.2 TB/s; in launches of their own, one kind after
+// the other, 170); 64 x 8 beams behind 256 .. 2048 tokens, codes, 57 (67); one request's four behind
+// 2048 tokens 12 (13.6). 2 x 16 behind 27000, codes, fp32 outputs 70: 570 TF/s with the pieces of
+// q and p, whose cutting costs as much again.
 #include "kept_attend.hpp"
 #include "lds_dma.hpp"
 
@@ -674,24 +681,26 @@ static SharedPlan shared_plan(int32_t B, int32_t n_groups, int32_t n_q_heads, in
   const int G = n_q_heads / n_kv_heads;
   const int64_t avg = n_groups > 0 ? std::max<int64_t>(1, ((int64_t)B + n_groups - 1) / n_groups) : 1;
   const int64_t cols = avg * G;
-  // Shapes by the even group's query heads, us of the first launch (64 groups of 256 .. 2048 shared
-  // tokens, 8 kv heads): 32 heads, two waves of a tile 35 (codes 29), four 40 (42); 64 heads,
-  // four waves of one tile 45 (44, fp32 outputs 55), two of two 50 (41, 58); 128 heads, four waves of
-  // two 43 (42), two of four 39 (43). 512 sequences behind one prompt of 2048 tokens:
-  // four waves of four tiles 45, of two 49.
+  // Shapes by the even group's query heads, us of the prefix's workgroups alone (64 groups of
+  // 256 .. 2048 shared tokens, 8 kv heads): 32 heads, two waves of a tile 35 (codes 29), four 40
+  // (42); 64 heads, four waves of one tile 45 (44, fp32 outputs 55), two of two 50 (41, 58);
+  // 128 heads, four waves of two 43 (42). Four waves of four tiles are faster alone (512
+  // sequences behind one prompt of 2048 tokens 45, of two 49), but leave own blocks no room beside
+  // them: 155 for both, 148.
   p.wq = cols <= 32 || (cols <= 64 && blk && !fine) ? 2 : 4;
-  p.nt = cols <= 32 ? 1 : cols <= 64 ? 4 / p.wq : cols <= 128 || fine ? 2 : 4;
+  p.nt = cols <= 32 || (cols <= 64 && p.wq == 4) ? 1 : 2;
   p.per = 16 * p.nt * p.wq / G;
   // (as many tiles a group has room for as all of the even size need, and one)
   const int64_t each = (avg + p.per - 1) / p.per;
   p.tiles_each = (int)each + 1;
   p.tiles = p.tiles_each * (int64_t)n_groups;
-  // Parts of equal steps, so that long groups have more of them and no workgroup is
-  // longer than the rest; as many as the GPU holds at once (2 x 16 sequences behind 27000 tokens,
-  // fp32 outputs: 1024 workgroups 61 us and 14 for the second launch, 768 59 and 12.5).
+  // Parts of equal steps, so that long groups have more of them and no workgroup is longer than
+  // the rest; as many as the GPU holds at once, or half of that where a wave's registers are many
+  // (2 x 16 sequences behind 27000 tokens, fp32 outputs, both launches: 512 workgroups 70 us,
+  // 768 71, 1024 71; 512 sequences behind 2048 tokens 148, 768 155).
   const int64_t busy = std::max<int64_t>(n_groups * each * n_kv_heads, 1);
   const int64_t steps = ((int64_t)max_shared + 1) / 2;
-  const int64_t wgs = p.nt == 4 ? 512 : p.nt == 2 && !(blk && !fine) ? 768 : p.nt == 1 && p.wq == 4 ? 2048 : 1024;
+  const int64_t wgs = p.nt == 2 && !(blk && !fine) ? 512 : p.nt == 1 && p.wq == 4 ? 2048 : 1024;
   const int64_t room = std::max<int64_t>(1, kSharedPieces / std::max(B, 1));
   const int least = 4 * (kSharedWaves / p.wq);
   const int64_t splits = std::min({wgs / busy, room, (steps + least - 1) / least});
@@ -724,10 +733,8 @@ static void launch_read(const SharedPlan &p, dim3 grid, hipStream_t hs, const Sh
       hipLaunchKernelGGL((shared_read_kernel<BLK, 2, 2, FINE>), grid, block, 0, hs, s);
   } else if (p.nt == 1)
     hipLaunchKernelGGL((shared_read_kernel<BLK, 1, 4, FINE>), grid, block, 0, hs, s);
-  else if (p.nt == 2)
+  else
     hipLaunchKernelGGL((shared_read_kernel<BLK, 2, 4, FINE>), grid, block, 0, hs, s);
-  else if constexpr (!FINE)
-    hipLaunchKernelGGL((shared_read_kernel<BLK, 4, 4, false>), grid, block, 0, hs, s);
 }
 
 } // namespace gkv
@@ -809,11 +816,11 @@ extern "C" int gkv_shared_decode(void *stream, int32_t B, int32_t n_groups, cons
   s.own_steps = kOwnSteps;
   if (B == 0)
     return GKV_OK;
-  // waves per (sequence, head): a few steps each, more where few sequences are there
+  // waves per (sequence, head): more where few sequences are there, or long ones
   const int64_t own = std::min<int64_t>((((int64_t)max_own + 15) / 16 + 1) / 2, kOwnSteps);
   const int64_t pairs = (int64_t)B * Hkv;
   a.parts = 1;
-  while (a.parts < kSharedWaves && (2 * a.parts * pairs <= 2048 || own > 16 * a.parts))
+  while (a.parts < kSharedWaves && (2 * a.parts * pairs <= 2048 || own > 64 * a.parts))
     a.parts *= 2;
   s.join_parts = p.splits + p.own_pieces > 4 && pairs <= 1024 ? kSharedWaves : 1;
   const int64_t own_wgs = p.own_pieces * ((pairs * a.parts + kSharedWaves - 1) / kSharedWaves);
