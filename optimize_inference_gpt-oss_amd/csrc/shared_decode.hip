@@ -40,7 +40,7 @@ struct SharedArgs {
   int own_pieces, own_steps; // parts of a sequence's own blocks, at most; steps of one, at least
   float *ws_ml, *ws_o;   // [splits + own_pieces][B][Hq]: (m, l), o[64]
   int32_t *first;        // [B] shared blocks of a sequence that it does not read itself
-  int prefix_wgs, own_wgs; // of the first launch
+  int prefix_wgs;        // of the first launch; behind them, those of own blocks
   int join_parts;        // waves per (sequence, kv head) of the second
 };
 
@@ -210,20 +210,11 @@ void shared_read_kernel(SharedArgs s) {
   static_assert(sizeof(s_mem) >= kOwnBytes, "room for either kind");
   const KeptDecodeArgs &a = s.a;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15, kg = lane >> 4;
-  // Both kinds of workgroups in turn, 256 at a time (one a CU), then what is left of either.
-  const int turns = min(s.prefix_wgs, s.own_wgs) >> 8;
+  // (the prefix's workgroups, which are the longer ones, first, own blocks in the room beside them; both
+  // in turn, 256 each, ran level)
   int item = blockIdx.x;
-  bool own;
-  if (item < 2 * turns << 8) {
-    own = item >> 8 & 1;
-    item = (item >> 9 << 8) + (item & 255);
-  } else {
-    item -= turns << 8;
-    own = item >= s.prefix_wgs;
-    item -= own ? s.prefix_wgs - (turns << 8) : 0;
-  }
-  if (own) {
-    own_piece<BLK, FINE>(s, item, (float *)s_mem);
+  if (item >= s.prefix_wgs) {
+    own_piece<BLK, FINE>(s, item - s.prefix_wgs, (float *)s_mem);
     return;
   }
   const int g = item % a.n_kv_heads;
@@ -834,7 +825,6 @@ extern "C" int gkv_shared_decode(void *stream, int32_t B, int32_t n_groups, cons
   s.ws_ml = (float *)((char *)workspace + p.ml);
   s.ws_o = (float *)((char *)workspace + p.o);
   s.prefix_wgs = (int)prefix_wgs;
-  s.own_wgs = (int)own_wgs;
   hipStream_t hs = (hipStream_t)stream;
   const dim3 grid((unsigned)(prefix_wgs + own_wgs));
   if (blk && fine)
