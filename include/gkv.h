@@ -549,8 +549,8 @@ size_t gkv_shared_workspace_bytes(int32_t B, int32_t n_groups, int32_t n_q_heads
  *                  sequence in no group is read on its own.
  *   shared_blocks  device int32 [n_groups]: the first shared_blocks[g] blocks (16 positions each,
  *                  all full) are the same for the whole group, and are read through
- *                  the table row of the group's first sequence; the other rows' entries
- *                  there are not looked at (one more than a table row has is taken at the row's
+ *                  the table row of the group's first sequence, which holds them all; the other
+ *                  rows' entries there are not looked at (one more than a table row has is taken at the row's
  *                  length: GKV_DEVERR_LENGTH). A sequence that ends before them is read on
  *                  its own, through its own row. gkv_tables_reorder counts them; forks of the
  *                  pool share what gkv_pool_seq_fork was given, in full blocks.

@@ -304,3 +304,10 @@ def test_blocks_past_4_gib(gkv, cuda, fmt):
     gkv.shared_decode(x, 64, dev(s.cu), dev(s.shared), dev(s.c.lens), 310, view, again, 17, 38, workspace=s.ws,
                       dev_err=s.c.err)
     assert torch.equal(again, out) and int(s.c.err.item()) == 0
+
+
+@pytest.mark.parametrize("fmt,bf16", FORMS)
+def test_no_groups(gkv, cuda, fmt, bf16):
+    """Every sequence on its own: short ones, and ones of several pieces."""
+    check(gkv, [17, 0, 1, 300], [], [], 16, 2, fmt, bf16)
+    check(gkv, [5000, 17], [], [], 8, 1, fmt, bf16)
