@@ -610,21 +610,17 @@ def _there(t, what):
 
 
 def _of(n, t, what, dtype=None):
-    """Address of a contiguous device tensor of n int32 (or dtype) elements, which may be None."""
+    """Address of a contiguous device tensor of n int32 (or dtype) elements (n None: any number of
+    them), which may be None."""
     if t is None:
         return None
-    if t.numel() != n:
+    if n is not None and t.numel() != n:
         _refuse(what, f"not {n} elements")
-    if dtype is None:
-        return _ints(t, what)
-    if t.dtype is not dtype or not t.is_contiguous():
-        _refuse(what, f"not contiguous {dtype}")
-    return _there(t, what)
-
-
-def _table(t, what):
-    """Address of contiguous fp32, which may be None."""
-    return None if t is None else _of(t.numel(), t, what, _torch.float32)
+    if t.dtype is not (dtype or _torch.int32) or not t.is_contiguous():
+        _refuse(what, f"not contiguous {dtype or _torch.int32}")
+    if not t.is_cuda and not t.is_pinned():
+        _refuse(what, "not in GPU memory")
+    return t.data_ptr()
 
 
 def _ws(t):
@@ -649,18 +645,21 @@ def shared_decode(q, n_q_heads, cu_groups, shared_blocks, seq_lens, max_seq_len,
     max_own (tokens behind them) size the launches only. The types of kept_decode; ValueError
     otherwise."""
     L = lib()
-    B, n_groups = q.shape[0], shared_blocks.shape[0]
+    B, width = q.shape
+    rows, out_width = out.shape
+    n_groups = shared_blocks.numel()
     out_stride, out_dtype = _out_rows(out)
-    if q.shape[1] < n_q_heads * 64:
+    if width < n_q_heads * 64:
         _refuse("q", f"not {n_q_heads} heads of 64")
-    if out.shape[0] != B or out.shape[1] < n_q_heads * 64:
+    if rows != B or out_width < n_q_heads * 64:
         _refuse("out", f"not {B} rows of {n_q_heads} heads of 64")
     ws, ws_bytes = _ws(workspace)
     st = L.gkv_shared_decode(stream_handle(stream), B, n_groups,
                              _of(n_groups + 1, cu_groups, "cu_groups"),
                              _of(n_groups, shared_blocks, "shared_blocks"), max_shared_blocks,
                              max_own, n_q_heads, _there(q, "q"), _row_stride(q, "q"),
-                             _table(cos_tab, "cos_tab"), _table(sin_tab, "sin_tab"),
+                             _of(None, cos_tab, "cos_tab", _torch.float32),
+                             _of(None, sin_tab, "sin_tab", _torch.float32),
                              _of(B, seq_lens, "seq_lens"), max_seq_len, view,
                              _of(n_q_heads, sinks, "sinks", _torch.float32), ws, ws_bytes,
                              _there(out, "out"), out_stride, out_dtype, ptr(dev_err))
@@ -705,7 +704,7 @@ def block_tables(table, lens, refs) -> BlockTables:
     lib()
     n_seqs, stride = table.shape
     return BlockTables(_of(n_seqs * stride, table, "table"), _of(n_seqs, lens, "lens"),
-                       _ints(refs, "refs"), stride, n_seqs, refs.numel())
+                       _of(None, refs, "refs"), stride, n_seqs, refs.numel())
 
 
 def tables_init(tables: BlockTables, stream=None):
