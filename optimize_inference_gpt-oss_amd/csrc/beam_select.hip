@@ -10,8 +10,8 @@
 // Many long rows are bound by HBM: 64 x 8 rows of 131072 fp32 logits (a tenth of them of beams that
 // have ended, 242 MB), 16 best, 50 us, 4.8 TB/s, and 6 for the second launch. Where a wave has
 // but a few tiles, the sorts and the first threshold show: 24 x 5 rows of 200000 in bf16, 10 best,
-// 38 MB, 20 and 7 us; 4 rows of 32001 7 and 6, all of it latency.
-#include "gkv_device.hpp"
+// 38 MB, 19 and 7 us; 4 rows of 32001 6.5 and 6, all of it latency.
+#include "lds_dma.hpp"
 
 #include <algorithm>
 
@@ -103,6 +103,14 @@ __device__ __forceinline__ void sort_step(uint64_t &key, bool down) {
   key = (x > y) == (lower == down) ? x : y;
 }
 
+template <int X>
+__device__ __forceinline__ void sort_step(uint32_t &key, bool down) {
+  uint32_t x, y;
+  pair_of<X>(key, x, y);
+  const bool lower = (threadIdx.x & X) == 0;
+  key = lower == down ? max(x, y) : min(x, y);
+}
+
 // Largest first, of keys that rise and then fall (or the reverse).
 __device__ __forceinline__ void sort_bitonic(uint64_t &key) {
   sort_step<32>(key, true);
@@ -115,7 +123,8 @@ __device__ __forceinline__ void sort_bitonic(uint64_t &key) {
 
 // The 64 lanes' keys, smallest first (so that the lanes of another, sorted the other way round, can
 // be compared one by one).
-__device__ __forceinline__ void sort_up(uint64_t &key) {
+template <typename Key>
+__device__ __forceinline__ void sort_up(Key &key) {
   const int lane = threadIdx.x & 63;
   auto down = [&](int size) { return (lane & size) != 0; };
   sort_step<1>(key, down(2));
@@ -182,18 +191,23 @@ struct Tile {
   }
 };
 
+// What the waves of a workgroup tell each other, in LDS: their n-th best so far, and what their first
+// tiles said of the four together. (Typed as LDS: a volatile access through a plain pointer would be one
+// to memory of any kind, which waits for the tiles under way.)
+typedef volatile __attribute__((address_space(3))) float *Told;
+constexpr int kListMost = 63 + 16 * 64; // candidates of a wave: fewer than a sort's, and a tile
+
 // One wave's tiles t0 .. t1 - 1 of a row: maximum and sum per lane, and the 64 best keys, best in
 // lane 0. What may be among the row's n best is put into the wave's list in LDS, 64 at a time are
 // sorted and joined with the best so far: a few hundred instructions for 64 candidates, where
 // putting them in one by one took some 80 each. Where it meets a NaN or +inf, l ends as NaN, and the
 // caller runs it again with PLAIN, which looks at every value.
-// low: the waves' n-th best so far, in LDS: what is below one of them is not among the row's n
+// low: the waves' n-th best so far: what is below one of them is not among the row's n
 // best, whoever reads it when. The waves begin with what their first tiles say: the n-th largest
 // of one wave's lanes' maxima, or the least of the four waves' n / 4-th.
 template <bool BF, bool PLAIN>
 __device__ __forceinline__ void row_part(const BeamArgs &a, const char *base, int off, int t0, int t1,
-                                         volatile float *low, uint64_t *list, uint64_t &best,
-                                         float &m, float &l) {
+                                         Told low, uint64_t *list, uint64_t &best, float &m, float &l) {
   constexpr int N = Tile<BF>::N;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   best = 0;
@@ -201,17 +215,14 @@ __device__ __forceinline__ void row_part(const BeamArgs &a, const char *base, in
   l = 0.0f;
   float over = -INFINITY; // the least logit that may join: above the n-th best, whose token is lower
   int listed = 0;
-  auto join = [&]() { // the first 64 of the list with the best
+  auto join = [&]() { // the last 64 of the list with the best
     wave_sync();
-    uint64_t key = lane < listed ? list[lane] : 0;
-    const uint64_t rest = lane + 64 < listed ? list[lane + 64] : 0;
+    listed = max(listed - 64, 0);
+    uint64_t key = list[listed + lane];
     sort_up(key);
     best = best > key ? best : key;
     sort_bitonic(best);
     const uint32_t nth = __builtin_amdgcn_readlane((uint32_t)(best >> 32), a.n - 1); // (0: there are fewer)
-    listed = max(listed - 64, 0);
-    wave_sync();
-    list[lane] = rest;
     wave_sync();
     if (nth != 0) {
       over = value_of(nth + 1);
@@ -219,40 +230,35 @@ __device__ __forceinline__ void row_part(const BeamArgs &a, const char *base, in
         low[wave] = value_of(nth);
     }
   };
-  Tile<BF> next, then; // two tiles under way
-  if (t0 < t1)
-    next.load(base, t0, off, a.V);
-  if (t0 + 1 < t1)
-    then.load(base, t0 + 1, off, a.V);
+  Tile<BF> tile[3]; // one looked at, two under way, in turn
+#pragma unroll
+  for (int i = 0; i < 3; i++)
+    if (t0 + i < t1)
+      tile[i].load(base, t0 + i, off, a.V);
   {
     float mx = -INFINITY;
-    if (t0 < t1)
 #pragma unroll
-      for (int k = 0; k < 16; k++)
-        mx = fmaxf(mx, PLAIN ? plain_logit(next.at(k)) : next.at(k));
-    if (t0 + 1 < t1)
+    for (int i = 0; i < 2; i++)
+      if (t0 + i < t1)
 #pragma unroll
-      for (int k = 0; k < 16; k++)
-        mx = fmaxf(mx, PLAIN ? plain_logit(then.at(k)) : then.at(k));
-    uint64_t top = key_of(mx, lane);
+        for (int k = 0; k < 16; k++)
+          mx = fmaxf(mx, PLAIN ? plain_logit(tile[i].at(k)) : tile[i].at(k));
+    uint32_t top = order_of(mx);
     sort_up(top);
-    mx = logit_of(top);
+    mx = value_of(top);
     if (lane == 64 - a.n)
       low[wave] = mx;
     if (lane == 64 - (a.n + kBeamWaves - 1) / kBeamWaves)
       low[kBeamWaves + wave] = mx;
-    __syncthreads();
+    lds_barrier(); // (the third tile stays under way)
   }
   const float fourth = fminf(fminf(low[4], low[5]), fminf(low[6], low[7]));
-  for (int t = t0; t < t1; t++) {
+  auto look = [&](Tile<BF> &now, int t) {
     float x[16], top[4], mx; // the largest of four, of all
     const float l0 = low[0], l1 = low[1], l2 = low[2], l3 = low[3]; // (here: nothing waits for them)
 #pragma unroll
     for (int k = 0; k < 16; k++)
-      x[k] = PLAIN ? plain_logit(next.at(k)) : next.at(k);
-    next = then;
-    if (t + 2 < t1)
-      then.load(base, t + 2, off, a.V);
+      x[k] = PLAIN ? plain_logit(now.at(k)) : now.at(k);
 #pragma unroll
     for (int q = 0; q < 4; q++)
       top[q] = fmaxf(fmaxf(x[4 * q], x[4 * q + 1]), fmaxf(x[4 * q + 2], x[4 * q + 3]));
@@ -264,36 +270,48 @@ __device__ __forceinline__ void row_part(const BeamArgs &a, const char *base, in
     for (int k = 0; k < 16; k++)
       l += __builtin_amdgcn_exp2f((x[k] - m) * kLog2e);
     const float least = fmaxf(fmaxf(fmaxf(l0, l1), fmaxf(l2, l3)), fmaxf(fourth, over));
-    if (!__any(mx >= least))
-      continue;
+    if (__any(mx >= least)) {
 #pragma unroll
-    for (int q = 0; q < 4; q++) {
-      if (!__any(top[q] >= least))
-        continue;
-#pragma unroll
-      for (int k = 4 * q; k < 4 * q + 4; k++) {
-        if (!__any(x[k] >= least))
+      for (int q = 0; q < 4; q++) {
+        if (!__any(top[q] >= least))
           continue;
-        const int e = Tile<BF>::first(t, k / N, off) + k % N;
-        const bool in = (uint32_t)e < (uint32_t)a.V && x[k] >= least;
-        const uint64_t who = __ballot(in);
-        if (in)
-          list[listed + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32),
-                                                  __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] =
-              key_of(x[k], e);
-        listed += __popcll(who);
-        if (listed >= 64)
-          join();
+#pragma unroll
+        for (int k = 4 * q; k < 4 * q + 4; k++) {
+          if (!__any(x[k] >= least))
+            continue;
+          const int e = Tile<BF>::first(t, k / N, off) + k % N;
+          const bool in = (uint32_t)e < (uint32_t)a.V && x[k] >= least;
+          const uint64_t who = __ballot(in);
+          if (in)
+            list[listed + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32),
+                                                    __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] =
+                key_of(x[k], e);
+          listed += __popcll(who);
+        }
       }
     }
+    if (t + 3 < t1)
+      now.load(base, t + 3, off, a.V);
+    while (listed >= 64)
+      join();
+  };
+  for (int t = t0; t < t1; t += 3) {
+    look(tile[0], t);
+    if (t + 1 < t1)
+      look(tile[1], t + 1);
+    if (t + 2 < t1)
+      look(tile[2], t + 2);
   }
-  if (listed > 0)
+  if (listed > 0) {
+    if (lane >= listed) // (what the sort takes beside them: none)
+      list[lane] = 0;
     join();
+  }
 }
 
 template <bool BF>
 __global__ __launch_bounds__(kBeamThreads) void beam_rows_kernel(BeamArgs a) {
-  __shared__ uint64_t s_list[kBeamWaves][2 * 64]; // candidates; then every wave's best
+  __shared__ uint64_t s_list[kBeamWaves][kListMost]; // candidates; then every wave's best
   __shared__ float2 s_ml[kBeamWaves];
   __shared__ float s_low[2][2 * kBeamWaves];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
@@ -304,19 +322,20 @@ __global__ __launch_bounds__(kBeamThreads) void beam_rows_kernel(BeamArgs a) {
     return;
   const char *start = (const char *)a.x + (int64_t)row * a.stride * (BF ? 2 : 4);
   const int off = (int)((uintptr_t)start & 15) / (BF ? 2 : 4);
-  const char *base = (const char *)((uintptr_t)start & ~(uintptr_t)15);
+  const char *base = start - ((uintptr_t)start & 15); // (not by masking: a pointer made of a number is one
+                                                      // to memory of any kind)
   // this wave's tiles, in order
   const int tiles = (int)(((int64_t)off + a.V + 1023) / 1024);
   const int64_t w = (int64_t)part * kBeamWaves + wave, n_waves = (int64_t)a.parts * kBeamWaves;
   const int t0 = (int)(w * tiles / n_waves), t1 = (int)((w + 1) * tiles / n_waves);
   uint64_t best;
   float m, l;
-  row_part<BF, false>(a, base, off, t0, t1, s_low[0], s_list[wave], best, m, l);
+  row_part<BF, false>(a, base, off, t0, t1, (Told)s_low[0], s_list[wave], best, m, l);
   if (__syncthreads_or(l != l)) {
     // (all waves again: what bounded them may have been taken from a NaN)
     if (threadIdx.x == 0 && a.dev_err)
       atomicOr(a.dev_err, GKV_DEVERR_RANGE);
-    row_part<BF, true>(a, base, off, t0, t1, s_low[1], s_list[wave], best, m, l);
+    row_part<BF, true>(a, base, off, t0, t1, (Told)s_low[1], s_list[wave], best, m, l);
   }
   // the lanes' sums, then the waves'
 #pragma unroll
