@@ -560,8 +560,9 @@ size_t gkv_shared_workspace_bytes(int32_t B, int32_t n_groups, int32_t n_q_heads
  *   q, cos_tab / sin_tab, seq_lens, max_seq_len, sinks (NULL: none), out   as in
  *                  gkv_kept_decode; the new tokens are appended
  * A window layer of such sequences reads its window only: gkv_kept_decode. Results do not
- * depend on the order in which workgroups run. For bf16 outputs, weights of shared tokens
- * are rounded to bf16 (each off by at most 2^-8 of itself), and q against e4m3 codes to 11 bits.
+ * depend on the order in which workgroups run. A token counts with the same precision whether its
+ * block is shared or not, gkv_kept_decode's: weights to 2^-16 of themselves (fp32 outputs 2^-24), q to 16
+ * bits against bf16 K (24) and to 22 against codes.
  * Calls that may overlap need workspaces of their own. */
 int gkv_shared_decode(void *stream, int32_t B, int32_t n_groups, const int32_t *cu_groups,
                       const int32_t *shared_blocks, int32_t max_shared_blocks, int32_t max_own,

@@ -17,11 +17,11 @@
 // A sequence shorter than the shared blocks is read on its own, so the prefix
 // needs no mask.
 //
-// 8 kv heads of 8 query heads, bf16 outputs, both launches: 512 sequences of 129 .. 1025 own
-// tokens behind a prompt of 2048, bf16, 149 us (4.2 TB/s; in launches of their own, one kind after
-// the other, 170); 64 x 8 beams behind 256 .. 2048 tokens, codes, 56 (67); one request's four behind
-// 2048 tokens 12 (13.6). 2 x 16 behind 27000, codes, fp32 outputs 68 (72): 580 TF/s with the pieces
-// of q and p; cutting those keeps the vector units longer than the matrix ones.
+// 8 kv heads of 8 query heads, bf16 outputs, both launches (in brackets: one kind of workgroup after
+// the other, in launches of their own): 512 sequences of 129 .. 1025 own tokens behind a prompt of
+// 2048, bf16, 145 us (170), 4.3 TB/s; 64 x 8 beams behind 256 .. 2048 tokens, codes, 58 (67); one
+// request's four behind 2048 tokens 12 (13.6). 2 x 16 behind 27000, codes, fp32 outputs 61: 590 TF/s
+// with the pieces of q and p; cutting those keeps the vector units longer than the matrix ones.
 #include "kept_attend.hpp"
 #include "lds_dma.hpp"
 
@@ -191,16 +191,18 @@ __device__ __forceinline__ void own_piece(const SharedArgs &s, int item, float *
 // it takes registers. One barrier a step. A block's scales come the same way, and the block ids
 // 64 at a time into a register's lanes: a scalar load in the loop would be waited for with
 // the step's LDS reads, which share its counter (8 beams of 64 requests, codes: 65 us so).
-// NT: tiles of 16 query heads per wave. Pieces of q: bf16 K two in bf16 (FINE three), codes one
-// in fp16 (FINE two); p: one in bf16 (FINE three). A bf16 output's own rounding is off by at most
-// 2^-8 of it; so is a weight here, each at random, and q's 11 (16) bits leave far less.
+// NT: tiles of 16 query heads per wave. Pieces of q and p as in kept_attend.hpp, whether a token is
+// shared or not: q against codes two in fp16 (22 bits), against bf16 K two in bf16 (FINE three); p two in
+// bf16 (FINE three), 2^-16 of a weight where the output's own rounding is 2^-8 of it. (One of
+// each leaves a weight off by 2^-8, and a score against codes by 2^-11 of sum |q k| / 8, which grows with
+// the score; 8 beams of 64 requests, codes, 55 us so, 58 with two.)
 template <bool BLK, int NT, int WQ, bool FINE>
 __global__ __launch_bounds__(64 * kSharedWaves)
-__attribute__((amdgpu_waves_per_eu(NT == 1 ? (FINE ? 3 : 4) : NT == 2 && BLK && !FINE ? 4 : 2)))
+__attribute__((amdgpu_waves_per_eu(NT == 1 ? (FINE ? 3 : 4) : BLK ? 3 : 2)))
 void shared_read_kernel(SharedArgs s) {
   constexpr int D = kHeadDim, WT = kSharedWaves / WQ;
   constexpr int kHeadBytes = kBlockTokens * D * (BLK ? 1 : 2);
-  constexpr int QP = BLK ? (FINE ? 2 : 1) : (FINE ? 3 : 2);
+  constexpr int QP = BLK || !FINE ? 2 : 3, PP = FINE ? 3 : 2; // pieces of q, of p
   constexpr int kData = 4 * kHeadBytes;          // K and V of two blocks
   constexpr int kStage = kData + (BLK ? 256 : 0); // and their scales: K0, V0, K1, V1, in the first lanes
   constexpr int DP = WQ == 4 || BLK ? 3 : 2; // (deeper rings cost workgroups, and ran level)
@@ -498,7 +500,7 @@ void shared_read_kernel(SharedArgs s) {
               p[i][r] *= sc[i][1];
           }
 #pragma unroll
-        for (int piece = 0; piece < (FINE ? 3 : 1); piece++) {
+        for (int piece = 0; piece < PP; piece++) {
           u32x4 w;
 #pragma unroll
           for (int i = 0; i < 2; i++)
@@ -506,7 +508,7 @@ void shared_read_kernel(SharedArgs s) {
             for (int r = 0; r < 2; r++) {
               const uint32_t y = f32x2_to_bf16_rne(p[i][2 * r], p[i][2 * r + 1]);
               w[2 * i + r] = y;
-              if (FINE) {
+              if (piece + 1 < PP) {
                 p[i][2 * r] -= __uint_as_float(y << 16);
                 p[i][2 * r + 1] -= __uint_as_float(y & 0xffff0000u);
               }
@@ -673,12 +675,11 @@ static SharedPlan shared_plan(int32_t B, int32_t n_groups, int32_t n_q_heads, in
   const int G = n_q_heads / n_kv_heads;
   const int64_t avg = n_groups > 0 ? std::max<int64_t>(1, ((int64_t)B + n_groups - 1) / n_groups) : 1;
   const int64_t cols = avg * G;
-  // Shapes by the even group's query heads, us of the prefix's workgroups alone (64 groups of
-  // 256 .. 2048 shared tokens, 8 kv heads): 32 heads, two waves of a tile 35 (codes 29), four 40
-  // (42); 64 heads, four waves of one tile 45 (44, fp32 outputs 55), two of two 50 (41, 58);
-  // 128 heads, four waves of two 43 (42). Four waves of four tiles are faster alone (512
-  // sequences behind one prompt of 2048 tokens 45, of two 49), but leave own blocks no room beside
-  // them: 155 for both, 148.
+  // Shapes by the even group's query heads, us of both launches (64 groups of 256 .. 2048 shared
+  // tokens and a token of each sequence's own, 8 kv heads, bf16 outputs): 32 heads, two waves of a tile 41 (codes
+  // 38), four 48 (49); 64 heads, four waves of one tile 59 (57), two of two 54 (58), and with 1 .. 256
+  // own tokens 84 (61) and 71 (58); 128 heads, four waves of two 85 (102), of one 88 (91);
+  // 32 groups of 128 heads with own tokens 56 (60) and 66 (62).
   p.wq = cols <= 32 || (cols <= 64 && blk && !fine) ? 2 : 4;
   p.nt = cols <= 32 || (cols <= 64 && p.wq == 4) ? 1 : 2;
   p.per = 16 * p.nt * p.wq / G;
@@ -687,12 +688,13 @@ static SharedPlan shared_plan(int32_t B, int32_t n_groups, int32_t n_q_heads, in
   p.tiles_each = (int)each + 1;
   p.tiles = p.tiles_each * (int64_t)n_groups;
   // Parts of equal steps, so that long groups have more of them and no workgroup is longer than
-  // the rest; as many as the GPU holds at once, or half of that where a wave's registers are many
-  // (2 x 16 sequences behind 27000 tokens, fp32 outputs, both launches: 512 workgroups 70 us,
-  // 768 71, 1024 71; 512 sequences behind 2048 tokens 148, 768 155).
+  // the rest; as many as the GPU holds at once, or fewer where a wave's registers are many: four waves
+  // of two tiles 512 (512 sequences behind one prompt of 2048 tokens 145 us, 768 workgroups 168; codes
+  // 110 and 120; 2 x 16 behind 27000, codes, 55 and 57), two of two 768 (8 beams of 64 requests, codes,
+  // 58, 512 workgroups 59, 1024 63).
   const int64_t busy = std::max<int64_t>(n_groups * each * n_kv_heads, 1);
   const int64_t steps = ((int64_t)max_shared + 1) / 2;
-  const int64_t wgs = p.nt == 2 && !(blk && !fine) ? 512 : p.nt == 1 && p.wq == 4 ? 2048 : 1024;
+  const int64_t wgs = p.nt == 2 ? (p.wq == 2 ? 768 : 512) : p.wq == 4 ? 2048 : 1024;
   const int64_t room = std::max<int64_t>(1, kSharedPieces / std::max(B, 1));
   const int least = 4 * (kSharedWaves / p.wq);
   const int64_t splits = std::min({wgs / busy, room, (steps + least - 1) / least});
