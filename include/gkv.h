@@ -588,8 +588,10 @@ size_t gkv_beam_workspace_bytes(int32_t n_requests, int32_t n_beams, int32_t voc
  *               one continuation is the token eos at the score that it has
  * and its continuation by token t scores cum_scores + logit[t] - log sum exp(logits). The n_out
  * largest logits of every beam (of equal ones the lower token) compete, best score
- * first, of equal scores the lower beam's (scores of -inf too, where too few others are there;
- * formed and compared in 64 bits):
+ * first, of equal scores the lower beam's (scores of -inf too, where too few others are there).
+ * Scores are formed and compared in 64 bits, from a sum of fp32 exponentials (16 neighbouring tokens'
+ * in fp32, 2^-19 of it at most; the rest in 64 bits): equal rows have the same sum wherever they lie, and a row's
+ * changes by some 2^-50 with the batch that it is in (where its largest logit is past 600, by 2^-20).
  *   scores      fp32 [n_requests][n_out]
  *   parents     int32 [n_requests][n_out]: the row continued, r * n_beams + k
  *   tokens      int32 [n_requests][n_out]

@@ -1,16 +1,27 @@
 // Beam search's choice: for every request the n best of its beams' continuations.
 //
 // A continuation of beam b by token t scores cum[b] + x[b][t] - log sum_v exp x[b][v]. The
-// logits are read once: a wave takes a run of a row, keeps the row's running maximum and sum
-// per lane, and its n best so far in one register across its lanes, sorted. Inside a row the
+// logits are read once: a wave takes a run of a row, keeps its sum per lane, and its n best
+// so far in one register across its lanes, sorted. Inside a row the
 // order is that of the logits, so nothing but their values is compared until the rows meet;
 // scores are formed and compared in 64 bits (two beams' scores differ by as little as
 // their sums' last bits).
 //
+// A row's sum does not depend on where the row lies or how it is cut, which would decide between
+// equal beams: tiles are counted from token 0, whatever the row's alignment; a lane's 16 logits
+// of a tile are summed in fp32 against their largest, r, so that the sum s depends on those 16 alone;
+// and s exp(r), a number of its own for the same reason, is added up in 64 bits, as a power of two
+// times an fp32 number: n = rint(r log2 e), 2^n (s 2^(r log2 e - n)), log2 e in two pieces. What the
+// order of the additions changes is 2^-53 of it; the fp32 terms are off by 2^-22 of theirs. That reaches
+// over |r| <= 700; a row whose largest logit is past 600 takes a second sum, in fp32
+// against a running maximum (of masked values alone it is their number). Both sums for 16 logits are some 20
+// instructions: 24 x 5 rows of 200000 in bf16 25.5 us for 24.6 with the second alone, 64 x 8 of
+// 131072 fp32 55.7 for 54.8.
+//
 // Many long rows are bound by HBM: 64 x 8 rows of 131072 fp32 logits (a tenth of them of beams that
 // have ended, 242 MB), 16 best, 50 us, 4.8 TB/s, and 6 for the second launch. Where a wave has
 // but a few tiles, the sorts and the first threshold show: 24 x 5 rows of 200000 in bf16, 10 best,
-// 38 MB, 19 and 7 us; 4 rows of 32001 6.5 and 6, all of it latency.
+// 38 MB, 19.5 and 7 us; 4 rows of 32001 6.8 and 6, all of it latency.
 #include "lds_dma.hpp"
 
 #include <algorithm>
@@ -23,6 +34,13 @@ constexpr int kBeamWaves = kBeamThreads / 64;
 constexpr int kMergeWaves = 8;
 constexpr float kFloatMax = 3.402823466e38f;
 
+// What a run of a row adds up to: the largest logit m, sum of exp(x - m), and sum of exp(x).
+struct RowSum {
+  float m, l;
+  double sum;
+};
+constexpr float kPlainMost = 600.0f; // |m| up to here: sum is the one that counts
+
 struct BeamArgs {
   const void *x;
   int64_t stride;
@@ -30,7 +48,7 @@ struct BeamArgs {
   const int32_t *done;
   int R, K, V, n, eos;
   int parts;        // workgroups per row
-  float2 *ml;       // [rows][parts] maximum, sum of exp2((x - maximum) log2 e)
+  RowSum *sums;     // [rows][parts]
   float *best;      // [rows][parts][n] logits, best first
   int32_t *token;   // and their tokens; -1: there is none
   float *scores;
@@ -150,32 +168,32 @@ __device__ __forceinline__ void sort_up(Key &key) {
   sort_step<1>(key, false);
 }
 
-// A lane's 16 logits of tile t of a row as fp32: 16-byte granules, 64 lanes side by side, counted
-// from the 16-byte line that the row begins in, off elements before it. Elements outside the row
-// are -inf and not read.
+// A lane's 16 logits of tile t of a row as fp32: granules of 16 bytes, 64 lanes side by side, from
+// token 0 on at whatever address the row begins (rows that begin on no 16-byte line cost little: 64 x 8
+// of 131071 fp32 54.2 us, of 131072 55.7; 24 x 5 of 200001 in bf16 26.3, of 200000 25.5). Elements past
+// the row are -inf and not read.
+typedef uint32_t Granule __attribute__((ext_vector_type(4), aligned(2)));
 template <bool BF>
 struct Tile {
   static constexpr int N = BF ? 8 : 4, U = 16 / N; // of a granule; granules
   u32x4 raw[U];
-  // The element (token) that the lane's granule u begins with.
-  __device__ __forceinline__ static int first(int t, int u, int off) {
-    return (t * 64 * U + u * 64 + (int)(threadIdx.x & 63)) * N - off;
+  // The token that the lane's granule u begins with.
+  __device__ __forceinline__ static int first(int t, int u) {
+    return (t * 64 * U + u * 64 + (int)(threadIdx.x & 63)) * N;
   }
-  __device__ __forceinline__ void load(const char *base, int t, int off, int V) {
+  __device__ __forceinline__ void load(const char *row, int t, int V) {
 #pragma unroll
     for (int u = 0; u < U; u++) {
-      const int e = first(t, u, off);
-      const int64_t i = (int64_t)t * 64 * U + u * 64 + (threadIdx.x & 63);
-      if (e >= 0 && e <= V - N) {
-        raw[u] = __builtin_nontemporal_load((const u32x4 *)base + i);
+      const int e = first(t, u);
+      if (e <= V - N) {
+        raw[u] = __builtin_nontemporal_load((const Granule *)(row + (int64_t)e * (BF ? 2 : 4)));
       } else {
         float v[N];
 #pragma unroll
         for (int j = 0; j < N; j++) {
           v[j] = -INFINITY;
-          if (e + j >= 0 && e + j < V)
-            v[j] = BF ? bf16_to_f32(((const uint16_t *)base)[i * N + j])
-                      : ((const float *)base)[i * N + j];
+          if (e + j < V)
+            v[j] = BF ? bf16_to_f32(((const uint16_t *)row)[e + j]) : ((const float *)row)[e + j];
         }
 #pragma unroll
         for (int j = 0; j < 4; j++)
@@ -197,22 +215,21 @@ struct Tile {
 typedef volatile __attribute__((address_space(3))) float *Told;
 constexpr int kListMost = 63 + 16 * 64; // candidates of a wave: fewer than a sort's, and a tile
 
-// One wave's tiles t0 .. t1 - 1 of a row: maximum and sum per lane, and the 64 best keys, best in
-// lane 0. What may be among the row's n best is put into the wave's list in LDS, 64 at a time are
+// One wave's tiles t0 .. t1 - 1 of a row: sums per lane, and the 64 best keys, best in lane 0. What may be among the row's n best is put into the wave's list in LDS, 64 at a time are
 // sorted and joined with the best so far: a few hundred instructions for 64 candidates, where
-// putting them in one by one took some 80 each. Where it meets a NaN or +inf, l ends as NaN, and the
+// putting them in one by one took some 80 each. Where it meets a NaN or +inf, at.l ends as NaN, and the
 // caller runs it again with PLAIN, which looks at every value.
 // low: the waves' n-th best so far: what is below one of them is not among the row's n
 // best, whoever reads it when. The waves begin with what their first tiles say: the n-th largest
 // of one wave's lanes' maxima, or the least of the four waves' n / 4-th.
 template <bool BF, bool PLAIN>
-__device__ __forceinline__ void row_part(const BeamArgs &a, const char *base, int off, int t0, int t1,
-                                         Told low, uint64_t *list, uint64_t &best, float &m, float &l) {
+__device__ __forceinline__ void row_part(const BeamArgs &a, const char *row, int t0, int t1, Told low,
+                                         uint64_t *list, uint64_t &best, RowSum &at) {
   constexpr int N = Tile<BF>::N;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   best = 0;
-  m = -kFloatMax;
-  l = 0.0f;
+  float m = -kFloatMax, l = 0.0f;
+  double sum = 0;
   float over = -INFINITY; // the least logit that may join: above the n-th best, whose token is lower
   int listed = 0;
   auto join = [&]() { // the last 64 of the list with the best
@@ -234,7 +251,7 @@ __device__ __forceinline__ void row_part(const BeamArgs &a, const char *base, in
 #pragma unroll
   for (int i = 0; i < 2; i++)
     if (t0 + i < t1)
-      tile[i].load(base, t0 + i, off, a.V);
+      tile[i].load(row, t0 + i, a.V);
   {
     float mx = -INFINITY;
 #pragma unroll
@@ -263,12 +280,21 @@ __device__ __forceinline__ void row_part(const BeamArgs &a, const char *base, in
     for (int q = 0; q < 4; q++)
       top[q] = fmaxf(fmaxf(x[4 * q], x[4 * q + 1]), fmaxf(x[4 * q + 2], x[4 * q + 3]));
     mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-    const float mn = fmaxf(m, mx);
-    l *= __builtin_amdgcn_exp2f((m - mn) * kLog2e);
-    m = mn;
+    const float r = fmaxf(mx, -kFloatMax);
+    float s = 0.0f;
 #pragma unroll
     for (int k = 0; k < 16; k++)
-      l += __builtin_amdgcn_exp2f((x[k] - m) * kLog2e);
+      s += __builtin_amdgcn_exp2f((x[k] - r) * kLog2e);
+    {
+      constexpr float kLog2eRest = 1.925963033e-8f; // log2 e - kLog2e
+      const float y = fminf(fmaxf(r, -1000.0f), 1000.0f); // (past 700 the power of two is 0 or inf)
+      const float n = __builtin_rintf(y * kLog2e);
+      const float p = __builtin_amdgcn_exp2f(fmaf(y, kLog2eRest, fmaf(y, kLog2e, -n)));
+      sum += __builtin_ldexp((double)(s * p), (int)n);
+      const float f = __builtin_amdgcn_exp2f(-fabsf(m - r) * kLog2e);
+      l = r > m ? fmaf(l, f, s) : fmaf(s, f, l);
+      m = fmaxf(m, r);
+    }
     const float least = fmaxf(fmaxf(fmaxf(l0, l1), fmaxf(l2, l3)), fmaxf(fourth, over));
     if (__any(mx >= least)) {
 #pragma unroll
@@ -279,8 +305,8 @@ __device__ __forceinline__ void row_part(const BeamArgs &a, const char *base, in
         for (int k = 4 * q; k < 4 * q + 4; k++) {
           if (!__any(x[k] >= least))
             continue;
-          const int e = Tile<BF>::first(t, k / N, off) + k % N;
-          const bool in = (uint32_t)e < (uint32_t)a.V && x[k] >= least;
+          const int e = Tile<BF>::first(t, k / N) + k % N;
+          const bool in = e < a.V && x[k] >= least;
           const uint64_t who = __ballot(in);
           if (in)
             list[listed + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32),
@@ -291,7 +317,7 @@ __device__ __forceinline__ void row_part(const BeamArgs &a, const char *base, in
       }
     }
     if (t + 2 < t1)
-      now.load(base, t + 2, off, a.V);
+      now.load(row, t + 2, a.V);
     while (listed >= 64)
       join();
   };
@@ -305,12 +331,13 @@ __device__ __forceinline__ void row_part(const BeamArgs &a, const char *base, in
       list[lane] = 0;
     join();
   }
+  at = RowSum{m, l, sum};
 }
 
 template <bool BF>
 __global__ __launch_bounds__(kBeamThreads) void beam_rows_kernel(BeamArgs a) {
   __shared__ uint64_t s_list[kBeamWaves][kListMost]; // candidates; then every wave's best
-  __shared__ float2 s_ml[kBeamWaves];
+  __shared__ RowSum s_sums[kBeamWaves];
   __shared__ float s_low[2][2 * kBeamWaves];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int row = blockIdx.x / a.parts, part = blockIdx.x % a.parts;
@@ -319,42 +346,39 @@ __global__ __launch_bounds__(kBeamThreads) void beam_rows_kernel(BeamArgs a) {
   if ((a.done && a.done[row] != 0) || !(cum > -INFINITY))
     return;
   const char *start = (const char *)a.x + (int64_t)row * a.stride * (BF ? 2 : 4);
-  const int off = (int)((uintptr_t)start & 15) / (BF ? 2 : 4);
-  const char *base = start - ((uintptr_t)start & 15); // (not by masking: a pointer made of a number is one
-                                                      // to memory of any kind)
   // this wave's tiles, in order
-  const int tiles = (int)(((int64_t)off + a.V + 1023) / 1024);
+  const int tiles = (int)(((int64_t)a.V + 1023) / 1024);
   const int64_t w = (int64_t)part * kBeamWaves + wave, n_waves = (int64_t)a.parts * kBeamWaves;
   const int t0 = (int)(w * tiles / n_waves), t1 = (int)((w + 1) * tiles / n_waves);
   uint64_t best;
-  float m, l;
-  row_part<BF, false>(a, base, off, t0, t1, (Told)s_low[0], s_list[wave], best, m, l);
-  if (__syncthreads_or(l != l)) {
+  RowSum at;
+  row_part<BF, false>(a, start, t0, t1, (Told)s_low[0], s_list[wave], best, at);
+  if (__syncthreads_or(at.l != at.l)) {
     // (all waves again: what bounded them may have been taken from a NaN)
     if (threadIdx.x == 0 && a.dev_err)
       atomicOr(a.dev_err, GKV_DEVERR_RANGE);
-    row_part<BF, true>(a, base, off, t0, t1, (Told)s_low[1], s_list[wave], best, m, l);
+    row_part<BF, true>(a, start, t0, t1, (Told)s_low[1], s_list[wave], best, at);
   }
   // the lanes' sums, then the waves'
+  auto join = [&](const RowSum &x) {
+    const float mn = fmaxf(at.m, x.m);
+    at.l = at.l * __builtin_amdgcn_exp2f((at.m - mn) * kLog2e) +
+           x.l * __builtin_amdgcn_exp2f((x.m - mn) * kLog2e);
+    at.m = mn;
+    at.sum += x.sum;
+  };
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    const float m2 = __shfl_xor(m, o), l2 = __shfl_xor(l, o), mn = fmaxf(m, m2);
-    l = l * __builtin_amdgcn_exp2f((m - mn) * kLog2e) + l2 * __builtin_amdgcn_exp2f((m2 - mn) * kLog2e);
-    m = mn;
-  }
+  for (int o = 32; o >= 1; o >>= 1)
+    join(RowSum{__shfl_xor(at.m, o), __shfl_xor(at.l, o), __shfl_xor(at.sum, o)});
   if (lane == 0)
-    s_ml[wave] = float2{m, l};
+    s_sums[wave] = at;
   s_list[wave][lane] = best;
   __syncthreads();
-  const int64_t at = (int64_t)row * a.parts + part;
+  const int64_t piece = (int64_t)row * a.parts + part;
   if (threadIdx.x == 0) {
-    for (int k = 1; k < kBeamWaves; k++) {
-      const float mn = fmaxf(m, s_ml[k].x);
-      l = l * __builtin_amdgcn_exp2f((m - mn) * kLog2e) +
-          s_ml[k].y * __builtin_amdgcn_exp2f((s_ml[k].x - mn) * kLog2e);
-      m = mn;
-    }
-    a.ml[at] = float2{m, l};
+    for (int k = 1; k < kBeamWaves; k++)
+      join(s_sums[k]);
+    a.sums[piece] = at;
   }
   // the first wave: the waves' best to the n best of all
   if (wave != 0)
@@ -366,8 +390,8 @@ __global__ __launch_bounds__(kBeamThreads) void beam_rows_kernel(BeamArgs a) {
     sort_bitonic(best);
   }
   if (lane < a.n) {
-    a.best[at * a.n + lane] = logit_of(best);
-    a.token[at * a.n + lane] = best != 0 ? token_of(best) : -1;
+    a.best[piece * a.n + lane] = logit_of(best);
+    a.token[piece * a.n + lane] = best != 0 ? token_of(best) : -1;
   }
 }
 
@@ -433,22 +457,22 @@ __global__ __launch_bounds__(64 * kMergeWaves) void beam_merge_kernel(BeamArgs a
       best = best > key ? best : key;
       sort_bitonic(best);
     }
+    const RowSum *sums = a.sums + (int64_t)row * a.parts;
     float m = -kFloatMax;
     for (int p = lane; p < a.parts; p += 64)
-      m = fmaxf(m, a.ml[(int64_t)row * a.parts + p].x);
+      m = fmaxf(m, sums[p].m);
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1)
       m = fmaxf(m, __shfl_xor(m, o));
+    const bool plain = fabsf(m) <= kPlainMost;
     double l = 0;
-    for (int p = lane; p < a.parts; p += 64) {
-      const float2 ml = a.ml[(int64_t)row * a.parts + p];
-      l += (double)ml.y * exp2(((double)ml.x - (double)m) * 1.4426950408889634);
-    }
+    for (int p = lane; p < a.parts; p += 64)
+      l += plain ? sums[p].sum : (double)sums[p].l * exp2(((double)sums[p].m - (double)m) * 1.4426950408889634);
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1)
       l += __shfl_xor(l, o);
     // (a row of -inf alone: every score is -inf)
-    const double lse = l > 0 ? (double)m + log(l) : 0.0;
+    const double lse = plain ? log(l) : l > 0 ? (double)m + log(l) : 0.0;
     if (lane < a.n) {
       s_score[k * a.n + lane] = c + ((double)logit_of(best) - lse);
       s_token[k * a.n + lane] = token_of(best);
@@ -508,7 +532,7 @@ static BeamWorkspace beam_workspace(int64_t rows, int n) {
   auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
   BeamWorkspace w;
   const size_t pieces = std::max<int64_t>(rows, kBeamWgs); // (what fewer rows need too)
-  w.best = up(pieces * sizeof(float2));
+  w.best = up(pieces * sizeof(RowSum));
   w.token = w.best + up(pieces * n * 4);
   w.total = w.token + pieces * n * 4;
   return w;
@@ -567,7 +591,7 @@ extern "C" int gkv_beam_select(void *stream, int32_t n_requests, int32_t n_beams
   a.n = n_out;
   a.eos = eos;
   a.parts = parts;
-  a.ml = (float2 *)ws;
+  a.sums = (RowSum *)ws;
   a.best = (float *)(ws + w.best);
   a.token = (int32_t *)(ws + w.token);
   a.scores = scores;
