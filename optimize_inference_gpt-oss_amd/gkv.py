@@ -642,8 +642,9 @@ def shared_decode(q, n_q_heads, cu_groups, shared_blocks, seq_lens, max_seq_len,
                   workspace=None, dev_err=None, stream=None):
     """gkv_shared_decode: kept_decode (window 0) for groups of sequences whose first
     shared_blocks[g] blocks are the same, which are read once a group. max_shared_blocks and
-    max_own (tokens behind them) size the launches only. The types of kept_decode; ValueError
-    otherwise."""
+    max_own (tokens behind them) size the launches only. The types of kept_decode, and cos_tab
+    and sin_tab with a row of 32 for every position below max_seq_len and the block table's end;
+    ValueError otherwise."""
     L = lib()
     B, width = q.shape
     rows, out_width = out.shape
@@ -653,14 +654,19 @@ def shared_decode(q, n_q_heads, cu_groups, shared_blocks, seq_lens, max_seq_len,
         _refuse("q", f"not {n_q_heads} heads of 64")
     if rows != B or out_width < n_q_heads * 64:
         _refuse("out", f"not {B} rows of {n_q_heads} heads of 64")
+    cos = _of(None, cos_tab, "cos_tab", _torch.float32)
+    sin = _of(None, sin_tab, "sin_tab", _torch.float32)
+    positions = min(max_seq_len, view.table_stride * 16)
+    if cos_tab is not None and cos_tab.numel() < positions * 32:
+        _refuse("cos_tab", f"not {positions} rows of 32")
+    if sin_tab is not None and sin_tab.numel() < positions * 32:
+        _refuse("sin_tab", f"not {positions} rows of 32")
     ws, ws_bytes = _ws(workspace)
     st = L.gkv_shared_decode(stream_handle(stream), B, n_groups,
                              _of(n_groups + 1, cu_groups, "cu_groups"),
                              _of(n_groups, shared_blocks, "shared_blocks"), max_shared_blocks,
                              max_own, n_q_heads, _there(q, "q"), _row_stride(q, "q"),
-                             _of(None, cos_tab, "cos_tab", _torch.float32),
-                             _of(None, sin_tab, "sin_tab", _torch.float32),
-                             _of(B, seq_lens, "seq_lens"), max_seq_len, view,
+                             cos, sin, _of(B, seq_lens, "seq_lens"), max_seq_len, view,
                              _of(n_q_heads, sinks, "sinks", _torch.float32), ws, ws_bytes,
                              _there(out, "out"), out_stride, out_dtype, ptr(dev_err))
     check("gkv_shared_decode", st)
