@@ -623,6 +623,12 @@ def _of(n, t, what, dtype=None):
     return t.data_ptr()
 
 
+def _map(n, t, what, dtype=None):
+    """_of for a row map: one without elements is not None (torch has no address for it)."""
+    address = _of(n, t, what, dtype)
+    return 16 if t is not None and n == 0 else address
+
+
 def _ws(t):
     """Address and bytes of a workspace, which may be None."""
     if t is None:
@@ -727,16 +733,16 @@ def tables_resize(tables: BlockTables, new_lens, copy_src=None, copy_dst=None, c
                   stream=None):
     """gkv_tables_resize: the lengths new_lens, blocks taken and given back, the copies that shared
     last blocks need (pairs for copy_blocks) and the map of the new rows (row_seq and row_pos int32,
-    row_slot int64, of one size, which bounds the rows). int32 tensors; ValueError otherwise."""
+    row_slot int64, of one size, which bounds the rows, also where it is 0). int32 tensors; ValueError otherwise."""
     L = lib()
     n = tables.n_seqs
     rows = next((t.numel() for t in (row_seq, row_pos, row_slot) if t is not None), 0)
     ws, ws_bytes = _ws(workspace)
     st = L.gkv_tables_resize(stream_handle(stream), tables, _of(n, new_lens, "new_lens"),
                              _of(n, copy_src, "copy_src"), _of(n, copy_dst, "copy_dst"), rows,
-                             _of(n + 1, cu_rows, "cu_rows"), _of(rows, row_seq, "row_seq"),
-                             _of(rows, row_pos, "row_pos"),
-                             _of(rows, row_slot, "row_slot", _torch.int64), ws, ws_bytes,
+                             _of(n + 1, cu_rows, "cu_rows"), _map(rows, row_seq, "row_seq"),
+                             _map(rows, row_pos, "row_pos"),
+                             _map(rows, row_slot, "row_slot", _torch.int64), ws, ws_bytes,
                              ptr(dev_err))
     check("gkv_tables_resize", st)
 

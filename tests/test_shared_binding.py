@@ -30,3 +30,28 @@ def test_tables_of_enough_angles(gkv, monkeypatch, kw):
     with pytest.raises(gkv.GkvError) as e:
         decode(gkv, **kw)
     assert e.value.status == gkv.GKV_ERR_ARG
+
+
+class Calls:
+    """Stands for the library: keeps what a call was given."""
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.name, self.args = name, args
+            return 0
+        return call
+
+
+@pytest.mark.parametrize("given", [("row_seq",), ("row_pos",), ("row_slot",), ("row_seq", "row_pos", "row_slot")])
+@pytest.mark.parametrize("rows", [0, 5])
+def test_row_maps_that_are_empty_are_asked_for_all_the_same(gkv, monkeypatch, given, rows):
+    """A tensor without elements has no address; as none at all it would lift the bound of the rows."""
+    monkeypatch.setattr(torch.Tensor, "is_pinned", lambda self: True)
+    calls = Calls()
+    monkeypatch.setattr(gkv, "lib", lambda: calls)
+    maps = {n: torch.zeros(rows, dtype=torch.int64 if n == "row_slot" else torch.int32) for n in given}
+    gkv.tables_resize(gkv.BlockTables(0x1000, 0x1000, 0x1000, 4, 8, 16), ints(8), stream=NO_STREAM, **maps)
+    assert calls.name == "gkv_tables_resize" and calls.args[5] == rows
+    for n, address in zip(("row_seq", "row_pos", "row_slot"), calls.args[7:10]):
+        assert bool(address) == (n in given)
+        assert not address or address % 8 == 0
