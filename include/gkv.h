@@ -535,8 +535,8 @@ int gkv_copy_blocks(void *stream, const gkv_cache_view *views, int32_t n_views, 
 
 /* ---- Sequences that share their first blocks ------------------------------ */
 
-/* Bytes of workspace that gkv_shared_decode needs for these sizes. Fewer sequences may need more:
- * calls of several sizes that share one take the most of theirs. */
+/* Bytes of workspace that gkv_shared_decode needs for these sizes, and for fewer sequences, any
+ * number of groups and smaller bounds. */
 size_t gkv_shared_workspace_bytes(int32_t B, int32_t n_groups, int32_t n_q_heads,
                                   int32_t n_kv_heads, int32_t max_shared_blocks, int32_t max_own);
 

@@ -661,6 +661,7 @@ __global__ __launch_bounds__(64 * kSharedWaves) void shared_join_kernel(SharedAr
 
 constexpr int kSharedPieces = 2048; // pieces (times sequences) per kind, at most, or one per sequence
 constexpr int kOwnSteps = 72;      // steps of own blocks of a piece, at least
+constexpr int kLeastSteps = 4;     // of shared blocks of a part, per wave's share of the tokens
 
 struct SharedPlan {
   int nt, wq, per, tiles_each;
@@ -668,6 +669,13 @@ struct SharedPlan {
   int splits, part_steps, own_pieces;
   size_t ml, o, total; // workspace (the sequences' first blocks come first)
 };
+
+static void shared_layout(SharedPlan &p, int32_t B, int64_t rows) {
+  auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
+  p.ml = up((size_t)B * 4);
+  p.o = p.ml + up((size_t)rows * 8);
+  p.total = p.o + (size_t)rows * kHeadDim * 4;
+}
 
 static SharedPlan shared_plan(int32_t B, int32_t n_groups, int32_t n_q_heads, int32_t n_kv_heads,
                               int32_t max_shared, int32_t max_own, bool blk, bool fine) {
@@ -696,18 +704,27 @@ static SharedPlan shared_plan(int32_t B, int32_t n_groups, int32_t n_q_heads, in
   const int64_t steps = ((int64_t)max_shared + 1) / 2;
   const int64_t wgs = p.nt == 2 ? (p.wq == 2 ? 768 : 512) : p.wq == 4 ? 2048 : 1024;
   const int64_t room = std::max<int64_t>(1, kSharedPieces / std::max(B, 1));
-  const int least = 4 * (kSharedWaves / p.wq);
+  const int least = kLeastSteps * (kSharedWaves / p.wq);
   const int64_t splits = std::min({wgs / busy, room, (steps + least - 1) / least});
   p.splits = (int)std::max<int64_t>(1, splits);
   p.part_steps = (int)std::max<int64_t>(least, (steps + p.splits - 1) / p.splits);
   const int64_t own_steps = (((int64_t)max_own + kBlockTokens - 1) / kBlockTokens + 1) / 2;
   p.own_pieces = (int)std::max<int64_t>(1, std::min((own_steps + kOwnSteps - 1) / kOwnSteps, room));
-  auto up = [](size_t x) { return (x + 255) & ~(size_t)255; };
-  const size_t rows = (size_t)(p.splits + p.own_pieces) * B * n_q_heads;
-  p.ml = up((size_t)B * 4);
-  p.o = p.ml + up(rows * 8);
-  p.total = p.o + rows * kHeadDim * 4;
+  shared_layout(p, B, (int64_t)(p.splits + p.own_pieces) * B * n_q_heads);
   return p;
+}
+
+// Room for any plan of up to B sequences, in groups of any number: of either kind at most room's
+// pieces, which are kSharedPieces sequences' or one each, and at most what the steps make for each.
+static size_t shared_room(int32_t B, int32_t n_q_heads, int32_t max_shared, int32_t max_own) {
+  const int64_t most = std::max(kSharedPieces, B);
+  const int64_t steps = ((int64_t)max_shared + 1) / 2;
+  const int64_t own_steps = (((int64_t)max_own + kBlockTokens - 1) / kBlockTokens + 1) / 2;
+  const int64_t splits = std::max<int64_t>(1, (steps + kLeastSteps - 1) / kLeastSteps);
+  const int64_t own = std::max<int64_t>(1, (own_steps + kOwnSteps - 1) / kOwnSteps);
+  SharedPlan p{};
+  shared_layout(p, B, (std::min(most, splits * B) + std::min(most, own * B)) * n_q_heads);
+  return p.total;
 }
 
 static bool shared_sizes_ok(int32_t B, int32_t n_groups, int32_t n_q_heads, int32_t n_kv_heads,
@@ -739,11 +756,7 @@ extern "C" size_t gkv_shared_workspace_bytes(int32_t B, int32_t n_groups, int32_
   using namespace gkv;
   if (!shared_sizes_ok(B, n_groups, n_q_heads, n_kv_heads, max_shared_blocks, max_own))
     return 0;
-  size_t most = 0; // (whatever the formats)
-  for (int k = 0; k < 4; k++)
-    most = std::max(most, shared_plan(B, n_groups, n_q_heads, n_kv_heads, max_shared_blocks, max_own,
-                                      k & 1, k & 2).total);
-  return most;
+  return shared_room(B, n_q_heads, max_shared_blocks, max_own);
 }
 
 extern "C" int gkv_shared_decode(void *stream, int32_t B, int32_t n_groups, const int32_t *cu_groups,
