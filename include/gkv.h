@@ -546,7 +546,8 @@ size_t gkv_shared_workspace_bytes(int32_t B, int32_t n_groups, int32_t n_q_heads
  * once for all of them. No counterpart in the reference.
  *   cu_groups      device int32 [n_groups + 1]: group g is the sequences cu_groups[g] ..
  *                  cu_groups[g + 1] - 1, in order, groups of any size (0, 1: nothing gained). A
- *                  sequence in no group is read on its own.
+ *                  sequence in no group is read on its own. Offsets that fall or lie outside 0 .. B:
+ *                  GKV_DEVERR_LENGTH, and any values in the outputs.
  *   shared_blocks  device int32 [n_groups]: the first shared_blocks[g] blocks (16 positions each,
  *                  all full) are the same for the whole group, and are read through
  *                  the table row of the group's first sequence, which holds them all; the other

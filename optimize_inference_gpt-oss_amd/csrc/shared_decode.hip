@@ -81,6 +81,15 @@ __device__ __forceinline__ int group_of(const SharedArgs &s, int b) {
   return g < 0 || g >= s.n_groups || s.cu_groups[g] > b || s.cu_groups[g + 1] <= b ? -1 : g;
 }
 
+// Whether group i's offsets are none: falling, or outside the batch. (What is read and written stays in
+// range by itself; but parts of the prefix may then be nobody's, and what is joined instead anything.)
+__device__ __forceinline__ bool offsets_fall(const SharedArgs &s, int64_t i) {
+  if (i >= s.n_groups)
+    return false;
+  const int from = s.cu_groups[i], to = s.cu_groups[i + 1];
+  return from < 0 || to < from || to > s.a.B;
+}
+
 __device__ __forceinline__ int shared_of(const SharedArgs &s, int grp) {
   return max(min(s.shared[grp], s.a.table_stride), 0);
 }
@@ -115,13 +124,23 @@ __device__ __forceinline__ void own_piece(const SharedArgs &s, int item, float *
   const int slot = wave / a.parts, part = wave % a.parts;
   const int e = item / wgs, pair = item % wgs * each_wg + slot;
   const int b = min(pair, pairs - 1) / a.n_kv_heads, g = min(pair, pairs - 1) % a.n_kv_heads;
+  const bool says = e == 0 && g == 0 && part == 0 && pair < pairs; // this wave speaks for its sequence
+  // (and looks at some of the offsets, 64 of every 64 B: their loads go out before the others')
+  bool none = false;
+  if (says)
+    none = offsets_fall(s, (int64_t)b * 64 + lane);
   const int len = uniform(a.seq_lens[b]), L = max(min(len, a.max_len), 0);
   const int grp = group_of(s, b), shared = grp < 0 ? 0 : uniform(shared_of(s, grp));
   const int first = L / kBlockTokens < shared ? 0 : shared;
-  if (e == 0 && g == 0 && part == 0 && lane == 0 && pair < pairs) {
-    s.first[b] = first;
-    if (a.dev_err && (len > a.max_len || (grp >= 0 && shared != s.shared[grp])))
-      atomicOr(a.dev_err, GKV_DEVERR_LENGTH);
+  if (says) {
+    for (int64_t i = (int64_t)(a.B + b) * 64 + lane; i < s.n_groups; i += (int64_t)a.B * 64)
+      none |= offsets_fall(s, i);
+    const bool wrong = __any(none) || len > a.max_len || (grp >= 0 && shared != s.shared[grp]);
+    if (lane == 0) {
+      s.first[b] = first;
+      if (a.dev_err && wrong)
+        atomicOr(a.dev_err, GKV_DEVERR_LENGTH);
+    }
   }
   Span sp;
   sp.L = L;
