@@ -650,7 +650,11 @@ size_t gkv_tables_workspace_bytes(int32_t n_seqs, int32_t num_blocks);
  * rows behind the last one are left as they were. Too few free blocks, or more new rows than
  * max_rows (of no account without the row arrays): GKV_DEVERR_CAPACITY, and nothing
  * changes (cu_rows and the pairs are 0). A length below 0 or beyond a row: GKV_DEVERR_LENGTH, and
- * that sequence stays as it is. new_lens may be lens itself (nothing happens). */
+ * that sequence stays as it is. new_lens may be lens itself (nothing happens).
+ * Counts of shared blocks (gkv_tables_reorder's, gkv_shared_decode's) are not looked at. A row cut below its
+ * group's count no longer holds those blocks, and once it has grown again it holds others there:
+ * before the next decode the caller lowers the count to the full blocks that were left of the shortest such
+ * row, or has the group counted again (a reorder in which every row is its own parent). */
 int gkv_tables_resize(void *stream, gkv_tables tables, const int32_t *new_lens, int32_t *copy_src,
                       int32_t *copy_dst, int32_t max_rows, int32_t *cu_rows, int32_t *row_seq,
                       int32_t *row_pos, int64_t *row_slot, void *workspace,
@@ -662,7 +666,7 @@ int gkv_tables_resize(void *stream, gkv_tables tables, const int32_t *new_lens, 
  * group_size - 1 the first; n_seqs is a multiple of it, group_size <= 2048); one outside:
  * GKV_DEVERR_BLOCK_ID, and the sequence stays. shared_blocks: NULL, or int32
  * [n_seqs / group_size]: the leading full blocks that all rows of the group now
- * have in common (gkv_shared_decode's). */
+ * have in common (gkv_shared_decode's; 0 where a row is empty). */
 int gkv_tables_reorder(void *stream, gkv_tables tables, int32_t group_size,
                        const int32_t *parents, int32_t *shared_blocks, uint32_t *dev_err);
 
