@@ -678,8 +678,14 @@ __global__ __launch_bounds__(64 * kSharedWaves) void shared_join_kernel(SharedAr
 
 // ---- host side ------------------------------------------------------------------------
 
-constexpr int kSharedPieces = 2048; // pieces (times sequences) per kind, at most, or one per sequence
-constexpr int kOwnSteps = 72;      // steps of own blocks of a piece, at least
+// Pieces (times sequences) per kind, at most, or one per sequence: what the workspace holds, and no time
+// lost (2 x 16 sequences behind 27000 tokens, codes: 512 67 us, 1024 56, 2048 56, 8192 55; 64 x 8 beams and
+// 128 sequences on their own level).
+constexpr int kSharedPieces = 2048;
+// Steps of own blocks of a piece, at least (us with 18, 36, 72, 144, 288: 4 sequences of 8000 ..
+// 16000 own tokens 27, 27, 24, 33, 53; 64 of 4000 .. 9000, codes, 117, 103, 101, 106, 101; 512 of 1000 .. 3000,
+// codes, 235, 227, 219, 223, 223).
+constexpr int kOwnSteps = 72;
 constexpr int kLeastSteps = 4;     // of shared blocks of a part, per wave's share of the tokens
 
 struct SharedPlan {
@@ -842,7 +848,11 @@ extern "C" int gkv_shared_decode(void *stream, int32_t B, int32_t n_groups, cons
   s.own_steps = kOwnSteps;
   if (B == 0)
     return GKV_OK;
-  // waves per (sequence, head): more where few sequences are there, or long ones
+  // Waves per (sequence, head): more where few sequences are there (up to 512 pairs, 1024, 2048, 4096:
+  // 64 sequences of 100 .. 1000 own tokens, codes, 30 us, 22, 20, 20; 128 of them 35, 35, 28, 31), or long
+  // ones (from 32 steps a wave on, 64, 128: 512 of 1000 .. 3000, codes, 225 us, 219, 231; 1024 of 100 .. 1200
+  // 168, 173, 173). The join's waves the same way (four for up to 256 pairs, 1024: 64 sequences of
+  // eight groups 23.7 us, 22.1; 512 level).
   const int64_t own = std::min<int64_t>((((int64_t)max_own + 15) / 16 + 1) / 2, kOwnSteps);
   const int64_t pairs = (int64_t)B * Hkv;
   a.parts = 1;
