@@ -1,10 +1,9 @@
 // Beam search's choice: for every request the n best of its beams' continuations.
 //
 // A continuation of beam b by token t scores cum[b] + x[b][t] - log sum_v exp x[b][v]. The
-// logits are read once: a wave takes a run of a row, keeps its sum per lane, and its n best
-// so far in one register across its lanes, sorted. Inside a row the
-// order is that of the logits, so nothing but their values is compared until the rows meet;
-// scores are formed and compared in 64 bits (two beams' scores differ by as little as
+// logits are read once: a wave takes a run of a row, keeps its sum per lane, and its n best so
+// far in one register across its lanes, sorted. Inside a row the order is that of the logits, so
+// nothing but their values is compared until the rows meet; scores are formed and compared in 64 bits (two beams' scores differ by as little as
 // their sums' last bits).
 //
 // A row's sum does not depend on where the row lies or how it is cut, which would decide between
@@ -12,11 +11,11 @@
 // of a tile are summed in fp32 against their largest, r, so that the sum s depends on those 16 alone;
 // and s exp(r), a number of its own for the same reason, is added up in 64 bits, as a power of two
 // times an fp32 number: n = rint(r log2 e), 2^n (s 2^(r log2 e - n)), log2 e in two pieces. What the
-// order of the additions changes is 2^-53 of it; the fp32 terms are off by 2^-22 of theirs. That reaches
-// over |r| <= 700; a row whose largest logit is past 600 takes a second sum, in fp32
-// against a running maximum (of masked values alone it is their number). Both sums for 16 logits are some 20
-// instructions: 24 x 5 rows of 200000 in bf16 25.5 us for 24.6 with the second alone, 64 x 8 of
-// 131072 fp32 55.7 for 54.8.
+// order of the additions changes is 2^-53 of it; the fp32 sums are off by 2^-19 of theirs at most. That
+// reaches over |r| <= 700; a row whose largest logit is past 600 takes a second sum, in fp32 against a
+// running maximum (of masked values alone it is their number). Both together are some 20
+// instructions for 16 logits: 24 x 5 rows of 200000 in bf16 25.5 us for 24.6 with the second
+// alone, 64 x 8 of 131072 fp32 55.7 for 54.8.
 //
 // Many long rows are bound by HBM: 64 x 8 rows of 131072 fp32 logits (a tenth of them of beams that
 // have ended, 242 MB), 16 best, 50 us, 4.8 TB/s, and 6 for the second launch. Where a wave has
@@ -215,10 +214,11 @@ struct Tile {
 typedef volatile __attribute__((address_space(3))) float *Told;
 constexpr int kListMost = 63 + 16 * 64; // candidates of a wave: fewer than a sort's, and a tile
 
-// One wave's tiles t0 .. t1 - 1 of a row: sums per lane, and the 64 best keys, best in lane 0. What may be among the row's n best is put into the wave's list in LDS, 64 at a time are
+// One wave's tiles t0 .. t1 - 1 of a row: sums per lane, and the 64 best keys, best in lane 0.
+// What may be among the row's n best is put into the wave's list in LDS, 64 at a time are
 // sorted and joined with the best so far: a few hundred instructions for 64 candidates, where
-// putting them in one by one took some 80 each. Where it meets a NaN or +inf, at.l ends as NaN, and the
-// caller runs it again with PLAIN, which looks at every value.
+// putting them in one by one took some 80 each. Where it meets a NaN or +inf, at.l ends as NaN, and
+// the caller runs it again with PLAIN, which looks at every value.
 // low: the waves' n-th best so far: what is below one of them is not among the row's n
 // best, whoever reads it when. The waves begin with what their first tiles say: the n-th largest
 // of one wave's lanes' maxima, or the least of the four waves' n / 4-th.

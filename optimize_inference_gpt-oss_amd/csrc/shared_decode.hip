@@ -686,7 +686,10 @@ constexpr int kSharedPieces = 2048;
 // 16000 own tokens 27, 27, 24, 33, 53; 64 of 4000 .. 9000, codes, 117, 103, 101, 106, 101; 512 of 1000 .. 3000,
 // codes, 235, 227, 219, 223, 223).
 constexpr int kOwnSteps = 72;
-constexpr int kLeastSteps = 4;     // of shared blocks of a part, per wave's share of the tokens
+// Steps of shared blocks of a part, at least, per wave that shares its tokens (us with 1, 2, 4, 8, 16: one
+// request's four sequences behind 2048 tokens 12, 12, 12, 13, 18; 8 x 8 beams, codes, 25, 25, 22, 20, 28;
+// 64 x 4 behind 64 .. 256 tokens 30, 30, 22, 23, 22).
+constexpr int kLeastSteps = 4;
 
 struct SharedPlan {
   int nt, wq, per, tiles_each;
@@ -848,7 +851,7 @@ extern "C" int gkv_shared_decode(void *stream, int32_t B, int32_t n_groups, cons
   s.own_steps = kOwnSteps;
   if (B == 0)
     return GKV_OK;
-  // Waves per (sequence, head): more where few sequences are there (up to 512 pairs, 1024, 2048, 4096:
+  // Waves per (sequence, head): more where few sequences are there (up to 512 waves in all, 1024, 2048, 4096:
   // 64 sequences of 100 .. 1000 own tokens, codes, 30 us, 22, 20, 20; 128 of them 35, 35, 28, 31), or long
   // ones (from 32 steps a wave on, 64, 128: 512 of 1000 .. 3000, codes, 225 us, 219, 231; 1024 of 100 .. 1200
   // 168, 173, 173). The join's waves the same way (four for up to 256 pairs, 1024: 64 sequences of
