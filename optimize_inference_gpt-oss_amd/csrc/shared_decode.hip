@@ -19,7 +19,7 @@
 //
 // 8 kv heads of 8 query heads, bf16 outputs, both launches (in brackets: one kind of workgroup after
 // the other, in launches of their own): 512 sequences of 129 .. 1025 own tokens behind a prompt of
-// 2048, bf16, 145 us (170), 4.3 TB/s; 64 x 8 beams behind 256 .. 2048 tokens, codes, 58 (67); one
+// 2048, bf16, 147 us (170), 4.3 TB/s; 64 x 8 beams behind 256 .. 2048 tokens, codes, 58 (67); one
 // request's four behind 2048 tokens 12 (13.6). 2 x 16 behind 27000, codes, fp32 outputs 61: 590 TF/s
 // with the pieces of q and p; cutting those keeps the vector units longer than the matrix ones.
 #include "kept_attend.hpp"
